@@ -9,21 +9,24 @@ with the source tree to the GPU machine.
 from __future__ import annotations
 
 import os
+import re
 import shutil
 import subprocess
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libravel_b200.so"
+OBJ = PKG / "_build"
 HOST_EXT = PKG / ("_ravel_host" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
     "-Xcompiler", "-fvisibility=default",
 ]
 
@@ -39,19 +42,38 @@ def nvcc_path() -> str:
     return found
 
 
-def sources() -> list[Path]:
-    return sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + [ROOT / "include" / "ravel_b200.h"]
+def units() -> list[Path]:
+    """The translation units of the library."""
+    return sorted(CSRC.glob("*.cu"))
+
+
+def includes(src: Path, seen: set[Path] | None = None) -> set[Path]:
+    """``src`` and every file of this repository that it includes, directly or not."""
+    seen = set() if seen is None else seen
+    if src in seen:
+        return seen
+    seen.add(src)
+    for name in re.findall(r'^\s*#include "([^"]+)"', src.read_text(), flags=re.M):
+        dep = (src.parent / name).resolve()
+        if dep.exists():
+            includes(dep, seen)
+    return seen
 
 
 def host_sources() -> list[Path]:
     return [CSRC / "host_ext.cpp", ROOT / "include" / "ravel_b200.h", LIB]
 
 
+def obj_path(unit: Path) -> Path:
+    return OBJ / (unit.stem + ".o")
+
+
+def stale(unit: Path, target: Path) -> bool:
+    return not target.exists() or any(p.stat().st_mtime > target.stat().st_mtime for p in includes(unit))
+
+
 def needs_build() -> bool:
-    if not LIB.exists():
-        return True
-    mtime = LIB.stat().st_mtime
-    return any(p.stat().st_mtime > mtime for p in sources())
+    return any(stale(u, LIB) for u in units())
 
 
 def build_host(force: bool = False, verbose: bool = False) -> Path:
@@ -76,15 +98,29 @@ def build_host(force: bool = False, verbose: bool = False) -> Path:
 
 
 def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | None = None) -> Path:
-    """Compile ``csrc/ravel_b200.cu`` into ``libravel_b200.so`` when it is stale, then the host extension."""
+    """Compile the stale translation units of ``csrc`` (in parallel) and link ``libravel_b200.so``, then build
+    the host extension."""
     if not force and not needs_build():
         build_host(force=force, verbose=verbose)
         return LIB
-    cmd = [nvcc_path(), *NVCC_FLAGS, *(extra_flags or []), "-o", str(LIB), str(CSRC / "ravel_b200.cu")]
+    OBJ.mkdir(exist_ok=True)
+
+    def compile_unit(unit: Path) -> None:
+        obj = obj_path(unit)
+        tmp = obj.with_suffix(".o.tmp")
+        cmd = [nvcc_path(), *NVCC_FLAGS, *(extra_flags or []), "-c", "-o", str(tmp), str(unit)]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        subprocess.run(cmd, check=True)
+        os.replace(tmp, obj)
+
+    todo = [u for u in units() if force or extra_flags or stale(u, obj_path(u))]
+    with ThreadPoolExecutor(max_workers=max(1, len(todo))) as pool:
+        list(pool.map(compile_unit, todo))
+    tmp = LIB.with_suffix(".so.tmp")
+    cmd = [nvcc_path(), *NVCC_FLAGS, "-shared", "-o", str(tmp), *(str(obj_path(u)) for u in units())]
     if verbose:
         print(" ".join(cmd), flush=True)
-    tmp = LIB.with_suffix(".so.tmp")
-    cmd[cmd.index(str(LIB))] = str(tmp)
     subprocess.run(cmd, check=True)
     os.replace(tmp, LIB)
     build_host(force=True, verbose=verbose)

@@ -1,0 +1,59 @@
+// host.cuh -- host-side plumbing shared by the library's translation units
+// (defined in ravel_b200.cu): launch accounting, launch attributes, per-entry
+// timing, the device error word, and TMA tensor maps.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "../../include/ravel_b200.h"
+
+namespace ravel {
+
+// SMs of the current device.
+int sm_count();
+
+// Called once after every kernel launch of this library: counts it and returns
+// RAVEL_OK or RAVEL_ERR_CUDA.
+int check_launch();
+
+// Raise a kernel's dynamic shared-memory limit to `bytes` (once per kernel and device).
+int raise_smem(const void* kernel, size_t bytes);
+
+template <typename K>
+int set_smem(K kernel, size_t bytes) {
+    return raise_smem(reinterpret_cast<const void*>(kernel), bytes);
+}
+
+// Device addresses of the current device's error word and wait limit, for
+// kernels of other translation units (looked up once per device).
+struct DeviceWords {
+    unsigned int* error;
+    const unsigned int* wait_limit;
+};
+int device_words(DeviceWords* out);
+
+// cuTensorMapEncodeTiled of a row-major 2-D tensor (inner x outer elements,
+// `pitch` bytes between rows), boxes of box_inner x box_outer, 128-byte swizzle,
+// zero fill outside.  type: CU_TENSOR_MAP_DATA_TYPE_*.
+int encode_map_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t inner, int64_t outer,
+                  int64_t pitch, int box_inner, int box_outer);
+
+// One timing record around the rest of the enclosing entry point (a pair of CUDA
+// events while ravel_timing_start's recording is on, nothing otherwise).
+class EntryTimer {
+  public:
+    EntryTimer(const char* entry, void* stream);
+    ~EntryTimer();
+    EntryTimer(const EntryTimer&) = delete;
+    EntryTimer& operator=(const EntryTimer&) = delete;
+
+  private:
+    cudaStream_t st_;
+    int64_t slot_ = -1;
+};
+#define RAVEL_TIMED(entry, stream) ravel::EntryTimer ravel_entry_timer_(entry, stream)
+
+}  // namespace ravel

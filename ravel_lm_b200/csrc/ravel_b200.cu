@@ -16,6 +16,7 @@
 #include <vector>
 
 #include "common.cuh"
+#include "host.cuh"
 #include "sort.cuh"
 #include "latestk.cuh"
 #include "segsum.cuh"
@@ -222,6 +223,8 @@ int64_t max_ranges(int64_t T) { return T > 0 ? (T + RAVEL_RS_RLMIN - 1) / RAVEL_
 #endif
 static_assert(RAVEL_RS_VPL2_NVEC >= 2 && RAVEL_RS_VPL2_NVEC <= 64, "two vectors per lane need two per row");
 
+}  // namespace
+
 int sm_count() {
     static int n = 0;
     if (n == 0) {
@@ -232,6 +235,8 @@ int sm_count() {
     }
     return n;
 }
+
+namespace {
 
 struct ScratchLayout {
     size_t off_sort, off_flags, off_ticket, off_agg, off_incl, off_bflags, off_bval, off_big, total;
@@ -297,13 +302,6 @@ constexpr bool vb_ok() {
 
 std::atomic<uint64_t> g_launches{0};
 
-// Called once after every kernel launch of this library.
-int check_launch() {
-    g_launches.fetch_add(1, std::memory_order_relaxed);
-    const cudaError_t e = cudaGetLastError();
-    return e == cudaSuccess ? RAVEL_OK : RAVEL_ERR_CUDA;
-}
-
 // Per-(kernel, device) results of CUDA attribute calls, so that a launch pays for
 // them once per process instead of on every call.
 std::mutex g_attr_mu;
@@ -315,11 +313,18 @@ int current_device() {
     return cudaGetDevice(&dev) == cudaSuccess ? dev : 0;
 }
 
-template <typename K>
-int set_smem(K kernel, size_t bytes) {
+}  // namespace
+
+int check_launch() {
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? RAVEL_OK : RAVEL_ERR_CUDA;
+}
+
+int raise_smem(const void* kernel, size_t bytes) {
     if (bytes <= 48 * 1024) return RAVEL_OK;
     if (bytes > 227 * 1024) return RAVEL_ERR_UNSUPPORTED;
-    const auto key = std::make_pair(reinterpret_cast<const void*>(kernel), current_device());
+    const auto key = std::make_pair(kernel, current_device());
     std::lock_guard<std::mutex> lock(g_attr_mu);
     auto it = g_smem_set.find(key);
     if (it != g_smem_set.end() && it->second >= bytes) return RAVEL_OK;
@@ -329,6 +334,25 @@ int set_smem(K kernel, size_t bytes) {
     g_smem_set[key] = bytes;
     return RAVEL_OK;
 }
+
+int device_words(DeviceWords* out) {
+    static std::mutex mu;
+    static std::map<int, DeviceWords> found;
+    const int dev = current_device();
+    std::lock_guard<std::mutex> lock(mu);
+    auto it = found.find(dev);
+    if (it == found.end()) {
+        void *e = nullptr, *w = nullptr;
+        if (cudaGetSymbolAddress(&e, g_error_word) != cudaSuccess ||
+            cudaGetSymbolAddress(&w, g_wait_limit) != cudaSuccess)
+            return RAVEL_ERR_CUDA;
+        it = found.emplace(dev, DeviceWords{static_cast<unsigned int*>(e), static_cast<const unsigned int*>(w)}).first;
+    }
+    *out = it->second;
+    return RAVEL_OK;
+}
+
+namespace {
 
 // cudaOccupancyMaxActiveBlocksPerMultiprocessor, remembered per (kernel, device, block, smem).
 template <typename K>
@@ -1154,46 +1178,13 @@ int elem_vec_ok(int64_t n, int esize, std::initializer_list<const void*> ptrs) {
     return 1;
 }
 // ------------------------------------------------------------------ fused gather + fuse Linear
-// cuTensorMapEncodeTiled through the runtime's driver entry point (no libcuda link).
 int encode_weight_map(CUtensorMap* map, const float* W, int64_t N, int64_t K, int box_rows) {
-    static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
-    if (encode == nullptr) {
-        cudaDriverEntryPointQueryResult q;
-        void* fn = nullptr;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess || fn == nullptr)
-            return RAVEL_ERR_CUDA;
-        encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-    }
-    cuuint64_t dims[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(N)};
-    cuuint64_t strides[1] = {static_cast<cuuint64_t>(K) * 4};
-    cuuint32_t box[2] = {static_cast<cuuint32_t>(ravel::GG_BK), static_cast<cuuint32_t>(box_rows)};
-    cuuint32_t estr[2] = {1, 1};
-    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<float*>(W), dims, strides, box,
-                              estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? RAVEL_OK : RAVEL_ERR_CUDA;
+    return ravel::encode_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, W, K, N, K * 4, ravel::GG_BK, box_rows);
 }
 
 // Rows of `rows` x D floats (payload or sums) for TMA gather4: boxes of one row x 32 floats.
 int encode_rows_map(CUtensorMap* map, const float* base, int64_t rows, int64_t D) {
-    static PFN_cuTensorMapEncodeTiled_v12000 encode = nullptr;
-    if (encode == nullptr) {
-        cudaDriverEntryPointQueryResult q;
-        void* fn = nullptr;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
-            q != cudaDriverEntryPointSuccess || fn == nullptr)
-            return RAVEL_ERR_CUDA;
-        encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-    }
-    cuuint64_t dims[2] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(rows)};
-    cuuint64_t strides[1] = {static_cast<cuuint64_t>(D) * 4};
-    cuuint32_t box[2] = {static_cast<cuuint32_t>(ravel::GG_BK), 1};
-    cuuint32_t estr[2] = {1, 1};
-    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<float*>(base), dims, strides, box,
-                              estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                              CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? RAVEL_OK : RAVEL_ERR_CUDA;
+    return ravel::encode_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, base, D, rows, D * 4, ravel::GG_BK, 1);
 }
 
 int gather_args(ravel::GatherArgs& g, const float* payload, const int32_t* src, const float* sums, int64_t B, int64_t T,
@@ -1227,28 +1218,6 @@ struct EntryTiming {
 };
 EntryTiming g_timing;
 
-class EntryTimer {
-  public:
-    EntryTimer(const char* entry, void* stream) : st_(static_cast<cudaStream_t>(stream)) {
-        if (!g_timing.on.load(std::memory_order_acquire)) return;
-        cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-        if (cudaStreamIsCapturing(st_, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone) return;
-        const int64_t i = g_timing.next.fetch_add(1, std::memory_order_relaxed);
-        if (i >= g_timing.cap) return;
-        g_timing.name[i] = entry;
-        if (cudaEventRecord(g_timing.ev[2 * i], st_) == cudaSuccess) slot_ = i;
-    }
-    ~EntryTimer() {
-        if (slot_ >= 0 && cudaEventRecord(g_timing.ev[2 * slot_ + 1], st_) == cudaSuccess) g_timing.closed[slot_] = 1;
-    }
-    EntryTimer(const EntryTimer&) = delete;
-    EntryTimer& operator=(const EntryTimer&) = delete;
-
-  private:
-    cudaStream_t st_;
-    int64_t slot_ = -1;
-};
-
 void timing_release() {
     if (g_timing.device >= 0) {
         int cur = 0;
@@ -1266,8 +1235,53 @@ void timing_release() {
 }
 }  // namespace
 
-// one timing record around the rest of the enclosing entry point
-#define RAVEL_TIMED(entry, stream) EntryTimer ravel_entry_timer_(entry, stream)
+namespace ravel {
+
+EntryTimer::EntryTimer(const char* entry, void* stream) : st_(static_cast<cudaStream_t>(stream)) {
+    if (!g_timing.on.load(std::memory_order_acquire)) return;
+    cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(st_, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone) return;
+    const int64_t i = g_timing.next.fetch_add(1, std::memory_order_relaxed);
+    if (i >= g_timing.cap) return;
+    g_timing.name[i] = entry;
+    if (cudaEventRecord(g_timing.ev[2 * i], st_) == cudaSuccess) slot_ = i;
+}
+
+EntryTimer::~EntryTimer() {
+    if (slot_ >= 0 && cudaEventRecord(g_timing.ev[2 * slot_ + 1], st_) == cudaSuccess) g_timing.closed[slot_] = 1;
+}
+
+// cuTensorMapEncodeTiled through the runtime's driver entry point (no libcuda link).
+int encode_map_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t inner, int64_t outer,
+                  int64_t pitch, int box_inner, int box_outer) {
+    static const PFN_cuTensorMapEncodeTiled_v12000 encode = [] {
+        cudaDriverEntryPointQueryResult q;
+        void* fn = nullptr;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            fn = nullptr;
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    }();
+    if (encode == nullptr) return RAVEL_ERR_CUDA;
+    cuuint64_t dims[2] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer)};
+    cuuint64_t strides[1] = {static_cast<cuuint64_t>(pitch)};
+    cuuint32_t box[2] = {static_cast<cuuint32_t>(box_inner), static_cast<cuuint32_t>(box_outer)};
+    cuuint32_t estr[2] = {1, 1};
+    auto make = [&] {
+        return encode(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult r = make();
+    if (r == CUDA_ERROR_INVALID_CONTEXT || r == CUDA_ERROR_NOT_INITIALIZED) {
+        // a thread's first call (an autograd thread's backward): bind the device's context to it
+        if (cudaSetDevice(current_device()) != cudaSuccess) return RAVEL_ERR_CUDA;
+        r = make();
+    }
+    return r == CUDA_SUCCESS ? RAVEL_OK : RAVEL_ERR_CUDA;
+}
+
+}  // namespace ravel
 
 using namespace ravel;
 
