@@ -318,6 +318,51 @@ int ravel_rms_norm_bwd(const void* x, const void* weight, const void* grad_y, co
                        void* grad_weight, int64_t M, int64_t K, int dtype, void* scratch, size_t scratch_bytes,
                        void* stream);
 
+/* ---- the dense path around the memory ------------------------------------
+ * 16-bit matrix products (bfloat16 or float16, float32 accumulation on the
+ * tensor cores, one rounding).  Rows are `ld` elements apart.
+ */
+/* activations of a product's epilogue */
+#define RAVEL_ACT_NONE 0
+#define RAVEL_ACT_RELU 1
+#define RAVEL_ACT_GELU 2 /* z * Phi(z), with the error function */
+#define RAVEL_ACT_SILU 3 /* z * sigmoid(z) */
+
+/*
+ * y[m][n] = residual[m][n] + act(sum_k A[m][k] * B[n][k] + bias[n]).
+ * A is [M, K] with rows lda apart, or with a_mn stored [K, M]; B is [N, K], or
+ * with b_mn stored [K, N].  The three products of a Linear with weight W [N, K]:
+ *   y  = x W^T:   A = x, B = W
+ *   dx = dz W:    A = dz [M, N], B = W, b_mn   (sum over N)
+ *   dW = dz^T x:  A = dz, a_mn, B = x, b_mn    (sum over M)
+ * a_mn needs b_mn.  bias [N], residual, z (receives the sum before the
+ * activation) are NULL where not wanted; they and act need both operands
+ * K-major.  A and B: 16-byte aligned, lda and ldb multiples of 8
+ * (ravel_pad_rows makes such a copy); y, z, residual and bias may lie anyhow.
+ * Every dimension is at most 2^30.  The summation order depends on the sizes and
+ * the device only: the same inputs give the same bits.
+ */
+int ravel_matmul(const void* A, int64_t lda, int a_mn, const void* B, int64_t ldb, int b_mn, int64_t M, int64_t N,
+                 int64_t K, const void* bias, const void* residual, int64_t ldr, int act, void* y, int64_t ldy,
+                 void* z, int64_t ldz, int dtype, void* stream);
+
+/* Scratch bytes of ravel_linear_dz (per-block column sums). */
+size_t ravel_linear_dz_scratch_bytes(int64_t M, int64_t N);
+
+/*
+ * dz = grad_y * act'(z) over [M, N] (rows ldg, ldz and ldd apart), and
+ * grad_bias[n] = sum_m dz[m][n] from the unrounded products (deterministic: no
+ * atomics).  dz or grad_bias may be NULL; z is not read for RAVEL_ACT_NONE;
+ * scratch is needed for grad_bias only.
+ */
+int ravel_linear_dz(const void* grad_y, int64_t ldg, const void* z, int64_t ldz, int act, void* dz, int64_t ldd,
+                    void* grad_bias, int64_t M, int64_t N, int dtype, void* scratch, size_t scratch_bytes,
+                    void* stream);
+
+/* rows x cols 16-bit elements from row pitch ld to row pitch ldd (elements). */
+int ravel_pad_rows(const void* src, int64_t ld, int64_t rows, int64_t cols, void* dst, int64_t ldd, int dtype,
+                   void* stream);
+
 /*
  * Poll limit of every wait on another block, on the current device (default
  * 2^22 polls, about a second of waiting; 1 .. 2^28).  A copy to device memory:

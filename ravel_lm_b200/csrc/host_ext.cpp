@@ -14,14 +14,23 @@
 // returned to the caller, which raises the library's own errors.  The cache step
 // returns None when its arguments are not the common case (the caller then
 // takes the fully checked Python path, with its error messages).
+//
+// The dense operators (fused_linear) live here whole: argument checks, outputs and
+// workspaces, and the autograd node, so that a decoded token's call or a small
+// training step is not bound by Python.  Workspaces come from the caching
+// allocator on the current stream of the tensors' device.
 
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <optional>
+#include <string>
 #include <tuple>
+#include <vector>
 
 #include "../../include/ravel_b200.h"
 
@@ -169,6 +178,198 @@ std::tuple<int, at::Tensor> latestk_bwd(const at::Tensor& tape, int flags, const
     return {rc, grad};
 }
 
+// ------------------------------------------------------------------ dense operators
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptTensor = std::optional<at::Tensor>;
+
+// A failed library call as the Python error _lib.check raises for its status.
+void check_status(const char* entry, int rc) {
+    if (rc == RAVEL_OK) return;
+    const std::string msg =
+        std::string(entry) + " failed: " + ravel_status_string(rc) + " (status " + std::to_string(rc) + ")";
+    if (rc == RAVEL_ERR_INVALID_ARG || rc == RAVEL_ERR_UNSUPPORTED) throw py::value_error(msg);
+    throw std::runtime_error(msg);
+}
+
+void require_cuda(const at::Tensor& first, std::initializer_list<const OptTensor*> others) {
+    auto cuda = [](const at::Tensor& t) {
+        if (!t.is_cuda())
+            throw std::runtime_error("ravel_lm_b200 runs on CUDA tensors only (got a " + t.device().str() +
+                                     " tensor); there is no CPU fallback");
+    };
+    cuda(first);
+    for (const OptTensor* t : others) {
+        if (!t->has_value()) continue;
+        cuda(**t);
+        if ((*t)->device() != first.device())
+            throw std::runtime_error("tensors are on different devices: " + first.device().str() + " and " +
+                                     (*t)->device().str());
+    }
+}
+
+int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
+
+// A row-major matrix as the kernels take it: elements of a row adjacent, rows `ld` apart.
+struct Rows {
+    at::Tensor t;  // holds the memory
+    int64_t ld = 0;
+};
+
+int64_t leading(const at::Tensor& t) {
+    int64_t n = 1;
+    for (int64_t d = 0; d + 1 < t.dim(); ++d) n *= t.size(d);
+    return n;
+}
+
+// [..., n] as [leading, n] with adjacent elements (a view where the strides allow one).
+Rows rows_of(const at::Tensor& x) {
+    const int64_t n = x.size(-1), m = leading(x);
+    at::Tensor t = x.dim() == 2 ? x : x.reshape({m, n});
+    if ((n > 1 && t.stride(1) != 1) || (m > 1 && t.stride(0) < n)) t = t.contiguous();
+    return {t, m > 1 ? t.stride(0) : up8(n)};
+}
+
+// The same for an operand that TMA reads: 16-byte aligned rows, copied to such a pitch when
+// the tensor has none.
+Rows tma_rows(const at::Tensor& x) {
+    Rows r = rows_of(x);
+    const int64_t m = r.t.size(0), n = r.t.size(1);
+    if (m == 0 || n == 0) return r;
+    if (r.ld % 8 == 0 && reinterpret_cast<uintptr_t>(r.t.data_ptr()) % 16 == 0) return r;
+    Rows p{at::empty({m, up8(n)}, r.t.options()), up8(n)};
+    check_status("ravel_pad_rows", ravel_pad_rows(r.t.data_ptr(), r.ld, m, n, p.t.data_ptr(), p.ld,
+                                                  payload_code(r.t.scalar_type()), stream_of(r.t)));
+    return p;
+}
+
+// y = residual + act(x W^T + bias); x2 and w2 from tma_rows.  z (when wanted): the sum before
+// the activation, rows up8(N) apart.
+at::Tensor linear_forward(const Rows& x2, const Rows& w2, int64_t M, int64_t K, int64_t N, const OptTensor& bias,
+                          const OptTensor& residual, int act, at::IntArrayRef out_shape, at::Tensor* z) {
+    at::Tensor y = at::empty(out_shape, x2.t.options());
+    OptTensor b = bias ? OptTensor(bias->contiguous()) : std::nullopt;
+    Rows res;
+    if (residual) res = rows_of(*residual);
+    if (z != nullptr) *z = at::empty({M, up8(N)}, x2.t.options());
+    check_status("ravel_matmul",
+                 ravel_matmul(x2.t.data_ptr(), x2.ld, 0, w2.t.data_ptr(), w2.ld, 0, M, N, K, ptr_or_null(b),
+                              residual ? res.t.data_ptr() : nullptr, res.ld, act, y.data_ptr(), N,
+                              z != nullptr ? z->data_ptr() : nullptr, up8(N), payload_code(y.scalar_type()),
+                              stream_of(y)));
+    return y;
+}
+
+struct FusedLinear : public torch::autograd::Function<FusedLinear> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight,
+                              const OptTensor& bias, const OptTensor& residual, int64_t act) {
+        const int64_t K = x.size(-1), M = leading(x), N = weight.size(0);
+        const Rows x2 = tma_rows(x), w2 = tma_rows(weight);
+        std::vector<int64_t> shape = x.sizes().vec();
+        shape.back() = N;
+        // without an activation d z is the output's gradient, and z is not needed
+        const bool keep_z = act != RAVEL_ACT_NONE && (x.requires_grad() || weight.requires_grad() ||
+                                                      (bias && bias->requires_grad()));
+        at::Tensor z;
+        at::Tensor y = linear_forward(x2, w2, M, K, N, bias, residual, static_cast<int>(act), shape,
+                                      keep_z ? &z : nullptr);
+        ctx->save_for_backward({x2.t, w2.t, z});
+        ctx->saved_data["x_ld"] = x2.ld;
+        ctx->saved_data["w_ld"] = w2.ld;
+        ctx->saved_data["x_shape"] = x.sizes().vec();
+        ctx->saved_data["N"] = N;
+        ctx->saved_data["act"] = act;
+        ctx->saved_data["bias"] = bias.has_value();
+        ctx->saved_data["residual"] = residual.has_value();
+        return y;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &x2 = saved[0], &w2 = saved[1], &z = saved[2];
+        const std::vector<int64_t> x_shape = ctx->saved_data["x_shape"].toIntVector();
+        const int64_t x_ld = ctx->saved_data["x_ld"].toInt(), w_ld = ctx->saved_data["w_ld"].toInt();
+        const int64_t N = ctx->saved_data["N"].toInt(), K = x_shape.back();
+        const int act = static_cast<int>(ctx->saved_data["act"].toInt());
+        // the gradients this pass asks for; edges are counted over the tensors that were given
+        const bool has_b = ctx->saved_data["bias"].toBool(), has_r = ctx->saved_data["residual"].toBool();
+        const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+        const bool need_b = has_b && ctx->needs_input_grad(2);
+        const bool need_r = has_r && ctx->needs_input_grad(has_b ? 3 : 2);
+        int64_t M = 1;
+        for (size_t d = 0; d + 1 < x_shape.size(); ++d) M *= x_shape[d];
+        variable_list out(5);
+        if (!grads[0].defined()) return out;
+        const c10::cuda::CUDAGuard guard(x2.device());
+        if (need_r) out[3] = grads[0];
+        if (!need_x && !need_w && !need_b) return out;
+        const Rows gy = rows_of(grads[0]);
+        void* const st = stream_of(gy.t);
+        const int dt = payload_code(gy.t.scalar_type());
+        const bool products = need_x || need_w;
+        // the operand of the products: dy itself, or dz (16 bits, TMA-readable rows)
+        Rows dz = gy;
+        const bool own_dz = products && (act != RAVEL_ACT_NONE || gy.ld % 8 != 0 ||
+                                         reinterpret_cast<uintptr_t>(gy.t.data_ptr()) % 16 != 0);
+        if (own_dz) dz = Rows{at::empty({M, up8(N)}, gy.t.options()), up8(N)};
+        if (own_dz || need_b) {
+            at::Tensor scratch;
+            size_t sb = 0;
+            if (need_b) {
+                out[2] = at::empty({N}, gy.t.options());
+                sb = ravel_linear_dz_scratch_bytes(M, N);
+                scratch = bytes(sb, gy.t);
+            }
+            check_status("ravel_linear_dz",
+                         ravel_linear_dz(gy.t.data_ptr(), gy.ld, z.defined() ? z.data_ptr() : nullptr, up8(N), act,
+                                         own_dz ? dz.t.data_ptr() : nullptr, dz.ld,
+                                         need_b ? out[2].data_ptr() : nullptr, M, N, dt,
+                                         need_b ? scratch.data_ptr() : nullptr, sb, st));
+        }
+        if (need_x) {
+            at::Tensor dx = at::empty(x_shape, gy.t.options());
+            check_status("ravel_matmul", ravel_matmul(dz.t.data_ptr(), dz.ld, 0, w2.data_ptr(), w_ld, 1, M, K, N,
+                                                      nullptr, nullptr, 0, RAVEL_ACT_NONE, dx.data_ptr(), K, nullptr,
+                                                      0, dt, st));
+            out[0] = dx;
+        }
+        if (need_w) {
+            at::Tensor dw = at::empty({N, K}, gy.t.options());
+            check_status("ravel_matmul", ravel_matmul(dz.t.data_ptr(), dz.ld, 1, x2.data_ptr(), x_ld, 1, N, K, M,
+                                                      nullptr, nullptr, 0, RAVEL_ACT_NONE, dw.data_ptr(), K, nullptr,
+                                                      0, dt, st));
+            out[1] = dw;
+        }
+        return out;
+    }
+};
+
+at::Tensor fused_linear(const at::Tensor& x, const at::Tensor& weight, const OptTensor& bias,
+                        const OptTensor& residual, int64_t act) {
+    if (x.dim() < 1 || weight.dim() != 2 || weight.size(1) != x.size(-1))
+        throw py::value_error("fused_linear expects x [..., K] and a weight [N, K]");
+    const auto dt = x.scalar_type();
+    if (dt != at::kBFloat16 && dt != at::kHalf)
+        throw py::type_error(std::string("fused_linear takes bfloat16 or float16 tensors, got ") + toString(dt));
+    if (weight.scalar_type() != dt || (bias && bias->scalar_type() != dt) || (residual && residual->scalar_type() != dt))
+        throw py::type_error("fused_linear expects x, weight, bias and residual of one dtype");
+    const int64_t N = weight.size(0);
+    if (bias && (bias->dim() != 1 || bias->size(0) != N)) throw py::value_error("bias must have shape [N]");
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = N;
+    if (residual && residual->sizes() != at::IntArrayRef(shape))
+        throw py::value_error("residual must have the output's shape [..., N]");
+    const OptTensor w(weight);
+    require_cuda(x, {&w, &bias, &residual});
+    const c10::cuda::CUDAGuard guard(x.device());
+    const bool grad = at::GradMode::is_enabled() &&
+                      (x.requires_grad() || weight.requires_grad() || (bias && bias->requires_grad()) ||
+                       (residual && residual->requires_grad()));
+    if (grad) return FusedLinear::apply(x, weight, bias, residual, act);
+    return linear_forward(tma_rows(x), tma_rows(weight), leading(x), x.size(-1), N, bias, residual,
+                          static_cast<int>(act), shape, nullptr);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_ravel_host, m) {
@@ -179,4 +380,5 @@ PYBIND11_MODULE(_ravel_host, m) {
     m.def("segsum_fwd", &segsum_fwd);
     m.def("segsum_bwd", &segsum_bwd);
     m.def("latestk_bwd", &latestk_bwd);
+    m.def("fused_linear", &fused_linear);
 }
