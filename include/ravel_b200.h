@@ -61,9 +61,10 @@ extern "C" {
 /* ---- device-side error bits (ravel_device_error) ------------------------ */
 /* A wait on another block (a scan's look-back, the fused GEMM's pipeline
  * barriers) hit its poll limit and gave up instead of hanging.  Sizes,
- * pointers, alignment and workspace are checked on the host before any launch,
- * so kernels carry no other error bit. */
+ * pointers, alignment and workspace are checked on the host before any launch. */
 #define RAVEL_DEVERR_SPIN 1
+/* an index read from device memory lay outside its range and was not used */
+#define RAVEL_DEVERR_INDEX 2
 
 /* Bytes of the tape written by a forward call and read by its backward call. */
 size_t ravel_tape_bytes(int64_t B, int64_t T, int64_t C, int64_t A, int tape_flags);
@@ -362,6 +363,63 @@ int ravel_linear_dz(const void* grad_y, int64_t ldg, const void* z, int64_t ldz,
 /* rows x cols 16-bit elements from row pitch ld to row pitch ldd (elements). */
 int ravel_pad_rows(const void* src, int64_t ld, int64_t rows, int64_t cols, void* dst, int64_t ldd, int dtype,
                    void* stream);
+
+/*
+ * LayerNorm over the last dimension: y = (x - mean) / sqrt(var + eps) * weight +
+ * bias for M rows of K elements (x's rows ldx apart, y contiguous), float32,
+ * bfloat16 or float16 with float32 statistics.  weight and bias (K elements of
+ * the same type) may be NULL: ones and zeros.  mean and rstd [M] (float32) are
+ * kept for the backward; both NULL where there is none.
+ */
+int ravel_layer_norm_fwd(const void* x, int64_t ldx, const void* weight, const void* bias, float eps, void* y,
+                         float* mean, float* rstd, int64_t M, int64_t K, int dtype, void* stream);
+
+/* Scratch bytes of ravel_layer_norm_bwd (per-block partial weight gradients). */
+size_t ravel_layer_norm_scratch_bytes(int64_t M, int64_t K);
+
+/*
+ * LayerNorm backward: grad_x [M, K] contiguous (NULL: not wanted), grad_weight and
+ * grad_bias [K] (both or neither; deterministic: no atomics, a fixed order).
+ * scratch is needed for the latter only.
+ */
+int ravel_layer_norm_bwd(const void* x, int64_t ldx, const void* weight, const void* grad_y, int64_t ldg,
+                         const float* mean, const float* rstd, void* grad_x, void* grad_weight, void* grad_bias,
+                         int64_t M, int64_t K, int dtype, void* scratch, size_t scratch_bytes, void* stream);
+
+/* reductions of the rows' losses */
+#define RAVEL_REDUCE_NONE 0
+#define RAVEL_REDUCE_SUM 1
+#define RAVEL_REDUCE_MEAN 2 /* over the rows that have a live teacher entry */
+
+/*
+ * Distillation from a teacher's top logits.  Row r has student logits s [V] (rows
+ * ld apart) and k teacher entries (ids[r][j], teacher[r][j]).  An entry is live
+ * when 0 <= id < V and its logit is not -inf; an id >= V also sets
+ * RAVEL_DEVERR_INDEX.  With p = softmax(teacher / T) over the live entries
+ * and q = softmax(s / T) over the vocabulary:
+ *   loss_r = weight T^2 sum_j p_j (log p_j - log q[id_j]);  0 without a live entry
+ * losses [R] receives them, out their sum or mean (RAVEL_REDUCE_SUM / _MEAN; not
+ * used for _NONE), count (MEAN) the rows that have a live entry.  stat [R][2] is
+ * kept for the backward, NULL where there is none.  grad [R, V] contiguous or
+ * NULL: the gradient of out with respect to the logits, made while each row is
+ * still in cache (not for _NONE).  logits: float32, bfloat16 or float16; teacher:
+ * any of those; k <= 4096.
+ */
+int ravel_distill_topk_fwd(const void* logits, int64_t ld, const void* ids, int ids_dtype, const void* teacher,
+                           int teacher_dtype, int64_t R, int64_t V, int64_t k, float temperature, float weight,
+                           int reduction, float* losses, float* stat, uint32_t* count, float* out, void* grad,
+                           int dtype, void* stream);
+
+/*
+ * Its backward for any upstream gradient (on the device: one float32, or [R] for
+ * _NONE): grad[r][v] = u weight T (q_v - sum_{j: id_j = v} p_j) (/ count for MEAN).
+ * With grad_is_unit, grad already holds the forward's gradient: the kernel leaves
+ * it as it is when the upstream gradient is 1, and writes it anew otherwise.
+ */
+int ravel_distill_topk_bwd(const void* logits, int64_t ld, const void* ids, int ids_dtype, const void* teacher,
+                           int teacher_dtype, int64_t R, int64_t V, int64_t k, float temperature, float weight,
+                           int reduction, const float* stat, const uint32_t* count, const float* upstream,
+                           int grad_is_unit, void* grad, int dtype, void* stream);
 
 /*
  * Poll limit of every wait on another block, on the current device (default

@@ -22,11 +22,13 @@ RAVEL_ERR_DEVICE = 5
 
 RAVEL_F32, RAVEL_BF16, RAVEL_F16, RAVEL_F64 = 0, 1, 2, 3
 RAVEL_I32, RAVEL_I64 = 0, 1
+RAVEL_REDUCE_NONE, RAVEL_REDUCE_SUM, RAVEL_REDUCE_MEAN = 0, 1, 2
 RAVEL_ACT_NONE, RAVEL_ACT_RELU, RAVEL_ACT_GELU, RAVEL_ACT_SILU = 0, 1, 2, 3
 RAVEL_TAPE_GENERAL_READS = 1
 RAVEL_TAPE_WRITE_MASK = 2
 RAVEL_NOALLOC_SCRATCH_BYTES = 32 << 20
 RAVEL_DEVERR_SPIN = 1
+RAVEL_DEVERR_INDEX = 2
 
 _c_i64 = ctypes.c_int64
 _c_int = ctypes.c_int
@@ -79,6 +81,15 @@ SIGNATURES = {
     "ravel_linear_dz": (_c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_int, _c_vp, _c_i64, _c_vp, _c_i64, _c_i64, _c_int,
                                  _c_vp, _c_sz, _c_vp]),
     "ravel_pad_rows": (_c_int, [_c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_int, _c_vp]),
+    "ravel_layer_norm_fwd": (_c_int, [_c_vp, _c_i64, _c_vp, _c_vp, ctypes.c_float, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64,
+                                      _c_int, _c_vp]),
+    "ravel_layer_norm_scratch_bytes": (_c_sz, [_c_i64, _c_i64]),
+    "ravel_layer_norm_bwd": (_c_int, [_c_vp, _c_i64, _c_vp, _c_vp, _c_i64] + [_c_vp] * 5 + [_c_i64, _c_i64, _c_int, _c_vp,
+                                      _c_sz, _c_vp]),
+    "ravel_distill_topk_fwd": (_c_int, [_c_vp, _c_i64, _c_vp, _c_int, _c_vp, _c_int] + [_c_i64] * 3 +
+                               [ctypes.c_float, ctypes.c_float, _c_int] + [_c_vp] * 5 + [_c_int, _c_vp]),
+    "ravel_distill_topk_bwd": (_c_int, [_c_vp, _c_i64, _c_vp, _c_int, _c_vp, _c_int] + [_c_i64] * 3 +
+                               [ctypes.c_float, ctypes.c_float, _c_int] + [_c_vp] * 3 + [_c_int, _c_vp, _c_int, _c_vp]),
     "ravel_set_wait_limit": (_c_int, [ctypes.c_uint32]),
     "ravel_wait_selftest": (_c_int, [_c_vp, _c_vp]),
     "ravel_device_error": (_c_int, [ctypes.POINTER(_c_int), _c_vp]),

@@ -1,14 +1,18 @@
 // dense.cu -- C ABI of the dense operators around the event memory: the matrix product with
-// its epilogue.  Argument validation and launch plumbing; the kernels live in the headers.
+// its epilogue, LayerNorm, distillation.  Argument validation and launch plumbing; the kernels
+// live in the headers.
 #include <algorithm>
+#include <cmath>
 #include <cstring>
 #include <map>
 #include <mutex>
 #include <utility>
 
 #include "colsum.cuh"
+#include "distill.cuh"
 #include "host.cuh"
 #include "linear.cuh"
+#include "norm.cuh"
 
 namespace ravel {
 namespace {
@@ -166,6 +170,100 @@ unsigned grid_for(int64_t blocks) {
     return static_cast<unsigned>(std::max<int64_t>(1, std::min<int64_t>(blocks, int64_t{sm_count()} * 32)));
 }
 
+// ------------------------------------------------------------------ LayerNorm
+template <int V> using IC = std::integral_constant<int, V>;
+
+template <typename F>
+int with_float_type(int dtype, F&& f) {
+    if (dtype == RAVEL_F32) return f(float());
+    return with_half_type(dtype, f);
+}
+
+constexpr int64_t kNormMaxK = int64_t{1} << 30;
+
+int esize(int dtype) { return dtype == RAVEL_F32 ? 4 : 2; }
+
+// How a row of K elements is shared: W warps (1, 4, 16; 0: the wide kernels), NV vectors a lane.
+struct NormPlan {
+    int vec, W, NV;
+};
+
+NormPlan plan_norm(int64_t M, int64_t K, int dtype, bool vec) {
+    const int64_t units = vec ? K / (16 / esize(dtype)) : K;
+    const int most = vec ? 4 : 16;  // vectors, or single elements, of a row in a lane's registers
+    // Rows for every SM: as few warps per row as hold it (shuffles alone add up a warp's row).
+    // Fewer rows: more warps per row, for a shorter chain.
+    const bool few = M < static_cast<int64_t>(sm_count()) * 8;
+    for (int w : {1, 4, 16}) {
+        const int64_t per = (units + 32 * w - 1) / (32 * w);
+        if (per > most || (few && w < 16 && per > most / 4)) continue;
+        int nv = most / 4;
+        while (nv < per) nv *= 2;
+        return {vec ? 1 : 0, w, nv};
+    }
+    return {0, 0, 0};
+}
+
+int64_t norm_bwd_blocks(int64_t M, const NormPlan& p) {
+    const int64_t sms = sm_count();
+    if (p.W == 1) return std::max<int64_t>(1, std::min((M + LN_ROWS - 1) / LN_ROWS, sms * 4));
+    return std::max<int64_t>(1, std::min(M, p.W == 4 ? sms * 8 : sms * 2));
+}
+
+// f(VEC, W, NV as integral constants) for a plan with W > 0.
+template <typename T, typename F>
+int with_norm_plan(const NormPlan& p, F&& f) {
+    auto nv = [&](auto vec, auto w) -> int {
+        constexpr int S = decltype(vec)::value == 1 ? 4 : 1;  // NV 4, 8, 16 single elements; 1, 2, 4 vectors
+        if (p.NV == S) return f(vec, w, IC<S>{});
+        if (p.NV == 2 * S) return f(vec, w, IC<2 * S>{});
+        return f(vec, w, IC<4 * S>{});
+    };
+    auto ww = [&](auto vec) -> int {
+        if (p.W == 1) return nv(vec, IC<1>{});
+        if (p.W == 4) return nv(vec, IC<4>{});
+        return nv(vec, IC<16>{});
+    };
+    return p.vec ? ww(IC<16 / sizeof(T)>{}) : ww(IC<1>{});
+}
+
+// ------------------------------------------------------------------ distillation
+constexpr int64_t kDistillMaxK = 4096;
+
+// Threads of a row's block.
+int distill_threads(int64_t R, int64_t V, int dtype) {
+    const int64_t bytes = V * esize(dtype);
+    if (bytes <= 4096) return 128;
+    return R < sm_count() || bytes > 65536 ? 512 : 256;
+}
+
+template <typename F>
+int with_threads(int th, F&& f) {
+    if (th == 128) return f(IC<128>{});
+    if (th == 256) return f(IC<256>{});
+    return f(IC<512>{});
+}
+
+int distill_args(DistillArgs& a, const void* logits, int64_t lds, const void* ids, int ids_dtype, const void* teacher,
+                 int64_t R, int64_t V, int64_t k, float tau, int dtype, int teacher_dtype) {
+    std::memset(&a, 0, sizeof(a));
+    if (R < 0 || V <= 0 || k < 0 || !(tau > 0.0f) || !std::isfinite(tau)) return RAVEL_ERR_INVALID_ARG;
+    if (ids_dtype != RAVEL_I32 && ids_dtype != RAVEL_I64) return RAVEL_ERR_INVALID_ARG;
+    for (int d : {dtype, teacher_dtype})
+        if (d != RAVEL_F32 && d != RAVEL_BF16 && d != RAVEL_F16) return RAVEL_ERR_UNSUPPORTED;
+    if (V > kMaxDim || k > kDistillMaxK || R > 2147483647LL) return RAVEL_ERR_UNSUPPORTED;
+    if (R > 0 && (logits == nullptr || (R > 1 && lds < V) || (k > 0 && (ids == nullptr || teacher == nullptr))))
+        return RAVEL_ERR_INVALID_ARG;
+    a.s = logits; a.ids = ids; a.t = teacher;
+    a.R = R; a.lds = lds; a.V = static_cast<int>(V); a.k = static_cast<int>(k);
+    a.ids64 = ids_dtype == RAVEL_I64;
+    a.tau = tau;
+    DeviceWords w;
+    if (int e = device_words(&w)) return e;
+    a.err = w.error;
+    return RAVEL_OK;
+}
+
 }  // namespace
 }  // namespace ravel
 
@@ -272,6 +370,172 @@ int ravel_pad_rows(const void* src, int64_t ld, int64_t rows, int64_t cols, void
     k_pad_rows<<<grid_for((rows + 7) / 8), 256, 0, static_cast<cudaStream_t>(stream)>>>(
         static_cast<const unsigned short*>(src), ld, rows, cols, static_cast<unsigned short*>(dst), ldd);
     return check_launch();
+}
+
+int ravel_layer_norm_fwd(const void* x, int64_t ldx, const void* weight, const void* bias, float eps, void* y,
+                         float* mean, float* rstd, int64_t M, int64_t K, int dtype, void* stream) {
+    RAVEL_TIMED("ravel_layer_norm_fwd", stream);
+    if (M < 0 || K <= 0 || (mean == nullptr) != (rstd == nullptr)) return RAVEL_ERR_INVALID_ARG;
+    if (dtype != RAVEL_F32 && dtype != RAVEL_BF16 && dtype != RAVEL_F16) return RAVEL_ERR_UNSUPPORTED;
+    if (K > kNormMaxK || M > 2147483647LL) return RAVEL_ERR_UNSUPPORTED;
+    if (M == 0) return RAVEL_OK;
+    if (x == nullptr || y == nullptr || (M > 1 && ldx < K)) return RAVEL_ERR_INVALID_ARG;
+    NormArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.x = x; a.g = weight; a.b = bias; a.out = y; a.mean = mean; a.rstd = rstd;
+    a.M = M; a.ldx = ldx; a.K = static_cast<int>(K); a.eps = eps;
+    const int es = esize(dtype);
+    const bool vec = (K * es) % 16 == 0 && vec16(x, M > 1 ? ldx * es : 0) && aligned16(y) && aligned16(weight) &&
+                     aligned16(bias);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const NormPlan p = plan_norm(M, K, dtype, vec);
+    return with_float_type(dtype, [&](auto tv) -> int {
+        using T = decltype(tv);
+        if (p.W == 0) {
+            k_ln_fwd_wide<T><<<static_cast<unsigned>(M), 32 * LN_WIDE_WARPS, 0, st>>>(a);
+            return check_launch();
+        }
+        return with_norm_plan<T>(p, [&](auto vc, auto wc, auto nc) -> int {
+            constexpr int W = decltype(wc)::value;
+            const int64_t blocks = W == 1 ? (M + LN_ROWS - 1) / LN_ROWS : M;
+            k_ln_fwd<T, decltype(vc)::value, W, decltype(nc)::value>
+                <<<static_cast<unsigned>(blocks), ln_threads<W>(), 0, st>>>(a);
+            return check_launch();
+        });
+    });
+}
+
+size_t ravel_layer_norm_scratch_bytes(int64_t M, int64_t K) {
+    if (M < 0 || K <= 0) return 0;
+    return static_cast<size_t>(std::max<int64_t>(1, std::min<int64_t>(M, int64_t{sm_count()} * 8)) * 2 * K) *
+           sizeof(float);
+}
+
+int ravel_layer_norm_bwd(const void* x, int64_t ldx, const void* weight, const void* grad_y, int64_t ldg,
+                         const float* mean, const float* rstd, void* grad_x, void* grad_weight, void* grad_bias,
+                         int64_t M, int64_t K, int dtype, void* scratch, size_t scratch_bytes, void* stream) {
+    RAVEL_TIMED("ravel_layer_norm_bwd", stream);
+    if (M < 0 || K <= 0 || (grad_weight == nullptr) != (grad_bias == nullptr)) return RAVEL_ERR_INVALID_ARG;
+    if (dtype != RAVEL_F32 && dtype != RAVEL_BF16 && dtype != RAVEL_F16) return RAVEL_ERR_UNSUPPORTED;
+    if (K > kNormMaxK || M > 2147483647LL) return RAVEL_ERR_UNSUPPORTED;
+    if (grad_weight == nullptr && (M == 0 || grad_x == nullptr)) return RAVEL_OK;
+    if (M > 0 && (x == nullptr || grad_y == nullptr || mean == nullptr || rstd == nullptr ||
+                  (M > 1 && (ldx < K || ldg < K))))
+        return RAVEL_ERR_INVALID_ARG;
+    if (grad_weight != nullptr && (scratch == nullptr || scratch_bytes < ravel_layer_norm_scratch_bytes(M, K)))
+        return RAVEL_ERR_WORKSPACE;
+    NormArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.x = x; a.g = weight; a.gy = grad_y; a.out = grad_x;
+    a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
+    a.part = grad_weight != nullptr ? static_cast<float*>(scratch) : nullptr;
+    a.M = M; a.ldx = ldx; a.ldg = ldg; a.K = static_cast<int>(K);
+    const int es = esize(dtype);
+    const bool vec = (K * es) % 16 == 0 && vec16(x, M > 1 ? ldx * es : 0) && vec16(grad_y, M > 1 ? ldg * es : 0) &&
+                     aligned16(grad_x) && aligned16(weight);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const NormPlan p = plan_norm(M, K, dtype, vec);
+    const int64_t blocks = p.W == 0 ? std::max<int64_t>(1, std::min<int64_t>(M, int64_t{sm_count()} * 2))
+                                    : norm_bwd_blocks(M, p);
+    return with_float_type(dtype, [&](auto tv) -> int {
+        using T = decltype(tv);
+        int rc;
+        if (p.W == 0) {
+            k_ln_bwd_wide<T><<<static_cast<unsigned>(blocks), 32 * LN_WIDE_WARPS, 0, st>>>(a);
+            rc = check_launch();
+        } else {
+            rc = with_norm_plan<T>(p, [&](auto vc, auto wc, auto nc) -> int {
+                constexpr int W = decltype(wc)::value;
+                k_ln_bwd<T, decltype(vc)::value, W, decltype(nc)::value>
+                    <<<static_cast<unsigned>(blocks), ln_threads<W>(), 0, st>>>(a);
+                return check_launch();
+            });
+        }
+        if (rc != RAVEL_OK || grad_weight == nullptr) return rc;
+        k_col_reduce<T><<<static_cast<unsigned>((2 * K + CR_COLS - 1) / CR_COLS), CR_COLS * CR_ROWS, 0, st>>>(
+            a.part, static_cast<int>(blocks), 2 * K, K, static_cast<T*>(grad_weight), static_cast<T*>(grad_bias));
+        return check_launch();
+    });
+}
+
+int ravel_distill_topk_fwd(const void* logits, int64_t ld, const void* ids, int ids_dtype, const void* teacher,
+                           int teacher_dtype, int64_t R, int64_t V, int64_t k, float temperature, float weight,
+                           int reduction, float* losses, float* stat, uint32_t* count, float* out, void* grad,
+                           int dtype, void* stream) {
+    RAVEL_TIMED("ravel_distill_topk_fwd", stream);
+    DistillArgs a;
+    if (int e = distill_args(a, logits, ld, ids, ids_dtype, teacher, R, V, k, temperature, dtype, teacher_dtype))
+        return e;
+    if (reduction < RAVEL_REDUCE_NONE || reduction > RAVEL_REDUCE_MEAN) return RAVEL_ERR_INVALID_ARG;
+    if ((R > 0 && losses == nullptr) || (reduction == RAVEL_REDUCE_MEAN && count == nullptr) ||
+        (reduction != RAVEL_REDUCE_NONE && out == nullptr) || (grad != nullptr && reduction == RAVEL_REDUCE_NONE))
+        return RAVEL_ERR_INVALID_ARG;
+    a.weight = weight;
+    a.losses = losses; a.stat = reinterpret_cast<float2*>(stat); a.grad = grad;
+    a.count = reduction == RAVEL_REDUCE_MEAN ? count : nullptr;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const size_t smem = static_cast<size_t>(k) * 8;
+    return with_float_type(teacher_dtype, [&](auto ttv) -> int {
+        using TT = decltype(ttv);
+        if (a.count != nullptr) {
+            if (cudaMemsetAsync(count, 0, sizeof(*count), st) != cudaSuccess) return RAVEL_ERR_CUDA;
+            if (R > 0) {
+                const int64_t blocks = std::min<int64_t>((R + 7) / 8, int64_t{sm_count()} * 4);
+                k_distill_count<TT><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a, count);
+                if (int e = check_launch()) return e;
+            }
+        }
+        if (R > 0) {
+            const int rc = with_float_type(dtype, [&](auto tv) -> int {
+                using T = decltype(tv);
+                return with_threads(distill_threads(R, V, dtype), [&](auto th) -> int {
+                    constexpr int TH = decltype(th)::value;
+                    if (grad != nullptr) k_distill<T, TT, TH, true><<<static_cast<unsigned>(R), TH, smem, st>>>(a);
+                    else k_distill<T, TT, TH, false><<<static_cast<unsigned>(R), TH, smem, st>>>(a);
+                    return check_launch();
+                });
+            });
+            if (rc != RAVEL_OK) return rc;
+        }
+        if (reduction == RAVEL_REDUCE_NONE) return RAVEL_OK;
+        k_distill_total<<<1, 1024, 0, st>>>(losses, R, a.count, out);
+        return check_launch();
+    });
+}
+
+int ravel_distill_topk_bwd(const void* logits, int64_t ld, const void* ids, int ids_dtype, const void* teacher,
+                           int teacher_dtype, int64_t R, int64_t V, int64_t k, float temperature, float weight,
+                           int reduction, const float* stat, const uint32_t* count, const float* upstream,
+                           int grad_is_unit, void* grad, int dtype, void* stream) {
+    RAVEL_TIMED("ravel_distill_topk_bwd", stream);
+    DistillArgs a;
+    if (int e = distill_args(a, logits, ld, ids, ids_dtype, teacher, R, V, k, temperature, dtype, teacher_dtype))
+        return e;
+    if (reduction < RAVEL_REDUCE_NONE || reduction > RAVEL_REDUCE_MEAN) return RAVEL_ERR_INVALID_ARG;
+    if (R == 0) return RAVEL_OK;
+    if (stat == nullptr || upstream == nullptr || grad == nullptr ||
+        (reduction == RAVEL_REDUCE_MEAN && count == nullptr) || (grad_is_unit && reduction == RAVEL_REDUCE_NONE))
+        return RAVEL_ERR_INVALID_ARG;
+    a.weight = weight;
+    a.stat = reinterpret_cast<float2*>(const_cast<float*>(stat));
+    a.grad = grad;
+    a.count = reduction == RAVEL_REDUCE_MEAN ? count : nullptr;
+    a.up = upstream;
+    a.up_rows = reduction == RAVEL_REDUCE_NONE;
+    a.done = grad_is_unit;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    return with_float_type(teacher_dtype, [&](auto ttv) -> int {
+        using TT = decltype(ttv);
+        return with_float_type(dtype, [&](auto tv) -> int {
+            using T = decltype(tv);
+            return with_threads(distill_threads(R, V, dtype), [&](auto th) -> int {
+                constexpr int TH = decltype(th)::value;
+                const int64_t blocks = std::min<int64_t>(R, int64_t{sm_count()} * (2048 / TH));
+                k_distill_bwd<T, TT, TH><<<static_cast<unsigned>(blocks), TH, static_cast<size_t>(k) * 8, st>>>(a);
+                return check_launch();
+            });
+        });
+    });
 }
 
 }  // extern "C"

@@ -15,7 +15,7 @@
 // returns None when its arguments are not the common case (the caller then
 // takes the fully checked Python path, with its error messages).
 //
-// The dense operators (fused_linear) live here whole: argument checks, outputs and
+// The dense operators (fused_linear, layer_norm, distill_topk_loss) live here whole: argument checks, outputs and
 // workspaces, and the autograd node, so that a decoded token's call or a small
 // training step is not bound by Python.  Workspaces come from the caching
 // allocator on the current stream of the tensors' device.
@@ -27,6 +27,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <cmath>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -370,6 +371,213 @@ at::Tensor fused_linear(const at::Tensor& x, const at::Tensor& weight, const Opt
                           static_cast<int>(act), shape, nullptr);
 }
 
+// The element types of LayerNorm and of logits.
+int float_code(const at::Tensor& t, const char* what) {
+    const int c = payload_code(t.scalar_type());
+    if (c != RAVEL_F32 && c != RAVEL_BF16 && c != RAVEL_F16)
+        throw py::type_error(std::string(what) + " takes float32, bfloat16 or float16 tensors, got " +
+                             toString(t.scalar_type()));
+    return c;
+}
+
+at::Tensor norm_forward(const Rows& x2, at::IntArrayRef shape, const OptTensor& weight, const OptTensor& bias,
+                        double eps, at::Tensor* mean, at::Tensor* rstd) {
+    const int64_t M = x2.t.size(0), K = x2.t.size(1);
+    at::Tensor y = at::empty(shape, x2.t.options());
+    if (mean != nullptr) {
+        *mean = at::empty({M}, x2.t.options().dtype(at::kFloat));
+        *rstd = at::empty({M}, x2.t.options().dtype(at::kFloat));
+    }
+    check_status("ravel_layer_norm_fwd",
+                 ravel_layer_norm_fwd(x2.t.data_ptr(), x2.ld, ptr_or_null(weight), ptr_or_null(bias),
+                                      static_cast<float>(eps), y.data_ptr(),
+                                      mean != nullptr ? mean->data_ptr<float>() : nullptr,
+                                      rstd != nullptr ? rstd->data_ptr<float>() : nullptr, M, K,
+                                      payload_code(y.scalar_type()), stream_of(y)));
+    return y;
+}
+
+struct LayerNorm : public torch::autograd::Function<LayerNorm> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const OptTensor& weight, const OptTensor& bias,
+                              double eps) {
+        const Rows x2 = rows_of(x);
+        const OptTensor w = weight ? OptTensor(weight->contiguous()) : std::nullopt;
+        const OptTensor b = bias ? OptTensor(bias->contiguous()) : std::nullopt;
+        at::Tensor mean, rstd;
+        at::Tensor y = norm_forward(x2, x.sizes(), w, b, eps, &mean, &rstd);
+        ctx->save_for_backward({x2.t, w ? *w : at::Tensor(), mean, rstd});
+        ctx->saved_data["ld"] = x2.ld;
+        ctx->saved_data["shape"] = x.sizes().vec();
+        ctx->saved_data["weight"] = weight.has_value();
+        ctx->saved_data["bias"] = bias.has_value();
+        return y;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &x2 = saved[0], &w = saved[1], &mean = saved[2], &rstd = saved[3];
+        const bool has_w = ctx->saved_data["weight"].toBool(), has_b = ctx->saved_data["bias"].toBool();
+        const bool need_x = ctx->needs_input_grad(0), need_w = has_w && ctx->needs_input_grad(1);
+        const bool need_b = has_b && ctx->needs_input_grad(has_w ? 2 : 1);
+        variable_list out(4);
+        if (!grads[0].defined() || !(need_x || need_w || need_b)) return out;
+        const c10::cuda::CUDAGuard guard(x2.device());
+        const int64_t M = x2.size(0), K = x2.size(1);
+        const Rows gy = rows_of(grads[0]);
+        at::Tensor scratch, dw, db;
+        size_t sb = 0;
+        if (need_x) out[0] = at::empty(ctx->saved_data["shape"].toIntVector(), x2.options());
+        if (need_w || need_b) {  // one pass makes both
+            dw = at::empty({K}, x2.options());
+            db = at::empty({K}, x2.options());
+            sb = ravel_layer_norm_scratch_bytes(M, K);
+            scratch = bytes(sb, x2);
+        }
+        check_status("ravel_layer_norm_bwd",
+                     ravel_layer_norm_bwd(x2.data_ptr(), ctx->saved_data["ld"].toInt(),
+                                          w.defined() ? w.data_ptr() : nullptr, gy.t.data_ptr(), gy.ld,
+                                          mean.data_ptr<float>(), rstd.data_ptr<float>(),
+                                          need_x ? out[0].data_ptr() : nullptr, dw.defined() ? dw.data_ptr() : nullptr,
+                                          db.defined() ? db.data_ptr() : nullptr, M, K,
+                                          payload_code(x2.scalar_type()), sb ? scratch.data_ptr() : nullptr, sb,
+                                          stream_of(x2)));
+        if (need_w) out[1] = dw;
+        if (need_b) out[2] = db;
+        return out;
+    }
+};
+
+at::Tensor layer_norm(const at::Tensor& x, const OptTensor& weight, const OptTensor& bias, double eps) {
+    if (x.dim() < 1 || x.size(-1) < 1) throw py::value_error("layer_norm expects x [..., K] with K >= 1");
+    const int64_t K = x.size(-1);
+    for (const OptTensor* t : {&weight, &bias})
+        if (t->has_value() && ((*t)->dim() != 1 || (*t)->size(0) != K))
+            throw py::value_error("layer_norm expects weight and bias of shape [x.shape[-1]]");
+    float_code(x, "layer_norm");
+    for (const OptTensor* t : {&weight, &bias})
+        if (t->has_value() && (*t)->scalar_type() != x.scalar_type())
+            throw py::type_error("layer_norm expects x, weight and bias of one dtype");
+    require_cuda(x, {&weight, &bias});
+    const c10::cuda::CUDAGuard guard(x.device());
+    if (at::GradMode::is_enabled() &&
+        (x.requires_grad() || (weight && weight->requires_grad()) || (bias && bias->requires_grad())))
+        return LayerNorm::apply(x, weight, bias, eps);
+    return norm_forward(rows_of(x), x.sizes(), weight ? OptTensor(weight->contiguous()) : std::nullopt,
+                        bias ? OptTensor(bias->contiguous()) : std::nullopt, eps, nullptr, nullptr);
+}
+
+// The tensors of a distillation call, and its launch.
+struct DistillCall {
+    Rows s;
+    at::Tensor ids, teacher, losses, stat, count, out;
+    int64_t R, V, k;
+    float tau, weight;
+    int reduction, dtype;
+
+    DistillCall(const at::Tensor& logits, const at::Tensor& ids_, const at::Tensor& teacher_, double tau_,
+                double weight_, int64_t reduction_)
+        : s(rows_of(logits)), ids(ids_.contiguous()), teacher(teacher_.contiguous()), R(s.t.size(0)), V(s.t.size(1)),
+          k(ids_.size(-1)), tau(static_cast<float>(tau_)), weight(static_cast<float>(weight_)),
+          reduction(static_cast<int>(reduction_)), dtype(payload_code(logits.scalar_type())) {}
+
+    int ids_code() const { return ids.scalar_type() == at::kLong ? RAVEL_I64 : RAVEL_I32; }
+
+    // losses (and their reduction); stat is kept and grad written where wanted.
+    at::Tensor forward(at::IntArrayRef rows_shape, bool keep, const at::Tensor& grad) {
+        const auto f32 = s.t.options().dtype(at::kFloat);
+        losses = at::empty(rows_shape, f32);
+        if (keep) stat = at::empty({R, 2}, f32);
+        if (reduction == RAVEL_REDUCE_MEAN) count = at::empty({1}, f32.dtype(at::kInt));
+        if (reduction != RAVEL_REDUCE_NONE) out = at::empty({}, f32);
+        check_status("ravel_distill_topk_fwd",
+                     ravel_distill_topk_fwd(s.t.data_ptr(), s.ld, ids.data_ptr(), ids_code(), teacher.data_ptr(),
+                                            payload_code(teacher.scalar_type()), R, V, k, tau, weight, reduction,
+                                            losses.data_ptr<float>(), keep ? stat.data_ptr<float>() : nullptr,
+                                            count.defined() ? reinterpret_cast<uint32_t*>(count.data_ptr<int>()) : nullptr,
+                                            out.defined() ? out.data_ptr<float>() : nullptr,
+                                            grad.defined() ? grad.data_ptr() : nullptr, dtype, stream_of(s.t)));
+        return reduction == RAVEL_REDUCE_NONE ? losses : out;
+    }
+};
+
+struct DistillTopk : public torch::autograd::Function<DistillTopk> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& logits, const at::Tensor& ids,
+                              const at::Tensor& teacher, double tau, double weight, int64_t reduction) {
+        DistillCall c(logits, ids, teacher, tau, weight, reduction);
+        // The gradient for an upstream gradient of 1 while the rows are in cache: a training step
+        // then reads the logits from memory once.  Not for float16, where it may underflow before
+        // the loss scaling of the upstream gradient reaches it, nor for single rows' losses, whose
+        // upstream gradients are rarely 1.
+        at::Tensor unit;
+        if (reduction != RAVEL_REDUCE_NONE && c.dtype != RAVEL_F16) unit = at::empty(logits.sizes(), c.s.t.options());
+        const auto sizes = logits.sizes();
+        at::Tensor loss = c.forward(sizes.slice(0, sizes.size() - 1), true, unit);
+        ctx->save_for_backward({c.s.t, c.ids, c.teacher, c.stat, c.count});
+        if (unit.defined()) ctx->saved_data["unit"] = unit;
+        ctx->saved_data["ld"] = c.s.ld;
+        ctx->saved_data["shape"] = sizes.vec();
+        ctx->saved_data["tau"] = tau;
+        ctx->saved_data["weight"] = weight;
+        ctx->saved_data["reduction"] = reduction;
+        return loss;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &s = saved[0], &ids = saved[1], &teacher = saved[2], &stat = saved[3], &count = saved[4];
+        variable_list out(6);
+        if (!grads[0].defined()) return out;
+        const c10::cuda::CUDAGuard guard(s.device());
+        // The forward's gradient is given away once; a second backward pass writes a new one.
+        at::Tensor grad;
+        const auto it = ctx->saved_data.find("unit");
+        const bool unit = it != ctx->saved_data.end();
+        if (unit) {
+            grad = it->second.toTensor();
+            ctx->saved_data.erase(it);
+        } else {
+            grad = at::empty(ctx->saved_data["shape"].toIntVector(), s.options());
+        }
+        const at::Tensor up = grads[0].contiguous();
+        check_status(
+            "ravel_distill_topk_bwd",
+            ravel_distill_topk_bwd(s.data_ptr(), ctx->saved_data["ld"].toInt(), ids.data_ptr(),
+                                   ids.scalar_type() == at::kLong ? RAVEL_I64 : RAVEL_I32, teacher.data_ptr(),
+                                   payload_code(teacher.scalar_type()), s.size(0), s.size(1), ids.size(-1),
+                                   static_cast<float>(ctx->saved_data["tau"].toDouble()),
+                                   static_cast<float>(ctx->saved_data["weight"].toDouble()),
+                                   static_cast<int>(ctx->saved_data["reduction"].toInt()), stat.data_ptr<float>(),
+                                   count.defined() ? reinterpret_cast<const uint32_t*>(count.data_ptr<int>()) : nullptr,
+                                   up.data_ptr<float>(), unit ? 1 : 0, grad.data_ptr(),
+                                   payload_code(s.scalar_type()), stream_of(s)));
+        out[0] = grad;
+        return out;
+    }
+};
+
+at::Tensor distill_topk_loss(const at::Tensor& logits, const at::Tensor& ids, const at::Tensor& teacher, double tau,
+                             double weight, int64_t reduction) {
+    if (logits.dim() < 1 || logits.size(-1) < 1)
+        throw py::value_error("distill_topk_loss expects logits [..., V] with V >= 1");
+    if (ids.dim() != logits.dim() || ids.sizes() != teacher.sizes() ||
+        ids.sizes().slice(0, ids.dim() - 1) != logits.sizes().slice(0, logits.dim() - 1))
+        throw py::value_error("teacher_ids and teacher_logits must both be [..., k] with the logits' leading dimensions");
+    if (ids.scalar_type() != at::kInt && ids.scalar_type() != at::kLong)
+        throw py::type_error("teacher_ids must be int32 or int64");
+    float_code(logits, "distill_topk_loss");
+    float_code(teacher, "distill_topk_loss");
+    if (!(tau > 0.0) || !std::isfinite(tau)) throw py::value_error("temperature must be positive and finite");
+    if (teacher.requires_grad() && at::GradMode::is_enabled())
+        throw py::value_error("teacher_logits must not require a gradient (detach them)");
+    const OptTensor i(ids), t(teacher);
+    require_cuda(logits, {&i, &t});
+    const c10::cuda::CUDAGuard guard(logits.device());
+    if (at::GradMode::is_enabled() && logits.requires_grad())
+        return DistillTopk::apply(logits, ids, teacher, tau, weight, reduction);
+    DistillCall c(logits, ids, teacher, tau, weight, reduction);
+    return c.forward(logits.sizes().slice(0, logits.dim() - 1), false, at::Tensor());
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_ravel_host, m) {
@@ -381,4 +589,6 @@ PYBIND11_MODULE(_ravel_host, m) {
     m.def("segsum_bwd", &segsum_bwd);
     m.def("latestk_bwd", &latestk_bwd);
     m.def("fused_linear", &fused_linear);
+    m.def("layer_norm", &layer_norm);
+    m.def("distill_topk_loss", &distill_topk_loss);
 }

@@ -1,0 +1,318 @@
+// norm.cuh -- LayerNorm over the last dimension, forward and backward.
+//
+//   k_ln_fwd   y = (x - mean) * rstd * g + b, rstd = 1 / sqrt(var + eps).  A row is held in
+//              registers by W warps, NV vectors of VEC elements per lane: read once, the mean and
+//              then the variance around it summed from registers (no cancellation), written once.
+//   k_ln_bwd   with a = dy * g and xh = (x - mean) * rstd:
+//              dx = rstd * (a - mean(a) - xh * mean(a * xh)); d g = sum_rows dy * xh,
+//              d b = sum_rows dy.  A lane owns the same columns in every row its group takes, so the
+//              weight gradients accumulate in registers; one row of partial sums per block leaves
+//              the kernel and k_col_reduce adds them in block order (deterministic, no atomics).
+//   k_ln_*_wide  any row length: a block per row that reads it again instead of holding it.
+// All are bound by HBM: 2 (forward) and 3 (backward) row passes.  Statistics, sums and the weight
+// gradients are float32; each output is rounded once.
+#pragma once
+
+#include "colsum.cuh"
+#include "host.cuh"
+
+namespace ravel {
+
+template <typename T> __device__ __forceinline__ float as_float(T v);
+template <> __device__ __forceinline__ float as_float<float>(float v) { return v; }
+template <> __device__ __forceinline__ float as_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <> __device__ __forceinline__ float as_float<__half>(__half v) { return __half2float(v); }
+
+// VEC elements as loaded: one 16-byte load, or a single element.
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC) Pack {
+    T v[VEC];
+};
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> load_pack(const T* p) {
+    Pack<T, VEC> r;
+    if constexpr (sizeof(T) * VEC == 16)
+        *reinterpret_cast<uint4*>(&r) = __ldg(reinterpret_cast<const uint4*>(p));
+    else
+        r = *reinterpret_cast<const Pack<T, VEC>*>(p);
+    return r;
+}
+
+struct NormArgs {
+    const void* x;       // [M, K], rows ldx apart
+    const void* g;       // [K] or null (ones)
+    const void* b;       // [K] or null (zeros)
+    const void* gy;      // [M, K], rows ldg apart (backward)
+    void* out;           // y or dx, [M, K] contiguous; the backward's may be null
+    float* mean;         // [M]; forward: null when not wanted
+    float* rstd;
+    float* part;         // backward: [blocks][2K] partial d g | d b, or null
+    int64_t M, ldx, ldg;
+    int K;
+    float eps;
+};
+
+// Sums of two values over the W warps of a group; every lane gets them.  For W > 1 the group is
+// the block; `red` has two halves used in turn, so one barrier per call is enough.
+template <int W>
+__device__ __forceinline__ float2 group_sum2(float a, float b, float2* red, int& turn) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        a += __shfl_xor_sync(0xffffffffu, a, o);
+        b += __shfl_xor_sync(0xffffffffu, b, o);
+    }
+    if constexpr (W > 1) {
+        float2* const r = red + turn * W;
+        turn ^= 1;
+        if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = make_float2(a, b);
+        __syncthreads();
+        a = b = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            a += r[w].x;
+            b += r[w].y;
+        }
+    }
+    return make_float2(a, b);
+}
+
+// rows (one per warp) of a block when a row takes one warp
+constexpr int LN_ROWS = 8;
+template <int W> constexpr int ln_threads() { return W == 1 ? 32 * LN_ROWS : 32 * W; }
+
+template <typename T, int VEC, int W, int NV>
+__global__ void __launch_bounds__(ln_threads<W>()) k_ln_fwd(const NormArgs a) {
+    __shared__ float2 red[2 * W];
+    int turn = 0;
+    const int lane = W == 1 ? (threadIdx.x & 31) : threadIdx.x;
+    const int64_t row = W == 1 ? static_cast<int64_t>(blockIdx.x) * LN_ROWS + (threadIdx.x >> 5) : blockIdx.x;
+    if (row >= a.M) return;  // whole warps; with W > 1 every row exists
+    const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
+    Pack<T, VEC> v[NV];
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * 32 * W + lane) * VEC;
+        if (c < a.K) v[i] = load_pack<T, VEC>(x + c);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if ((i * 32 * W + lane) * VEC < a.K) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) s += as_float(v[i].v[e]);
+        }
+    }
+    const float inv_k = 1.0f / static_cast<float>(a.K);
+    const float mean = group_sum2<W>(s, 0.0f, red, turn).x * inv_k;
+    float ss = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if ((i * 32 * W + lane) * VEC < a.K) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float d = as_float(v[i].v[e]) - mean;
+                ss = fmaf(d, d, ss);
+            }
+        }
+    }
+    const float rstd = rsqrtf(group_sum2<W>(ss, 0.0f, red, turn).x * inv_k + a.eps);
+    if (lane == 0 && a.mean != nullptr) {
+        a.mean[row] = mean;
+        a.rstd[row] = rstd;
+    }
+    T* const y = static_cast<T*>(a.out) + row * a.K;
+    const T* const g = static_cast<const T*>(a.g);
+    const T* const b = static_cast<const T*>(a.b);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * 32 * W + lane) * VEC;
+        if (c < a.K) {
+            Pack<T, VEC> gv, bv, o;
+            if (g != nullptr) gv = load_pack<T, VEC>(g + c);
+            if (b != nullptr) bv = load_pack<T, VEC>(b + c);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                float t = (as_float(v[i].v[e]) - mean) * rstd;
+                if (g != nullptr) t *= as_float(gv.v[e]);
+                if (b != nullptr) t += as_float(bv.v[e]);
+                o.v[e] = round_to<T>(t);
+            }
+            *reinterpret_cast<Pack<T, VEC>*>(y + c) = o;
+        }
+    }
+}
+
+template <typename T, int VEC, int W, int NV>
+__global__ void __launch_bounds__(ln_threads<W>()) k_ln_bwd(const NormArgs a) {
+    constexpr int COLS = 32 * W * NV * VEC;
+    __shared__ float2 red[2 * W];
+    __shared__ float wsum[W == 1 ? 2 * COLS : 1];
+    int turn = 0;
+    const int lane = W == 1 ? (threadIdx.x & 31) : threadIdx.x;
+    const int warp = threadIdx.x >> 5;
+    const T* const g = static_cast<const T*>(a.g);
+    float dg[NV * VEC], db[NV * VEC];
+#pragma unroll
+    for (int i = 0; i < NV * VEC; ++i) dg[i] = db[i] = 0.0f;
+    const float inv_k = 1.0f / static_cast<float>(a.K);
+    const int64_t first = W == 1 ? static_cast<int64_t>(blockIdx.x) * LN_ROWS + warp : blockIdx.x;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * (W == 1 ? LN_ROWS : 1);
+    for (int64_t row = first; row < a.M; row += step) {
+        const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
+        const T* const gy = static_cast<const T*>(a.gy) + row * a.ldg;
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        Pack<T, VEC> xv[NV], yv[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * 32 * W + lane) * VEC;
+            if (c < a.K) {
+                xv[i] = load_pack<T, VEC>(x + c);
+                yv[i] = load_pack<T, VEC>(gy + c);
+            }
+        }
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * 32 * W + lane) * VEC;
+            if (c < a.K) {
+                Pack<T, VEC> gv;
+                if (g != nullptr) gv = load_pack<T, VEC>(g + c);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float dy = as_float(yv[i].v[e]);
+                    const float xh = (as_float(xv[i].v[e]) - mean) * rstd;
+                    const float t = g != nullptr ? dy * as_float(gv.v[e]) : dy;
+                    s1 += t;
+                    s2 = fmaf(t, xh, s2);
+                    dg[i * VEC + e] = fmaf(dy, xh, dg[i * VEC + e]);
+                    db[i * VEC + e] += dy;
+                }
+            }
+        }
+        const float2 s = group_sum2<W>(s1, s2, red, turn);
+        if (a.out == nullptr) continue;
+        const float m1 = s.x * inv_k, m2 = s.y * inv_k;
+        T* const dx = static_cast<T*>(a.out) + row * a.K;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * 32 * W + lane) * VEC;
+            if (c < a.K) {
+                Pack<T, VEC> gv, o;
+                if (g != nullptr) gv = load_pack<T, VEC>(g + c);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    const float dy = as_float(yv[i].v[e]);
+                    const float xh = (as_float(xv[i].v[e]) - mean) * rstd;
+                    const float t = g != nullptr ? dy * as_float(gv.v[e]) : dy;
+                    o.v[e] = round_to<T>(rstd * (t - m1 - xh * m2));
+                }
+                *reinterpret_cast<Pack<T, VEC>*>(dx + c) = o;
+            }
+        }
+    }
+    if (a.part == nullptr) return;
+    float* const part = a.part + static_cast<int64_t>(blockIdx.x) * 2 * a.K;
+    if constexpr (W == 1) {
+        // the block's warps add their columns in warp order
+        for (int w = 0; w < LN_ROWS; ++w) {
+            if (warp == w) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        const int c = (i * 32 + lane) * VEC + e;
+                        wsum[c] = (w == 0 ? 0.0f : wsum[c]) + dg[i * VEC + e];
+                        wsum[COLS + c] = (w == 0 ? 0.0f : wsum[COLS + c]) + db[i * VEC + e];
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        for (int c = threadIdx.x; c < a.K; c += 32 * LN_ROWS) {
+            part[c] = wsum[c];
+            part[a.K + c] = wsum[COLS + c];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const int c = (i * 32 * W + lane) * VEC + e;
+                if (c < a.K) {
+                    part[c] = dg[i * VEC + e];
+                    part[a.K + c] = db[i * VEC + e];
+                }
+            }
+        }
+    }
+}
+
+// ------------------------------------------------------------------ rows of any length
+constexpr int LN_WIDE_WARPS = 32;
+
+template <typename T>
+__global__ void __launch_bounds__(32 * LN_WIDE_WARPS) k_ln_fwd_wide(const NormArgs a) {
+    __shared__ float2 red[2 * LN_WIDE_WARPS];
+    int turn = 0;
+    const int64_t row = blockIdx.x;
+    const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
+    const float inv_k = 1.0f / static_cast<float>(a.K);
+    float s = 0.0f, ss = 0.0f;
+    for (int c = threadIdx.x; c < a.K; c += blockDim.x) s += as_float(x[c]);
+    const float mean = group_sum2<LN_WIDE_WARPS>(s, 0.0f, red, turn).x * inv_k;
+    for (int c = threadIdx.x; c < a.K; c += blockDim.x) {
+        const float d = as_float(x[c]) - mean;
+        ss = fmaf(d, d, ss);
+    }
+    const float rstd = rsqrtf(group_sum2<LN_WIDE_WARPS>(ss, 0.0f, red, turn).x * inv_k + a.eps);
+    if (threadIdx.x == 0 && a.mean != nullptr) {
+        a.mean[row] = mean;
+        a.rstd[row] = rstd;
+    }
+    T* const y = static_cast<T*>(a.out) + row * a.K;
+    for (int c = threadIdx.x; c < a.K; c += blockDim.x) {
+        float t = (as_float(x[c]) - mean) * rstd;
+        if (a.g != nullptr) t *= as_float(static_cast<const T*>(a.g)[c]);
+        if (a.b != nullptr) t += as_float(static_cast<const T*>(a.b)[c]);
+        y[c] = round_to<T>(t);
+    }
+}
+
+// The partial sums of a block stay in its row of `part` (a thread's own columns only).
+template <typename T>
+__global__ void __launch_bounds__(32 * LN_WIDE_WARPS) k_ln_bwd_wide(const NormArgs a) {
+    __shared__ float2 red[2 * LN_WIDE_WARPS];
+    int turn = 0;
+    const T* const g = static_cast<const T*>(a.g);
+    const float inv_k = 1.0f / static_cast<float>(a.K);
+    float* const part = a.part == nullptr ? nullptr : a.part + static_cast<int64_t>(blockIdx.x) * 2 * a.K;
+    if (part != nullptr)
+        for (int c = threadIdx.x; c < a.K; c += blockDim.x) part[c] = part[a.K + c] = 0.0f;
+    for (int64_t row = blockIdx.x; row < a.M; row += gridDim.x) {
+        const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
+        const T* const gy = static_cast<const T*>(a.gy) + row * a.ldg;
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        float s1 = 0.0f, s2 = 0.0f;
+        for (int c = threadIdx.x; c < a.K; c += blockDim.x) {
+            const float dy = as_float(gy[c]), xh = (as_float(x[c]) - mean) * rstd;
+            const float t = g != nullptr ? dy * as_float(g[c]) : dy;
+            s1 += t;
+            s2 = fmaf(t, xh, s2);
+            if (part != nullptr) {
+                part[c] = fmaf(dy, xh, part[c]);
+                part[a.K + c] += dy;
+            }
+        }
+        const float2 s = group_sum2<LN_WIDE_WARPS>(s1, s2, red, turn);
+        if (a.out == nullptr) continue;
+        const float m1 = s.x * inv_k, m2 = s.y * inv_k;
+        T* const dx = static_cast<T*>(a.out) + row * a.K;
+        for (int c = threadIdx.x; c < a.K; c += blockDim.x) {
+            const float dy = as_float(gy[c]), xh = (as_float(x[c]) - mean) * rstd;
+            const float t = g != nullptr ? dy * as_float(g[c]) : dy;
+            dx[c] = round_to<T>(rstd * (t - m1 - xh * m2));
+        }
+    }
+}
+
+}  // namespace ravel

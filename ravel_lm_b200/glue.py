@@ -13,8 +13,14 @@ Drop-ins for two functions ``ravel_lm/model.py`` imports from
 
 Both take CUDA tensors of float32 or bfloat16 (``rms_norm``: last dimension
 up to 4096) and raise on anything else; there is no CPU path.
+
+``layer_norm(x, weight, bias, eps)`` is LayerNorm over the last dimension, for
+blocks that centre their rows: float32, bfloat16 or float16, any length, each row
+read once and held in registers, weight gradients reduced without atomics.
 """
 from __future__ import annotations
+
+from typing import Optional
 
 import torch
 
@@ -98,4 +104,16 @@ def rms_norm(x: Tensor, g: Tensor, eps: float) -> Tensor:
     return _RMSNormFn.apply(x, g, float(eps))
 
 
-__all__ = ["gate_residual", "rms_norm"]
+def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor] = None, eps: float = 1e-5) -> Tensor:
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the last dimension (the biased variance).
+
+    Args:
+        x:            [..., K], float32, bfloat16 or float16; rows may be strided.
+        weight, bias: optional [K] of x's dtype (ones and zeros when absent).
+    Returns:
+        [..., K] of x's dtype; differentiable in x, weight and bias.
+    """
+    return _lib.host().layer_norm(x, weight, bias, float(eps))
+
+
+__all__ = ["gate_residual", "layer_norm", "rms_norm"]

@@ -290,6 +290,15 @@ def test_another_stream_and_graph_replay():
     assert torch.equal(out, fused_linear(x, w, b, activation="gelu", residual=r))
 
 
+def test_offsets_past_32_bits():
+    from ravel_lm_b200.dense import fused_linear
+    M, K, N = 40000, 64, 65536  # 2.6e9 outputs
+    x, w, b, _ = make(M, K, N, torch.bfloat16, seed=13, residual=False)
+    y = fused_linear(x, w, b, activation="silu")
+    for rows in (slice(0, 128), slice(M // 2, M // 2 + 128), slice(M - 128, M)):
+        check(x[rows], w, b, None, "silu", y[rows])
+
+
 def test_refusals():
     from ravel_lm_b200.dense import fused_linear
     x, w, b, r = make(4, 8, 16, torch.bfloat16, seed=12)
