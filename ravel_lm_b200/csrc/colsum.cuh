@@ -13,7 +13,7 @@ template <> __device__ __forceinline__ float round_to<float>(float v) { return v
 template <> __device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half round_to<__half>(float v) { return __float2half_rn(v); }
 
-constexpr int CR_COLS = 32, CR_ROWS = 16;
+constexpr int CR_COLS = 16, CR_ROWS = 32;
 
 // out[n] = sum_b part[b][n], n < N: CR_ROWS threads per column take every CR_ROWS-th block,
 // their sums are added in order.  Columns from `split` on go to out2 (two weights' partial

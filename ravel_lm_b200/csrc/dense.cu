@@ -17,6 +17,8 @@
 namespace ravel {
 namespace {
 
+template <int V> using IC = std::integral_constant<int, V>;
+
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 int vec16(const void* p, int64_t ld_bytes) { return aligned16(p) && ld_bytes % 16 == 0 ? 1 : 0; }
 
@@ -79,7 +81,7 @@ Plan plan_matmul(int64_t M, int64_t N, int64_t K) {
     if (c1 < cost) cost = c1, best = {SINGLE, 1};
     for (int s = 2; s <= 8; s *= 2) {
         if (kc < 2 * s) break;
-        const double c = std::ceil(t1 * s / sms) * 1.25 * std::ceil(kc / s) + 20.0;
+        const double c = std::ceil(t1 * s / sms) * (1.25 * std::ceil(kc / s) + 24.0);
         if (c < cost) cost = c, best = {SPLIT, s};
     }
     return best;
@@ -128,6 +130,34 @@ int launch_matmul(const Operand& A, const Operand& B, int64_t K, MatmulArgs a, c
     return check_launch();
 }
 
+constexpr int64_t kGemvRows = 4;
+
+// At most kGemvRows rows.  Warps per weight row: at least 16 warps an SM in all while every lane keeps
+// a few loads of its row.
+template <typename T>
+int launch_gemv(const Operand& X, const Operand& W, int64_t K, const MatmulArgs& e, cudaStream_t st) {
+    GemvArgs a;
+    a.x = X.p; a.w = W.p; a.ldx = X.ld; a.ldw = W.ld; a.K = K;
+    a.e = e;
+    int s = 1;
+    while (s < GV_WARPS && e.N * s < static_cast<int64_t>(sm_count()) * 16 && K >= 512 * s) s *= 2;
+    auto rows = [&](auto sc) -> int {
+        constexpr int S = decltype(sc)::value;
+        const unsigned grid = static_cast<unsigned>((e.N + GV_WARPS / S - 1) / (GV_WARPS / S));
+        switch (e.M) {
+            case 1: k_gemv<T, 1, S><<<grid, 32 * GV_WARPS, 0, st>>>(a); break;
+            case 2: k_gemv<T, 2, S><<<grid, 32 * GV_WARPS, 0, st>>>(a); break;
+            case 3: k_gemv<T, 3, S><<<grid, 32 * GV_WARPS, 0, st>>>(a); break;
+            default: k_gemv<T, 4, S><<<grid, 32 * GV_WARPS, 0, st>>>(a); break;
+        }
+        return check_launch();
+    };
+    if (s == 1) return rows(IC<1>{});
+    if (s == 2) return rows(IC<2>{});
+    if (s == 4) return rows(IC<4>{});
+    return rows(IC<8>{});
+}
+
 template <typename T, bool A_MN, bool B_MN, bool FULL>
 int matmul_shape(const Operand& A, const Operand& B, int64_t K, MatmulArgs& a, cudaStream_t st) {
     const Plan p = plan_matmul(a.M, a.N, K);
@@ -171,8 +201,6 @@ unsigned grid_for(int64_t blocks) {
 }
 
 // ------------------------------------------------------------------ LayerNorm
-template <int V> using IC = std::integral_constant<int, V>;
-
 template <typename F>
 int with_float_type(int dtype, F&& f) {
     if (dtype == RAVEL_F32) return f(float());
@@ -183,12 +211,16 @@ constexpr int64_t kNormMaxK = int64_t{1} << 30;
 
 int esize(int dtype) { return dtype == RAVEL_F32 ? 4 : 2; }
 
+#ifndef RAVEL_LN_BWD_MOST
+#define RAVEL_LN_BWD_MOST 1
+#endif
+
 // How a row of K elements is shared: W warps (1, 4, 16; 0: the wide kernels), NV vectors a lane.
 struct NormPlan {
     int vec, W, NV;
 };
 
-NormPlan plan_norm(int64_t M, int64_t K, int dtype, bool vec) {
+NormPlan plan_norm(int64_t M, int64_t K, int dtype, bool vec, bool backward) {
     const int64_t units = vec ? K / (16 / esize(dtype)) : K;
     const int most = vec ? 4 : 16;  // vectors, or single elements, of a row in a lane's registers
     // Rows for every SM: as few warps per row as hold it (shuffles alone add up a warp's row).
@@ -197,6 +229,8 @@ NormPlan plan_norm(int64_t M, int64_t K, int dtype, bool vec) {
     for (int w : {1, 4, 16}) {
         const int64_t per = (units + 32 * w - 1) / (32 * w);
         if (per > most || (few && w < 16 && per > most / 4)) continue;
+        // the backward also accumulates two weight gradients per column
+        if (backward && w < 16 && per > RAVEL_LN_BWD_MOST * most / 4) continue;
         int nv = most / 4;
         while (nv < per) nv *= 2;
         return {vec ? 1 : 0, w, nv};
@@ -313,6 +347,7 @@ int ravel_matmul(const void* A, int64_t lda, int a_mn, const void* B, int64_t ld
         const Operand oa{A, lda, a_mn}, ob{B, ldb, b_mn};
         if (a_mn) return matmul_shape<T, true, true, false>(oa, ob, K, a, st);
         if (b_mn) return matmul_shape<T, false, true, false>(oa, ob, K, a, st);
+        if (M <= kGemvRows) return launch_gemv<T>(oa, ob, K, a, st);
         return matmul_shape<T, false, false, true>(oa, ob, K, a, st);
     });
 }
@@ -388,7 +423,7 @@ int ravel_layer_norm_fwd(const void* x, int64_t ldx, const void* weight, const v
     const bool vec = (K * es) % 16 == 0 && vec16(x, M > 1 ? ldx * es : 0) && aligned16(y) && aligned16(weight) &&
                      aligned16(bias);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const NormPlan p = plan_norm(M, K, dtype, vec);
+    const NormPlan p = plan_norm(M, K, dtype, vec, false);
     return with_float_type(dtype, [&](auto tv) -> int {
         using T = decltype(tv);
         if (p.W == 0) {
@@ -434,7 +469,7 @@ int ravel_layer_norm_bwd(const void* x, int64_t ldx, const void* weight, const v
     const bool vec = (K * es) % 16 == 0 && vec16(x, M > 1 ? ldx * es : 0) && vec16(grad_y, M > 1 ? ldg * es : 0) &&
                      aligned16(grad_x) && aligned16(weight);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const NormPlan p = plan_norm(M, K, dtype, vec);
+    const NormPlan p = plan_norm(M, K, dtype, vec, true);
     const int64_t blocks = p.W == 0 ? std::max<int64_t>(1, std::min<int64_t>(M, int64_t{sm_count()} * 2))
                                     : norm_bwd_blocks(M, p);
     return with_float_type(dtype, [&](auto tv) -> int {

@@ -22,6 +22,8 @@
 //                     workspace), each CTA finishing an equal share of the columns.  For few
 //                     rows (decoding), where the weights' bytes bound the call and one CTA per
 //                     column tile would leave most SMs idle.
+//   k_gemv          the forward of at most 4 rows: a warp (or 2, 4, 8 warps) per weight row, plain
+//                   16-byte loads, one multiply-add per weight and row.
 //   k_linear_dz     dz = dy * act'(z) in 16 bits (the operand of the two gradient products) and
 //                   per-block column sums of dz in float32 (the bias gradient) in one pass.
 //   k_col_reduce    those partial sums added in block order: deterministic, no atomics.
@@ -100,22 +102,59 @@ __device__ __forceinline__ void store8(T* row, int64_t c, int64_t n, bool vec, c
 }
 
 // ------------------------------------------------------------------ activations
-// gelu is z Phi(z) with the error function; silu is z sigma(z).  Every one keeps a NaN.
+// gelu is z Phi(z), silu is z sigma(z).  Every one keeps a NaN.
+//
+// The normal tail 1 - Phi(x) = erfc(x / sqrt 2) / 2 of x = |z| comes from exp(-x^2 / 2) and, with
+// t = 1 / (1 + 0.44 y), y = x / sqrt 2, a polynomial: erfc(y) exp(y^2) is one of degree 6 in t without
+// constant term to 5.2e-6 of its value for 0 <= y <= 9 (a weighted least-squares fit driven to equal
+// ripples); beyond that the exponential is zero in float32.  With the float32 exponential the tail is good to
+// 1.6e-5 of itself, 1 / 30 of float16's roundoff.  One reciprocal and one exponential serve Phi and the
+// density; erff and expf made the epilogue and k_linear_dz issue-bound (the latter 345 us at 16384 x 8192
+// against 123 us for its bytes).
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float ex2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Phi(z); e receives exp(-z^2 / 2).
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+    const float t = rcp_approx(fmaf(fabsf(z), 0.44f * 0.70710678118654752f, 1.0f));
+    e = ex2_approx(z * z * (-0.5f * 1.4426950408889634f));
+    float p = -0.073042055f;
+    p = fmaf(p, t, 0.17529081f);
+    p = fmaf(p, t, 0.020410425f);
+    p = fmaf(p, t, 0.13176596f);
+    p = fmaf(p, t, 0.12129263f);
+    p = fmaf(p, t, 0.12427965f);
+    const float h = p * t * e;
+    return z < 0.0f ? h : 1.0f - h;
+}
 template <int ACT>
 __device__ __forceinline__ float act_fwd(float z) {
     if constexpr (ACT == RAVEL_ACT_RELU) return z < 0.0f ? 0.0f : z;
-    if constexpr (ACT == RAVEL_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-    if constexpr (ACT == RAVEL_ACT_SILU) return __fdividef(z, 1.0f + __expf(-z));
+    if constexpr (ACT == RAVEL_ACT_GELU) {
+        float e;
+        return z * normal_cdf(z, e);
+    }
+    if constexpr (ACT == RAVEL_ACT_SILU) return z * rcp_approx(1.0f + ex2_approx(-1.4426950408889634f * z));
     return z;
 }
 template <int ACT>
 __device__ __forceinline__ float act_grad(float z) {
     if constexpr (ACT == RAVEL_ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
-    if constexpr (ACT == RAVEL_ACT_GELU)
-        return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * __expf(-0.5f * z * z);
+    if constexpr (ACT == RAVEL_ACT_GELU) {
+        float e;
+        const float c = normal_cdf(z, e);
+        return fmaf(z * 0.39894228040143268f, e, c);
+    }
     if constexpr (ACT == RAVEL_ACT_SILU) {
-        const float s = __fdividef(1.0f, 1.0f + __expf(-z));
-        return s * (1.0f + z * (1.0f - s));
+        const float s = rcp_approx(1.0f + ex2_approx(-1.4426950408889634f * z));
+        return s * fmaf(z, 1.0f - s, 1.0f);
     }
     return 1.0f;
 }
@@ -203,22 +242,40 @@ __device__ __forceinline__ uint32_t epi_piece(int row, int piece) {
 template <typename T>
 __device__ __forceinline__ void epi_load(unsigned char* st, const T* g, int64_t ld, int64_t m0, int64_t M, int64_t c0,
                                          int64_t N, bool vec, int lane) {
+    if (vec) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = i * 8 + (lane >> 2), piece = lane & 3;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (m0 + row < M) v = load8(g + (m0 + row) * ld, c0 + piece * 8, N, vec);
-        *reinterpret_cast<uint4*>(st + epi_piece(row, piece)) = v;
+        for (int i = 0; i < 4; ++i) {
+            const int row = i * 8 + (lane >> 2), piece = lane & 3;
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (m0 + row < M) v = load8(g + (m0 + row) * ld, c0 + piece * 8, N, true);
+            *reinterpret_cast<uint4*>(st + epi_piece(row, piece)) = v;
+        }
+    } else {  // an element per lane, a row at a time: adjacent addresses whatever the rows' alignment
+        const bool col = c0 + lane < N;
+        const int rows = (M - m0) < 32 ? static_cast<int>(M - m0) : 32;
+        const T* p = g + m0 * ld + c0 + lane;
+#pragma unroll 8
+        for (int row = 0; row < rows; ++row, p += ld)
+            if (col) *reinterpret_cast<T*>(st + epi_piece(row, lane >> 3) + (lane & 7) * 2) = *p;
     }
 }
 template <typename T>
 __device__ __forceinline__ void epi_store(const unsigned char* st, T* g, int64_t ld, int64_t m0, int64_t M, int64_t c0,
                                           int64_t N, bool vec, int lane) {
+    if (vec) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = i * 8 + (lane >> 2), piece = lane & 3;
-        const uint4 v = *reinterpret_cast<const uint4*>(st + epi_piece(row, piece));
-        if (m0 + row < M) store8(g + (m0 + row) * ld, c0 + piece * 8, N, vec, v);
+        for (int i = 0; i < 4; ++i) {
+            const int row = i * 8 + (lane >> 2), piece = lane & 3;
+            const uint4 v = *reinterpret_cast<const uint4*>(st + epi_piece(row, piece));
+            if (m0 + row < M) store8(g + (m0 + row) * ld, c0 + piece * 8, N, true, v);
+        }
+    } else {
+        const bool col = c0 + lane < N;
+        const int rows = (M - m0) < 32 ? static_cast<int>(M - m0) : 32;
+        T* p = g + m0 * ld + c0 + lane;
+#pragma unroll 8
+        for (int row = 0; row < rows; ++row, p += ld)
+            if (col) *p = *reinterpret_cast<const T*>(st + epi_piece(row, lane >> 3) + (lane & 7) * 2);
     }
 }
 
@@ -461,6 +518,90 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
     tc_fence_after();
     if (*abort && threadIdx.x == 0) atomicOr(a.err, RAVEL_DEVERR_SPIN);
     if (warp == 2) tmem_free<CG>(tmem, COLS);
+}
+
+// ------------------------------------------------------------------ few rows
+constexpr int GV_WARPS = 8;
+constexpr int GV_DEPTH = 8;  // 16-byte weight loads in flight per lane
+
+struct GemvArgs {
+    const void* x;       // [M, K], rows ldx apart
+    const void* w;       // [N, K], rows ldw apart; both 16-byte rows
+    int64_t ldx, ldw, K;
+    MatmulArgs e;        // the epilogue
+};
+
+// MR rows of x against the weights' rows: S warps share a weight row's K, each lane taking
+// 16 bytes of it at a time, MR products per weight; the warp's (then the block's, in warp order)
+// partial sums are added and one lane finishes the element.
+template <typename T, int MR, int S>
+__global__ void __launch_bounds__(32 * GV_WARPS) k_gemv(const GemvArgs a) {
+    __shared__ float part[GV_WARPS][MR];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t n = static_cast<int64_t>(blockIdx.x) * (GV_WARPS / S) + warp / S;
+    float acc[MR];
+#pragma unroll
+    for (int m = 0; m < MR; ++m) acc[m] = 0.0f;
+    if (n < a.e.N) {
+        const T* const w = static_cast<const T*>(a.w) + n * a.ldw;
+        const T* const x = static_cast<const T*>(a.x);
+        const int64_t first = ((warp % S) * 32 + lane) * 8, step = S * 32 * 8;
+        auto add = [&](const uint4& wv, int64_t k) {
+            float wf[8];
+            unpack8<T>(wv, wf);
+#pragma unroll
+            for (int m = 0; m < MR; ++m) {
+                float xf[8];
+                unpack8<T>(load8(x + m * a.ldx, k, a.K, true), xf);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[m] = fmaf(wf[e], xf[e], acc[m]);
+            }
+        };
+        int64_t k = first;
+        for (; k + (GV_DEPTH - 1) * step + 8 <= a.K; k += GV_DEPTH * step) {
+            uint4 wv[GV_DEPTH];
+#pragma unroll
+            for (int i = 0; i < GV_DEPTH; ++i) wv[i] = __ldg(reinterpret_cast<const uint4*>(w + k + i * step));
+#pragma unroll
+            for (int i = 0; i < GV_DEPTH; ++i) add(wv[i], k + i * step);
+        }
+        for (; k < a.K; k += step) add(load8(w, k, a.K, true), k);
+    }
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) acc[m] += __shfl_xor_sync(0xffffffffu, acc[m], o);
+    }
+    if constexpr (S > 1) {
+        if (lane == 0) {
+#pragma unroll
+            for (int m = 0; m < MR; ++m) part[warp][m] = acc[m];
+        }
+        __syncthreads();
+        if (warp % S != 0) return;
+#pragma unroll
+        for (int m = 0; m < MR; ++m) {
+            acc[m] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < S; ++i) acc[m] += part[warp + i][m];
+        }
+    }
+    if (n >= a.e.N) return;
+#pragma unroll
+    for (int m = 0; m < MR; ++m) {
+        if (lane != m) continue;
+        float v = acc[m];
+        if (a.e.bias != nullptr) v += static_cast<float>(static_cast<const T*>(a.e.bias)[n]);
+        if (a.e.z != nullptr) static_cast<T*>(a.e.z)[m * a.e.ldz + n] = static_cast<T>(v);
+        switch (a.e.act) {
+            case RAVEL_ACT_RELU: v = act_fwd<RAVEL_ACT_RELU>(v); break;
+            case RAVEL_ACT_GELU: v = act_fwd<RAVEL_ACT_GELU>(v); break;
+            case RAVEL_ACT_SILU: v = act_fwd<RAVEL_ACT_SILU>(v); break;
+            default: break;
+        }
+        if (a.e.res != nullptr) v += static_cast<float>(static_cast<const T*>(a.e.res)[m * a.e.ldr + n]);
+        static_cast<T*>(a.e.y)[m * a.e.ldy + n] = static_cast<T>(v);
+    }
 }
 
 // ------------------------------------------------------------------ the backward's elementwise pass
