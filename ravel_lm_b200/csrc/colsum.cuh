@@ -2,16 +2,11 @@
 // (float32) added in block order, so that the result depends on nothing but the inputs.
 #pragma once
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <stdint.h>
 
-namespace ravel {
+#include "pack.cuh"
 
-template <typename T> __device__ __forceinline__ T round_to(float v);
-template <> __device__ __forceinline__ float round_to<float>(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 round_to<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half round_to<__half>(float v) { return __float2half_rn(v); }
+namespace ravel {
 
 constexpr int CR_COLS = 16, CR_ROWS = 32;
 

@@ -200,11 +200,11 @@ __device__ __forceinline__ void distill_grad_row(const DistillArgs& a, int64_t r
     if (same) {
 #pragma unroll 4
         for (int i = threadIdx.x; i < rs.vecs; i += TH) {
-            const Pack<T, E> v = load_pack<T, E>(s + rs.head + i * E);
-            Pack<T, E> o;
+            float f[E];
+            to_floats<T, E>(load_pack<T, E>(s + rs.head + i * E), f);
 #pragma unroll
-            for (int e = 0; e < E; ++e) o.v[e] = one(v.v[e]);
-            *reinterpret_cast<Pack<T, E>*>(d + rs.head + i * E) = o;
+            for (int e = 0; e < E; ++e) f[e] = gl * ex2(fmaf(f[e], c, -st.m));
+            store_pack<T, E>(d + rs.head + i * E, from_floats<T, E>(f));
         }
         for (int i = threadIdx.x; i < rs.head; i += TH) d[i] = one(s[i]);
         for (int i = rs.head + rs.vecs * E + threadIdx.x; i < a.V; i += TH) d[i] = one(s[i]);
@@ -249,13 +249,11 @@ __global__ void __launch_bounds__(TH) k_distill(const DistillArgs a) {
     };
 #pragma unroll 4
     for (int i = threadIdx.x; i < rs.vecs; i += TH) {
-        const Pack<T, E> p = load_pack<T, E>(s + rs.head + i * E);
         float x[E], m = -INFINITY;
+        to_floats<T, E>(load_pack<T, E>(s + rs.head + i * E), x);
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            x[e] = as_float(p.v[e]);
-            m = fmaxf(m, x[e] * c);
-        }
+        for (int e = 0; e < E; ++e) m = fmaxf(m, x[e]);
+        m *= c;
         if (m > v.m) {
             v.l *= ex2(v.m - m);
             v.m = m;

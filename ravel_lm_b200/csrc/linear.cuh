@@ -33,33 +33,15 @@
 // its copies in flight, frees its TMEM and returns.
 #pragma once
 
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include <type_traits>
 
 #include "host.cuh"
+#include "pack.cuh"
 #include "ptx.cuh"
 
 namespace ravel {
 
 // ------------------------------------------------------------------ 16-bit element types
-template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t w);
-template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
-    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
-}
-template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
-    return __half22float2(*reinterpret_cast<const __half2*>(&w));
-}
-template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
-template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-    const __half2 v = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
 template <typename T>
 __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -606,7 +588,8 @@ __global__ void __launch_bounds__(32 * GV_WARPS) k_gemv(const GemvArgs a) {
 
 // ------------------------------------------------------------------ the backward's elementwise pass
 constexpr int DZ_COLS = 256;   // columns per block: 32 lanes x 8
-constexpr int DZ_WARPS = 8;    // rows in flight per block
+constexpr int DZ_WARPS = 8;    // rows per block at a time
+constexpr int DZ_ROWS = 4;     // rows per warp whose loads are in flight together
 
 struct DzArgs {
     int64_t M, N, ldg, ldz, ldd;
@@ -620,7 +603,7 @@ struct DzArgs {
 
 // Bound by HBM: reads dy and z, writes dz, 6 bytes an element.
 template <typename T, int ACT>
-__global__ void __launch_bounds__(32 * DZ_WARPS) k_linear_dz(const DzArgs a) {
+__global__ void __launch_bounds__(32 * DZ_WARPS, 3) k_linear_dz(const DzArgs a) {
     __shared__ float sums[DZ_WARPS][DZ_COLS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t c = static_cast<int64_t>(blockIdx.x) * DZ_COLS + lane * 8;
@@ -628,19 +611,36 @@ __global__ void __launch_bounds__(32 * DZ_WARPS) k_linear_dz(const DzArgs a) {
     const int64_t r1 = (r0 + a.rows) < a.M ? (r0 + a.rows) : a.M;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     if (c < a.N) {
-#pragma unroll 4
-        for (int64_t r = r0 + warp; r < r1; r += DZ_WARPS) {
-            float g[8];
-            unpack8<T>(load8(static_cast<const T*>(a.gy) + r * a.ldg, c, a.N, a.vec_g), g);
-            if constexpr (ACT != RAVEL_ACT_NONE) {
-                float z[8];
-                unpack8<T>(load8(static_cast<const T*>(a.z) + r * a.ldz, c, a.N, a.vec_z), z);
+        const T* const gy = static_cast<const T*>(a.gy);
+        const T* const zz = static_cast<const T*>(a.z);
+        T* const dz = static_cast<T*>(a.dz);
+        for (int64_t r = r0 + warp; r < r1; r += DZ_WARPS * DZ_ROWS) {
+            uint4 gv[DZ_ROWS], zv[DZ_ROWS];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) g[e] *= act_grad<ACT>(z[e]);
+            for (int i = 0; i < DZ_ROWS; ++i) {
+                const int64_t row = r + i * DZ_WARPS;
+                if (row < r1) {
+                    gv[i] = load8(gy + row * a.ldg, c, a.N, a.vec_g);
+                    if constexpr (ACT != RAVEL_ACT_NONE) zv[i] = load8(zz + row * a.ldz, c, a.N, a.vec_z);
+                }
             }
-            if (a.dz != nullptr) store8(static_cast<T*>(a.dz) + r * a.ldd, c, a.N, a.vec_d, pack8<T>(g));
 #pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] += g[e];
+            for (int i = 0; i < DZ_ROWS; ++i) {
+                const int64_t row = r + i * DZ_WARPS;
+                if (row < r1) {
+                    float g[8];
+                    unpack8<T>(gv[i], g);
+                    if constexpr (ACT != RAVEL_ACT_NONE) {
+                        float z[8];
+                        unpack8<T>(zv[i], z);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) g[e] *= act_grad<ACT>(z[e]);
+                    }
+                    if (dz != nullptr) store8(dz + row * a.ldd, c, a.N, a.vec_d, pack8<T>(g));
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) acc[e] += g[e];
+                }
+            }
         }
     }
     if (a.part == nullptr) return;

@@ -15,28 +15,9 @@
 
 #include "colsum.cuh"
 #include "host.cuh"
+#include "pack.cuh"
 
 namespace ravel {
-
-template <typename T> __device__ __forceinline__ float as_float(T v);
-template <> __device__ __forceinline__ float as_float<float>(float v) { return v; }
-template <> __device__ __forceinline__ float as_float<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <> __device__ __forceinline__ float as_float<__half>(__half v) { return __half2float(v); }
-
-// VEC elements as loaded: one 16-byte load, or a single element.
-template <typename T, int VEC>
-struct alignas(sizeof(T) * VEC) Pack {
-    T v[VEC];
-};
-template <typename T, int VEC>
-__device__ __forceinline__ Pack<T, VEC> load_pack(const T* p) {
-    Pack<T, VEC> r;
-    if constexpr (sizeof(T) * VEC == 16)
-        *reinterpret_cast<uint4*>(&r) = __ldg(reinterpret_cast<const uint4*>(p));
-    else
-        r = *reinterpret_cast<const Pack<T, VEC>*>(p);
-    return r;
-}
 
 struct NormArgs {
     const void* x;       // [M, K], rows ldx apart
@@ -76,6 +57,22 @@ __device__ __forceinline__ float2 group_sum2(float a, float b, float2* red, int&
     return make_float2(a, b);
 }
 
+template <int W>
+__device__ __forceinline__ float group_sum(float a, float* red, int& turn) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+    if constexpr (W > 1) {
+        float* const r = red + turn * W;
+        turn ^= 1;
+        if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = a;
+        __syncthreads();
+        a = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; ++w) a += r[w];
+    }
+    return a;
+}
+
 // rows (one per warp) of a block when a row takes one warp
 constexpr int LN_ROWS = 8;
 template <int W> constexpr int ln_threads() { return W == 1 ? 32 * LN_ROWS : 32 * W; }
@@ -88,34 +85,38 @@ __global__ void __launch_bounds__(ln_threads<W>()) k_ln_fwd(const NormArgs a) {
     const int64_t row = W == 1 ? static_cast<int64_t>(blockIdx.x) * LN_ROWS + (threadIdx.x >> 5) : blockIdx.x;
     if (row >= a.M) return;  // whole warps; with W > 1 every row exists
     const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
-    Pack<T, VEC> v[NV];
+    float v[NV * VEC];
     float s = 0.0f;
+    {
+        Pack<T, VEC> p[NV];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int c = (i * 32 * W + lane) * VEC;
-        if (c < a.K) v[i] = load_pack<T, VEC>(x + c);
-    }
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * 32 * W + lane) * VEC;
+            if (c < a.K) p[i] = load_pack<T, VEC>(x + c);
+        }
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        if ((i * 32 * W + lane) * VEC < a.K) {
+        for (int i = 0; i < NV; ++i) {
+            if ((i * 32 * W + lane) * VEC < a.K) {
+                to_floats<T, VEC>(p[i], v + i * VEC);
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) s += as_float(v[i].v[e]);
+                for (int e = 0; e < VEC; ++e) s += v[i * VEC + e];
+            }
         }
     }
     const float inv_k = 1.0f / static_cast<float>(a.K);
-    const float mean = group_sum2<W>(s, 0.0f, red, turn).x * inv_k;
+    const float mean = group_sum<W>(s, reinterpret_cast<float*>(red), turn) * inv_k;
     float ss = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         if ((i * 32 * W + lane) * VEC < a.K) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
-                const float d = as_float(v[i].v[e]) - mean;
-                ss = fmaf(d, d, ss);
+                v[i * VEC + e] -= mean;
+                ss = fmaf(v[i * VEC + e], v[i * VEC + e], ss);
             }
         }
     }
-    const float rstd = rsqrtf(group_sum2<W>(ss, 0.0f, red, turn).x * inv_k + a.eps);
+    const float rstd = rsqrtf(group_sum<W>(ss, reinterpret_cast<float*>(red), turn) * inv_k + a.eps);
     if (lane == 0 && a.mean != nullptr) {
         a.mean[row] = mean;
         a.rstd[row] = rstd;
@@ -127,17 +128,20 @@ __global__ void __launch_bounds__(ln_threads<W>()) k_ln_fwd(const NormArgs a) {
     for (int i = 0; i < NV; ++i) {
         const int c = (i * 32 * W + lane) * VEC;
         if (c < a.K) {
-            Pack<T, VEC> gv, bv, o;
-            if (g != nullptr) gv = load_pack<T, VEC>(g + c);
-            if (b != nullptr) bv = load_pack<T, VEC>(b + c);
+            float t[VEC], w[VEC];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                float t = (as_float(v[i].v[e]) - mean) * rstd;
-                if (g != nullptr) t *= as_float(gv.v[e]);
-                if (b != nullptr) t += as_float(bv.v[e]);
-                o.v[e] = round_to<T>(t);
+            for (int e = 0; e < VEC; ++e) t[e] = v[i * VEC + e] * rstd;
+            if (g != nullptr) {
+                to_floats<T, VEC>(load_pack<T, VEC>(g + c), w);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) t[e] *= w[e];
             }
-            *reinterpret_cast<Pack<T, VEC>*>(y + c) = o;
+            if (b != nullptr) {
+                to_floats<T, VEC>(load_pack<T, VEC>(b + c), w);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) t[e] += w[e];
+            }
+            store_pack<T, VEC>(y + c, from_floats<T, VEC>(t));
         }
     }
 }
@@ -170,43 +174,42 @@ __global__ void __launch_bounds__(ln_threads<W>()) k_ln_bwd(const NormArgs a) {
                 yv[i] = load_pack<T, VEC>(gy + c);
             }
         }
+        float xh[NV * VEC], t[NV * VEC];  // (x - mean) rstd, dy g
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * 32 * W + lane) * VEC;
             if (c < a.K) {
-                Pack<T, VEC> gv;
-                if (g != nullptr) gv = load_pack<T, VEC>(g + c);
+                to_floats<T, VEC>(xv[i], xh + i * VEC);
+                to_floats<T, VEC>(yv[i], t + i * VEC);
+                float w[VEC];
+                if (g != nullptr) to_floats<T, VEC>(load_pack<T, VEC>(g + c), w);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
-                    const float dy = as_float(yv[i].v[e]);
-                    const float xh = (as_float(xv[i].v[e]) - mean) * rstd;
-                    const float t = g != nullptr ? dy * as_float(gv.v[e]) : dy;
-                    s1 += t;
-                    s2 = fmaf(t, xh, s2);
-                    dg[i * VEC + e] = fmaf(dy, xh, dg[i * VEC + e]);
-                    db[i * VEC + e] += dy;
+                    const int k = i * VEC + e;
+                    xh[k] = (xh[k] - mean) * rstd;
+                    dg[k] = fmaf(t[k], xh[k], dg[k]);
+                    db[k] += t[k];
+                    if (g != nullptr) t[k] *= w[e];
+                    s1 += t[k];
+                    s2 = fmaf(t[k], xh[k], s2);
                 }
             }
         }
         const float2 s = group_sum2<W>(s1, s2, red, turn);
         if (a.out == nullptr) continue;
-        const float m1 = s.x * inv_k, m2 = s.y * inv_k;
+        const float m1 = s.x * inv_k * rstd, m2 = s.y * inv_k * rstd;
         T* const dx = static_cast<T*>(a.out) + row * a.K;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * 32 * W + lane) * VEC;
             if (c < a.K) {
-                Pack<T, VEC> gv, o;
-                if (g != nullptr) gv = load_pack<T, VEC>(g + c);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
-                    const float dy = as_float(yv[i].v[e]);
-                    const float xh = (as_float(xv[i].v[e]) - mean) * rstd;
-                    const float t = g != nullptr ? dy * as_float(gv.v[e]) : dy;
-                    o.v[e] = round_to<T>(rstd * (t - m1 - xh * m2));
+                    const int k = i * VEC + e;
+                    t[k] = fmaf(t[k], rstd, -m1) - xh[k] * m2;
                 }
-                *reinterpret_cast<Pack<T, VEC>*>(dx + c) = o;
+                store_pack<T, VEC>(dx + c, from_floats<T, VEC>(t + i * VEC));
             }
         }
     }
