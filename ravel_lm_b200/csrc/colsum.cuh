@@ -5,6 +5,7 @@
 #include <stdint.h>
 
 #include "pack.cuh"
+#include "ptx.cuh"
 
 namespace ravel {
 
@@ -18,6 +19,8 @@ __global__ void __launch_bounds__(CR_COLS* CR_ROWS) k_col_reduce(const float* __
                                                                  int64_t split, T* __restrict__ out,
                                                                  T* __restrict__ out2) {
     __shared__ float sums[CR_ROWS][CR_COLS + 1];
+    grid_wait();
+    grid_trigger();
     const int x = threadIdx.x % CR_COLS, y = threadIdx.x / CR_COLS;
     const int64_t n = static_cast<int64_t>(blockIdx.x) * CR_COLS + x;
     float s = 0.0f;

@@ -22,8 +22,8 @@ template <int V> using IC = std::integral_constant<int, V>;
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 int vec16(const void* p, int64_t ld_bytes) { return aligned16(p) && ld_bytes % 16 == 0 ? 1 : 0; }
 
-// Clusters of `size` CTAs of a kernel that fit the device at once (queried once per kernel).
-int resident_clusters(const void* kernel, int size, size_t smem) {
+// Clusters of `size` matrix-product CTAs that fit the device at once (queried once per kernel).
+int resident_clusters(const void* kernel, int size) {
     static std::mutex mu;
     static std::map<std::pair<const void*, int>, int> known;
     int dev = 0;
@@ -32,15 +32,14 @@ int resident_clusters(const void* kernel, int size, size_t smem) {
     const auto key = std::make_pair(kernel, dev);
     const auto it = known.find(key);
     if (it != known.end()) return it->second;
-    cudaLaunchConfig_t cfg;
-    std::memset(&cfg, 0, sizeof(cfg));
-    cudaLaunchAttribute at;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at = {};
     at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = size;
+    at.val.clusterDim.x = static_cast<unsigned>(size);
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.gridDim = dim3(static_cast<unsigned>(sm_count() / size * size));
     cfg.blockDim = dim3(MM_THREADS);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = MM_SMEM;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
     int n = 0;
@@ -56,78 +55,76 @@ struct Operand {
     int mn;  // stored [k][rows]
 };
 
-enum Shape { PAIRS, SINGLE, SPLIT };
 struct Plan {
-    Shape shape;
-    int splits;
+    int cg, bn, splits;
 };
 
-// The launch shape: an estimate of each shape's time in units of a 128 x 128 x 64 product at
-// the tensor peak.  Per wave of tiles a pair spends 2 units a chunk on each of its SMs; a single
-// CTA 1.25 (its operands come from shared memory at twice the bytes per product); the constants
-// are the fill of the pipeline and the last epilogue.
-Plan plan_matmul(int64_t M, int64_t N, int64_t K) {
-#ifdef RAVEL_MM_FORCE_SHAPE  // build-time tuning knob (sweeps): 0 pairs, 1 single, 2/4/8 split
-    if (RAVEL_MM_FORCE_SHAPE == 0) return {PAIRS, 1};
-    if (RAVEL_MM_FORCE_SHAPE == 1) return {SINGLE, 1};
-    return {SPLIT, RAVEL_MM_FORCE_SHAPE};
+// The launch shape, by an estimate of each one's time in microseconds: a launch's fixed part plus, per wave
+// of tiles, the larger of a tile's chunks and its epilogue (which runs under the next tile's chunks).  Clusters that
+// split k pay their setup and the exchange of sums per tile; clusters of 4 and 8 fill the SMs less well (35 and 16
+// of them are resident).  Measured (graph replays, outputs 128 x 4096, k = 64 / 1024 / 4096 / 8192, us):
+//   single 32: 3.5 / 5.3 / 11.6 / 21.3    single 64: 3.5 / 5.5 / 12.2 / 21.2    single 128: 4.4 / 6.8 / 14.6 / 31.6
+//   pairs 128: 4.4 / 6.7 / 13.7 / 23.8    pairs 256: 6.0 / 10.3 / 23.6 / 41.8
+//   split 2: - / 8.4 / 12.5 / 19.7        split 4: - / 10.7 / 13.5 / 17.4
+Plan plan_matmul(int64_t M, int64_t N, int64_t K, bool b_mn) {
+#ifdef RAVEL_MM_FORCE_SHAPE  // build-time tuning knob (sweeps): cg * 10000 + bn * 10 + splits
+    return {RAVEL_MM_FORCE_SHAPE / 10000, RAVEL_MM_FORCE_SHAPE / 10 % 1000, RAVEL_MM_FORCE_SHAPE % 10};
 #endif
     const double sms = sm_count(), kc = static_cast<double>((K + MM_BK - 1) / MM_BK);
-    const double t2 = static_cast<double>((M + 255) / 256) * static_cast<double>((N + 255) / 256);
-    const double t1 = static_cast<double>((M + 127) / 128) * static_cast<double>((N + 127) / 128);
-    Plan best = {PAIRS, 1};
-    double cost = std::ceil(t2 / std::floor(sms / 2)) * 2.0 * kc + 26.0;
-    const double c1 = std::ceil(t1 / sms) * 1.25 * kc + 16.0;
-    if (c1 < cost) cost = c1, best = {SINGLE, 1};
+    auto waves = [&](int bm, int bn, double slots) {
+        return std::ceil(static_cast<double>((M + bm - 1) / bm) * static_cast<double>((N + bn - 1) / bn) / slots);
+    };
+    struct Kind {
+        int cg, bn;
+        double fixed, chunk, epilogue;
+    };
+    const Kind kinds[] = {{2, 256, 5.5, 0.280, 2.2}, {2, 128, 4.4, 0.145, 1.2}, {1, 128, 4.2, 0.160, 1.2},
+                          {1, 64, 3.4, 0.135, 1.0},  {1, 32, 3.4, 0.125, 0.9}};
+    Plan best = {1, 128, 1};
+    double cost = 1e30;
+    for (const Kind& k : kinds) {
+        if (b_mn && k.bn / k.cg < 64) continue;
+        const double us = k.fixed + waves(128 * k.cg, k.bn, std::floor(sms / k.cg)) * std::max(kc * k.chunk, k.epilogue);
+        if (us < cost) cost = us, best = {k.cg, k.bn, 1};
+    }
     for (int s = 2; s <= 8; s *= 2) {
-        if (kc < 2 * s) break;
-        const double c = std::ceil(t1 * s / sms) * (1.25 * std::ceil(kc / s) + 24.0);
-        if (c < cost) cost = c, best = {SPLIT, s};
+        if (kc < 4 * s) break;
+        const double slots = s == 2 ? std::floor(sms / 2) : (s == 4 ? std::floor(sms * 35 / 148) : std::floor(sms * 16 / 148));
+        const double us = 1.2 + waves(128, 128, slots) * (std::ceil(kc / s) * 0.160 + 5.0 + 0.5 * s);
+        if (us < cost) cost = us, best = {1, 128, s};
     }
     return best;
 }
 
-template <typename T, int CG, bool A_MN, bool B_MN, bool FULL, bool SPLIT>
+template <typename T, int CG, int BN, bool A_MN, bool B_MN, bool FULL, int ACT, bool SPLIT>
 int launch_matmul(const Operand& A, const Operand& B, int64_t K, MatmulArgs a, cudaStream_t st) {
-    const auto kern = k_matmul<T, CG, A_MN, B_MN, FULL, SPLIT>;
+    const auto kern = k_matmul<T, CG, BN, A_MN, B_MN, FULL, ACT, SPLIT>;
     constexpr CUtensorMapDataType TY =
         std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    constexpr int B_ROWS = BN / CG;
     a.mtiles = static_cast<int>((a.M + 128 * CG - 1) / (128 * CG));
-    a.ntiles = static_cast<int>((a.N + 128 * CG - 1) / (128 * CG));
-    // few rows: load (and wait for) no more of A's tile than exists; the accumulator rows past it
-    // hold products of stale shared memory and are never read
+    a.ntiles = static_cast<int>((a.N + BN - 1) / BN);
+    // few rows: load (and wait for) no more of A's tile than exists, in more and smaller stages; the
+    // accumulator rows past it hold products of whatever lies there and are never read
     a.a_rows = A_MN || a.M >= 128 ? 128 : static_cast<int>((a.M + 7) / 8 * 8);
+    a.a_bytes = static_cast<uint32_t>(a.a_rows) * 128u;
+    a.stage_bytes = mm_ksub(CG) * (a.a_bytes + B_ROWS * 128u);
+    a.ksteps = static_cast<int>((K + mm_ksub(CG) * MM_BK - 1) / (mm_ksub(CG) * MM_BK));
+    a.stages = static_cast<int>(std::min<uint32_t>(MM_MAX_STAGES, MM_RING / a.stage_bytes));
     CUtensorMap ma, mb;
     if (int e = A_MN ? encode_map_2d(&ma, TY, A.p, a.M, K, A.ld * 2, 64, MM_BK)
                      : encode_map_2d(&ma, TY, A.p, K, a.M, A.ld * 2, MM_BK, a.a_rows))
         return e;
     if (int e = B_MN ? encode_map_2d(&mb, TY, B.p, a.N, K, B.ld * 2, 64, MM_BK)
-                     : encode_map_2d(&mb, TY, B.p, K, a.N, B.ld * 2, MM_BK, 128))
+                     : encode_map_2d(&mb, TY, B.p, K, a.N, B.ld * 2, MM_BK, B_ROWS))
         return e;
     if (int e = set_smem(kern, MM_SMEM)) return e;
     const int64_t tiles = static_cast<int64_t>(a.mtiles) * a.ntiles;
     const int size = CG == 2 ? 2 : (SPLIT ? a.splits : 1);
     const int64_t groups =
         SPLIT ? tiles
-              : std::min<int64_t>(tiles, CG == 2 ? resident_clusters(reinterpret_cast<const void*>(kern), 2, MM_SMEM)
-                                                 : sm_count());
-    cudaLaunchConfig_t cfg;
-    std::memset(&cfg, 0, sizeof(cfg));
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = static_cast<unsigned>(size);
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    cfg.gridDim = dim3(static_cast<unsigned>(groups * size));
-    cfg.blockDim = dim3(MM_THREADS);
-    cfg.dynamicSmemBytes = MM_SMEM;
-    cfg.stream = st;
-    cfg.attrs = &at;
-    cfg.numAttrs = 1;
-    if (cudaLaunchKernelEx(&cfg, kern, ma, mb, a) != cudaSuccess) {
-        (void)check_launch();
-        return RAVEL_ERR_CUDA;
-    }
-    return check_launch();
+              : std::min<int64_t>(tiles, CG == 2 ? resident_clusters(reinterpret_cast<const void*>(kern), 2) : sm_count());
+    return launch(kern, dim3(static_cast<unsigned>(groups * size)), MM_THREADS, MM_SMEM, st, size, ma, mb, a);
 }
 
 constexpr int64_t kGemvRows = 4;
@@ -135,22 +132,22 @@ constexpr int64_t kGemvRows = 4;
 // At most kGemvRows rows.  Warps per weight row: at least 16 warps an SM in all while every lane keeps
 // a few loads of its row.
 template <typename T>
-int launch_gemv(const Operand& X, const Operand& W, int64_t K, const MatmulArgs& e, cudaStream_t st) {
+int launch_gemv(const Operand& X, const Operand& W, int64_t K, int act, const MatmulArgs& e, cudaStream_t st) {
     GemvArgs a;
     a.x = X.p; a.w = W.p; a.ldx = X.ld; a.ldw = W.ld; a.K = K;
+    a.act = act;
     a.e = e;
     int s = 1;
     while (s < GV_WARPS && e.N * s < static_cast<int64_t>(sm_count()) * 16 && K >= 512 * s) s *= 2;
     auto rows = [&](auto sc) -> int {
         constexpr int S = decltype(sc)::value;
-        const unsigned grid = static_cast<unsigned>((e.N + GV_WARPS / S - 1) / (GV_WARPS / S));
+        const dim3 grid(static_cast<unsigned>((e.N + GV_WARPS / S - 1) / (GV_WARPS / S)));
         switch (e.M) {
-            case 1: k_gemv<T, 1, S><<<grid, 32 * GV_WARPS, 0, st>>>(a); break;
-            case 2: k_gemv<T, 2, S><<<grid, 32 * GV_WARPS, 0, st>>>(a); break;
-            case 3: k_gemv<T, 3, S><<<grid, 32 * GV_WARPS, 0, st>>>(a); break;
-            default: k_gemv<T, 4, S><<<grid, 32 * GV_WARPS, 0, st>>>(a); break;
+            case 1: return launch(k_gemv<T, 1, S>, grid, 32 * GV_WARPS, 0, st, 1, a);
+            case 2: return launch(k_gemv<T, 2, S>, grid, 32 * GV_WARPS, 0, st, 1, a);
+            case 3: return launch(k_gemv<T, 3, S>, grid, 32 * GV_WARPS, 0, st, 1, a);
+            default: return launch(k_gemv<T, 4, S>, grid, 32 * GV_WARPS, 0, st, 1, a);
         }
-        return check_launch();
     };
     if (s == 1) return rows(IC<1>{});
     if (s == 2) return rows(IC<2>{});
@@ -158,15 +155,20 @@ int launch_gemv(const Operand& X, const Operand& W, int64_t K, const MatmulArgs&
     return rows(IC<8>{});
 }
 
-template <typename T, bool A_MN, bool B_MN, bool FULL>
+template <typename T, bool A_MN, bool B_MN, bool FULL, int ACT>
 int matmul_shape(const Operand& A, const Operand& B, int64_t K, MatmulArgs& a, cudaStream_t st) {
-    const Plan p = plan_matmul(a.M, a.N, K);
+    const Plan p = plan_matmul(a.M, a.N, K, B_MN);
     a.splits = p.splits;
-    switch (p.shape) {
-        case PAIRS: return launch_matmul<T, 2, A_MN, B_MN, FULL, false>(A, B, K, a, st);
-        case SINGLE: return launch_matmul<T, 1, A_MN, B_MN, FULL, false>(A, B, K, a, st);
-        default: return launch_matmul<T, 1, A_MN, B_MN, FULL, true>(A, B, K, a, st);
+    if (p.splits > 1) return launch_matmul<T, 1, 128, A_MN, B_MN, FULL, ACT, true>(A, B, K, a, st);
+    if (p.cg == 2) {
+        if (p.bn == 256) return launch_matmul<T, 2, 256, A_MN, B_MN, FULL, ACT, false>(A, B, K, a, st);
+        return launch_matmul<T, 2, 128, A_MN, B_MN, FULL, ACT, false>(A, B, K, a, st);
     }
+    if constexpr (!B_MN) {
+        if (p.bn == 32) return launch_matmul<T, 1, 32, A_MN, B_MN, FULL, ACT, false>(A, B, K, a, st);
+    }
+    if (p.bn == 64) return launch_matmul<T, 1, 64, A_MN, B_MN, FULL, ACT, false>(A, B, K, a, st);
+    return launch_matmul<T, 1, 128, A_MN, B_MN, FULL, ACT, false>(A, B, K, a, st);
 }
 
 template <typename F>
@@ -325,8 +327,6 @@ int ravel_matmul(const void* A, int64_t lda, int a_mn, const void* B, int64_t ld
     MatmulArgs a;
     std::memset(&a, 0, sizeof(a));
     a.M = M; a.N = N;
-    a.kchunks = static_cast<int>((K + MM_BK - 1) / MM_BK);
-    a.act = act;
     a.bias = bias; a.res = residual; a.y = y; a.z = z;
     a.ldr = ldr; a.ldy = ldy; a.ldz = ldz;
     a.vec_bias = bias != nullptr && aligned16(bias);
@@ -340,15 +340,16 @@ int ravel_matmul(const void* A, int64_t lda, int a_mn, const void* B, int64_t ld
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     return with_half_type(dtype, [&](auto tv) -> int {
         using T = decltype(tv);
-        if (K == 0) {
-            k_epilogue_only<T><<<grid_for((M * ((N + 7) / 8) + 255) / 256), 256, 0, st>>>(a);
-            return check_launch();
-        }
         const Operand oa{A, lda, a_mn}, ob{B, ldb, b_mn};
-        if (a_mn) return matmul_shape<T, true, true, false>(oa, ob, K, a, st);
-        if (b_mn) return matmul_shape<T, false, true, false>(oa, ob, K, a, st);
-        if (M <= kGemvRows) return launch_gemv<T>(oa, ob, K, a, st);
-        return matmul_shape<T, false, false, true>(oa, ob, K, a, st);
+        if (K > 0 && a_mn) return matmul_shape<T, true, true, false, RAVEL_ACT_NONE>(oa, ob, K, a, st);
+        if (K > 0 && b_mn) return matmul_shape<T, false, true, false, RAVEL_ACT_NONE>(oa, ob, K, a, st);
+        if (K > 0 && M <= kGemvRows) return launch_gemv<T>(oa, ob, K, act, a, st);
+        return with_act(act, [&](auto av) -> int {
+            constexpr int ACT = decltype(av)::value;
+            if (K == 0)
+                return launch(k_epilogue_only<T, ACT>, dim3(grid_for((M * ((N + 7) / 8) + 255) / 256)), 256, 0, st, 1, a);
+            return matmul_shape<T, false, false, true, ACT>(oa, ob, K, a, st);
+        });
     });
 }
 
@@ -385,13 +386,12 @@ int ravel_linear_dz(const void* grad_y, int64_t ldg, const void* z, int64_t ldz,
     return with_half_type(dtype, [&](auto tv) -> int {
         using T = decltype(tv);
         const int rc = with_act(act, [&](auto av) -> int {
-            k_linear_dz<T, decltype(av)::value><<<grid, 32 * DZ_WARPS, 0, st>>>(a);
-            return check_launch();
+            return launch(k_linear_dz<T, decltype(av)::value>, grid, 32 * DZ_WARPS, 0, st, 1, a);
         });
         if (rc != RAVEL_OK || grad_bias == nullptr) return rc;
-        k_col_reduce<T><<<static_cast<unsigned>((N + CR_COLS - 1) / CR_COLS), CR_COLS * CR_ROWS, 0, st>>>(
-            a.part, static_cast<int>(blocks), N, N, static_cast<T*>(grad_bias), nullptr);
-        return check_launch();
+        return launch(k_col_reduce<T>, dim3(static_cast<unsigned>((N + CR_COLS - 1) / CR_COLS)), CR_COLS * CR_ROWS, 0,
+                      st, 1, a.part, static_cast<int>(blocks), N, N, static_cast<T*>(grad_bias),
+                      static_cast<T*>(nullptr));
     });
 }
 
@@ -402,9 +402,8 @@ int ravel_pad_rows(const void* src, int64_t ld, int64_t rows, int64_t cols, void
     if (dtype != RAVEL_BF16 && dtype != RAVEL_F16) return RAVEL_ERR_UNSUPPORTED;
     if (rows == 0 || cols == 0) return RAVEL_OK;
     if (src == nullptr || dst == nullptr || (rows > 1 && ld < cols) || ldd < cols) return RAVEL_ERR_INVALID_ARG;
-    k_pad_rows<<<grid_for((rows + 7) / 8), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-        static_cast<const unsigned short*>(src), ld, rows, cols, static_cast<unsigned short*>(dst), ldd);
-    return check_launch();
+    return launch(k_pad_rows, dim3(grid_for((rows + 7) / 8)), 256, 0, static_cast<cudaStream_t>(stream), 1,
+                  static_cast<const unsigned short*>(src), ld, rows, cols, static_cast<unsigned short*>(dst), ldd);
 }
 
 int ravel_layer_norm_fwd(const void* x, int64_t ldx, const void* weight, const void* bias, float eps, void* y,
@@ -427,15 +426,13 @@ int ravel_layer_norm_fwd(const void* x, int64_t ldx, const void* weight, const v
     return with_float_type(dtype, [&](auto tv) -> int {
         using T = decltype(tv);
         if (p.W == 0) {
-            k_ln_fwd_wide<T><<<static_cast<unsigned>(M), 32 * LN_WIDE_WARPS, 0, st>>>(a);
-            return check_launch();
+            return launch(k_ln_fwd_wide<T>, dim3(static_cast<unsigned>(M)), 32 * LN_WIDE_WARPS, 0, st, 1, a);
         }
         return with_norm_plan<T>(p, [&](auto vc, auto wc, auto nc) -> int {
             constexpr int W = decltype(wc)::value;
             const int64_t blocks = W == 1 ? (M + LN_ROWS - 1) / LN_ROWS : M;
-            k_ln_fwd<T, decltype(vc)::value, W, decltype(nc)::value>
-                <<<static_cast<unsigned>(blocks), ln_threads<W>(), 0, st>>>(a);
-            return check_launch();
+            return launch(k_ln_fwd<T, decltype(vc)::value, W, decltype(nc)::value>, dim3(static_cast<unsigned>(blocks)),
+                          ln_threads<W>(), 0, st, 1, a);
         });
     });
 }
@@ -476,20 +473,18 @@ int ravel_layer_norm_bwd(const void* x, int64_t ldx, const void* weight, const v
         using T = decltype(tv);
         int rc;
         if (p.W == 0) {
-            k_ln_bwd_wide<T><<<static_cast<unsigned>(blocks), 32 * LN_WIDE_WARPS, 0, st>>>(a);
-            rc = check_launch();
+            rc = launch(k_ln_bwd_wide<T>, dim3(static_cast<unsigned>(blocks)), 32 * LN_WIDE_WARPS, 0, st, 1, a);
         } else {
             rc = with_norm_plan<T>(p, [&](auto vc, auto wc, auto nc) -> int {
                 constexpr int W = decltype(wc)::value;
-                k_ln_bwd<T, decltype(vc)::value, W, decltype(nc)::value>
-                    <<<static_cast<unsigned>(blocks), ln_threads<W>(), 0, st>>>(a);
-                return check_launch();
+                return launch(k_ln_bwd<T, decltype(vc)::value, W, decltype(nc)::value>,
+                              dim3(static_cast<unsigned>(blocks)), ln_threads<W>(), 0, st, 1, a);
             });
         }
         if (rc != RAVEL_OK || grad_weight == nullptr) return rc;
-        k_col_reduce<T><<<static_cast<unsigned>((2 * K + CR_COLS - 1) / CR_COLS), CR_COLS * CR_ROWS, 0, st>>>(
-            a.part, static_cast<int>(blocks), 2 * K, K, static_cast<T*>(grad_weight), static_cast<T*>(grad_bias));
-        return check_launch();
+        return launch(k_col_reduce<T>, dim3(static_cast<unsigned>((2 * K + CR_COLS - 1) / CR_COLS)), CR_COLS * CR_ROWS,
+                      0, st, 1, a.part, static_cast<int>(blocks), 2 * K, K, static_cast<T*>(grad_weight),
+                      static_cast<T*>(grad_bias));
     });
 }
 
@@ -516,8 +511,8 @@ int ravel_distill_topk_fwd(const void* logits, int64_t ld, const void* ids, int 
             if (cudaMemsetAsync(count, 0, sizeof(*count), st) != cudaSuccess) return RAVEL_ERR_CUDA;
             if (R > 0) {
                 const int64_t blocks = std::min<int64_t>((R + 7) / 8, int64_t{sm_count()} * 4);
-                k_distill_count<TT><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a, count);
-                if (int e = check_launch()) return e;
+                if (int e = launch(k_distill_count<TT>, dim3(static_cast<unsigned>(blocks)), 256, 0, st, 1, a, count))
+                    return e;
             }
         }
         if (R > 0) {
@@ -525,16 +520,14 @@ int ravel_distill_topk_fwd(const void* logits, int64_t ld, const void* ids, int 
                 using T = decltype(tv);
                 return with_threads(distill_threads(R, V, dtype), [&](auto th) -> int {
                     constexpr int TH = decltype(th)::value;
-                    if (grad != nullptr) k_distill<T, TT, TH, true><<<static_cast<unsigned>(R), TH, smem, st>>>(a);
-                    else k_distill<T, TT, TH, false><<<static_cast<unsigned>(R), TH, smem, st>>>(a);
-                    return check_launch();
+                    return launch(grad != nullptr ? k_distill<T, TT, TH, true> : k_distill<T, TT, TH, false>,
+                                  dim3(static_cast<unsigned>(R)), TH, smem, st, 1, a);
                 });
             });
             if (rc != RAVEL_OK) return rc;
         }
         if (reduction == RAVEL_REDUCE_NONE) return RAVEL_OK;
-        k_distill_total<<<1, 1024, 0, st>>>(losses, R, a.count, out);
-        return check_launch();
+        return launch(k_distill_total, dim3(1), 1024, 0, st, 1, losses, R, a.count, out);
     });
 }
 
@@ -566,8 +559,8 @@ int ravel_distill_topk_bwd(const void* logits, int64_t ld, const void* ids, int 
             return with_threads(distill_threads(R, V, dtype), [&](auto th) -> int {
                 constexpr int TH = decltype(th)::value;
                 const int64_t blocks = std::min<int64_t>(R, int64_t{sm_count()} * (2048 / TH));
-                k_distill_bwd<T, TT, TH><<<static_cast<unsigned>(blocks), TH, static_cast<size_t>(k) * 8, st>>>(a);
-                return check_launch();
+                return launch(k_distill_bwd<T, TT, TH>, dim3(static_cast<unsigned>(blocks)), TH,
+                              static_cast<size_t>(k) * 8, st, 1, a);
             });
         });
     });

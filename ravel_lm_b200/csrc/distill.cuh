@@ -57,6 +57,8 @@ __device__ __forceinline__ bool distill_entry(const DistillArgs& a, int64_t row,
 template <typename TT>
 __global__ void __launch_bounds__(256) k_distill_count(const DistillArgs a, unsigned int* count) {
     __shared__ unsigned int n;
+    grid_wait();
+    grid_trigger();
     if (threadIdx.x == 0) n = 0u;
     __syncthreads();
     const int lane = threadIdx.x & 31;
@@ -234,6 +236,8 @@ __global__ void __launch_bounds__(TH) k_distill(const DistillArgs a) {
     __shared__ float sred[1];
     float* const sp = dyn;
     int* const sid = reinterpret_cast<int*>(dyn + a.k);
+    grid_wait();
+    grid_trigger();
     const int64_t row = blockIdx.x;
     const T* const s = static_cast<const T*>(a.s) + row * a.lds;
     const float c = 1.4426950408889634f / a.tau;
@@ -283,6 +287,8 @@ __global__ void __launch_bounds__(TH) k_distill_bwd(const DistillArgs a) {
     __shared__ float sred[1];
     float* const sp = dyn;
     int* const sid = reinterpret_cast<int*>(dyn + a.k);
+    grid_wait();
+    grid_trigger();
     if (a.done && *a.up == 1.0f) return;
     const float n = a.count != nullptr ? fmaxf(static_cast<float>(*a.count), 1.0f) : 1.0f;
     for (int64_t row = blockIdx.x; row < a.R; row += gridDim.x) {
@@ -301,6 +307,8 @@ __global__ void __launch_bounds__(1024) k_distill_total(const float* __restrict_
                                                         float* __restrict__ out) {
     __shared__ float2 red[64];
     int turn = 0;
+    grid_wait();
+    grid_trigger();
     float s = 0.0f;
 #pragma unroll 4
     for (int64_t i = threadIdx.x; i < R; i += 1024) s += losses[i];

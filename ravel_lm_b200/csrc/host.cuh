@@ -27,6 +27,28 @@ int set_smem(K kernel, size_t bytes) {
     return raise_smem(reinterpret_cast<const void*>(kernel), bytes);
 }
 
+// Launch a kernel that calls grid_wait() (programmatic dependent launch: its blocks may be set up while the
+// previous kernel of the stream drains), in clusters of `cluster` blocks where that is more than 1.
+template <typename... P, typename... A>
+int launch(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, int cluster, A&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[2] = {};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = static_cast<unsigned>(cluster);
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    const int rc = check_launch();
+    return e == cudaSuccess ? rc : RAVEL_ERR_CUDA;
+}
+
 // Device addresses of the current device's error word and wait limit, for
 // kernels of other translation units (looked up once per device).
 struct DeviceWords {

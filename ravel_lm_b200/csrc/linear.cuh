@@ -10,12 +10,14 @@
 //                   Warp 0 loads 64-deep chunks of both operands by TMA into a ring of
 //                   128-byte-swizzled stages, warp 1 issues the tcgen05.mma, warps 4-11 turn
 //                   accumulators into outputs.  Three shapes of it:
-//                   - pairs (CG 2): a cluster of two CTAs computes 256 x 256 outputs, each
-//                     CTA holding 128 rows of A and 128 of B per chunk, so shared memory
-//                     feeds 128 x 256 outputs per SM with 32 KB per chunk.  Two accumulators
-//                     (all 512 TMEM columns) let the epilogue of one tile run under the
-//                     products of the next; the grid is persistent.
-//                   - single (CG 1): 128 x 128 outputs per CTA, same structure.
+//                   - pairs (CG 2): a cluster of two CTAs computes 256 x BN outputs (BN 256 or
+//                     128), each CTA holding 128 rows of A and BN / 2 of B per chunk: 32 KB feed
+//                     128 x 256 outputs per SM.  An SM takes in at most 64 bytes a clock from L2,
+//                     so the bytes per output decide: a 64-deep chunk of 256 x 256 takes 600 clocks
+//                     (512 at the tensor peak), one of 128 x 128 per SM the same 600.  Two
+//                     accumulators let the epilogue of one tile run under the products of the next;
+//                     the grid is persistent.
+//                   - single (CG 1): 128 x BN outputs per CTA (BN 128, 64 or 32), same structure.
 //                   - split (CG 1, clusters of 2, 4 or 8): the CTAs of a cluster share one
 //                     output tile and divide k; their partial sums meet through distributed
 //                     shared memory, added in rank order (deterministic, one launch, no
@@ -144,26 +146,36 @@ __device__ __forceinline__ float act_grad(float z) {
 // ------------------------------------------------------------------ the matrix product
 constexpr int MM_BM = 128;         // rows of A per CTA
 constexpr int MM_BK = 64;          // elements per chunk: one 128-byte swizzle row
-constexpr int MM_STAGES = 6;       // x 32 KB of operands
+constexpr int MM_MAX_STAGES = 16;
+// Chunks per stage.  Issuing a stage (a wait, its products, a commit) takes one thread some 250 clocks and 40 a
+// product: below the 512 clocks of a pair's 256 x 256 chunk, above the 256 and fewer of a single CTA's, whose
+// stages therefore hold two chunks.
+#ifndef RAVEL_MM_KS2
+#define RAVEL_MM_KS2 1
+#endif
+#ifndef RAVEL_MM_KS1
+#define RAVEL_MM_KS1 2
+#endif
+__host__ __device__ constexpr int mm_ksub(int cg) { return cg == 2 ? RAVEL_MM_KS2 : RAVEL_MM_KS1; }
+constexpr uint32_t MM_RING = 6 * 32768;  // bytes of operand stages
 constexpr int MM_EPI_WARPS = 8;
 constexpr int MM_THREADS = 128 + 32 * MM_EPI_WARPS;
 constexpr int MM_GROUP = 8;        // row tiles per column sweep: their A stays in L2
-constexpr uint32_t MM_A_BYTES = MM_BM * MM_BK * 2;
-constexpr uint32_t MM_B_BYTES = 128 * MM_BK * 2;
-constexpr uint32_t MM_STAGE_BYTES = MM_A_BYTES + MM_B_BYTES;
 constexpr uint32_t MM_EPI_BYTES = 4096;  // per epilogue warp: 32 rows x 32 columns of y (and residual), and of z
-constexpr uint32_t MM_SMEM = 1024 /* alignment */ + MM_STAGES * MM_STAGE_BYTES + MM_EPI_WARPS * MM_EPI_BYTES + 256;
+constexpr uint32_t MM_SMEM = 1024 /* alignment */ + MM_RING + MM_EPI_WARPS * MM_EPI_BYTES + 512 /* barriers */;
 constexpr int MM_PART_LD = 132;    // floats per row of a split tile's partial sums (128 + 4: no bank conflicts)
 static_assert(MM_SMEM <= 227 * 1024, "one CTA per SM");
-static_assert(MM_BM * MM_PART_LD * 4 <= MM_STAGES * MM_STAGE_BYTES, "partial sums reuse the ring");
+static_assert(MM_BM * MM_PART_LD * 4 <= MM_RING, "partial sums reuse the ring");
+static_assert(MM_MAX_STAGES * 16 + 40 <= 512, "barriers");
 
 struct MatmulArgs {
     int64_t M, N;           // outputs
-    int kchunks;            // ceil(k / 64)
+    int ksteps;             // stages of k
     int a_rows;             // rows of A per load (128, or fewer when M is smaller; K-major A)
+    int stages;             // chunks in the ring
+    uint32_t stage_bytes, a_bytes;  // of one stage, and of one chunk of A (multiples of 1024)
     int mtiles, ntiles;
     int splits;             // CTAs per tile of the split shape
-    int act;
     const void* bias;       // [N] or null
     const void* res;        // [M, N], rows ldr apart, or null
     void* y;                // [M, N], rows ldy apart
@@ -174,9 +186,11 @@ struct MatmulArgs {
     const unsigned int* wait_limit;
 };
 
+// The barriers order tensor-memory and asynchronous-proxy accesses only, so every wait has the default
+// scope; an acquire at cluster scope here cost 600 clocks a chunk whatever the tile.
 __device__ __forceinline__ bool mm_wait(uint32_t bar, uint32_t parity, uint32_t limit, volatile int* abort) {
     for (uint32_t it = 0; it < limit; ++it) {
-        if (mbar_try_wait_cluster(bar, parity)) return true;
+        if (mbar_try_wait(bar, parity)) return true;
         if ((it & 255u) == 255u && *abort) return false;
         if (it > 4096u) __nanosleep(64);
     }
@@ -194,27 +208,6 @@ __device__ __forceinline__ void mm_tile(const MatmulArgs& a, int t, int& mt, int
     mt = first + (r - nt * gm);
 }
 
-// act(v + bias) over 8 columns; zp receives the rounded sum before the activation.
-template <typename T, int ACT>
-__device__ __forceinline__ void mm_finish8(float (&v)[8], const uint4& bias, uint4& zp, bool want_z) {
-    float b[8];
-    unpack8<T>(bias, b);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] += b[e];
-    if (want_z) zp = pack8<T>(v);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = act_fwd<ACT>(v[e]);
-}
-template <typename T>
-__device__ __forceinline__ void mm_finish8_act(int act, float (&v)[8], const uint4& bias, uint4& zp, bool want_z) {
-    switch (act) {
-        case RAVEL_ACT_RELU: mm_finish8<T, RAVEL_ACT_RELU>(v, bias, zp, want_z); break;
-        case RAVEL_ACT_GELU: mm_finish8<T, RAVEL_ACT_GELU>(v, bias, zp, want_z); break;
-        case RAVEL_ACT_SILU: mm_finish8<T, RAVEL_ACT_SILU>(v, bias, zp, want_z); break;
-        default: mm_finish8<T, RAVEL_ACT_NONE>(v, bias, zp, want_z); break;
-    }
-}
-
 // One warp's 32 rows x 32 columns: rows copied between global memory and the warp's
 // staging (64 bytes per row, its four 16-byte pieces rotated so that neither the row-wise
 // nor the piece-wise accesses meet in a bank).
@@ -223,23 +216,14 @@ __device__ __forceinline__ uint32_t epi_piece(int row, int piece) {
 }
 template <typename T>
 __device__ __forceinline__ void epi_load(unsigned char* st, const T* g, int64_t ld, int64_t m0, int64_t M, int64_t c0,
-                                         int64_t N, bool vec, int lane) {
-    if (vec) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int row = i * 8 + (lane >> 2), piece = lane & 3;
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (m0 + row < M) v = load8(g + (m0 + row) * ld, c0 + piece * 8, N, true);
-            *reinterpret_cast<uint4*>(st + epi_piece(row, piece)) = v;
-        }
-    } else {  // an element per lane, a row at a time: adjacent addresses whatever the rows' alignment
-        const bool col = c0 + lane < N;
-        const int rows = (M - m0) < 32 ? static_cast<int>(M - m0) : 32;
-        const T* p = g + m0 * ld + c0 + lane;
+                                         int64_t N, int lane) {
+    // rows without 16-byte access: an element per lane, a row at a time (adjacent addresses)
+    const bool col = c0 + lane < N;
+    const int rows = (M - m0) < 32 ? static_cast<int>(M - m0) : 32;
+    const T* p = g + m0 * ld + c0 + lane;
 #pragma unroll 8
-        for (int row = 0; row < rows; ++row, p += ld)
-            if (col) *reinterpret_cast<T*>(st + epi_piece(row, lane >> 3) + (lane & 7) * 2) = *p;
-    }
+    for (int row = 0; row < rows; ++row, p += ld)
+        if (col) *reinterpret_cast<T*>(st + epi_piece(row, lane >> 3) + (lane & 7) * 2) = *p;
 }
 template <typename T>
 __device__ __forceinline__ void epi_store(const unsigned char* st, T* g, int64_t ld, int64_t m0, int64_t M, int64_t c0,
@@ -261,34 +245,75 @@ __device__ __forceinline__ void epi_store(const unsigned char* st, T* g, int64_t
     }
 }
 
-// T: element type.  CG: CTAs per product.  A_MN / B_MN: the operand is stored [k][rows].
-// FULL: bias, activation, residual and z (the forward); else a plain store.  SPLIT: see above.
-template <typename T, int CG, bool A_MN, bool B_MN, bool FULL, bool SPLIT>
+// The residual of a warp's next 32 x 32 outputs, in registers until its turn (16-byte rows).
+template <typename T>
+__device__ __forceinline__ void epi_fetch(uint4 (&v)[4], const T* g, int64_t ld, int64_t m0, int64_t M, int64_t c0,
+                                          int64_t N, int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = i * 8 + (lane >> 2), piece = lane & 3;
+        v[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (m0 + row < M && c0 < N) v[i] = load8(g + (m0 + row) * ld, c0 + piece * 8, N, true);
+    }
+}
+__device__ __forceinline__ void epi_put(unsigned char* st, const uint4 (&v)[4], int lane) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<uint4*>(st + epi_piece(i * 8 + (lane >> 2), lane & 3)) = v[i];
+}
+
+// act(v + bias) over 8 columns (z: the rounded sum before the activation) plus the residual.
+template <typename T, int ACT>
+__device__ __forceinline__ void mm_finish8(float (&v)[8], const MatmulArgs& a, int64_t row, int64_t col) {
+    if (a.bias != nullptr) {
+        float b[8];
+        unpack8<T>(load8(static_cast<const T*>(a.bias), col, a.N, a.vec_bias), b);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += b[e];
+    }
+    if (a.z != nullptr) store8(static_cast<T*>(a.z) + row * a.ldz, col, a.N, a.vec_z, pack8<T>(v));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = act_fwd<ACT>(v[e]);
+    if (a.res != nullptr) {
+        float r[8];
+        unpack8<T>(load8(static_cast<const T*>(a.res) + row * a.ldr, col, a.N, a.vec_res), r);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] += r[e];
+    }
+}
+
+// T: element type.  CG: CTAs per product.  BN: columns of a tile.  A_MN / B_MN: the operand is stored
+// [k][rows].  FULL: bias, activation ACT, residual and z (the forward); else a plain store.  SPLIT: see above.
+template <typename T, int CG, int BN, bool A_MN, bool B_MN, bool FULL, int ACT, bool SPLIT>
 __global__ void __launch_bounds__(MM_THREADS, 1)
     k_matmul(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
              const __grid_constant__ MatmulArgs a) {
-    static_assert(!(SPLIT && CG == 2), "the split shape uses single CTAs");
-    constexpr int BN = 128 * CG;                        // columns of a tile
+    static_assert(!SPLIT || (CG == 1 && BN == 128), "the split shape uses single CTAs of 128 columns");
+    static_assert(CG == 2 ? (BN == 256 || BN == 128) : (BN == 128 || BN == 64 || BN == 32), "tile widths");
+    static_assert(!B_MN || BN / CG % 64 == 0, "MN-major tiles come in blocks of 64");
+    constexpr int B_ROWS = BN / CG;                     // rows of B per CTA
     constexpr uint32_t BUFS = SPLIT ? 1 : 2;            // accumulators
     constexpr uint32_t COLS = BN * BUFS;
+    constexpr int KS = mm_ksub(CG);                     // chunks per stage
+    constexpr int UNITS = BN >= 64 ? BN / 64 : 1;       // 32-column units of an epilogue warp
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ unsigned char smem_raw[];
     const uint32_t raw = static_cast<uint32_t>(__cvta_generic_to_shared(smem_raw));
     const uint32_t base = (raw + 1023u) & ~1023u;       // swizzled tiles need 1024-byte alignment
     unsigned char* const gen = smem_raw + (base - raw);
-    const uint32_t sbar = base + MM_STAGES * MM_STAGE_BYTES + MM_EPI_WARPS * MM_EPI_BYTES;
-    const uint32_t bar_full = sbar, bar_empty = sbar + 8 * MM_STAGES;
-    const uint32_t bar_tfull = sbar + 16 * MM_STAGES, bar_tempty = bar_tfull + 16;
+    const uint32_t sbar = base + MM_RING + MM_EPI_WARPS * MM_EPI_BYTES;
+    const uint32_t bar_full = sbar, bar_empty = sbar + 8 * MM_MAX_STAGES;
+    const uint32_t bar_tfull = sbar + 16 * MM_MAX_STAGES, bar_tempty = bar_tfull + 16;
     unsigned char* const tail = gen + (bar_tempty + 16 - base);
     volatile uint32_t* const tmem_slot = reinterpret_cast<volatile uint32_t*>(tail);
     volatile int* const abort = reinterpret_cast<volatile int*>(tail + 4);
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
     const uint32_t rank = (CG == 2 || SPLIT) ? cluster_rank() : 0u;
-    const uint32_t limit = 4u * *const_cast<volatile const unsigned int*>(a.wait_limit);
+    const uint32_t stages = static_cast<uint32_t>(a.stages);
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < MM_STAGES; ++s) {
+        for (uint32_t s = 0; s < stages; ++s) {
             mbar_init(bar_full + 8 * s, 1);
             mbar_init(bar_empty + 8 * s, 1);
         }
@@ -299,82 +324,99 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
         *abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (threadIdx.x == 32) {
+        prefetch_map(&map_a);
+        prefetch_map(&map_b);
+    }
     if (warp == 2) tmem_alloc<CG>(bar_tempty + 16, COLS);
     tc_fence_before();
     __syncthreads();
     if (CG == 2 || SPLIT) cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
+    grid_wait();
+    grid_trigger();
+    const uint32_t limit = 4u * *const_cast<volatile const unsigned int*>(a.wait_limit);
 
     // this cluster's tiles and this CTA's share of k
     const int group = CG == 2 ? 2 : (SPLIT ? a.splits : 1);
     const int tiles = a.mtiles * a.ntiles;
     const int t0 = static_cast<int>(blockIdx.x) / group, tstep = static_cast<int>(gridDim.x) / group;
-    const int k0 = SPLIT ? static_cast<int>(static_cast<int64_t>(a.kchunks) * rank / a.splits) : 0;
-    const int k1 = SPLIT ? static_cast<int>(static_cast<int64_t>(a.kchunks) * (rank + 1) / a.splits) : a.kchunks;
+    const int k0 = SPLIT ? static_cast<int>(static_cast<int64_t>(a.ksteps) * rank / a.splits) : 0;
+    const int k1 = SPLIT ? static_cast<int>(static_cast<int64_t>(a.ksteps) * (rank + 1) / a.splits) : a.ksteps;
 
-    if (warp == 0 && lane == 0) {
+    if (warp == 0 && elect_one()) {
         // ---------------- operand chunks by TMA (this GPU's memory, no multicast)
-        const uint32_t a_bytes = A_MN ? MM_A_BYTES : static_cast<uint32_t>(a.a_rows) * 128u;
-        uint32_t it = 0;
+        const uint32_t load_bytes =
+            KS * ((A_MN ? 16384u : static_cast<uint32_t>(a.a_rows) * 128u) + B_ROWS * 128u);
+        uint32_t it = 0, s = 0, ph = 1;  // ph: the parity of an empty stage (1 at first: free)
         bool ok = true;
         for (int t = t0; t < tiles && ok; t += tstep) {
             int mt, nt;
             mm_tile(a, t, mt, nt);
             const int m0 = mt * (MM_BM * CG) + static_cast<int>(CG == 2 ? rank : 0u) * MM_BM;
-            const int n0 = nt * BN + static_cast<int>(CG == 2 ? rank : 0u) * 128;
+            const int n0 = nt * BN + static_cast<int>(CG == 2 ? rank : 0u) * B_ROWS;
             for (int kc = k0; kc < k1; ++kc, ++it) {
-                const uint32_t s = it % MM_STAGES;
-                if (it >= MM_STAGES && !(ok = mm_wait(bar_empty + 8 * s, (it / MM_STAGES - 1) & 1, limit, abort))) break;
-                const uint32_t sa = base + s * MM_STAGE_BYTES, sb = sa + MM_A_BYTES;
-                if (CG == 1 || rank == 0) mbar_arrive_expect_tx(bar_full + 8 * s, CG * (a_bytes + MM_B_BYTES));
+                if (it >= stages && !(ok = mm_wait(bar_empty + 8 * s, ph, limit, abort))) break;
+                uint32_t sa = base + s * a.stage_bytes, sb = sa + KS * a.a_bytes;
+                if (CG == 1 || rank == 0) mbar_arrive_expect_tx(bar_full + 8 * s, CG * load_bytes);
                 const uint32_t bar = CG == 2 ? map_to_rank(bar_full + 8 * s, 0) : bar_full + 8 * s;
                 auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y) {
                     if constexpr (CG == 2) tma_load_2d_pair(dst, map, x, y, bar);
                     else tma_load_2d(dst, map, x, y, bar);
                 };
-                if constexpr (A_MN) {
-                    load(sa, &map_a, m0, kc * MM_BK);
-                    load(sa + 8192, &map_a, m0 + 64, kc * MM_BK);
-                } else {
-                    load(sa, &map_a, kc * MM_BK, m0);
+#pragma unroll
+                for (int i = 0; i < KS; ++i, sa += a.a_bytes, sb += B_ROWS * 128u) {
+                    const int k = (kc * KS + i) * MM_BK;  // past the end: zeros
+                    if constexpr (A_MN) {
+                        load(sa, &map_a, m0, k);
+                        load(sa + 8192, &map_a, m0 + 64, k);
+                    } else {
+                        load(sa, &map_a, k, m0);
+                    }
+                    if constexpr (B_MN) {
+#pragma unroll
+                        for (int c = 0; c < B_ROWS / 64; ++c) load(sb + c * 8192, &map_b, n0 + c * 64, k);
+                    } else {
+                        load(sb, &map_b, k, n0);
+                    }
                 }
-                if constexpr (B_MN) {
-                    load(sb, &map_b, n0, kc * MM_BK);
-                    load(sb + 8192, &map_b, n0 + 64, kc * MM_BK);
-                } else {
-                    load(sb, &map_b, kc * MM_BK, n0);
-                }
+                if (++s == stages) s = 0, ph ^= 1u;
             }
         }
         // every stage handed back before this CTA may leave (its barriers are arrived on
         // by the pair's first CTA)
-        for (uint32_t i = it < MM_STAGES ? 0 : it - MM_STAGES; i < it && ok; ++i)
-            ok = mm_wait(bar_empty + 8 * (i % MM_STAGES), (i / MM_STAGES) & 1, limit, abort);
+        for (uint32_t i = it < stages ? 0 : it - stages; i < it && ok; ++i)
+            ok = mm_wait(bar_empty + 8 * (i % stages), (i / stages) & 1, limit, abort);
         if (!ok)  // loads still in flight land within microseconds
             for (int i = 0; i < 256; ++i) __nanosleep(4000);
-    } else if (warp == 1 && lane == 0 && (CG == 1 || rank == 0)) {
+    } else if (warp == 1 && (CG == 1 || rank == 0) && elect_one()) {
         // ---------------- the products
         const uint32_t idesc = idesc_f16(BF16, A_MN, B_MN, MM_BM * CG, BN);
-        uint32_t it = 0, j = 0;
+        // 16 k on: 32 bytes along a K-major row, two 8-row groups of an MN-major block
+        constexpr uint32_t A_STEP = A_MN ? 2048 >> 4 : 32 >> 4, B_STEP = B_MN ? 2048 >> 4 : 32 >> 4;
+        const uint32_t a_lo = umma_desc_lo<A_MN>(base), b_lo = umma_desc_lo<B_MN>(base + KS * a.a_bytes);
+        uint32_t s = 0, ph = 0, j = 0;
         bool ok = true;
         for (int t = t0; t < tiles && ok; t += tstep, ++j) {
             const uint32_t buf = j % BUFS;
             if (j >= BUFS && !(ok = mm_wait(bar_tempty + 8 * buf, (j / BUFS - 1) & 1, limit, abort))) break;
             tc_fence_after();
-            for (int kc = k0; kc < k1; ++kc, ++it) {
-                const uint32_t s = it % MM_STAGES;
-                if (!(ok = mm_wait(bar_full + 8 * s, (it / MM_STAGES) & 1, limit, abort))) break;
+            uint32_t more = 0;  // 0: the tile's first product overwrites the accumulator
+            for (int kc = k0; kc < k1; ++kc) {
+                if (!(ok = mm_wait(bar_full + 8 * s, ph, limit, abort))) break;
                 tc_fence_after();
-                const uint32_t sa = base + s * MM_STAGE_BYTES, sb = sa + MM_A_BYTES;
+                uint32_t da = a_lo + s * (a.stage_bytes >> 4), db = b_lo + s * (a.stage_bytes >> 4);
 #pragma unroll
-                for (int kk = 0; kk < MM_BK / 16; ++kk) {
-                    // 16 k on: 32 bytes along a K-major row, two 8-row groups of an MN-major block
-                    const uint64_t da = A_MN ? smem_desc_mn_sw128(sa + kk * 2048, 8192) : smem_desc_sw128(sa + kk * 32);
-                    const uint64_t db = B_MN ? smem_desc_mn_sw128(sb + kk * 2048, 8192) : smem_desc_sw128(sb + kk * 32);
-                    umma_f16<CG>(tmem + buf * BN, da, db, idesc, (kc > k0 || kk > 0) ? 1u : 0u);
+                for (int i = 0; i < KS; ++i, da += a.a_bytes >> 4, db += B_ROWS * 128 >> 4) {
+#pragma unroll
+                    for (int kk = 0; kk < MM_BK / 16; ++kk) {
+                        umma_f16<CG>(tmem + buf * BN, da + kk * A_STEP, db + kk * B_STEP, idesc, more);
+                        more = 1;
+                    }
                 }
                 umma_commit_to<CG>(bar_empty + 8 * s);
+                if (++s == stages) s = 0, ph ^= 1u;
             }
             if (ok) umma_commit_to<CG>(bar_tfull + 8 * buf);
         }
@@ -382,46 +424,67 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
             for (int i = 0; i < 256; ++i) __nanosleep(4000);
     } else if (warp >= 4) {
         // ---------------- outputs.  Warps w and w + 4 share the TMEM lanes (rows) 32 (w % 4) ..,
-        // each takes half of the columns.
+        // each takes half of the columns, 32 at a time.
         const int q = warp & 3, half = (warp - 4) >> 2;
-        unsigned char* const st = gen + MM_STAGES * MM_STAGE_BYTES + (warp - 4) * MM_EPI_BYTES;
+        unsigned char* const st = gen + MM_RING + (warp - 4) * MM_EPI_BYTES;
         const T* const bias = static_cast<const T*>(a.bias);
+        const T* const res = static_cast<const T*>(a.res);
+        const bool idle = BN == 32 && half == 1;  // a tile of one unit
+        const uint32_t done_bar = map_to_rank(bar_tempty, CG == 2 ? 0u : cluster_rank());
         uint32_t j = 0;
         for (int t = t0; t < tiles; t += tstep, ++j) {
             const uint32_t buf = j % BUFS;
             int mt, nt;
             mm_tile(a, t, mt, nt);
             const int64_t m0 = static_cast<int64_t>(mt) * (MM_BM * CG) + (CG == 2 ? rank : 0u) * MM_BM + q * 32;
-            const int64_t n0 = static_cast<int64_t>(nt) * BN;
+            const int c0 = half * UNITS * 32;
+            const int64_t n0 = static_cast<int64_t>(nt) * BN + c0;
+            const bool rows = m0 < a.M && !idle;
+            uint4 rv[4];
+            float bl = 0.0f;  // the bias of column `lane` of the unit
+            if constexpr (FULL && !SPLIT) {
+                if (res != nullptr && a.vec_res && rows) epi_fetch(rv, res, a.ldr, m0, a.M, n0, a.N, lane);
+                if (bias != nullptr && n0 + lane < a.N) bl = static_cast<float>(bias[n0 + lane]);
+            }
             const bool ok = __all_sync(0xffffffffu, mm_wait(bar_tfull + 8 * buf, (j / BUFS) & 1, limit, abort));
             tc_fence_after();
             if (!ok) break;
-            const uint32_t tm = tmem + buf * BN + (static_cast<uint32_t>(q * 32) << 16);
-            for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 32) {
-                const int64_t col = n0 + c;
-                const bool live = m0 < a.M && col < a.N;  // the same for the whole warp
+            const uint32_t tm = tmem + buf * BN + (static_cast<uint32_t>(q * 32) << 16) + c0;
+#pragma unroll 1
+            for (int u = 0; u < UNITS; ++u) {
+                const int64_t col = n0 + u * 32;
+                const bool live = rows && col < a.N;  // the same for the whole warp
                 uint32_t r[32];
+                if (!idle) tmem_ld32(tm + u * 32, r);
+                if (!SPLIT && u == UNITS - 1) {  // this warp has read its part of the accumulator
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(done_bar + 8 * buf);
+                }
+                if (!live) continue;
                 if constexpr (SPLIT) {
                     // partial sums into the ring's space (every load and product of it is done)
-                    tmem_ld32(tm + c, r);
-                    float* const p = reinterpret_cast<float*>(gen) + (q * 32 + lane) * MM_PART_LD + c;
-                    if (live && m0 + lane < a.M) {
+                    if (m0 + lane < a.M) {
+                        float* const p = reinterpret_cast<float*>(gen) + (q * 32 + lane) * MM_PART_LD + c0 + u * 32;
 #pragma unroll
                         for (int e = 0; e < 32; e += 4)
                             *reinterpret_cast<uint4*>(p + e) = make_uint4(r[e], r[e + 1], r[e + 2], r[e + 3]);
                     }
                 } else {
-                    if (FULL && a.res != nullptr && live)
-                        epi_load(st, static_cast<const T*>(a.res), a.ldr, m0, a.M, col, a.N, a.vec_res, lane);
-                    tmem_ld32(tm + c, r);
-                    if (c + 32 == (half + 1) * (BN / 2)) {  // this warp has read its part of the accumulator
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0)
-                            mbar_arrive_cluster(map_to_rank(bar_tempty + 8 * buf, CG == 2 ? 0u : cluster_rank()));
+                    const float bu = bl;
+                    if constexpr (FULL) {
+                        if (res != nullptr) {
+                            if (a.vec_res) {
+                                epi_put(st, rv, lane);
+                                if (u + 1 < UNITS) epi_fetch(rv, res, a.ldr, m0, a.M, col + 32, a.N, lane);
+                            } else {
+                                epi_load(st, res, a.ldr, m0, a.M, col, a.N, lane);
+                            }
+                            __syncwarp();
+                        }
+                        if (bias != nullptr && u + 1 < UNITS)
+                            bl = col + 32 + lane < a.N ? static_cast<float>(bias[col + 32 + lane]) : 0.0f;
                     }
-                    if (!live) continue;
-                    __syncwarp();
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
                         float v[8];
@@ -429,11 +492,14 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
                         for (int e = 0; e < 8; ++e) v[e] = __uint_as_float(r[p * 8 + e]);
                         uint4* const mine = reinterpret_cast<uint4*>(st + epi_piece(lane, p));
                         if constexpr (FULL) {
-                            uint4 b = make_uint4(0u, 0u, 0u, 0u), zp;
-                            if (bias != nullptr) b = load8(bias, col + p * 8, a.N, a.vec_bias);
-                            mm_finish8_act<T>(a.act, v, b, zp, a.z != nullptr);
-                            if (a.z != nullptr) *reinterpret_cast<uint4*>(st + 2048 + epi_piece(lane, p)) = zp;
-                            if (a.res != nullptr) {
+                            if (bias != nullptr) {
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) v[e] += __shfl_sync(0xffffffffu, bu, p * 8 + e);
+                            }
+                            if (a.z != nullptr) *reinterpret_cast<uint4*>(st + 2048 + epi_piece(lane, p)) = pack8<T>(v);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) v[e] = act_fwd<ACT>(v[e]);
+                            if (res != nullptr) {
                                 float rs[8];
                                 unpack8<T>(*mine, rs);
 #pragma unroll
@@ -463,7 +529,6 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
         const int64_t m0 = static_cast<int64_t>(mt) * MM_BM;
         const int rows = (a.M - m0) < MM_BM ? static_cast<int>(a.M - m0) : MM_BM;
         const int width = BN / a.splits / 8;  // pieces of 8 columns per row
-        const T* const bias = static_cast<const T*>(a.bias);
         if (!*abort) {
             for (int u = threadIdx.x; u < rows * width; u += MM_THREADS) {
                 const int row = u / width, piece = u - row * width;
@@ -478,18 +543,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
                     v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
                     v[4] += w.x; v[5] += w.y; v[6] += w.z; v[7] += w.w;
                 }
-                if constexpr (FULL) {
-                    uint4 b = make_uint4(0u, 0u, 0u, 0u), zp;
-                    if (bias != nullptr) b = load8(bias, col, a.N, a.vec_bias);
-                    mm_finish8_act<T>(a.act, v, b, zp, a.z != nullptr);
-                    if (a.z != nullptr) store8(static_cast<T*>(a.z) + (m0 + row) * a.ldz, col, a.N, a.vec_z, zp);
-                    if (a.res != nullptr) {
-                        float rs[8];
-                        unpack8<T>(load8(static_cast<const T*>(a.res) + (m0 + row) * a.ldr, col, a.N, a.vec_res), rs);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] += rs[e];
-                    }
-                }
+                if constexpr (FULL) mm_finish8<T, ACT>(v, a, m0 + row, col);
                 store8(static_cast<T*>(a.y) + (m0 + row) * a.ldy, col, a.N, a.vec_y, pack8<T>(v));
             }
         }
@@ -510,6 +564,7 @@ struct GemvArgs {
     const void* x;       // [M, K], rows ldx apart
     const void* w;       // [N, K], rows ldw apart; both 16-byte rows
     int64_t ldx, ldw, K;
+    int act;
     MatmulArgs e;        // the epilogue
 };
 
@@ -519,6 +574,8 @@ struct GemvArgs {
 template <typename T, int MR, int S>
 __global__ void __launch_bounds__(32 * GV_WARPS) k_gemv(const GemvArgs a) {
     __shared__ float part[GV_WARPS][MR];
+    grid_wait();
+    grid_trigger();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t n = static_cast<int64_t>(blockIdx.x) * (GV_WARPS / S) + warp / S;
     float acc[MR];
@@ -575,7 +632,7 @@ __global__ void __launch_bounds__(32 * GV_WARPS) k_gemv(const GemvArgs a) {
         float v = acc[m];
         if (a.e.bias != nullptr) v += static_cast<float>(static_cast<const T*>(a.e.bias)[n]);
         if (a.e.z != nullptr) static_cast<T*>(a.e.z)[m * a.e.ldz + n] = static_cast<T>(v);
-        switch (a.e.act) {
+        switch (a.act) {
             case RAVEL_ACT_RELU: v = act_fwd<RAVEL_ACT_RELU>(v); break;
             case RAVEL_ACT_GELU: v = act_fwd<RAVEL_ACT_GELU>(v); break;
             case RAVEL_ACT_SILU: v = act_fwd<RAVEL_ACT_SILU>(v); break;
@@ -605,6 +662,8 @@ struct DzArgs {
 template <typename T, int ACT>
 __global__ void __launch_bounds__(32 * DZ_WARPS, 3) k_linear_dz(const DzArgs a) {
     __shared__ float sums[DZ_WARPS][DZ_COLS];
+    grid_wait();
+    grid_trigger();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t c = static_cast<int64_t>(blockIdx.x) * DZ_COLS + lane * 8;
     const int64_t r0 = static_cast<int64_t>(blockIdx.y) * a.rows;
@@ -659,6 +718,8 @@ __global__ void __launch_bounds__(32 * DZ_WARPS, 3) k_linear_dz(const DzArgs a) 
 // Rows of `cols` 16-bit elements from pitch ld to pitch ldd (elements).
 __global__ void __launch_bounds__(256) k_pad_rows(const unsigned short* __restrict__ src, int64_t ld, int64_t rows,
                                                   int64_t cols, unsigned short* __restrict__ dst, int64_t ldd) {
+    grid_wait();
+    grid_trigger();
     const int lane = threadIdx.x & 31;
     const int64_t nw = static_cast<int64_t>(gridDim.x) * 8;
     for (int64_t r = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); r < rows; r += nw) {
@@ -669,23 +730,16 @@ __global__ void __launch_bounds__(256) k_pad_rows(const unsigned short* __restri
 }
 
 // y = res + act(bias): a product over nothing.
-template <typename T>
+template <typename T, int ACT>
 __global__ void __launch_bounds__(256) k_epilogue_only(const MatmulArgs a) {
+    grid_wait();
+    grid_trigger();
     const int64_t pieces = (a.N + 7) / 8;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < a.M * pieces;
          i += static_cast<int64_t>(gridDim.x) * 256) {
         const int64_t row = i / pieces, col = (i - row * pieces) * 8;
         float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        uint4 b = make_uint4(0u, 0u, 0u, 0u), zp;
-        if (a.bias != nullptr) b = load8(static_cast<const T*>(a.bias), col, a.N, a.vec_bias);
-        mm_finish8_act<T>(a.act, v, b, zp, a.z != nullptr);
-        if (a.z != nullptr) store8(static_cast<T*>(a.z) + row * a.ldz, col, a.N, a.vec_z, zp);
-        if (a.res != nullptr) {
-            float rs[8];
-            unpack8<T>(load8(static_cast<const T*>(a.res) + row * a.ldr, col, a.N, a.vec_res), rs);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += rs[e];
-        }
+        mm_finish8<T, ACT>(v, a, row, col);
         store8(static_cast<T*>(a.y) + row * a.ldy, col, a.N, a.vec_y, pack8<T>(v));
     }
 }

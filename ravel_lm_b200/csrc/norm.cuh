@@ -16,6 +16,7 @@
 #include "colsum.cuh"
 #include "host.cuh"
 #include "pack.cuh"
+#include "ptx.cuh"
 
 namespace ravel {
 
@@ -81,6 +82,8 @@ template <typename T, int VEC, int W, int NV>
 __global__ void __launch_bounds__(ln_threads<W>()) k_ln_fwd(const NormArgs a) {
     __shared__ float2 red[2 * W];
     int turn = 0;
+    grid_wait();
+    grid_trigger();
     const int lane = W == 1 ? (threadIdx.x & 31) : threadIdx.x;
     const int64_t row = W == 1 ? static_cast<int64_t>(blockIdx.x) * LN_ROWS + (threadIdx.x >> 5) : blockIdx.x;
     if (row >= a.M) return;  // whole warps; with W > 1 every row exists
@@ -152,6 +155,8 @@ __global__ void __launch_bounds__(ln_threads<W>()) k_ln_bwd(const NormArgs a) {
     __shared__ float2 red[2 * W];
     __shared__ float wsum[W == 1 ? 2 * COLS : 1];
     int turn = 0;
+    grid_wait();
+    grid_trigger();
     const int lane = W == 1 ? (threadIdx.x & 31) : threadIdx.x;
     const int warp = threadIdx.x >> 5;
     const T* const g = static_cast<const T*>(a.g);
@@ -257,6 +262,8 @@ template <typename T>
 __global__ void __launch_bounds__(32 * LN_WIDE_WARPS) k_ln_fwd_wide(const NormArgs a) {
     __shared__ float2 red[2 * LN_WIDE_WARPS];
     int turn = 0;
+    grid_wait();
+    grid_trigger();
     const int64_t row = blockIdx.x;
     const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
     const float inv_k = 1.0f / static_cast<float>(a.K);
@@ -286,6 +293,8 @@ template <typename T>
 __global__ void __launch_bounds__(32 * LN_WIDE_WARPS) k_ln_bwd_wide(const NormArgs a) {
     __shared__ float2 red[2 * LN_WIDE_WARPS];
     int turn = 0;
+    grid_wait();
+    grid_trigger();
     const T* const g = static_cast<const T*>(a.g);
     const float inv_k = 1.0f / static_cast<float>(a.K);
     float* const part = a.part == nullptr ? nullptr : a.part + static_cast<int64_t>(blockIdx.x) * 2 * a.K;

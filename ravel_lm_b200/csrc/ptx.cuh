@@ -48,6 +48,24 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
+// One thread of a converged warp.  A role's loop under this predicate (not under lane == 0) is known to run
+// in one thread, so that its tcgen05 and TMA operands go to uniform registers directly.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+
+// ---- programmatic dependent launch: a kernel launched with it may start while the one before it on the
+// stream still runs.  wait returns when that one has finished (its writes visible); no global memory is
+// touched before.  The trigger lets the next kernel's blocks start as SMs come free.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---- thread-block clusters
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -73,18 +91,7 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
 }
 // Arrive on a barrier of any CTA of the cluster (an address from map_to_rank).
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait_cluster(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // A 2-D tile into this CTA's shared memory whose bytes complete on a barrier of
 // either CTA of the pair (bar: an address from map_to_rank).
@@ -108,17 +115,15 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t addr) {
     return d;
 }
 
-// MN-major operand in the 128-byte swizzle layout: 64 elements (128 bytes) of the
-// M or N extent per row, one row per K, 8-row groups 1024 bytes apart (SBO), the
-// next 64 elements `lbo` bytes on.
-__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t addr, uint32_t lbo) {
-    uint64_t d = 0;
-    d |= static_cast<uint64_t>((addr & 0x3FFFFu) >> 4);
-    d |= static_cast<uint64_t>(lbo >> 4) << 16;
-    d |= static_cast<uint64_t>(1024 >> 4) << 32;
-    d |= static_cast<uint64_t>(1) << 46;
-    d |= static_cast<uint64_t>(2) << 61;
-    return d;
+// The 128-byte-swizzle operand descriptors of the 16-bit products as two words: the low one holds the
+// address (16-byte units) and moves along the operand by additions; the high one is constant.
+//   K-major: rows of 128 bytes, 8-row groups 1024 bytes apart (as smem_desc_sw128).
+//   MN-major: 64 elements (128 bytes) of the M or N extent per row, one row per K, 8-row groups 1024 bytes
+//   apart, the next 64 elements 8192 bytes on (the leading byte offset).
+constexpr uint32_t UMMA_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+template <bool MN>
+__device__ __forceinline__ uint32_t umma_desc_lo(uint32_t addr) {
+    return ((addr & 0x3FFFFu) >> 4) | ((MN ? 8192u >> 4 : 1u) << 16);
 }
 
 // kind::f16, D float32; A and B both bfloat16 or both float16, each K-major or MN-major.
@@ -129,19 +134,21 @@ __host__ __device__ constexpr uint32_t idesc_f16(bool bf16, bool a_mn, bool b_mn
 
 // D (TMEM) (+)= A B^T, K = 16; CG 2: the pair's MMA, issued by one thread of its first CTA.
 template <int CG>
-__device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc,
+__device__ __forceinline__ void umma_f16(uint32_t tmem_d, uint32_t da_lo, uint32_t db_lo, uint32_t idesc,
                                          uint32_t accumulate) {
     if constexpr (CG == 1) {
         asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-            ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+            "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}"
+            ::"r"(tmem_d), "r"(da_lo), "r"(db_lo), "r"(idesc), "r"(accumulate), "r"(UMMA_DESC_HI)
             : "memory");
     } else {
         asm volatile(
-            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-            ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+            "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %3, p;\n\t}"
+            ::"r"(tmem_d), "r"(da_lo), "r"(db_lo), "r"(idesc), "r"(accumulate), "r"(UMMA_DESC_HI)
             : "memory");
     }
 }
