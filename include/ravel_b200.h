@@ -399,16 +399,17 @@ int ravel_layer_norm_bwd(const void* x, int64_t ldx, const void* weight, const v
  * and q = softmax(s / T) over the vocabulary:
  *   loss_r = weight T^2 sum_j p_j (log p_j - log q[id_j]);  0 without a live entry
  * losses [R] receives them, out their sum or mean (RAVEL_REDUCE_SUM / _MEAN; not
- * used for _NONE), count (MEAN) the rows that have a live entry.  stat [R][2] is
- * kept for the backward, NULL where there is none.  grad [R, V] contiguous or
- * NULL: the gradient of out with respect to the logits, made while each row is
- * still in cache (not for _NONE).  logits: float32, bfloat16 or float16; teacher:
- * any of those; k <= 4096.
+ * used for _NONE).  stat [R][2] is kept for the backward, NULL where there is
+ * none; scratch (MEAN) too, whose start then holds the count of rows.  grad
+ * [R, V] contiguous or NULL: the gradient of out with respect to the logits, made
+ * while each row is still in cache (not for _NONE; stat is given with it).  logits:
+ * float32, bfloat16 or float16; teacher: any of those; k <= 4096.
  */
+size_t ravel_distill_topk_scratch_bytes(int64_t R);
 int ravel_distill_topk_fwd(const void* logits, int64_t ld, const void* ids, int ids_dtype, const void* teacher,
                            int teacher_dtype, int64_t R, int64_t V, int64_t k, float temperature, float weight,
-                           int reduction, float* losses, float* stat, uint32_t* count, float* out, void* grad,
-                           int dtype, void* stream);
+                           int reduction, float* losses, float* stat, float* out, void* grad, int dtype, void* scratch,
+                           size_t scratch_bytes, void* stream);
 
 /*
  * Its backward for any upstream gradient (on the device: one float32, or [R] for
@@ -418,7 +419,7 @@ int ravel_distill_topk_fwd(const void* logits, int64_t ld, const void* ids, int 
  */
 int ravel_distill_topk_bwd(const void* logits, int64_t ld, const void* ids, int ids_dtype, const void* teacher,
                            int teacher_dtype, int64_t R, int64_t V, int64_t k, float temperature, float weight,
-                           int reduction, const float* stat, const uint32_t* count, const float* upstream,
+                           int reduction, const float* stat, const void* scratch, const float* upstream,
                            int grad_is_unit, void* grad, int dtype, void* stream);
 
 /*

@@ -86,8 +86,9 @@ SIGNATURES = {
     "ravel_layer_norm_scratch_bytes": (_c_sz, [_c_i64, _c_i64]),
     "ravel_layer_norm_bwd": (_c_int, [_c_vp, _c_i64, _c_vp, _c_vp, _c_i64] + [_c_vp] * 5 + [_c_i64, _c_i64, _c_int, _c_vp,
                                       _c_sz, _c_vp]),
+    "ravel_distill_topk_scratch_bytes": (_c_sz, [_c_i64]),
     "ravel_distill_topk_fwd": (_c_int, [_c_vp, _c_i64, _c_vp, _c_int, _c_vp, _c_int] + [_c_i64] * 3 +
-                               [ctypes.c_float, ctypes.c_float, _c_int] + [_c_vp] * 5 + [_c_int, _c_vp]),
+                               [ctypes.c_float, ctypes.c_float, _c_int] + [_c_vp] * 4 + [_c_int, _c_vp, _c_sz, _c_vp]),
     "ravel_distill_topk_bwd": (_c_int, [_c_vp, _c_i64, _c_vp, _c_int, _c_vp, _c_int] + [_c_i64] * 3 +
                                [ctypes.c_float, ctypes.c_float, _c_int] + [_c_vp] * 3 + [_c_int, _c_vp, _c_int, _c_vp]),
     "ravel_set_wait_limit": (_c_int, [ctypes.c_uint32]),

@@ -488,52 +488,58 @@ int ravel_layer_norm_bwd(const void* x, int64_t ldx, const void* weight, const v
     });
 }
 
+size_t ravel_distill_topk_scratch_bytes(int64_t R) {
+    return R < 0 ? 0 : DISTILL_COUNTS * sizeof(unsigned int) + static_cast<size_t>(R);
+}
+
 int ravel_distill_topk_fwd(const void* logits, int64_t ld, const void* ids, int ids_dtype, const void* teacher,
                            int teacher_dtype, int64_t R, int64_t V, int64_t k, float temperature, float weight,
-                           int reduction, float* losses, float* stat, uint32_t* count, float* out, void* grad,
-                           int dtype, void* stream) {
+                           int reduction, float* losses, float* stat, float* out, void* grad, int dtype, void* scratch,
+                           size_t scratch_bytes, void* stream) {
     RAVEL_TIMED("ravel_distill_topk_fwd", stream);
     DistillArgs a;
     if (int e = distill_args(a, logits, ld, ids, ids_dtype, teacher, R, V, k, temperature, dtype, teacher_dtype))
         return e;
     if (reduction < RAVEL_REDUCE_NONE || reduction > RAVEL_REDUCE_MEAN) return RAVEL_ERR_INVALID_ARG;
-    if ((R > 0 && losses == nullptr) || (reduction == RAVEL_REDUCE_MEAN && count == nullptr) ||
-        (reduction != RAVEL_REDUCE_NONE && out == nullptr) || (grad != nullptr && reduction == RAVEL_REDUCE_NONE))
+    if ((R > 0 && losses == nullptr) || (reduction != RAVEL_REDUCE_NONE && out == nullptr) ||
+        (grad != nullptr && reduction == RAVEL_REDUCE_NONE))
         return RAVEL_ERR_INVALID_ARG;
+    const bool mean = reduction == RAVEL_REDUCE_MEAN;
+    if (mean && (scratch == nullptr || scratch_bytes < ravel_distill_topk_scratch_bytes(R))) return RAVEL_ERR_WORKSPACE;
+    unsigned int* const counts = static_cast<unsigned int*>(scratch);
     a.weight = weight;
     a.losses = losses; a.stat = reinterpret_cast<float2*>(stat); a.grad = grad;
-    a.count = reduction == RAVEL_REDUCE_MEAN ? count : nullptr;
+    a.live = mean ? static_cast<unsigned char*>(scratch) + DISTILL_COUNTS * sizeof(unsigned int) : nullptr;
+    a.counts = mean ? counts : nullptr;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const size_t smem = static_cast<size_t>(k) * 8;
+    const size_t smem = static_cast<size_t>(k) * 12;
     return with_float_type(teacher_dtype, [&](auto ttv) -> int {
         using TT = decltype(ttv);
-        if (a.count != nullptr) {
-            if (cudaMemsetAsync(count, 0, sizeof(*count), st) != cudaSuccess) return RAVEL_ERR_CUDA;
-            if (R > 0) {
-                const int64_t blocks = std::min<int64_t>((R + 7) / 8, int64_t{sm_count()} * 4);
-                if (int e = launch(k_distill_count<TT>, dim3(static_cast<unsigned>(blocks)), 256, 0, st, 1, a, count))
-                    return e;
-            }
+        // the backward and a gradient written here divide by the count
+        if (mean && stat != nullptr) {
+            if (int e = launch(k_distill_count<TT>, dim3(DISTILL_COUNTS), 256, 0, st, 1, a, counts)) return e;
         }
         if (R > 0) {
             const int rc = with_float_type(dtype, [&](auto tv) -> int {
                 using T = decltype(tv);
                 return with_threads(distill_threads(R, V, dtype), [&](auto th) -> int {
                     constexpr int TH = decltype(th)::value;
-                    return launch(grad != nullptr ? k_distill<T, TT, TH, true> : k_distill<T, TT, TH, false>,
-                                  dim3(static_cast<unsigned>(R)), TH, smem, st, 1, a);
+                    const auto kern = grad != nullptr ? k_distill<T, TT, TH, true> : k_distill<T, TT, TH, false>;
+                    if (int e = set_smem(kern, smem)) return e;
+                    return launch(kern, dim3(static_cast<unsigned>(R)), TH, smem, st, 1, a);
                 });
             });
             if (rc != RAVEL_OK) return rc;
         }
         if (reduction == RAVEL_REDUCE_NONE) return RAVEL_OK;
-        return launch(k_distill_total, dim3(1), 1024, 0, st, 1, losses, R, a.count, out);
+        return launch(mean ? k_distill_total<true> : k_distill_total<false>, dim3(1), 1024, 0, st, 1, losses, a.live, R,
+                      out);
     });
 }
 
 int ravel_distill_topk_bwd(const void* logits, int64_t ld, const void* ids, int ids_dtype, const void* teacher,
                            int teacher_dtype, int64_t R, int64_t V, int64_t k, float temperature, float weight,
-                           int reduction, const float* stat, const uint32_t* count, const float* upstream,
+                           int reduction, const float* stat, const void* scratch, const float* upstream,
                            int grad_is_unit, void* grad, int dtype, void* stream) {
     RAVEL_TIMED("ravel_distill_topk_bwd", stream);
     DistillArgs a;
@@ -542,12 +548,12 @@ int ravel_distill_topk_bwd(const void* logits, int64_t ld, const void* ids, int 
     if (reduction < RAVEL_REDUCE_NONE || reduction > RAVEL_REDUCE_MEAN) return RAVEL_ERR_INVALID_ARG;
     if (R == 0) return RAVEL_OK;
     if (stat == nullptr || upstream == nullptr || grad == nullptr ||
-        (reduction == RAVEL_REDUCE_MEAN && count == nullptr) || (grad_is_unit && reduction == RAVEL_REDUCE_NONE))
+        (reduction == RAVEL_REDUCE_MEAN && scratch == nullptr) || (grad_is_unit && reduction == RAVEL_REDUCE_NONE))
         return RAVEL_ERR_INVALID_ARG;
     a.weight = weight;
     a.stat = reinterpret_cast<float2*>(const_cast<float*>(stat));
     a.grad = grad;
-    a.count = reduction == RAVEL_REDUCE_MEAN ? count : nullptr;
+    a.counts = reduction == RAVEL_REDUCE_MEAN ? static_cast<const unsigned int*>(scratch) : nullptr;
     a.up = upstream;
     a.up_rows = reduction == RAVEL_REDUCE_NONE;
     a.done = grad_is_unit;

@@ -9,7 +9,7 @@
 //
 // A row without a live entry has loss 0 and gradient 0 and is not counted by the mean.
 //
-//   k_distill_count  rows with a live entry (integers: any order gives the same sum).
+//   k_distill_count  rows with a live entry, counted before a gradient of the mean is written.
 //   k_distill        a block per row.  One pass over the logits keeps a running maximum and sum
 //                    (base 2: exp2 of one fused multiply-add per element); with GRAD a second pass
 //                    writes the gradient for upstream 1 while the row is still in L2, then the at
@@ -25,6 +25,8 @@
 
 namespace ravel {
 
+constexpr int DISTILL_COUNTS = 256;  // blocks of k_distill_count
+
 struct DistillArgs {
     const void* s;            // [R, V], rows lds apart
     const void* ids;          // [R, k] int32 or int64
@@ -32,7 +34,8 @@ struct DistillArgs {
     void* grad;               // [R, V] contiguous, or null
     float* losses;            // [R]
     float2* stat;             // [R] (m, l): m the largest s_v c, l = sum_v 2^(s_v c - m), c = log2(e) / tau
-    const unsigned int* count;  // rows counted by the mean, or null (sum, none)
+    unsigned char* live;      // [R] the row has a live entry, or null
+    const unsigned int* counts;  // [DISTILL_COUNTS] rows counted by the mean, in parts; null: sum, none
     const float* up;          // upstream gradient: one value (mean, sum) or [R]
     int up_rows;              // up has one value per row
     int done;                 // grad already holds the gradient of upstream 1
@@ -53,9 +56,9 @@ __device__ __forceinline__ bool distill_entry(const DistillArgs& a, int64_t row,
     return v >= 0 && !bad && t != -INFINITY;
 }
 
-// A block per 8 rows (a warp each).
+// counts[block] = the rows with a live entry among the block's (a warp per row).
 template <typename TT>
-__global__ void __launch_bounds__(256) k_distill_count(const DistillArgs a, unsigned int* count) {
+__global__ void __launch_bounds__(256) k_distill_count(const DistillArgs a, unsigned int* counts) {
     __shared__ unsigned int n;
     grid_wait();
     grid_trigger();
@@ -74,7 +77,16 @@ __global__ void __launch_bounds__(256) k_distill_count(const DistillArgs a, unsi
         if (__any_sync(0xffffffffu, any) && lane == 0) atomicAdd(&n, 1u);
     }
     __syncthreads();
-    if (threadIdx.x == 0 && n != 0u) atomicAdd(count, n);
+    if (threadIdx.x == 0) counts[blockIdx.x] = n;
+}
+
+// What the mean divides by, by one warp: all of it where a.counts is null.
+__device__ __forceinline__ float distill_counted(const DistillArgs& a) {
+    if (a.counts == nullptr) return 1.0f;
+    unsigned int n = 0u;
+    for (int i = threadIdx.x & 31; i < DISTILL_COUNTS; i += 32) n += a.counts[i];
+    n = __reduce_add_sync(0xffffffffu, n);
+    return fmaxf(static_cast<float>(n), 1.0f);
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -88,24 +100,25 @@ struct MaxSum {
     float m, l;
 };
 __device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.0f : m; }
-__device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b) {
-    const float m = fmaxf(a.m, b.m), r = finite_ref(m);
-    return {m, a.l * ex2(a.m - r) + b.l * ex2(b.m - r)};
+// The warp's (maximum, sum): the maxima first, then one rescaling of each lane's sum.
+__device__ __forceinline__ MaxSum warp_join(MaxSum v) {
+    float m = v.m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float l = v.l * ex2(v.m - finite_ref(m));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    return {m, l};
 }
-
 template <int TH>
 __device__ __forceinline__ MaxSum block_join(MaxSum v, MaxSum* red) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        MaxSum w = {__shfl_xor_sync(0xffffffffu, v.m, o), __shfl_xor_sync(0xffffffffu, v.l, o)};
-        v = join(v, w);
-    }
+    v = warp_join(v);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = red[0];
-#pragma unroll
-    for (int w = 1; w < TH / 32; ++w) v = join(v, red[w]);
-    return v;
+    const int lane = threadIdx.x & 31;
+    v = {-INFINITY, 0.0f};
+    if (lane < TH / 32) v = red[lane];
+    return warp_join(v);
 }
 
 // The row's elements as this block's threads share them: a head and a tail of single elements and
@@ -122,60 +135,54 @@ struct RowSplit {
     }
 };
 
-// Teacher entries into shared memory: p_j (0 for a dead entry) and ids (-1 for a dead one).  Every
-// thread gets whether the row has a live entry, and (thread 0 only) the loss.
+// Teacher entries into shared memory, by one warp: p_j (0 for a dead entry), ids (-1 for a dead one), and for the
+// loss d_j = log2 p_j - s[id_j] c.  Returns whether the row has a live entry.
 template <typename T, typename TT>
-__device__ __forceinline__ bool distill_teacher(const DistillArgs& a, int64_t row, MaxSum st, bool want_loss,
-                                                float* sp, int* sid, float* sred, float& loss) {
-    // warp 0 alone: k is small next to the vocabulary
-    if (threadIdx.x < 32) {
-        const int lane = threadIdx.x;
-        const float c = 1.4426950408889634f / a.tau;  // log2(e) / tau
-        float m = -INFINITY;
-        bool live = false, bad_any = false;
-        for (int j = lane; j < a.k; j += 32) {
-            int id;
-            float t;
-            bool bad;
-            const bool ok = distill_entry<TT>(a, row, j, id, t, bad);
-            bad_any |= bad;
-            sid[j] = ok ? id : -1;
-            sp[j] = ok ? t * c : -INFINITY;
-            live |= ok;
-            if (ok) m = fmaxf(m, t * c);
-        }
-        if (bad_any) atomicOr(a.err, RAVEL_DEVERR_INDEX);
-        live = __any_sync(0xffffffffu, live);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        float z = 0.0f;
-        for (int j = lane; j < a.k; j += 32)
-            if (sid[j] >= 0) z += ex2(sp[j] - m);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-        const float lz = m + __log2f(z), iz = 1.0f / z, ll = __log2f(st.l);
-        float acc = 0.0f;
-        for (int j = lane; j < a.k; j += 32) {
-            if (sid[j] < 0) {
-                sp[j] = 0.0f;
-                continue;
-            }
-            const float lp = sp[j] - lz, p = ex2(sp[j] - m) * iz;
-            if (want_loss && p != 0.0f) {
-                const float sv = as_float(static_cast<const T*>(a.s)[row * a.lds + sid[j]]);
-                acc += p * (lp + ll - fmaf(sv, c, -st.m));  // base 2; p = 0 contributes nothing
-            }
-            sp[j] = p;
-        }
-        if (want_loss) {
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-            loss = live ? acc * 0.6931471805599453f * a.tau * a.tau * a.weight : 0.0f;
-        }
-        if (lane == 0) sred[0] = live ? 1.0f : 0.0f;
+__device__ __forceinline__ bool distill_teacher(const DistillArgs& a, int64_t row, bool want_loss, float* sp, int* sid,
+                                                float* sd) {
+    const int lane = threadIdx.x & 31;
+    const float c = 1.4426950408889634f / a.tau;  // log2(e) / tau
+    float m = -INFINITY;
+    bool live = false, bad_any = false;
+    for (int j = lane; j < a.k; j += 32) {
+        int id;
+        float t;
+        bool bad;
+        const bool ok = distill_entry<TT>(a, row, j, id, t, bad);
+        bad_any |= bad;
+        sid[j] = ok ? id : -1;
+        sp[j] = ok ? t * c : -INFINITY;
+        if (want_loss) sd[j] = ok ? as_float(static_cast<const T*>(a.s)[row * a.lds + id]) * c : 0.0f;
+        live |= ok;
+        if (ok) m = fmaxf(m, t * c);
     }
-    __syncthreads();
-    return sred[0] != 0.0f;
+    if (bad_any) atomicOr(a.err, RAVEL_DEVERR_INDEX);
+    live = __any_sync(0xffffffffu, live);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float z = 0.0f;
+    for (int j = lane; j < a.k; j += 32)
+        if (sid[j] >= 0) z += ex2(sp[j] - m);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+    const float lz = m + __log2f(z), iz = 1.0f / z;
+    for (int j = lane; j < a.k; j += 32) {
+        const bool ok = sid[j] >= 0;
+        if (want_loss) sd[j] = sp[j] - lz - sd[j];
+        sp[j] = ok ? ex2(sp[j] - m) * iz : 0.0f;
+    }
+    return live;
+}
+
+// The row's loss from those and the student's (m, l), by the same warp.
+__device__ __forceinline__ float distill_loss(const DistillArgs& a, MaxSum st, const float* sp, const float* sd) {
+    const float lse = st.m + __log2f(st.l);
+    float acc = 0.0f;
+    for (int j = threadIdx.x & 31; j < a.k; j += 32)
+        if (sp[j] != 0.0f) acc += sp[j] * (sd[j] + lse);  // base 2; p = 0 contributes nothing
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+    return acc * 0.6931471805599453f * a.tau * a.tau * a.weight;
 }
 
 // grad row = gs * (2^(s c - m) / l - p at the entries); a row without a live entry gets zeros.
@@ -231,16 +238,25 @@ __device__ __forceinline__ void distill_grad_row(const DistillArgs& a, int64_t r
 template <typename T, typename TT, int TH, bool GRAD>
 __global__ void __launch_bounds__(TH) k_distill(const DistillArgs a) {
     constexpr int E = 16 / sizeof(T);
-    extern __shared__ float dyn[];  // p [k], ids [k]
+    extern __shared__ float dyn[];  // p [k], ids [k], d [k]
     __shared__ MaxSum red[TH / 32];
-    __shared__ float sred[1];
+    __shared__ float s_live, s_count;
     float* const sp = dyn;
     int* const sid = reinterpret_cast<int*>(dyn + a.k);
+    float* const sd = dyn + 2 * a.k;
     grid_wait();
     grid_trigger();
     const int64_t row = blockIdx.x;
     const T* const s = static_cast<const T*>(a.s) + row * a.lds;
     const float c = 1.4426950408889634f / a.tau;
+    // the teacher's part first: its chain of loads runs under the other warps' pass over the logits
+    if (threadIdx.x < 32) {
+        const bool live = distill_teacher<T, TT>(a, row, true, sp, sid, sd);
+        if (threadIdx.x == 0) s_live = live ? 1.0f : 0.0f;
+    } else if (GRAD && threadIdx.x < 64) {
+        const float n = distill_counted(a);
+        if (threadIdx.x == 32) s_count = n;
+    }
     const RowSplit<T> rs(s, a.V);
     MaxSum v = {-INFINITY, 0.0f};
     auto take = [&](float x) {
@@ -269,51 +285,60 @@ __global__ void __launch_bounds__(TH) k_distill(const DistillArgs a) {
     for (int i = threadIdx.x; i < rs.head; i += TH) take(as_float(s[i]));
     for (int i = rs.head + rs.vecs * E + threadIdx.x; i < a.V; i += TH) take(as_float(s[i]));
     v = block_join<TH>(v, red);
-    float loss = 0.0f;
-    const bool live = distill_teacher<T, TT>(a, row, v, true, sp, sid, sred, loss);
-    if (threadIdx.x == 0) {
-        a.losses[row] = loss;
-        if (a.stat != nullptr) a.stat[row] = make_float2(v.m, v.l);
+    const bool live = s_live != 0.0f;
+    if (threadIdx.x < 32) {
+        const float loss = live ? distill_loss(a, v, sp, sd) : 0.0f;
+        if (threadIdx.x == 0) {
+            a.losses[row] = loss;
+            if (a.live != nullptr) a.live[row] = live;
+            if (a.stat != nullptr) a.stat[row] = make_float2(v.m, v.l);
+        }
     }
-    if constexpr (GRAD) {
-        const float n = a.count != nullptr ? fmaxf(static_cast<float>(*a.count), 1.0f) : 1.0f;
-        distill_grad_row<T, TH>(a, row, v, a.weight * a.tau / n, live, sp, sid);
-    }
+    if constexpr (GRAD) distill_grad_row<T, TH>(a, row, v, a.weight * a.tau / s_count, live, sp, sid);
 }
 
 template <typename T, typename TT, int TH>
 __global__ void __launch_bounds__(TH) k_distill_bwd(const DistillArgs a) {
     extern __shared__ float dyn[];
-    __shared__ float sred[1];
+    __shared__ float s_live, s_count;
     float* const sp = dyn;
     int* const sid = reinterpret_cast<int*>(dyn + a.k);
     grid_wait();
     grid_trigger();
     if (a.done && *a.up == 1.0f) return;
-    const float n = a.count != nullptr ? fmaxf(static_cast<float>(*a.count), 1.0f) : 1.0f;
     for (int64_t row = blockIdx.x; row < a.R; row += gridDim.x) {
+        if (threadIdx.x < 32) {
+            const bool live = distill_teacher<T, TT>(a, row, false, sp, sid, nullptr);
+            if (threadIdx.x == 0) s_live = live ? 1.0f : 0.0f;
+        } else if (threadIdx.x < 64) {
+            const float n = distill_counted(a);
+            if (threadIdx.x == 32) s_count = n;
+        }
+        __syncthreads();
         const float2 f = a.stat[row];
-        const MaxSum st = {f.x, f.y};
-        float unused;
-        const bool live = distill_teacher<T, TT>(a, row, st, false, sp, sid, sred, unused);
-        distill_grad_row<T, TH>(a, row, st, a.up[a.up_rows ? row : 0] * a.weight * a.tau / n, live, sp, sid);
+        distill_grad_row<T, TH>(a, row, {f.x, f.y}, a.up[a.up_rows ? row : 0] * a.weight * a.tau / s_count,
+                                s_live != 0.0f, sp, sid);
         __syncthreads();
     }
 }
 
-// out = sum of the losses (/ count): one block, a fixed order.
-__global__ void __launch_bounds__(1024) k_distill_total(const float* __restrict__ losses, int64_t R,
-                                                        const unsigned int* __restrict__ count,
+// out = sum of the losses (MEAN: / the live rows): one block, a fixed order.
+template <bool MEAN>
+__global__ void __launch_bounds__(1024) k_distill_total(const float* __restrict__ losses,
+                                                        const unsigned char* __restrict__ live, int64_t R,
                                                         float* __restrict__ out) {
     __shared__ float2 red[64];
     int turn = 0;
     grid_wait();
     grid_trigger();
-    float s = 0.0f;
+    float s = 0.0f, n = 0.0f;  // at most R / 1024 rows a thread: exact
 #pragma unroll 4
-    for (int64_t i = threadIdx.x; i < R; i += 1024) s += losses[i];
-    s = group_sum2<32>(s, 0.0f, red, turn).x;
-    if (threadIdx.x == 0) out[0] = count != nullptr ? s / fmaxf(static_cast<float>(*count), 1.0f) : s;
+    for (int64_t i = threadIdx.x; i < R; i += 1024) {
+        s += losses[i];
+        if (MEAN && live[i]) n += 1.0f;
+    }
+    const float2 t = group_sum2<32>(s, n, red, turn);
+    if (threadIdx.x == 0) out[0] = MEAN ? t.x / fmaxf(t.y, 1.0f) : t.x;
 }
 
 }  // namespace ravel

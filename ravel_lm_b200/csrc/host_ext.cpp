@@ -469,7 +469,7 @@ at::Tensor layer_norm(const at::Tensor& x, const OptTensor& weight, const OptTen
 // The tensors of a distillation call, and its launch.
 struct DistillCall {
     Rows s;
-    at::Tensor ids, teacher, losses, stat, count, out;
+    at::Tensor ids, teacher, losses, stat, scratch, out;
     int64_t R, V, k;
     float tau, weight;
     int reduction, dtype;
@@ -487,15 +487,16 @@ struct DistillCall {
         const auto f32 = s.t.options().dtype(at::kFloat);
         losses = at::empty(rows_shape, f32);
         if (keep) stat = at::empty({R, 2}, f32);
-        if (reduction == RAVEL_REDUCE_MEAN) count = at::empty({1}, f32.dtype(at::kInt));
+        const size_t sb = reduction == RAVEL_REDUCE_MEAN ? ravel_distill_topk_scratch_bytes(R) : 0;
+        if (sb) scratch = bytes(sb, s.t);
         if (reduction != RAVEL_REDUCE_NONE) out = at::empty({}, f32);
         check_status("ravel_distill_topk_fwd",
                      ravel_distill_topk_fwd(s.t.data_ptr(), s.ld, ids.data_ptr(), ids_code(), teacher.data_ptr(),
                                             payload_code(teacher.scalar_type()), R, V, k, tau, weight, reduction,
                                             losses.data_ptr<float>(), keep ? stat.data_ptr<float>() : nullptr,
-                                            count.defined() ? reinterpret_cast<uint32_t*>(count.data_ptr<int>()) : nullptr,
                                             out.defined() ? out.data_ptr<float>() : nullptr,
-                                            grad.defined() ? grad.data_ptr() : nullptr, dtype, stream_of(s.t)));
+                                            grad.defined() ? grad.data_ptr() : nullptr, dtype,
+                                            sb ? scratch.data_ptr() : nullptr, sb, stream_of(s.t)));
         return reduction == RAVEL_REDUCE_NONE ? losses : out;
     }
 };
@@ -512,7 +513,7 @@ struct DistillTopk : public torch::autograd::Function<DistillTopk> {
         if (reduction != RAVEL_REDUCE_NONE && c.dtype != RAVEL_F16) unit = at::empty(logits.sizes(), c.s.t.options());
         const auto sizes = logits.sizes();
         at::Tensor loss = c.forward(sizes.slice(0, sizes.size() - 1), true, unit);
-        ctx->save_for_backward({c.s.t, c.ids, c.teacher, c.stat, c.count});
+        ctx->save_for_backward({c.s.t, c.ids, c.teacher, c.stat, c.scratch});
         if (unit.defined()) ctx->saved_data["unit"] = unit;
         ctx->saved_data["ld"] = c.s.ld;
         ctx->saved_data["shape"] = sizes.vec();
@@ -524,7 +525,7 @@ struct DistillTopk : public torch::autograd::Function<DistillTopk> {
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
-        const at::Tensor &s = saved[0], &ids = saved[1], &teacher = saved[2], &stat = saved[3], &count = saved[4];
+        const at::Tensor &s = saved[0], &ids = saved[1], &teacher = saved[2], &stat = saved[3], &scratch = saved[4];
         variable_list out(6);
         if (!grads[0].defined()) return out;
         const c10::cuda::CUDAGuard guard(s.device());
@@ -547,7 +548,7 @@ struct DistillTopk : public torch::autograd::Function<DistillTopk> {
                                    static_cast<float>(ctx->saved_data["tau"].toDouble()),
                                    static_cast<float>(ctx->saved_data["weight"].toDouble()),
                                    static_cast<int>(ctx->saved_data["reduction"].toInt()), stat.data_ptr<float>(),
-                                   count.defined() ? reinterpret_cast<const uint32_t*>(count.data_ptr<int>()) : nullptr,
+                                   scratch.defined() ? scratch.data_ptr() : nullptr,
                                    up.data_ptr<float>(), unit ? 1 : 0, grad.data_ptr(),
                                    payload_code(s.scalar_type()), stream_of(s)));
         out[0] = grad;
