@@ -266,17 +266,33 @@ int with_norm_plan(const NormPlan& p, F&& f) {
 // ------------------------------------------------------------------ distillation
 constexpr int64_t kDistillMaxK = 4096;
 
-// Threads of a row's block.
-int distill_threads(int64_t R, int64_t V, int dtype) {
+// How a row's block is made: threads, and vectors per thread held in registers (0: the row is read twice).  Rows up
+// to 8 KB are held by 128 threads, longer ones take 256 or, past 64 KB or when there are few rows, 512.  Measured with
+// the gradient (us): 16384 rows of 8 KB 84 held, 106 read twice; of 16 KB 143 held (8 vectors a thread), 133 read twice.
+struct DistillPlan {
+    int threads, held;
+};
+DistillPlan distill_plan(int64_t R, int64_t V, int dtype) {
     const int64_t bytes = V * esize(dtype);
-    if (bytes <= 4096) return 128;
-    return R < sm_count() || bytes > 65536 ? 512 : 256;
+    for (int nv : {1, 2, 4})
+        if (bytes <= 2048 * nv) return {128, nv};
+    return {R < sm_count() || bytes > 65536 ? 512 : 256, 0};
 }
 
 template <typename F>
-int with_threads(int th, F&& f) {
-    if (th == 128) return f(IC<128>{});
-    if (th == 256) return f(IC<256>{});
+int with_distill_plan(const DistillPlan& p, F&& f) {
+    switch (p.held) {
+        case 1: return f(IC<128>{}, IC<1>{});
+        case 2: return f(IC<128>{}, IC<2>{});
+        case 4: return f(IC<128>{}, IC<4>{});
+        default: return p.threads == 256 ? f(IC<256>{}, IC<0>{}) : f(IC<512>{}, IC<0>{});
+    }
+}
+
+template <typename F>
+int with_distill_threads(const DistillPlan& p, F&& f) {
+    if (p.threads == 128) return f(IC<128>{});
+    if (p.threads == 256) return f(IC<256>{});
     return f(IC<512>{});
 }
 
@@ -522,9 +538,10 @@ int ravel_distill_topk_fwd(const void* logits, int64_t ld, const void* ids, int 
         if (R > 0) {
             const int rc = with_float_type(dtype, [&](auto tv) -> int {
                 using T = decltype(tv);
-                return with_threads(distill_threads(R, V, dtype), [&](auto th) -> int {
-                    constexpr int TH = decltype(th)::value;
-                    const auto kern = grad != nullptr ? k_distill<T, TT, TH, true> : k_distill<T, TT, TH, false>;
+                return with_distill_plan(distill_plan(R, V, dtype), [&](auto th, auto nv) -> int {
+                    constexpr int TH = decltype(th)::value, NV = decltype(nv)::value;
+                    const auto kern =
+                        grad != nullptr ? k_distill<T, TT, TH, NV, true> : k_distill<T, TT, TH, NV, false>;
                     if (int e = set_smem(kern, smem)) return e;
                     return launch(kern, dim3(static_cast<unsigned>(R)), TH, smem, st, 1, a);
                 });
@@ -562,7 +579,7 @@ int ravel_distill_topk_bwd(const void* logits, int64_t ld, const void* ids, int 
         using TT = decltype(ttv);
         return with_float_type(dtype, [&](auto tv) -> int {
             using T = decltype(tv);
-            return with_threads(distill_threads(R, V, dtype), [&](auto th) -> int {
+            return with_distill_threads(distill_plan(R, V, dtype), [&](auto th) -> int {
                 constexpr int TH = decltype(th)::value;
                 const int64_t blocks = std::min<int64_t>(R, int64_t{sm_count()} * (2048 / TH));
                 return launch(k_distill_bwd<T, TT, TH>, dim3(static_cast<unsigned>(blocks)), TH,

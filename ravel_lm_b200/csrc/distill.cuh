@@ -12,8 +12,8 @@
 //   k_distill_count  rows with a live entry, counted before a gradient of the mean is written.
 //   k_distill        a block per row.  One pass over the logits keeps a running maximum and sum
 //                    (base 2: exp2 of one fused multiply-add per element); with GRAD a second pass
-//                    writes the gradient for upstream 1 while the row is still in L2, then the at
-//                    most k entries are written once more with their p, from float32.
+//                    writes the gradient for upstream 1 while the row is still in registers (up to 8 KB)
+//                    or L2, then the at most k entries are written once more with their p, from float32.
 //   k_distill_bwd    the second pass alone, for any upstream gradient.
 //   k_distill_total  the rows' losses added in a fixed order.
 // Bound by HBM: one read of the logits, and one write of the gradient.
@@ -185,10 +185,11 @@ __device__ __forceinline__ float distill_loss(const DistillArgs& a, MaxSum st, c
     return acc * 0.6931471805599453f * a.tau * a.tau * a.weight;
 }
 
-// grad row = gs * (2^(s c - m) / l - p at the entries); a row without a live entry gets zeros.
-template <typename T, int TH>
+// grad row = gs * (2^(s c - m) / l - p at the entries); a row without a live entry gets zeros.  The row's vectors are
+// in v (NV > 0: vector i * TH + thread in v[i]) or read again.
+template <typename T, int TH, int NV>
 __device__ __forceinline__ void distill_grad_row(const DistillArgs& a, int64_t row, MaxSum st, float gs, bool live,
-                                                 const float* sp, const int* sid) {
+                                                 const float* sp, const int* sid, const Pack<T, 16 / sizeof(T)>* v) {
     constexpr int E = 16 / sizeof(T);
     const T* const s = static_cast<const T*>(a.s) + row * a.lds;
     T* const d = static_cast<T*>(a.grad) + row * a.V;
@@ -205,15 +206,22 @@ __device__ __forceinline__ void distill_grad_row(const DistillArgs& a, int64_t r
         return;
     }
     const float gl = gs / st.l;
-    auto one = [&](T v) { return round_to<T>(gl * ex2(fmaf(as_float(v), c, -st.m))); };
+    auto one = [&](T x) { return round_to<T>(gl * ex2(fmaf(as_float(x), c, -st.m))); };
     if (same) {
-#pragma unroll 4
-        for (int i = threadIdx.x; i < rs.vecs; i += TH) {
+        auto put = [&](int i, const Pack<T, E>& x) {
             float f[E];
-            to_floats<T, E>(load_pack<T, E>(s + rs.head + i * E), f);
+            to_floats<T, E>(x, f);
 #pragma unroll
             for (int e = 0; e < E; ++e) f[e] = gl * ex2(fmaf(f[e], c, -st.m));
-            store_pack<T, E>(d + rs.head + i * E, from_floats<T, E>(f));
+            store_pack_stream<T, E>(d + rs.head + i * E, from_floats<T, E>(f));
+        };
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (threadIdx.x + i * TH < rs.vecs) put(threadIdx.x + i * TH, v[i]);
+        } else {
+#pragma unroll 4
+            for (int i = threadIdx.x; i < rs.vecs; i += TH) put(i, load_pack<T, E>(s + rs.head + i * E));
         }
         for (int i = threadIdx.x; i < rs.head; i += TH) d[i] = one(s[i]);
         for (int i = rs.head + rs.vecs * E + threadIdx.x; i < a.V; i += TH) d[i] = one(s[i]);
@@ -235,7 +243,8 @@ __device__ __forceinline__ void distill_grad_row(const DistillArgs& a, int64_t r
     }
 }
 
-template <typename T, typename TT, int TH, bool GRAD>
+// NV > 0: the row's vectors (at most NV * TH) stay in registers between the passes.
+template <typename T, typename TT, int TH, int NV, bool GRAD>
 __global__ void __launch_bounds__(TH) k_distill(const DistillArgs a) {
     constexpr int E = 16 / sizeof(T);
     extern __shared__ float dyn[];  // p [k], ids [k], d [k]
@@ -249,6 +258,13 @@ __global__ void __launch_bounds__(TH) k_distill(const DistillArgs a) {
     const int64_t row = blockIdx.x;
     const T* const s = static_cast<const T*>(a.s) + row * a.lds;
     const float c = 1.4426950408889634f / a.tau;
+    const RowSplit<T> rs(s, a.V);
+    Pack<T, E> held[NV > 0 ? NV : 1];
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (threadIdx.x + i * TH < rs.vecs) held[i] = load_pack<T, E>(s + rs.head + (threadIdx.x + i * TH) * E);
+    }
     // the teacher's part first: its chain of loads runs under the other warps' pass over the logits
     if (threadIdx.x < 32) {
         const bool live = distill_teacher<T, TT>(a, row, true, sp, sid, sd);
@@ -257,20 +273,10 @@ __global__ void __launch_bounds__(TH) k_distill(const DistillArgs a) {
         const float n = distill_counted(a);
         if (threadIdx.x == 32) s_count = n;
     }
-    const RowSplit<T> rs(s, a.V);
     MaxSum v = {-INFINITY, 0.0f};
-    auto take = [&](float x) {
-        const float x2 = x * c;
-        if (x2 > v.m) {
-            v.l *= ex2(v.m - x2);
-            v.m = x2;
-        }
-        v.l += ex2(fmaf(x, c, -finite_ref(v.m)));
-    };
-#pragma unroll 4
-    for (int i = threadIdx.x; i < rs.vecs; i += TH) {
+    auto add = [&](const Pack<T, E>& p) {
         float x[E], m = -INFINITY;
-        to_floats<T, E>(load_pack<T, E>(s + rs.head + i * E), x);
+        to_floats<T, E>(p, x);
 #pragma unroll
         for (int e = 0; e < E; ++e) m = fmaxf(m, x[e]);
         m *= c;
@@ -281,6 +287,22 @@ __global__ void __launch_bounds__(TH) k_distill(const DistillArgs a) {
         const float r = finite_ref(v.m);
 #pragma unroll
         for (int e = 0; e < E; ++e) v.l += ex2(fmaf(x[e], c, -r));
+    };
+    auto take = [&](float x) {
+        const float x2 = x * c;
+        if (x2 > v.m) {
+            v.l *= ex2(v.m - x2);
+            v.m = x2;
+        }
+        v.l += ex2(fmaf(x, c, -finite_ref(v.m)));
+    };
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (threadIdx.x + i * TH < rs.vecs) add(held[i]);
+    } else {
+#pragma unroll 4
+        for (int i = threadIdx.x; i < rs.vecs; i += TH) add(load_pack<T, E>(s + rs.head + i * E));
     }
     for (int i = threadIdx.x; i < rs.head; i += TH) take(as_float(s[i]));
     for (int i = rs.head + rs.vecs * E + threadIdx.x; i < a.V; i += TH) take(as_float(s[i]));
@@ -294,7 +316,7 @@ __global__ void __launch_bounds__(TH) k_distill(const DistillArgs a) {
             if (a.stat != nullptr) a.stat[row] = make_float2(v.m, v.l);
         }
     }
-    if constexpr (GRAD) distill_grad_row<T, TH>(a, row, v, a.weight * a.tau / s_count, live, sp, sid);
+    if constexpr (GRAD) distill_grad_row<T, TH, NV>(a, row, v, a.weight * a.tau / s_count, live, sp, sid, held);
 }
 
 template <typename T, typename TT, int TH>
@@ -316,8 +338,8 @@ __global__ void __launch_bounds__(TH) k_distill_bwd(const DistillArgs a) {
         }
         __syncthreads();
         const float2 f = a.stat[row];
-        distill_grad_row<T, TH>(a, row, {f.x, f.y}, a.up[a.up_rows ? row : 0] * a.weight * a.tau / s_count,
-                                s_live != 0.0f, sp, sid);
+        distill_grad_row<T, TH, 0>(a, row, {f.x, f.y}, a.up[a.up_rows ? row : 0] * a.weight * a.tau / s_count,
+                                   s_live != 0.0f, sp, sid, nullptr);
         __syncthreads();
     }
 }

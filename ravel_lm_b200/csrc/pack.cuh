@@ -56,6 +56,12 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, VEC>& v) {
     else
         *reinterpret_cast<Pack<T, VEC>*>(p) = v;
 }
+// Written once and not read again by the kernel: leaves the caches to what is.
+template <typename T, int VEC>
+__device__ __forceinline__ void store_pack_stream(T* p, const Pack<T, VEC>& v) {
+    static_assert(sizeof(T) * VEC == 16, "16-byte vectors");
+    __stcs(reinterpret_cast<uint4*>(p), *reinterpret_cast<const uint4*>(&v));
+}
 template <typename T, int VEC>
 __device__ __forceinline__ void to_floats(const Pack<T, VEC>& p, float* f) {
     if constexpr (sizeof(T) == 2 && VEC % 2 == 0) {

@@ -131,6 +131,26 @@ def test_step(R, V, k, dtype):
         assert torch.equal(distill_topk_loss(s, ids, t, temperature=2.0), loss.detach())
 
 
+# training steps of longer rows, around the lengths where the kernel's way changes; rows that start off 16 bytes;
+# repeated ids, every row dead
+@pytest.mark.parametrize("dtype,R,V,k", [
+    (torch.bfloat16, 700, 8192, 5), (torch.bfloat16, 301, 16887, 128), (torch.bfloat16, 160, 16896, 64),
+    (torch.bfloat16, 333, 32003, 31), (torch.bfloat16, 90, 65536, 64), (torch.bfloat16, 40, 131001, 33),
+    (torch.bfloat16, 20, 140000, 129), (torch.float32, 650, 4096, 1), (torch.float32, 300, 8443, 16),
+    (torch.float32, 200, 16001, 40), (torch.float32, 75, 50304, 100), (torch.float32, 9, 67500, 7),
+    (torch.float32, 3, 70000, 7)])
+def test_long_rows(dtype, R, V, k):
+    s, ids, t = make(R, V, k, dtype, seed=R + k)
+    for reduction, weight in (("mean", 1.0), ("sum", -0.5)):
+        loss, g = check(s, ids, t, 1.5, reduction, weight)
+        loss2, g2 = check(s, ids, t, 1.5, reduction, weight)
+        assert torch.equal(loss, loss2) and torch.equal(g, g2)
+    repeated = ids.clone()
+    repeated[:, : k // 2] = repeated[:, k // 2 : k // 2 * 2]
+    check(s, repeated, t, 1.0, "mean")
+    check(s, torch.full_like(ids, -1), t, 1.0, "mean")
+
+
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_reductions_temperatures_weights_and_upstream_gradients(dtype, reduction):
