@@ -48,6 +48,25 @@ int resident_clusters(const void* kernel, int size) {
     return n;
 }
 
+// Blocks per SM of a kernel without dynamic shared memory (queried once per kernel).
+int resident_blocks(const void* kernel, int threads) {
+    static std::mutex mu;
+    static std::map<std::pair<const void*, int>, int> known;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 1;
+    std::lock_guard<std::mutex> lock(mu);
+    const auto key = std::make_pair(kernel, dev);
+    const auto it = known.find(key);
+    if (it != known.end()) return it->second;
+    int n = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != cudaSuccess || n <= 0) {
+        (void)cudaGetLastError();
+        n = 1;
+    }
+    known[key] = n;
+    return n;
+}
+
 // ------------------------------------------------------------------ matrix product
 struct Operand {
     const void* p;
@@ -213,10 +232,6 @@ constexpr int64_t kNormMaxK = int64_t{1} << 30;
 
 int esize(int dtype) { return dtype == RAVEL_F32 ? 4 : 2; }
 
-#ifndef RAVEL_LN_BWD_MOST
-#define RAVEL_LN_BWD_MOST 1
-#endif
-
 // How a row of K elements is shared: W warps (1, 4, 16; 0: the wide kernels), NV vectors a lane.
 struct NormPlan {
     int vec, W, NV;
@@ -231,8 +246,8 @@ NormPlan plan_norm(int64_t M, int64_t K, int dtype, bool vec, bool backward) {
     for (int w : {1, 4, 16}) {
         const int64_t per = (units + 32 * w - 1) / (32 * w);
         if (per > most || (few && w < 16 && per > most / 4)) continue;
-        // the backward also accumulates two weight gradients per column
-        if (backward && w < 16 && per > RAVEL_LN_BWD_MOST * most / 4) continue;
+        // the backward also accumulates two weight gradients per column: one vector a lane where that can be
+        if (backward && w < 16 && per > most / 4) continue;
         int nv = most / 4;
         while (nv < per) nv *= 2;
         return {vec ? 1 : 0, w, nv};
@@ -240,11 +255,7 @@ NormPlan plan_norm(int64_t M, int64_t K, int dtype, bool vec, bool backward) {
     return {0, 0, 0};
 }
 
-int64_t norm_bwd_blocks(int64_t M, const NormPlan& p) {
-    const int64_t sms = sm_count();
-    if (p.W == 1) return std::max<int64_t>(1, std::min((M + LN_ROWS - 1) / LN_ROWS, sms * 4));
-    return std::max<int64_t>(1, std::min(M, p.W == 4 ? sms * 8 : sms * 2));
-}
+constexpr int kNormBwdBlocks = 8;  // blocks per SM at most (the backward's scratch)
 
 // f(VEC, W, NV as integral constants) for a plan with W > 0.
 template <typename T, typename F>
@@ -455,7 +466,7 @@ int ravel_layer_norm_fwd(const void* x, int64_t ldx, const void* weight, const v
 
 size_t ravel_layer_norm_scratch_bytes(int64_t M, int64_t K) {
     if (M < 0 || K <= 0) return 0;
-    return static_cast<size_t>(std::max<int64_t>(1, std::min<int64_t>(M, int64_t{sm_count()} * 8)) * 2 * K) *
+    return static_cast<size_t>(std::max<int64_t>(1, std::min<int64_t>(M, int64_t{sm_count()} * kNormBwdBlocks)) * 2 * K) *
            sizeof(float);
 }
 
@@ -483,8 +494,7 @@ int ravel_layer_norm_bwd(const void* x, int64_t ldx, const void* weight, const v
                      aligned16(grad_x) && aligned16(weight);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const NormPlan p = plan_norm(M, K, dtype, vec, true);
-    const int64_t blocks = p.W == 0 ? std::max<int64_t>(1, std::min<int64_t>(M, int64_t{sm_count()} * 2))
-                                    : norm_bwd_blocks(M, p);
+    int64_t blocks = std::max<int64_t>(1, std::min<int64_t>(M, int64_t{sm_count()} * 2));
     return with_float_type(dtype, [&](auto tv) -> int {
         using T = decltype(tv);
         int rc;
@@ -493,8 +503,11 @@ int ravel_layer_norm_bwd(const void* x, int64_t ldx, const void* weight, const v
         } else {
             rc = with_norm_plan<T>(p, [&](auto vc, auto wc, auto nc) -> int {
                 constexpr int W = decltype(wc)::value;
-                return launch(k_ln_bwd<T, decltype(vc)::value, W, decltype(nc)::value>,
-                              dim3(static_cast<unsigned>(blocks)), ln_threads<W>(), 0, st, 1, a);
+                const auto kern = k_ln_bwd<T, decltype(vc)::value, W, decltype(nc)::value>;
+                const int fit = std::min(kNormBwdBlocks, resident_blocks(reinterpret_cast<const void*>(kern), ln_threads<W>()));
+                blocks = std::max<int64_t>(1, std::min<int64_t>(W == 1 ? (M + LN_ROWS - 1) / LN_ROWS : M,
+                                                                int64_t{sm_count()} * fit));
+                return launch(kern, dim3(static_cast<unsigned>(blocks)), ln_threads<W>(), 0, st, 1, a);
             });
         }
         if (rc != RAVEL_OK || grad_weight == nullptr) return rc;

@@ -149,8 +149,14 @@ __global__ void __launch_bounds__(ln_threads<W>()) k_ln_fwd(const NormArgs a) {
     }
 }
 
+// Resident blocks asked of the backward's register allocation (its grid is what fits, so that no block waits for a
+// second wave: 131072 x 1024 bf16 took 200 us with 8 blocks an SM of which 7 fit, 157 with as many as fit).
+template <int VEC, int W, int NV> constexpr int ln_bwd_min_blocks() {
+    return NV * VEC <= 8 ? (W == 1 ? 3 : (W == 4 ? 8 : 2)) : 1;
+}
+
 template <typename T, int VEC, int W, int NV>
-__global__ void __launch_bounds__(ln_threads<W>()) k_ln_bwd(const NormArgs a) {
+__global__ void __launch_bounds__(ln_threads<W>(), ln_bwd_min_blocks<VEC, W, NV>()) k_ln_bwd(const NormArgs a) {
     constexpr int COLS = 32 * W * NV * VEC;
     __shared__ float2 red[2 * W];
     __shared__ float wsum[W == 1 ? 2 * COLS : 1];
@@ -166,11 +172,11 @@ __global__ void __launch_bounds__(ln_threads<W>()) k_ln_bwd(const NormArgs a) {
     const float inv_k = 1.0f / static_cast<float>(a.K);
     const int64_t first = W == 1 ? static_cast<int64_t>(blockIdx.x) * LN_ROWS + warp : blockIdx.x;
     const int64_t step = static_cast<int64_t>(gridDim.x) * (W == 1 ? LN_ROWS : 1);
-    for (int64_t row = first; row < a.M; row += step) {
+    Pack<T, VEC> xv[NV], yv[NV];
+    float mean = 0.0f, rstd = 0.0f;
+    auto load = [&](int64_t row) {
         const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
         const T* const gy = static_cast<const T*>(a.gy) + row * a.ldg;
-        const float mean = a.mean[row], rstd = a.rstd[row];
-        Pack<T, VEC> xv[NV], yv[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * 32 * W + lane) * VEC;
@@ -179,20 +185,30 @@ __global__ void __launch_bounds__(ln_threads<W>()) k_ln_bwd(const NormArgs a) {
                 yv[i] = load_pack<T, VEC>(gy + c);
             }
         }
+        mean = a.mean[row];
+        rstd = a.rstd[row];
+    };
+    if (first < a.M) load(first);
+    for (int64_t row = first; row < a.M; row += step) {
         float xh[NV * VEC], t[NV * VEC];  // (x - mean) rstd, dy g
+        const float mu = mean, rs = rstd;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            to_floats<T, VEC>(xv[i], xh + i * VEC);
+            to_floats<T, VEC>(yv[i], t + i * VEC);
+        }
+        if (row + step < a.M) load(row + step);  // in flight while this row is reduced and written
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             const int c = (i * 32 * W + lane) * VEC;
             if (c < a.K) {
-                to_floats<T, VEC>(xv[i], xh + i * VEC);
-                to_floats<T, VEC>(yv[i], t + i * VEC);
                 float w[VEC];
                 if (g != nullptr) to_floats<T, VEC>(load_pack<T, VEC>(g + c), w);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     const int k = i * VEC + e;
-                    xh[k] = (xh[k] - mean) * rstd;
+                    xh[k] = (xh[k] - mu) * rs;
                     dg[k] = fmaf(t[k], xh[k], dg[k]);
                     db[k] += t[k];
                     if (g != nullptr) t[k] *= w[e];
@@ -203,7 +219,7 @@ __global__ void __launch_bounds__(ln_threads<W>()) k_ln_bwd(const NormArgs a) {
         }
         const float2 s = group_sum2<W>(s1, s2, red, turn);
         if (a.out == nullptr) continue;
-        const float m1 = s.x * inv_k * rstd, m2 = s.y * inv_k * rstd;
+        const float m1 = s.x * inv_k * rs, m2 = s.y * inv_k * rs;
         T* const dx = static_cast<T*>(a.out) + row * a.K;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -212,7 +228,7 @@ __global__ void __launch_bounds__(ln_threads<W>()) k_ln_bwd(const NormArgs a) {
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     const int k = i * VEC + e;
-                    t[k] = fmaf(t[k], rstd, -m1) - xh[k] * m2;
+                    t[k] = fmaf(t[k], rs, -m1) - xh[k] * m2;
                 }
                 store_pack<T, VEC>(dx + c, from_floats<T, VEC>(t + i * VEC));
             }
