@@ -146,32 +146,18 @@ int launch_matmul(const Operand& A, const Operand& B, int64_t K, MatmulArgs a, c
     return launch(kern, dim3(static_cast<unsigned>(groups * size)), MM_THREADS, MM_SMEM, st, size, ma, mb, a);
 }
 
-constexpr int64_t kGemvRows = 4;
-
-// At most kGemvRows rows.  Warps per weight row: at least 16 warps an SM in all while every lane keeps
-// a few loads of its row.
+// One row.  Warps per weight row: at least 16 warps an SM in all while every lane keeps a few loads of its row.
 template <typename T>
 int launch_gemv(const Operand& X, const Operand& W, int64_t K, int act, const MatmulArgs& e, cudaStream_t st) {
     GemvArgs a;
-    a.x = X.p; a.w = W.p; a.ldx = X.ld; a.ldw = W.ld; a.K = K;
+    a.x = X.p; a.w = W.p; a.ldw = W.ld; a.K = K;
     a.act = act;
     a.e = e;
     int s = 1;
     while (s < GV_WARPS && e.N * s < static_cast<int64_t>(sm_count()) * 16 && K >= 512 * s) s *= 2;
-    auto rows = [&](auto sc) -> int {
-        constexpr int S = decltype(sc)::value;
-        const dim3 grid(static_cast<unsigned>((e.N + GV_WARPS / S - 1) / (GV_WARPS / S)));
-        switch (e.M) {
-            case 1: return launch(k_gemv<T, 1, S>, grid, 32 * GV_WARPS, 0, st, 1, a);
-            case 2: return launch(k_gemv<T, 2, S>, grid, 32 * GV_WARPS, 0, st, 1, a);
-            case 3: return launch(k_gemv<T, 3, S>, grid, 32 * GV_WARPS, 0, st, 1, a);
-            default: return launch(k_gemv<T, 4, S>, grid, 32 * GV_WARPS, 0, st, 1, a);
-        }
-    };
-    if (s == 1) return rows(IC<1>{});
-    if (s == 2) return rows(IC<2>{});
-    if (s == 4) return rows(IC<4>{});
-    return rows(IC<8>{});
+    const dim3 grid(static_cast<unsigned>((e.N + GV_WARPS / s - 1) / (GV_WARPS / s)));
+    const auto kern = s == 1 ? k_gemv<T, 1> : (s == 2 ? k_gemv<T, 2> : (s == 4 ? k_gemv<T, 4> : k_gemv<T, 8>));
+    return launch(kern, grid, 32 * GV_WARPS, 0, st, 1, a);
 }
 
 template <typename T, bool A_MN, bool B_MN, bool FULL, int ACT>
@@ -370,7 +356,7 @@ int ravel_matmul(const void* A, int64_t lda, int a_mn, const void* B, int64_t ld
         const Operand oa{A, lda, a_mn}, ob{B, ldb, b_mn};
         if (K > 0 && a_mn) return matmul_shape<T, true, true, false, RAVEL_ACT_NONE>(oa, ob, K, a, st);
         if (K > 0 && b_mn) return matmul_shape<T, false, true, false, RAVEL_ACT_NONE>(oa, ob, K, a, st);
-        if (K > 0 && M <= kGemvRows) return launch_gemv<T>(oa, ob, K, act, a, st);
+        if (K > 0 && M == 1) return launch_gemv<T>(oa, ob, K, act, a, st);
         return with_act(act, [&](auto av) -> int {
             constexpr int ACT = decltype(av)::value;
             if (K == 0)

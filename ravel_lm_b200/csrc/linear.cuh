@@ -24,8 +24,8 @@
 //                     workspace), each CTA finishing an equal share of the columns.  For few
 //                     rows (decoding), where the weights' bytes bound the call and one CTA per
 //                     column tile would leave most SMs idle.
-//   k_gemv          the forward of at most 4 rows: a warp (or 2, 4, 8 warps) per weight row, plain
-//                   16-byte loads, one multiply-add per weight and row.
+//   k_gemv          the forward of one row: a warp (or 2, 4, 8 warps) per weight row, plain 16-byte
+//                   loads, one multiply-add per weight.
 //   k_linear_dz     dz = dy * act'(z) in 16 bits (the operand of the two gradient products) and
 //                   per-block column sums of dz in float32 (the bias gradient) in one pass.
 //   k_col_reduce    those partial sums added in block order: deterministic, no atomics.
@@ -556,45 +556,40 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
     if (warp == 2) tmem_free<CG>(tmem, COLS);
 }
 
-// ------------------------------------------------------------------ few rows
+// ------------------------------------------------------------------ one row
 constexpr int GV_WARPS = 8;
 constexpr int GV_DEPTH = 8;  // 16-byte weight loads in flight per lane
 
 struct GemvArgs {
-    const void* x;       // [M, K], rows ldx apart
+    const void* x;       // [K]
     const void* w;       // [N, K], rows ldw apart; both 16-byte rows
-    int64_t ldx, ldw, K;
+    int64_t ldw, K;
     int act;
     MatmulArgs e;        // the epilogue
 };
 
-// MR rows of x against the weights' rows: S warps share a weight row's K, each lane taking
-// 16 bytes of it at a time, MR products per weight; the warp's (then the block's, in warp order)
-// partial sums are added and one lane finishes the element.
-template <typename T, int MR, int S>
+// S warps share a weight row's K, each lane taking 16 bytes of it at a time; the warp's (then the block's, in warp
+// order) partial sums are added and one lane finishes the element.  Bound by HBM: 8192 x 8192 in 24.9 us (82% of the
+// copy rate), 4096 x 4096 in 8.5 (the launch and the first loads' latency are 3).  Two rows and more repeat the
+// loads and conversions of x per weight (4 rows: 24.6 us at 4096 x 4096) and go to the tensor cores (9 us).
+template <typename T, int S>
 __global__ void __launch_bounds__(32 * GV_WARPS) k_gemv(const GemvArgs a) {
-    __shared__ float part[GV_WARPS][MR];
+    __shared__ float part[GV_WARPS];
     grid_wait();
     grid_trigger();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int64_t n = static_cast<int64_t>(blockIdx.x) * (GV_WARPS / S) + warp / S;
-    float acc[MR];
-#pragma unroll
-    for (int m = 0; m < MR; ++m) acc[m] = 0.0f;
+    float acc = 0.0f;
     if (n < a.e.N) {
         const T* const w = static_cast<const T*>(a.w) + n * a.ldw;
         const T* const x = static_cast<const T*>(a.x);
         const int64_t first = ((warp % S) * 32 + lane) * 8, step = S * 32 * 8;
         auto add = [&](const uint4& wv, int64_t k) {
-            float wf[8];
+            float wf[8], xf[8];
             unpack8<T>(wv, wf);
+            unpack8<T>(load8(x, k, a.K, true), xf);
 #pragma unroll
-            for (int m = 0; m < MR; ++m) {
-                float xf[8];
-                unpack8<T>(load8(x + m * a.ldx, k, a.K, true), xf);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) acc[m] = fmaf(wf[e], xf[e], acc[m]);
-            }
+            for (int e = 0; e < 8; ++e) acc = fmaf(wf[e], xf[e], acc);
         };
         int64_t k = first;
         for (; k + (GV_DEPTH - 1) * step + 8 <= a.K; k += GV_DEPTH * step) {
@@ -607,40 +602,26 @@ __global__ void __launch_bounds__(32 * GV_WARPS) k_gemv(const GemvArgs a) {
         for (; k < a.K; k += step) add(load8(w, k, a.K, true), k);
     }
 #pragma unroll
-    for (int m = 0; m < MR; ++m) {
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) acc[m] += __shfl_xor_sync(0xffffffffu, acc[m], o);
-    }
+    for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
     if constexpr (S > 1) {
-        if (lane == 0) {
-#pragma unroll
-            for (int m = 0; m < MR; ++m) part[warp][m] = acc[m];
-        }
+        if (lane == 0) part[warp] = acc;
         __syncthreads();
         if (warp % S != 0) return;
+        acc = 0.0f;
 #pragma unroll
-        for (int m = 0; m < MR; ++m) {
-            acc[m] = 0.0f;
-#pragma unroll
-            for (int i = 0; i < S; ++i) acc[m] += part[warp + i][m];
-        }
+        for (int i = 0; i < S; ++i) acc += part[warp + i];
     }
-    if (n >= a.e.N) return;
-#pragma unroll
-    for (int m = 0; m < MR; ++m) {
-        if (lane != m) continue;
-        float v = acc[m];
-        if (a.e.bias != nullptr) v += static_cast<float>(static_cast<const T*>(a.e.bias)[n]);
-        if (a.e.z != nullptr) static_cast<T*>(a.e.z)[m * a.e.ldz + n] = static_cast<T>(v);
-        switch (a.act) {
-            case RAVEL_ACT_RELU: v = act_fwd<RAVEL_ACT_RELU>(v); break;
-            case RAVEL_ACT_GELU: v = act_fwd<RAVEL_ACT_GELU>(v); break;
-            case RAVEL_ACT_SILU: v = act_fwd<RAVEL_ACT_SILU>(v); break;
-            default: break;
-        }
-        if (a.e.res != nullptr) v += static_cast<float>(static_cast<const T*>(a.e.res)[m * a.e.ldr + n]);
-        static_cast<T*>(a.e.y)[m * a.e.ldy + n] = static_cast<T>(v);
+    if (n >= a.e.N || lane != 0) return;
+    if (a.e.bias != nullptr) acc += static_cast<float>(static_cast<const T*>(a.e.bias)[n]);
+    if (a.e.z != nullptr) static_cast<T*>(a.e.z)[n] = static_cast<T>(acc);
+    switch (a.act) {
+        case RAVEL_ACT_RELU: acc = act_fwd<RAVEL_ACT_RELU>(acc); break;
+        case RAVEL_ACT_GELU: acc = act_fwd<RAVEL_ACT_GELU>(acc); break;
+        case RAVEL_ACT_SILU: acc = act_fwd<RAVEL_ACT_SILU>(acc); break;
+        default: break;
     }
+    if (a.e.res != nullptr) acc += static_cast<float>(static_cast<const T*>(a.e.res)[n]);
+    static_cast<T*>(a.e.y)[n] = static_cast<T>(acc);
 }
 
 // ------------------------------------------------------------------ the backward's elementwise pass
