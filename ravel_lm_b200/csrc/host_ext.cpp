@@ -209,6 +209,13 @@ void require_cuda(const at::Tensor& first, std::initializer_list<const OptTensor
     }
 }
 
+// The backward kernels have no derivative of their own: refuse create_graph rather than return gradients that
+// silently lack one.
+void once_differentiable(const char* op) {
+    if (at::GradMode::is_enabled())
+        throw std::runtime_error(std::string(op) + ": the backward pass is not differentiable (create_graph=True)");
+}
+
 int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 
 // A row-major matrix as the kernels take it: elements of a row adjacent, rows `ld` apart.
@@ -301,6 +308,7 @@ struct FusedLinear : public torch::autograd::Function<FusedLinear> {
         for (size_t d = 0; d + 1 < x_shape.size(); ++d) M *= x_shape[d];
         variable_list out(5);
         if (!grads[0].defined()) return out;
+        once_differentiable("fused_linear");
         const c10::cuda::CUDAGuard guard(x2.device());
         if (need_r) out[3] = grads[0];
         if (!need_x && !need_w && !need_b) return out;
@@ -420,6 +428,7 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
         const bool need_x = ctx->needs_input_grad(0), need_w = has_w && ctx->needs_input_grad(1);
         const bool need_b = has_b && ctx->needs_input_grad(has_w ? 2 : 1);
         variable_list out(4);
+        once_differentiable("layer_norm");
         if (!grads[0].defined() || !(need_x || need_w || need_b)) return out;
         const c10::cuda::CUDAGuard guard(x2.device());
         const int64_t M = x2.size(0), K = x2.size(1);
@@ -528,6 +537,7 @@ struct DistillTopk : public torch::autograd::Function<DistillTopk> {
         const at::Tensor &s = saved[0], &ids = saved[1], &teacher = saved[2], &stat = saved[3], &scratch = saved[4];
         variable_list out(6);
         if (!grads[0].defined()) return out;
+        once_differentiable("distill_topk_loss");
         const c10::cuda::CUDAGuard guard(s.device());
         // The forward's gradient is given away once; a second backward pass writes a new one.
         at::Tensor grad;

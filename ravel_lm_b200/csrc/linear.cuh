@@ -11,13 +11,12 @@
 //                   128-byte-swizzled stages, warp 1 issues the tcgen05.mma, warps 4-11 turn
 //                   accumulators into outputs.  Three shapes of it:
 //                   - pairs (CG 2): a cluster of two CTAs computes 256 x BN outputs (BN 256 or
-//                     128), each CTA holding 128 rows of A and BN / 2 of B per chunk: 32 KB feed
-//                     128 x 256 outputs per SM.  An SM takes in at most 64 bytes a clock from L2,
-//                     so the bytes per output decide: a 64-deep chunk of 256 x 256 takes 600 clocks
-//                     (512 at the tensor peak), one of 128 x 128 per SM the same 600.  Two
-//                     accumulators let the epilogue of one tile run under the products of the next;
-//                     the grid is persistent.
-//                   - single (CG 1): 128 x BN outputs per CTA (BN 128, 64 or 32), same structure.
+//                     128), each CTA holding 128 rows of A and BN / 2 of B per chunk, so that 32 KB
+//                     feed 128 x 256 outputs per SM: a 64-deep chunk takes 0.28 us (0.27 at the
+//                     tensor peak).  Two accumulators let the epilogue of one tile run under the
+//                     products of the next; the grid is persistent.
+//                   - single (CG 1): 128 x BN outputs per CTA (BN 128, 64 or 32; 0.16, 0.135 and
+//                     0.125 us a chunk, the last two bound by the issuing thread), same structure.
 //                   - split (CG 1, clusters of 2, 4 or 8): the CTAs of a cluster share one
 //                     output tile and divide k; their partial sums meet through distributed
 //                     shared memory, added in rank order (deterministic, one launch, no
@@ -147,16 +146,10 @@ __device__ __forceinline__ float act_grad(float z) {
 constexpr int MM_BM = 128;         // rows of A per CTA
 constexpr int MM_BK = 64;          // elements per chunk: one 128-byte swizzle row
 constexpr int MM_MAX_STAGES = 16;
-// Chunks per stage.  Issuing a stage (a wait, its products, a commit) takes one thread some 250 clocks and 40 a
-// product: below the 512 clocks of a pair's 256 x 256 chunk, above the 256 and fewer of a single CTA's, whose
+// Chunks per stage.  Handing a stage over (a wait, a commit) takes the issuing thread some 250 clocks and a product
+// 40: together below the 512 clocks of a pair's 256 x 256 chunk, above the 256 and fewer of a single CTA's, whose
 // stages therefore hold two chunks.
-#ifndef RAVEL_MM_KS2
-#define RAVEL_MM_KS2 1
-#endif
-#ifndef RAVEL_MM_KS1
-#define RAVEL_MM_KS1 2
-#endif
-__host__ __device__ constexpr int mm_ksub(int cg) { return cg == 2 ? RAVEL_MM_KS2 : RAVEL_MM_KS1; }
+__host__ __device__ constexpr int mm_ksub(int cg) { return cg == 2 ? 1 : 2; }
 constexpr uint32_t MM_RING = 6 * 32768;  // bytes of operand stages
 constexpr int MM_EPI_WARPS = 8;
 constexpr int MM_THREADS = 128 + 32 * MM_EPI_WARPS;
@@ -186,8 +179,7 @@ struct MatmulArgs {
     const unsigned int* wait_limit;
 };
 
-// The barriers order tensor-memory and asynchronous-proxy accesses only, so every wait has the default
-// scope; an acquire at cluster scope here cost 600 clocks a chunk whatever the tile.
+// The barriers order tensor-memory and asynchronous-proxy accesses only: every wait has the default scope.
 __device__ __forceinline__ bool mm_wait(uint32_t bar, uint32_t parity, uint32_t limit, volatile int* abort) {
     for (uint32_t it = 0; it < limit; ++it) {
         if (mbar_try_wait(bar, parity)) return true;
@@ -627,7 +619,7 @@ __global__ void __launch_bounds__(32 * GV_WARPS) k_gemv(const GemvArgs a) {
 // ------------------------------------------------------------------ the backward's elementwise pass
 constexpr int DZ_COLS = 256;   // columns per block: 32 lanes x 8
 constexpr int DZ_WARPS = 8;    // rows per block at a time
-constexpr int DZ_ROWS = 4;     // rows per warp whose loads are in flight together
+constexpr int DZ_ROWS = 2;     // rows per warp whose loads are in flight together
 
 struct DzArgs {
     int64_t M, N, ldg, ldz, ldd;
@@ -639,9 +631,11 @@ struct DzArgs {
     int vec_g, vec_z, vec_d;
 };
 
-// Bound by HBM: reads dy and z, writes dz, 6 bytes an element.
+// Reads dy and z, writes dz, 6 bytes an element: 16384 x 8192 with gelu in 158 us, 78% of the copy rate (two rows in
+// flight and four blocks an SM; four rows and three blocks 164).  The derivative's 20 instructions an element keep the
+// issue slots half busy.
 template <typename T, int ACT>
-__global__ void __launch_bounds__(32 * DZ_WARPS, 3) k_linear_dz(const DzArgs a) {
+__global__ void __launch_bounds__(32 * DZ_WARPS, 4) k_linear_dz(const DzArgs a) {
     __shared__ float sums[DZ_WARPS][DZ_COLS];
     grid_wait();
     grid_trigger();

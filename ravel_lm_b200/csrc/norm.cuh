@@ -188,16 +188,23 @@ __global__ void __launch_bounds__(ln_threads<W>(), ln_bwd_min_blocks<VEC, W, NV>
         mean = a.mean[row];
         rstd = a.rstd[row];
     };
+    // Rows of up to 16 elements a lane keep their floats between the passes, and the next row's loads fly
+    // meanwhile; longer ones keep the elements as loaded and convert them twice (registers: 4 vectors of 16-bit
+    // elements a lane spilled 750 bytes).
+    constexpr bool KEEP = NV * VEC <= 16;
+    float xh[KEEP ? NV * VEC : VEC], t[KEEP ? NV * VEC : VEC];  // (x - mean) rstd, dy g
+    auto convert = [&](int i, float* xf, float* tf) {
+        to_floats<T, VEC>(xv[i], xf);
+        to_floats<T, VEC>(yv[i], tf);
+    };
     if (first < a.M) load(first);
     for (int64_t row = first; row < a.M; row += step) {
-        float xh[NV * VEC], t[NV * VEC];  // (x - mean) rstd, dy g
         const float mu = mean, rs = rstd;
+        if constexpr (KEEP) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            to_floats<T, VEC>(xv[i], xh + i * VEC);
-            to_floats<T, VEC>(yv[i], t + i * VEC);
+            for (int i = 0; i < NV; ++i) convert(i, xh + i * VEC, t + i * VEC);
+            if (row + step < a.M) load(row + step);  // in flight while this row is reduced and written
         }
-        if (row + step < a.M) load(row + step);  // in flight while this row is reduced and written
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -205,34 +212,48 @@ __global__ void __launch_bounds__(ln_threads<W>(), ln_bwd_min_blocks<VEC, W, NV>
             if (c < a.K) {
                 float w[VEC];
                 if (g != nullptr) to_floats<T, VEC>(load_pack<T, VEC>(g + c), w);
+                if constexpr (!KEEP) convert(i, xh, t);
+                float* const xf = xh + (KEEP ? i * VEC : 0);
+                float* const tf = t + (KEEP ? i * VEC : 0);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) {
                     const int k = i * VEC + e;
-                    xh[k] = (xh[k] - mu) * rs;
-                    dg[k] = fmaf(t[k], xh[k], dg[k]);
-                    db[k] += t[k];
-                    if (g != nullptr) t[k] *= w[e];
-                    s1 += t[k];
-                    s2 = fmaf(t[k], xh[k], s2);
+                    xf[e] = (xf[e] - mu) * rs;
+                    dg[k] = fmaf(tf[e], xf[e], dg[k]);
+                    db[k] += tf[e];
+                    if (g != nullptr) tf[e] *= w[e];
+                    s1 += tf[e];
+                    s2 = fmaf(tf[e], xf[e], s2);
                 }
             }
         }
         const float2 s = group_sum2<W>(s1, s2, red, turn);
-        if (a.out == nullptr) continue;
-        const float m1 = s.x * inv_k * rs, m2 = s.y * inv_k * rs;
-        T* const dx = static_cast<T*>(a.out) + row * a.K;
+        if (a.out != nullptr) {
+            const float m1 = s.x * inv_k * rs, m2 = s.y * inv_k * rs;
+            T* const dx = static_cast<T*>(a.out) + row * a.K;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int c = (i * 32 * W + lane) * VEC;
-            if (c < a.K) {
+            for (int i = 0; i < NV; ++i) {
+                const int c = (i * 32 * W + lane) * VEC;
+                if (c < a.K) {
+                    float* const xf = xh + (KEEP ? i * VEC : 0);
+                    float* const tf = t + (KEEP ? i * VEC : 0);
+                    if constexpr (!KEEP) {
+                        convert(i, xh, t);
+                        float w[VEC];
+                        if (g != nullptr) to_floats<T, VEC>(load_pack<T, VEC>(g + c), w);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    const int k = i * VEC + e;
-                    t[k] = fmaf(t[k], rs, -m1) - xh[k] * m2;
+                        for (int e = 0; e < VEC; ++e) {
+                            xf[e] = (xf[e] - mu) * rs;
+                            if (g != nullptr) tf[e] *= w[e];
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) tf[e] = fmaf(tf[e], rs, -m1) - xf[e] * m2;
+                    store_pack<T, VEC>(dx + c, from_floats<T, VEC>(tf));
                 }
-                store_pack<T, VEC>(dx + c, from_floats<T, VEC>(t + i * VEC));
             }
         }
+        if (!KEEP && row + step < a.M) load(row + step);
     }
     if (a.part == nullptr) return;
     float* const part = a.part + static_cast<int64_t>(blockIdx.x) * 2 * a.K;

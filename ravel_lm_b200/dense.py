@@ -18,7 +18,7 @@ divide the contraction over a cluster of CTAs.
 Leading dimensions are arbitrary and may be strided or empty.  Rows that TMA
 cannot read in place (a pitch or an address that is no multiple of 16 bytes)
 are copied once to a padded pitch.  Every result is deterministic.  There is no
-CPU path.
+CPU path, and no second derivative (``create_graph`` is refused).
 """
 from __future__ import annotations
 

@@ -318,3 +318,6 @@ def test_refusals():
         fused_linear(x.cpu(), w.cpu())
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         fused_linear(x, w, b.cpu())
+    xs = x.clone().requires_grad_(True)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(fused_linear(xs, w, b).sum(), xs, create_graph=True)

@@ -378,3 +378,5 @@ def test_refusals():
         distill_topk_loss(s.cpu(), ids.cpu(), t.cpu())
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         distill_topk_loss(s, ids.cpu(), t)
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(distill_topk_loss(s, ids, t), s, create_graph=True)

@@ -244,3 +244,5 @@ def test_refusals():
         layer_norm(x.cpu())
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         layer_norm(x, w.cpu())
+    with pytest.raises(RuntimeError, match="not differentiable"):
+        torch.autograd.grad(layer_norm(x, w, b).sum(), x, create_graph=True)
