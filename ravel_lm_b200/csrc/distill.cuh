@@ -25,6 +25,10 @@
 
 namespace ravel {
 
+// Rows longer than this are dropped from L2 as the second pass reads them: the rows in flight (8 or 4 an SM) then
+// take more than half of it, and a third of the second reads went to memory.  With the gradient, us without and with:
+// 8192 rows of 128 KB 468 / 438, 4096 of 196 KB 392 / 344, 8192 of 62 KB 230 / 217, 16384 of 32 KB 206 / 223.
+constexpr int64_t DISTILL_DROP_BYTES = 48 * 1024;
 constexpr int DISTILL_COUNTS = 256;  // blocks of k_distill_count
 
 struct DistillArgs {
@@ -219,6 +223,9 @@ __device__ __forceinline__ void distill_grad_row(const DistillArgs& a, int64_t r
 #pragma unroll
             for (int i = 0; i < NV; ++i)
                 if (threadIdx.x + i * TH < rs.vecs) put(threadIdx.x + i * TH, v[i]);
+        } else if (static_cast<int64_t>(a.V) * sizeof(T) > DISTILL_DROP_BYTES) {
+#pragma unroll 4
+            for (int i = threadIdx.x; i < rs.vecs; i += TH) put(i, load_pack_last<T, E>(s + rs.head + i * E));
         } else {
 #pragma unroll 4
             for (int i = threadIdx.x; i < rs.vecs; i += TH) put(i, load_pack<T, E>(s + rs.head + i * E));

@@ -56,6 +56,18 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, VEC>& v) {
     else
         *reinterpret_cast<Pack<T, VEC>*>(p) = v;
 }
+// The last read of a row that was read before: its lines may leave L2 first.
+template <typename T, int VEC>
+__device__ __forceinline__ Pack<T, VEC> load_pack_last(const T* p) {
+    static_assert(sizeof(T) * VEC == 16, "16-byte vectors");
+    uint64_t policy;
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+    uint4 v;
+    asm volatile("ld.global.nc.L2::cache_hint.v4.u32 {%0, %1, %2, %3}, [%4], %5;"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p), "l"(policy));
+    return *reinterpret_cast<const Pack<T, VEC>*>(&v);
+}
 // Written once and not read again by the kernel: leaves the caches to what is.
 template <typename T, int VEC>
 __device__ __forceinline__ void store_pack_stream(T* p, const Pack<T, VEC>& v) {
