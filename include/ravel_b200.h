@@ -354,11 +354,14 @@ size_t ravel_linear_dz_scratch_bytes(int64_t M, int64_t N);
  * dz = grad_y * act'(z) over [M, N] (rows ldg, ldz and ldd apart), and
  * grad_bias[n] = sum_m dz[m][n] from the unrounded products (deterministic: no
  * atomics).  dz or grad_bias may be NULL; z is not read for RAVEL_ACT_NONE;
- * scratch is needed for grad_bias only.
+ * scratch is needed for grad_bias only.  x [M, K], weight [N, K] (16-byte rows) and
+ * bias are what z was made of: for RAVEL_ACT_RELU the sums whose sign the tensor
+ * cores' rounding leaves in doubt are added up again in float32 (x NULL: z's sign
+ * stands); other activations do not read them.
  */
 int ravel_linear_dz(const void* grad_y, int64_t ldg, const void* z, int64_t ldz, int act, void* dz, int64_t ldd,
-                    void* grad_bias, int64_t M, int64_t N, int dtype, void* scratch, size_t scratch_bytes,
-                    void* stream);
+                    void* grad_bias, int64_t M, int64_t N, const void* x, int64_t ldx, const void* weight, int64_t ldw,
+                    const void* bias, int64_t K, int dtype, void* scratch, size_t scratch_bytes, void* stream);
 
 /* rows x cols 16-bit elements from row pitch ld to row pitch ldd (elements). */
 int ravel_pad_rows(const void* src, int64_t ld, int64_t rows, int64_t cols, void* dst, int64_t ldd, int dtype,

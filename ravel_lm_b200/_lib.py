@@ -78,8 +78,8 @@ SIGNATURES = {
     "ravel_matmul": (_c_int, [_c_vp, _c_i64, _c_int, _c_vp, _c_i64, _c_int] + [_c_i64] * 3 +
                      [_c_vp, _c_vp, _c_i64, _c_int, _c_vp, _c_i64, _c_vp, _c_i64, _c_int, _c_vp]),
     "ravel_linear_dz_scratch_bytes": (_c_sz, [_c_i64, _c_i64]),
-    "ravel_linear_dz": (_c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_int, _c_vp, _c_i64, _c_vp, _c_i64, _c_i64, _c_int,
-                                 _c_vp, _c_sz, _c_vp]),
+    "ravel_linear_dz": (_c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_int, _c_vp, _c_i64, _c_vp, _c_i64, _c_i64] +
+                        [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_int, _c_vp, _c_sz, _c_vp]),
     "ravel_pad_rows": (_c_int, [_c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_int, _c_vp]),
     "ravel_layer_norm_fwd": (_c_int, [_c_vp, _c_i64, _c_vp, _c_vp, ctypes.c_float, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64,
                                       _c_int, _c_vp]),

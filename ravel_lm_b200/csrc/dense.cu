@@ -80,8 +80,9 @@ struct Plan {
 
 // The launch shape, by an estimate of each one's time in microseconds: a launch's fixed part plus, per wave
 // of tiles, the larger of a tile's chunks and its epilogue (which runs under the next tile's chunks).  Clusters that
-// split k pay their setup and the exchange of sums per tile; clusters of 4 and 8 fill the SMs less well (35 and 16
-// of them are resident).  Measured (graph replays, outputs 128 x 4096, k = 64 / 1024 / 4096 / 8192, us):
+// split k pay their setup and the exchange of sums per tile; clusters of 4 fill the SMs less well (35 of them are
+// resident), and clusters of 8 (16 resident) were slower at every size (24 x 2048 outputs, k 8192: 17.8 us against
+// 11.1 with 4).  Measured (graph replays, outputs 128 x 4096, k = 64 / 1024 / 4096 / 8192, us):
 //   single 32: 3.5 / 5.3 / 11.6 / 21.3    single 64: 3.5 / 5.5 / 12.2 / 21.2    single 128: 4.4 / 6.8 / 14.6 / 31.6
 //   pairs 128: 4.4 / 6.7 / 13.7 / 23.8    pairs 256: 6.0 / 10.3 / 23.6 / 41.8
 //   split 2: - / 8.4 / 12.5 / 19.7        split 4: - / 10.7 / 13.5 / 17.4
@@ -106,9 +107,9 @@ Plan plan_matmul(int64_t M, int64_t N, int64_t K, bool b_mn) {
         const double us = k.fixed + waves(128 * k.cg, k.bn, std::floor(sms / k.cg)) * std::max(kc * k.chunk, k.epilogue);
         if (us < cost) cost = us, best = {k.cg, k.bn, 1};
     }
-    for (int s = 2; s <= 8; s *= 2) {
+    for (int s = 2; s <= 4; s *= 2) {
         if (kc < 4 * s) break;
-        const double slots = s == 2 ? std::floor(sms / 2) : (s == 4 ? std::floor(sms * 35 / 148) : std::floor(sms * 16 / 148));
+        const double slots = s == 2 ? std::floor(sms / 2) : std::floor(sms * 35 / 148);
         const double us = 1.2 + waves(128, 128, slots) * (std::ceil(kc / s) * 0.160 + 5.0 + 0.5 * s);
         if (us < cost) cost = us, best = {1, 128, s};
     }
@@ -223,17 +224,17 @@ struct NormPlan {
     int vec, W, NV;
 };
 
-NormPlan plan_norm(int64_t M, int64_t K, int dtype, bool vec, bool backward) {
+NormPlan plan_norm(int64_t M, int64_t K, int dtype, bool vec) {
     const int64_t units = vec ? K / (16 / esize(dtype)) : K;
     const int most = vec ? 4 : 16;  // vectors, or single elements, of a row in a lane's registers
-    // Rows for every SM: as few warps per row as hold it (shuffles alone add up a warp's row).
+    // Rows for every SM: as few warps per row as hold it (shuffles alone add up a warp's row, and a row's fixed work
+    // is shared by more elements).  Backward, us with 1 and with 4 warps a row: 131072 x 1024 bf16 151 / 158, 8192 x
+    // 256 float32 9.2 / 11.4; with 4 and with 16: 16384 x 4096 bf16 90 / 98.
     // Fewer rows: more warps per row, for a shorter chain.
     const bool few = M < static_cast<int64_t>(sm_count()) * 8;
     for (int w : {1, 4, 16}) {
         const int64_t per = (units + 32 * w - 1) / (32 * w);
         if (per > most || (few && w < 16 && per > most / 4)) continue;
-        // the backward also accumulates two weight gradients per column: one vector a lane where that can be
-        if (backward && w < 16 && per > most / 4) continue;
         int nv = most / 4;
         while (nv < per) nv *= 2;
         return {vec ? 1 : 0, w, nv};
@@ -372,8 +373,8 @@ size_t ravel_linear_dz_scratch_bytes(int64_t M, int64_t N) {
 }
 
 int ravel_linear_dz(const void* grad_y, int64_t ldg, const void* z, int64_t ldz, int act, void* dz, int64_t ldd,
-                    void* grad_bias, int64_t M, int64_t N, int dtype, void* scratch, size_t scratch_bytes,
-                    void* stream) {
+                    void* grad_bias, int64_t M, int64_t N, const void* x, int64_t ldx, const void* weight, int64_t ldw,
+                    const void* bias, int64_t K, int dtype, void* scratch, size_t scratch_bytes, void* stream) {
     RAVEL_TIMED("ravel_linear_dz", stream);
     if (M < 0 || N < 0 || act < RAVEL_ACT_NONE || act > RAVEL_ACT_SILU) return RAVEL_ERR_INVALID_ARG;
     if (dtype != RAVEL_BF16 && dtype != RAVEL_F16) return RAVEL_ERR_UNSUPPORTED;
@@ -381,6 +382,9 @@ int ravel_linear_dz(const void* grad_y, int64_t ldg, const void* z, int64_t ldz,
     if (N == 0 || (M == 0 && grad_bias == nullptr) || (dz == nullptr && grad_bias == nullptr)) return RAVEL_OK;
     if (M > 0 && (grad_y == nullptr || ldg < N || (act != RAVEL_ACT_NONE && (z == nullptr || ldz < N)) ||
                   (dz != nullptr && ldd < N)))
+        return RAVEL_ERR_INVALID_ARG;
+    if (x != nullptr && (weight == nullptr || K < 0 || (M > 1 && ldx < K) || (N > 1 && ldw < K) ||
+                         !vec16(x, M > 1 ? ldx * 2 : 0) || !vec16(weight, N > 1 ? ldw * 2 : 0)))
         return RAVEL_ERR_INVALID_ARG;
     if (grad_bias != nullptr && (scratch == nullptr || scratch_bytes < ravel_linear_dz_scratch_bytes(M, N)))
         return RAVEL_ERR_WORKSPACE;
@@ -390,6 +394,10 @@ int ravel_linear_dz(const void* grad_y, int64_t ldg, const void* z, int64_t ldz,
     const int64_t blocks = dz_row_blocks(M, N);
     a.M = M; a.N = N; a.ldg = ldg; a.ldz = ldz; a.ldd = ldd;
     a.gy = grad_y; a.z = z; a.dz = dz;
+    if (act == RAVEL_ACT_RELU && K > 0) {
+        a.x = x; a.w = weight; a.bias = bias;
+        a.ldx = ldx; a.ldw = ldw; a.K = K;
+    }
     a.part = grad_bias != nullptr ? static_cast<float*>(scratch) : nullptr;
     a.rows = std::max<int64_t>(1, (M + blocks - 1) / blocks);
     a.vec_g = vec16(grad_y, ldg * 2);
@@ -435,7 +443,7 @@ int ravel_layer_norm_fwd(const void* x, int64_t ldx, const void* weight, const v
     const bool vec = (K * es) % 16 == 0 && vec16(x, M > 1 ? ldx * es : 0) && aligned16(y) && aligned16(weight) &&
                      aligned16(bias);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const NormPlan p = plan_norm(M, K, dtype, vec, false);
+    const NormPlan p = plan_norm(M, K, dtype, vec);
     return with_float_type(dtype, [&](auto tv) -> int {
         using T = decltype(tv);
         if (p.W == 0) {
@@ -479,7 +487,7 @@ int ravel_layer_norm_bwd(const void* x, int64_t ldx, const void* weight, const v
     const bool vec = (K * es) % 16 == 0 && vec16(x, M > 1 ? ldx * es : 0) && vec16(grad_y, M > 1 ? ldg * es : 0) &&
                      aligned16(grad_x) && aligned16(weight);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const NormPlan p = plan_norm(M, K, dtype, vec, true);
+    const NormPlan p = plan_norm(M, K, dtype, vec);
     int64_t blocks = std::max<int64_t>(1, std::min<int64_t>(M, int64_t{sm_count()} * 2));
     return with_float_type(dtype, [&](auto tv) -> int {
         using T = decltype(tv);

@@ -281,7 +281,9 @@ struct FusedLinear : public torch::autograd::Function<FusedLinear> {
         at::Tensor z;
         at::Tensor y = linear_forward(x2, w2, M, K, N, bias, residual, static_cast<int>(act), shape,
                                       keep_z ? &z : nullptr);
-        ctx->save_for_backward({x2.t, w2.t, z});
+        // the backward of relu settles the signs of sums near zero, bias included
+        const bool keep_b = act == RAVEL_ACT_RELU && bias.has_value();
+        ctx->save_for_backward({x2.t, w2.t, z, keep_b ? bias->contiguous() : at::Tensor()});
         ctx->saved_data["x_ld"] = x2.ld;
         ctx->saved_data["w_ld"] = w2.ld;
         ctx->saved_data["x_shape"] = x.sizes().vec();
@@ -294,7 +296,7 @@ struct FusedLinear : public torch::autograd::Function<FusedLinear> {
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto saved = ctx->get_saved_variables();
-        const at::Tensor &x2 = saved[0], &w2 = saved[1], &z = saved[2];
+        const at::Tensor &x2 = saved[0], &w2 = saved[1], &z = saved[2], &bias = saved[3];
         const std::vector<int64_t> x_shape = ctx->saved_data["x_shape"].toIntVector();
         const int64_t x_ld = ctx->saved_data["x_ld"].toInt(), w_ld = ctx->saved_data["w_ld"].toInt();
         const int64_t N = ctx->saved_data["N"].toInt(), K = x_shape.back();
@@ -332,7 +334,8 @@ struct FusedLinear : public torch::autograd::Function<FusedLinear> {
             check_status("ravel_linear_dz",
                          ravel_linear_dz(gy.t.data_ptr(), gy.ld, z.defined() ? z.data_ptr() : nullptr, up8(N), act,
                                          own_dz ? dz.t.data_ptr() : nullptr, dz.ld,
-                                         need_b ? out[2].data_ptr() : nullptr, M, N, dt,
+                                         need_b ? out[2].data_ptr() : nullptr, M, N, x2.data_ptr(), x_ld,
+                                         w2.data_ptr(), w_ld, bias.defined() ? bias.data_ptr() : nullptr, K, dt,
                                          need_b ? scratch.data_ptr() : nullptr, sb, st));
         }
         if (need_x) {

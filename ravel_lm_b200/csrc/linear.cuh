@@ -17,7 +17,7 @@
 //                     products of the next; the grid is persistent.
 //                   - single (CG 1): 128 x BN outputs per CTA (BN 128, 64 or 32; 0.16, 0.135 and
 //                     0.125 us a chunk, the last two bound by the issuing thread), same structure.
-//                   - split (CG 1, clusters of 2, 4 or 8): the CTAs of a cluster share one
+//                   - split (CG 1, clusters of 2 or 4): the CTAs of a cluster share one
 //                     output tile and divide k; their partial sums meet through distributed
 //                     shared memory, added in rank order (deterministic, one launch, no
 //                     workspace), each CTA finishing an equal share of the columns.  For few
@@ -26,7 +26,8 @@
 //   k_gemv          the forward of one row: a warp (or 2, 4, 8 warps) per weight row, plain 16-byte
 //                   loads, one multiply-add per weight.
 //   k_linear_dz     dz = dy * act'(z) in 16 bits (the operand of the two gradient products) and
-//                   per-block column sums of dz in float32 (the bias gradient) in one pass.
+//                   per-block column sums of dz in float32 (the bias gradient) in one pass; for relu
+//                   it adds up again in float32 the few sums whose sign is in doubt.
 //   k_col_reduce    those partial sums added in block order: deterministic, no atomics.
 //   k_pad_rows      rows copied to a 16-byte pitch, for operands that TMA cannot read in place.
 //
@@ -629,7 +630,55 @@ struct DzArgs {
     float* part;      // [row blocks][N] or null
     int64_t rows;     // rows per block
     int vec_g, vec_z, vec_d;
+    // relu: what z was made of, to settle the sign of sums near zero (x null: z's sign as it is)
+    const void* x;    // [M, K], rows ldx apart, 16-byte rows as w's
+    const void* w;    // [N, K]
+    const void* bias; // [N] or null
+    int64_t ldx, ldw, K;
 };
+
+// relu's derivative jumps where z changes sign, and a long sum on the tensor cores is off by some K 2^-31 of its
+// neighbours' size (rms 0.9e-6 at K 2048 and 2e-6 at 4096 for sums of size 1, ten times float32's own): enough to
+// turn one derivative in a million. Sums nearer to zero than ten times that, K 2^-28 of the largest of the 8
+// neighbouring ones, are added up again in float32, by the whole warp; one in some 10^5 is.
+template <typename T>
+__device__ __forceinline__ void relu_settle(const DzArgs& a, int64_t row, int64_t c, bool have, float (&z)[8]) {
+    float m = 0.0f;
+    unsigned near = 0u;
+    if (have) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(z[e]));
+        m *= static_cast<float>(a.K) * 3.7252903e-9f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (z[e] != 0.0f && fabsf(z[e]) < m && c + e < a.N) near |= 1u << e;
+    }
+    const int lane = threadIdx.x & 31;
+    for (unsigned who = __ballot_sync(0xffffffffu, near != 0u); who != 0u; who &= who - 1u) {
+        const int src = __ffs(static_cast<int>(who)) - 1;
+        const int64_t cs = __shfl_sync(0xffffffffu, c, src);
+        for (unsigned bits = __shfl_sync(0xffffffffu, near, src); bits != 0u; bits &= bits - 1u) {
+            const int e = __ffs(static_cast<int>(bits)) - 1;
+            const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
+            const T* const w = static_cast<const T*>(a.w) + (cs + e) * a.ldw;
+            float acc = 0.0f;
+#pragma unroll 4
+            for (int64_t k = lane * 8; k < a.K; k += 256) {
+                float xf[8], wf[8];
+                unpack8<T>(load8(x, k, a.K, true), xf);
+                unpack8<T>(load8(w, k, a.K, true), wf);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc = fmaf(xf[i], wf[i], acc);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+            if (a.bias != nullptr) acc += static_cast<float>(static_cast<const T*>(a.bias)[cs + e]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (lane == src && i == e) z[i] = acc;
+        }
+    }
+}
 
 // Reads dy and z, writes dz, 6 bytes an element: 16384 x 8192 with gelu in 158 us, 78% of the copy rate (two rows in
 // flight and four blocks an SM; four rows and three blocks 164).  The derivative's 20 instructions an element keep the
@@ -644,7 +693,9 @@ __global__ void __launch_bounds__(32 * DZ_WARPS, 4) k_linear_dz(const DzArgs a) 
     const int64_t r0 = static_cast<int64_t>(blockIdx.y) * a.rows;
     const int64_t r1 = (r0 + a.rows) < a.M ? (r0 + a.rows) : a.M;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (c < a.N) {
+    const bool settle = ACT == RAVEL_ACT_RELU && a.x != nullptr;
+    const bool mine = c < a.N;
+    if (mine || settle) {  // settling takes the whole warp
         const T* const gy = static_cast<const T*>(a.gy);
         const T* const zz = static_cast<const T*>(a.z);
         T* const dz = static_cast<T*>(a.dz);
@@ -653,7 +704,7 @@ __global__ void __launch_bounds__(32 * DZ_WARPS, 4) k_linear_dz(const DzArgs a) 
 #pragma unroll
             for (int i = 0; i < DZ_ROWS; ++i) {
                 const int64_t row = r + i * DZ_WARPS;
-                if (row < r1) {
+                if (row < r1 && mine) {
                     gv[i] = load8(gy + row * a.ldg, c, a.N, a.vec_g);
                     if constexpr (ACT != RAVEL_ACT_NONE) zv[i] = load8(zz + row * a.ldz, c, a.N, a.vec_z);
                 }
@@ -662,11 +713,14 @@ __global__ void __launch_bounds__(32 * DZ_WARPS, 4) k_linear_dz(const DzArgs a) 
             for (int i = 0; i < DZ_ROWS; ++i) {
                 const int64_t row = r + i * DZ_WARPS;
                 if (row < r1) {
-                    float g[8];
+                    float g[8], z[8];
+                    if constexpr (ACT != RAVEL_ACT_NONE) unpack8<T>(zv[i], z);
+                    if constexpr (ACT == RAVEL_ACT_RELU) {
+                        if (settle) relu_settle<T>(a, row, c, mine, z);
+                    }
+                    if (!mine) continue;
                     unpack8<T>(gv[i], g);
                     if constexpr (ACT != RAVEL_ACT_NONE) {
-                        float z[8];
-                        unpack8<T>(zv[i], z);
 #pragma unroll
                         for (int e = 0; e < 8; ++e) g[e] *= act_grad<ACT>(z[e]);
                     }

@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(ln_threads<W>()) k_ln_fwd(const NormArgs a) {
 // Resident blocks asked of the backward's register allocation (its grid is what fits, so that no block waits for a
 // second wave: 131072 x 1024 bf16 took 200 us with 8 blocks an SM of which 7 fit, 157 with as many as fit).
 template <int VEC, int W, int NV> constexpr int ln_bwd_min_blocks() {
-    return NV * VEC <= 8 ? (W == 1 ? 3 : (W == 4 ? 8 : 2)) : 1;
+    return NV * VEC <= 8 ? (W == 1 ? 3 : (W == 4 ? 8 : 2)) : (W == 1 && NV * VEC <= 16 ? 2 : 1);
 }
 
 template <typename T, int VEC, int W, int NV>
@@ -188,10 +188,10 @@ __global__ void __launch_bounds__(ln_threads<W>(), ln_bwd_min_blocks<VEC, W, NV>
         mean = a.mean[row];
         rstd = a.rstd[row];
     };
-    // Rows of up to 16 elements a lane keep their floats between the passes, and the next row's loads fly
-    // meanwhile; longer ones keep the elements as loaded and convert them twice (registers: 4 vectors of 16-bit
-    // elements a lane spilled 750 bytes).
-    constexpr bool KEEP = NV * VEC <= 16;
+    // The floats are kept between the passes, and the next row's loads fly meanwhile; blocks of 16 warps with
+    // more than 16 elements a lane (128 registers) keep the elements as loaded and convert them twice: 2048 x
+    // 16384 bf16 121 us spilling, 92 so.
+    constexpr bool KEEP = W < 16 || NV * VEC <= 16;
     float xh[KEEP ? NV * VEC : VEC], t[KEEP ? NV * VEC : VEC];  // (x - mean) rstd, dy g
     auto convert = [&](int i, float* xf, float* tf) {
         to_floats<T, VEC>(xv[i], xf);

@@ -39,10 +39,13 @@ def test_matmul_refuses_on_the_host(lib):
 
 
 def test_dz_pad_and_norm_refuse_on_the_host(lib):
-    dz = lib.ravel_linear_dz
+    def dz(g, ldg, z, ldz, act, out, ldd, gb, M, N, dtype, scratch, sb, stream, x=None, w=None):
+        return lib.ravel_linear_dz(g, ldg, z, ldz, act, out, ldd, gb, M, N, x, 8, w, 8, None, 8, dtype, scratch, sb, stream)
     assert dz(P, 8, None, 8, 2, P, 8, None, 4, 8, 1, None, 0, None) == INVALID      # gelu needs z
     assert dz(P, 8, None, 8, 0, None, 8, P, 4, 8, 1, None, 0, None) == WORKSPACE
     assert dz(P, 8, None, 8, 0, P, 8, None, 4, 8, 3, None, 0, None) == UNSUPPORTED
+    assert dz(P, 8, P, 8, 1, P, 8, None, 4, 8, 1, None, 0, None, x=P) == INVALID       # x without a weight
+    assert dz(P, 8, P, 8, 1, P, 8, None, 4, 8, 1, None, 0, None, x=P + 2, w=P) == INVALID
     assert lib.ravel_linear_dz_scratch_bytes(100, 256) >= 256 * 4
     assert lib.ravel_linear_dz_scratch_bytes(-1, 256) == 0
     assert lib.ravel_pad_rows(P, 4, 3, 8, P, 8, 1, None) == INVALID                 # rows overlap

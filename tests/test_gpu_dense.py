@@ -194,6 +194,32 @@ def test_gradient_against_differences(act):
         assert abs(got - want) <= tol, f"{n}: {got} vs {want} (tolerance {tol})"
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("M,K,N", [(256, 4096, 2048), (40, 8192, 4100), (1500, 1000, 515)])
+def test_relu_signs_of_sums_near_zero(M, K, N, dtype):
+    """The derivative is the exact sum's sign unless that lies within float32's own rounding of a sum of K terms in
+    lanes of K / 32 (K / 32 + 16 additions of partial sums no larger than a few times the sum's spread of 1)."""
+    x, w, b, _ = make(M, K, N, dtype, seed=K, residual=False, grad=True)
+    ones = torch.ones(M, N, device="cuda", dtype=dtype)  # the bias gradient counts a column's open elements
+    from ravel_lm_b200.dense import fused_linear
+    z = x.detach().double() @ w.detach().double().t() + b.detach().double()
+    db = torch.autograd.grad(fused_linear(x, w, b, activation="relu"), b, ones)[0]
+    sure = z.abs() > (K / 32 + 16) * 2.0 ** -24 * 4
+    low = ((z > 0) & sure).sum(0).double()
+    high = low + (~sure).sum(0)
+    # counts up to M are rounded to the type
+    u = U[dtype]
+    assert bool(((db.double() >= low * (1 - u)) & (db.double() <= high * (1 + u))).all())
+    part = torch.arange(0, M, max(1, M // 8), device="cuda")  # and rows one at a time, where counts are 0 or 1
+    for i in part.tolist():
+        xi = x.detach()[i:i + 1].expand(2, K).contiguous().requires_grad_(True)
+        gy = torch.zeros(2, N, device="cuda", dtype=dtype)
+        gy[0] = 1
+        di = torch.autograd.grad(fused_linear(xi, w, b, activation="relu"), b, gy)[0].double()
+        wrong = (di != (z[i] > 0).double()) & sure[i]
+        assert not wrong.any(), (i, z[i][wrong])
+
+
 def test_strides_views_and_leading_dimensions():
     from ravel_lm_b200.dense import fused_linear
     g = torch.Generator(device="cuda").manual_seed(5)
