@@ -128,17 +128,20 @@ __device__ __forceinline__ float act_fwd(float z) {
     if constexpr (ACT == RAVEL_ACT_SILU) return z * rcp_approx(1.0f + ex2_approx(-1.4426950408889634f * z));
     return z;
 }
+// The derivative, its limits 0 and 1 at infinite z (where a sum left float16's range): gelu and silu
+// have a factor z beside one that has vanished in float32 long before |z| = 128, where the former is held.
 template <int ACT>
 __device__ __forceinline__ float act_grad(float z) {
     if constexpr (ACT == RAVEL_ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
+    const float zc = fminf(fmaxf(z, -128.0f), 128.0f);  // loses a NaN; the other factors keep it
     if constexpr (ACT == RAVEL_ACT_GELU) {
         float e;
         const float c = normal_cdf(z, e);
-        return fmaf(z * 0.39894228040143268f, e, c);
+        return fmaf(zc * 0.39894228040143268f, e, c);
     }
     if constexpr (ACT == RAVEL_ACT_SILU) {
         const float s = rcp_approx(1.0f + ex2_approx(-1.4426950408889634f * z));
-        return s * fmaf(z, 1.0f - s, 1.0f);
+        return s * fmaf(zc, 1.0f - s, 1.0f);
     }
     return 1.0f;
 }

@@ -1,0 +1,75 @@
+"""``fused_linear`` where a sum leaves the 16-bit type's range or lies near zero.
+
+The inputs are powers of two and their small multiples, so that the exact sums, derivatives and gradients are
+known; where a tolerance is needed it is the accumulation's and the output's rounding, as in the general tests.
+"""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+TINY = {torch.bfloat16: 2.0 ** -133, torch.float16: 2.0 ** -24}
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _cuda():
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    import ravel_lm_b200._lib as L
+    L.load()
+    yield
+    torch.cuda.synchronize()
+    assert L.device_error(torch.cuda.current_stream().cuda_stream) == 0
+
+
+# one row (plain loads), few rows (single CTAs), a long sum (divided over a cluster), many rows (pairs)
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu"])
+@pytest.mark.parametrize("M,K,N", [(1, 64, 72), (5, 64, 72), (24, 8192, 512), (2100, 256, 2056)])
+def test_sums_beyond_float16(M, K, N, act):
+    """Sums of +-96000 are infinite in float16, where they are kept for the backward; the derivative is 1 or 0.
+
+    d x[m, k] = sum_n gy[m, n] act' w[n, k]: products of at most (N + 8) float32 roundings and the output's.
+    """
+    from ravel_lm_b200.dense import fused_linear
+    g = torch.Generator(device="cuda").manual_seed(M)
+    sign = torch.where(torch.rand(N, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    x = torch.full((M, K), 64.0, device="cuda").half().requires_grad_(True)
+    w = (sign[:, None] * (1500.0 / K)).expand(N, K).contiguous().half().requires_grad_(True)
+    b = torch.zeros(N, device="cuda").half().requires_grad_(True)
+    gy = torch.randn(M, N, generator=g, device="cuda").half()
+    y = fused_linear(x, w, b, activation=act)
+    assert bool((y[:, sign < 0] == 0).all()) and bool((y[:, sign > 0] == math.inf).all())
+    dx, dw, db = torch.autograd.grad(y, [x, w, b], gy)
+    dz = torch.where(sign > 0, gy.double(), torch.zeros_like(gy).double())
+    for name, got, want, size, n in (
+            ("dx", dx, dz @ w.detach().double(), dz.abs() @ w.detach().double().abs(), N),
+            ("dw", dw, dz.t() @ x.detach().double(), dz.abs().t() @ x.detach().double().abs(), M),
+            ("db", db, dz.sum(0), dz.abs().sum(0), M)):
+        tol = (n + 8) * 2.0 ** -23 * size + U[torch.float16] * want.abs() + TINY[torch.float16]
+        over = want.abs() > 65000  # d w may leave float16 itself
+        ok = ((got.double() - want).abs() <= tol) | over
+        assert bool(ok.all()), f"{name}: {int((~ok).sum())} of {ok.numel()} wrong"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu"])
+def test_derivative_at_infinity(act, dtype):
+    """dz of a kept sum of +inf is dy, of -inf zero; NaN stays NaN."""
+    import ravel_lm_b200._lib as L
+    M, N = 20, 264
+    z = torch.zeros(M, N, dtype=dtype, device="cuda")
+    z[:, 0::3], z[:, 1::3] = math.inf, -math.inf
+    z[3, 2], z[7, 5] = math.nan, math.nan
+    gy = torch.randn(M, N, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").to(dtype)
+    dz = torch.empty_like(gy)
+    code = L.RAVEL_BF16 if dtype == torch.bfloat16 else L.RAVEL_F16
+    codes = {"relu": L.RAVEL_ACT_RELU, "gelu": L.RAVEL_ACT_GELU, "silu": L.RAVEL_ACT_SILU}
+    L.call("ravel_linear_dz", gy.data_ptr(), N, z.data_ptr(), N, codes[act], dz.data_ptr(), N, None, M, N, None, 0, None,
+           0, None, 0, code, None, 0, torch.cuda.current_stream().cuda_stream)
+    assert torch.equal(dz[:, 0::3], gy[:, 0::3])
+    assert not dz[:, 1::3].any() and not torch.isnan(dz[:, 1::3]).any()
+    assert torch.isnan(dz[3, 2]) and torch.isnan(dz[7, 5]) and int(torch.isnan(dz).sum()) == 2
