@@ -331,6 +331,8 @@ int ravel_rms_norm_bwd(const void* x, const void* weight, const void* grad_y, co
 
 /*
  * y[m][n] = residual[m][n] + act(sum_k A[m][k] * B[n][k] + bias[n]).
+ * z holds those sums in the operands' type for ravel_linear_dz; with RAVEL_ACT_RELU a
+ * float16 sum that is not 0 but below 2^-24 is kept as +-2^-24 (its sign is what counts).
  * A is [M, K] with rows lda apart, or with a_mn stored [K, M]; B is [N, K], or
  * with b_mn stored [K, N].  The three products of a Linear with weight W [N, K]:
  *   y  = x W^T:   A = x, B = W

@@ -85,6 +85,8 @@ __device__ __forceinline__ void store8(T* row, int64_t c, int64_t n, bool vec, c
         if (c + e < n) p[c + e] = s[e];
 }
 
+constexpr float F16_TINY = 5.9604644775390625e-8f;  // 2^-24, float16's smallest subnormal
+
 // ------------------------------------------------------------------ activations
 // gelu is z Phi(z), silu is z sigma(z).  Every one keeps a NaN.
 //
@@ -144,6 +146,15 @@ __device__ __forceinline__ float act_grad(float z) {
         return s * fmaf(zc, 1.0f - s, 1.0f);
     }
     return 1.0f;
+}
+
+// The sum before the activation as it is kept for the backward.  relu's derivative needs no more of it than its sign,
+// which float16 would lose below 2^-25: such a sum is kept as the smallest subnormal, and 0 stands for exact zeros alone.
+template <typename T, int ACT>
+__device__ __forceinline__ float kept_sum(float z) {
+    if constexpr (ACT == RAVEL_ACT_RELU && std::is_same<T, __half>::value)
+        return z != 0.0f && fabsf(z) < F16_TINY ? copysignf(F16_TINY, z) : z;
+    return z;
 }
 
 // ------------------------------------------------------------------ the matrix product
@@ -267,7 +278,12 @@ __device__ __forceinline__ void mm_finish8(float (&v)[8], const MatmulArgs& a, i
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += b[e];
     }
-    if (a.z != nullptr) store8(static_cast<T*>(a.z) + row * a.ldz, col, a.N, a.vec_z, pack8<T>(v));
+    if (a.z != nullptr) {
+        float k[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) k[e] = kept_sum<T, ACT>(v[e]);
+        store8(static_cast<T*>(a.z) + row * a.ldz, col, a.N, a.vec_z, pack8<T>(k));
+    }
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = act_fwd<ACT>(v[e]);
     if (a.res != nullptr) {
@@ -492,7 +508,12 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
 #pragma unroll
                                 for (int e = 0; e < 8; ++e) v[e] += __shfl_sync(0xffffffffu, bu, p * 8 + e);
                             }
-                            if (a.z != nullptr) *reinterpret_cast<uint4*>(st + 2048 + epi_piece(lane, p)) = pack8<T>(v);
+                            if (a.z != nullptr) {
+                                float k[8];
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) k[e] = kept_sum<T, ACT>(v[e]);
+                                *reinterpret_cast<uint4*>(st + 2048 + epi_piece(lane, p)) = pack8<T>(k);
+                            }
 #pragma unroll
                             for (int e = 0; e < 8; ++e) v[e] = act_fwd<ACT>(v[e]);
                             if (res != nullptr) {
@@ -609,7 +630,9 @@ __global__ void __launch_bounds__(32 * GV_WARPS) k_gemv(const GemvArgs a) {
     }
     if (n >= a.e.N || lane != 0) return;
     if (a.e.bias != nullptr) acc += static_cast<float>(static_cast<const T*>(a.e.bias)[n]);
-    if (a.e.z != nullptr) static_cast<T*>(a.e.z)[n] = static_cast<T>(acc);
+    if (a.e.z != nullptr)
+        static_cast<T*>(a.e.z)[n] =
+            static_cast<T>(a.act == RAVEL_ACT_RELU ? kept_sum<T, RAVEL_ACT_RELU>(acc) : acc);
     switch (a.act) {
         case RAVEL_ACT_RELU: acc = act_fwd<RAVEL_ACT_RELU>(acc); break;
         case RAVEL_ACT_GELU: acc = act_fwd<RAVEL_ACT_GELU>(acc); break;
@@ -643,7 +666,8 @@ struct DzArgs {
 // relu's derivative jumps where z changes sign, and a long sum on the tensor cores is off by some K 2^-31 of its
 // neighbours' size (rms 0.9e-6 at K 2048 and 2e-6 at 4096 for sums of size 1, ten times float32's own): enough to
 // turn one derivative in a million. Sums nearer to zero than ten times that, K 2^-28 of the largest of the 8
-// neighbouring ones, are added up again in float32, by the whole warp; one in some 10^5 is.
+// neighbouring ones, are added up again in float32, by the whole warp; one in some 10^5 is.  So are all that float16
+// keeps as its smallest subnormal, whose size is not known: one in 10^3 of sums of size 1e-4.
 template <typename T>
 __device__ __forceinline__ void relu_settle(const DzArgs& a, int64_t row, int64_t c, bool have, float (&z)[8]) {
     float m = 0.0f;
@@ -654,7 +678,9 @@ __device__ __forceinline__ void relu_settle(const DzArgs& a, int64_t row, int64_
         m *= static_cast<float>(a.K) * 3.7252903e-9f;
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-            if (z[e] != 0.0f && fabsf(z[e]) < m && c + e < a.N) near |= 1u << e;
+            if (z[e] != 0.0f && (fabsf(z[e]) < m || (std::is_same<T, __half>::value && fabsf(z[e]) <= F16_TINY)) &&
+                c + e < a.N)
+                near |= 1u << e;
     }
     const int lane = threadIdx.x & 31;
     for (unsigned who = __ballot_sync(0xffffffffu, near != 0u); who != 0u; who &= who - 1u) {

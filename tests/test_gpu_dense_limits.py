@@ -73,3 +73,26 @@ def test_derivative_at_infinity(act, dtype):
     assert torch.equal(dz[:, 0::3], gy[:, 0::3])
     assert not dz[:, 1::3].any() and not torch.isnan(dz[:, 1::3]).any()
     assert torch.isnan(dz[3, 2]) and torch.isnan(dz[7, 5]) and int(torch.isnan(dz).sum()) == 2
+
+
+# one row (plain loads), few rows (single CTAs), a long sum (divided over a cluster), many rows (pairs)
+@pytest.mark.parametrize("M,K,N", [(1, 64, 72), (5, 64, 72), (24, 8192, 512), (2100, 256, 2056)])
+def test_relu_of_sums_that_underflow(M, K, N):
+    """z = +-2^-27 is 0 in float16, where it is kept for the backward; its derivative is 1 or 0, that of an exact
+    zero 0.  The bias gradient of a gradient of ones counts them (in float16: exactly to 2048, else to its rounding)."""
+    from ravel_lm_b200.dense import fused_linear
+    x = torch.zeros(M, K, device="cuda").half()
+    x[:, 3] = 2.0 ** -13
+    w = torch.zeros(N, K, device="cuda").half()
+    w[0::3, 3], w[1::3, 3] = 2.0 ** -14, -2.0 ** -14
+    b = torch.zeros(N, device="cuda").half()
+    for t in (x, w, b):
+        t.requires_grad_(True)
+    dx, dw, db = torch.autograd.grad(fused_linear(x, w, b, activation="relu"), [x, w, b],
+                                     torch.ones(M, N, device="cuda").half())
+    on = (torch.arange(N, device="cuda") % 3 == 0).double()
+    assert bool(((db.double() - M * on).abs() <= U[torch.float16] * M * on).all())
+    # d w[n, 3] = M 2^-13, d x[m, 3] = 2^-14 for each of the positive columns: exact sums, one rounding
+    assert bool(((dw[:, 3].double() - M * 2.0 ** -13 * on).abs() <= U[torch.float16] * M * 2.0 ** -13 * on).all())
+    want = float(on.sum()) * 2.0 ** -14
+    assert bool(((dx[:, 3].double() - want).abs() <= U[torch.float16] * want).all())
