@@ -664,24 +664,36 @@ struct DzArgs {
 };
 
 // relu's derivative jumps where z changes sign, and a long sum on the tensor cores is off by some K 2^-31 of its
-// neighbours' size (rms 0.9e-6 at K 2048 and 2e-6 at 4096 for sums of size 1, ten times float32's own): enough to
-// turn one derivative in a million. Sums nearer to zero than ten times that, K 2^-28 of the largest of the 8
-// neighbouring ones, are added up again in float32, by the whole warp; one in some 10^5 is.  So are all that float16
-// keeps as its smallest subnormal, whose size is not known: one in 10^3 of sums of size 1e-4.
+// terms' size (rms 0.9e-6 at K 2048 and 2e-6 at 4096 for sums of size 1, ten times float32's own): enough to
+// turn one derivative in a million. Sums nearer to zero than ten times that, K 2^-28 of the largest of the row's sums in
+// a window of 256 columns, are added up again in float32, by the whole warp; one in some 10^5 is.  So are all that
+// float16 keeps as its smallest subnormal, whose size is not known (one in 10^3 of sums of size 1e-4), and every sum
+// of a row of fewer than 8, which tell nothing about size.  Exact zeros keep the derivative 0: rows of zeros (padding)
+// and columns of zeros would otherwise be added up for nothing.
+//
+// z: the sums of columns c .. c + 7 where `mine`, else (past the last column) those of the strip before, which only
+// count for the size.
 template <typename T>
-__device__ __forceinline__ void relu_settle(const DzArgs& a, int64_t row, int64_t c, bool have, float (&z)[8]) {
-    float m = 0.0f;
-    unsigned near = 0u;
-    if (have) {
+__device__ __forceinline__ void relu_settle(const DzArgs& a, int64_t row, int64_t c, bool mine, float (&z)[8]) {
+    constexpr bool HALF = std::is_same<T, __half>::value;
+    float most = 0.0f, least = INFINITY;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf(z[e]));
-        m *= static_cast<float>(a.K) * 3.7252903e-9f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (z[e] != 0.0f && (fabsf(z[e]) < m || (std::is_same<T, __half>::value && fabsf(z[e]) <= F16_TINY)) &&
-                c + e < a.N)
-                near |= 1u << e;
+    for (int e = 0; e < 8; ++e) {
+        // a float16 sum that is infinite is of size 65504 at least; an infinite bfloat16 one tells no size
+        const float v = HALF ? fminf(fabsf(z[e]), 65504.0f) : (fabsf(z[e]) < INFINITY ? fabsf(z[e]) : 0.0f);
+        most = fmaxf(most, v);
+        least = fminf(least, fabsf(z[e]));
     }
+    most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));  // of positive floats
+    float limit = most * static_cast<float>(a.K) * 3.7252903e-9f;
+    if (HALF) limit = fmaxf(limit, 1.5f * F16_TINY);
+    if (a.N < 8) limit = INFINITY;
+    if (most == 0.0f) limit = 0.0f;
+    if (!__any_sync(0xffffffffu, mine && least < limit)) return;
+    unsigned near = 0u;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (mine && c + e < a.N && z[e] != 0.0f && fabsf(z[e]) < limit) near |= 1u << e;
     const int lane = threadIdx.x & 31;
     for (unsigned who = __ballot_sync(0xffffffffu, near != 0u); who != 0u; who &= who - 1u) {
         const int src = __ffs(static_cast<int>(who)) - 1;
@@ -724,6 +736,7 @@ __global__ void __launch_bounds__(32 * DZ_WARPS, 4) k_linear_dz(const DzArgs a) 
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     const bool settle = ACT == RAVEL_ACT_RELU && a.x != nullptr;
     const bool mine = c < a.N;
+    const bool look = settle && !mine && c >= DZ_COLS;  // lanes past the last column: the strip before, for its size
     if (mine || settle) {  // settling takes the whole warp
         const T* const gy = static_cast<const T*>(a.gy);
         const T* const zz = static_cast<const T*>(a.z);
@@ -736,6 +749,9 @@ __global__ void __launch_bounds__(32 * DZ_WARPS, 4) k_linear_dz(const DzArgs a) 
                 if (row < r1 && mine) {
                     gv[i] = load8(gy + row * a.ldg, c, a.N, a.vec_g);
                     if constexpr (ACT != RAVEL_ACT_NONE) zv[i] = load8(zz + row * a.ldz, c, a.N, a.vec_z);
+                } else if constexpr (ACT == RAVEL_ACT_RELU) {
+                    zv[i] = make_uint4(0u, 0u, 0u, 0u);
+                    if (row < r1 && look) zv[i] = load8(zz + row * a.ldz, c - DZ_COLS, a.N, a.vec_z);
                 }
             }
 #pragma unroll

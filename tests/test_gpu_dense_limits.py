@@ -96,3 +96,53 @@ def test_relu_of_sums_that_underflow(M, K, N):
     assert bool(((dw[:, 3].double() - M * 2.0 ** -13 * on).abs() <= U[torch.float16] * M * 2.0 ** -13 * on).all())
     want = float(on.sum()) * 2.0 ** -14
     assert bool(((dx[:, 3].double() - want).abs() <= U[torch.float16] * want).all())
+
+
+def near_zero(M, K, N, col, dtype, scale=1.0, sign=1.0, dead=()):
+    """Column `col` sums to sign scale (255 2^-26 - 2^-20) > 0 (sign 1), in an order in which a product of 1 hides
+    the 255 small ones from an accumulator of some 25 bits until a product of -1 takes it away.  The other columns
+    sum to scale, those in `dead` to 0."""
+    x = torch.zeros(M, K, device="cuda")
+    x[:, 0], x[:, 1:256], x[:, 256], x[:, 300] = 1.0, 2.0 ** -13, 1.0, 2.0 ** -10
+    w = torch.zeros(N, K, device="cuda")
+    w[:, 0] = scale
+    for n in dead:
+        w[n] = 0.0
+    w[col] = 0.0
+    w[col, 0], w[col, 1:256], w[col, 256], w[col, 300] = (sign * scale * v for v in (1.0, 2.0 ** -13, -1.0, -2.0 ** -10))
+    x, w = x.to(dtype), w.to(dtype)
+    exact = float(x[0].double() @ w[col].double())
+    assert exact == sign * scale * (255 * 2.0 ** -26 - 2.0 ** -20)
+    return x, w
+
+
+# the only column; the only one of its group of 8 (and of its strip of 256); a group whose other columns are dead
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N,col,dead", [(1, 0, ()), (3, 1, (0, 2)), (129, 128, ()), (257, 256, ()), (258, 257, (256,)),
+                                        (513, 512, ()), (64, 20, (16, 17, 18, 19, 21, 22, 23))])
+def test_relu_sign_without_neighbours(N, col, dead, dtype):
+    """Whatever stands beside a sum near zero, its derivative is that of the float32 sum: lanes of 8 elements a chunk
+    of 256 keep the 248 small products of lanes 1 to 31 (3.7e-6) beside the 2^-20 taken away."""
+    from ravel_lm_b200.dense import fused_linear
+    for M in (2, 40, 300):
+        for sign in (1.0, -1.0):
+            x, w = near_zero(M, 512, N, col, dtype, sign=sign, dead=dead)
+            b = torch.zeros(N, device="cuda", dtype=dtype).requires_grad_(True)
+            db, = torch.autograd.grad(fused_linear(x, w, b, activation="relu"), b, torch.ones(M, N, device="cuda", dtype=dtype))
+            want = torch.ones(N, device="cuda", dtype=torch.float64) * M
+            want[list(dead)] = 0
+            want[col] = M if sign > 0 else 0
+            assert bool(((db.double() - want).abs() <= U[dtype] * want).all()), (M, sign, db[col])
+
+
+def test_relu_sign_of_a_sum_that_underflows():
+    """The same with a sum of 1e-8, which float16 does not hold: its kept sign is only the tensor cores'."""
+    from ravel_lm_b200.dense import fused_linear
+    for M in (2, 40, 300):
+        for sign in (1.0, -1.0):
+            x, w = near_zero(M, 512, 72, 30, torch.float16, scale=2.0 ** -8, sign=sign)
+            b = torch.zeros(72, device="cuda").half().requires_grad_(True)
+            db, = torch.autograd.grad(fused_linear(x, w, b, activation="relu"), b, torch.ones(M, 72, device="cuda").half())
+            want = torch.full((72,), float(M), device="cuda")
+            want[30] = M if sign > 0 else 0
+            assert torch.equal(db.float(), want), (M, sign, db[30])
