@@ -11,7 +11,10 @@
 //
 //   k_distill_count  rows with a live entry, counted before a gradient of the mean is written.
 //   k_distill        a block per row.  One pass over the logits keeps a running maximum and sum
-//                    (base 2: exp2 of one fused multiply-add per element); with GRAD a second pass
+//                    (base 2: exp2 of (s - max) log2(e) / tau, subtracted before it is scaled, so that a row of the
+//                    type's lowest or highest values does not leave float32 and a common offset costs nothing.
+//                    In pairs; one fused multiply-add an element, which fails there, was 0 to 5% faster: 8192 x 65536
+//                    bf16 179 / 181 us, with the gradient 440 / 442, 16384 x 4096 85 / 89); with GRAD a second pass
 //                    writes the gradient for upstream 1 while the row is still in registers (up to 8 KB)
 //                    or L2, then the at most k entries are written once more with their p, from float32.
 //   k_distill_bwd    the second pass alone, for any upstream gradient.
@@ -37,7 +40,7 @@ struct DistillArgs {
     const void* t;            // [R, k] teacher logits
     void* grad;               // [R, V] contiguous, or null
     float* losses;            // [R]
-    float2* stat;             // [R] (m, l): m the largest s_v c, l = sum_v 2^(s_v c - m), c = log2(e) / tau
+    float2* stat;             // [R] (m, l): m the largest s_v, l = sum_v 2^((s_v - m) c), c = log2(e) / tau
     unsigned char* live;      // [R] the row has a live entry, or null
     const unsigned int* counts;  // [DISTILL_COUNTS] rows counted by the mean, in parts; null: sum, none
     const float* up;          // upstream gradient: one value (mean, sum) or [R]
@@ -99,30 +102,44 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// Running (maximum, sum of 2^(x - maximum)); an empty one is (-inf, 0).
+// x[i] = (x[i] - m) c for an even number of elements, two an instruction.
+template <int E>
+__device__ __forceinline__ void sub_scale(float (&x)[E], float m, float c) {
+    uint64_t m2, c2;
+    asm("mov.b64 %0, {%1, %1};" : "=l"(m2) : "f"(-m));
+    asm("mov.b64 %0, {%1, %1};" : "=l"(c2) : "f"(c));
+#pragma unroll
+    for (int e = 0; e < E; e += 2)
+        asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%0, %1};\n\tadd.rn.f32x2 t, t, %2;\n\tmul.rn.f32x2 t, t, %3;\n\t"
+            "mov.b64 {%0, %1}, t;\n\t}"
+            : "+f"(x[e]), "+f"(x[e + 1])
+            : "l"(m2), "l"(c2));
+}
+
+// Running (maximum, sum of 2^((x - maximum) c)); an empty one is (-inf, 0).
 struct MaxSum {
     float m, l;
 };
 __device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.0f : m; }
 // The warp's (maximum, sum): the maxima first, then one rescaling of each lane's sum.
-__device__ __forceinline__ MaxSum warp_join(MaxSum v) {
+__device__ __forceinline__ MaxSum warp_join(MaxSum v, float c) {
     float m = v.m;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float l = v.l * ex2(v.m - finite_ref(m));
+    float l = v.l * ex2((v.m - finite_ref(m)) * c);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     return {m, l};
 }
 template <int TH>
-__device__ __forceinline__ MaxSum block_join(MaxSum v, MaxSum* red) {
-    v = warp_join(v);
+__device__ __forceinline__ MaxSum block_join(MaxSum v, float c, MaxSum* red) {
+    v = warp_join(v, c);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
     __syncthreads();
     const int lane = threadIdx.x & 31;
     v = {-INFINITY, 0.0f};
     if (lane < TH / 32) v = red[lane];
-    return warp_join(v);
+    return warp_join(v, c);
 }
 
 // The row's elements as this block's threads share them: a head and a tail of single elements and
@@ -139,11 +156,11 @@ struct RowSplit {
     }
 };
 
-// Teacher entries into shared memory, by one warp: p_j (0 for a dead entry), ids (-1 for a dead one), and for the
-// loss d_j = log2 p_j - s[id_j] c.  Returns whether the row has a live entry.
+// Teacher entries into shared memory, by one warp: ids (-1 for a dead entry), p_j (0 for a dead one); for the
+// loss log2 p_j (-inf) in its place, and s[id_j].  Returns whether the row has a live entry.
 template <typename T, typename TT>
 __device__ __forceinline__ bool distill_teacher(const DistillArgs& a, int64_t row, bool want_loss, float* sp, int* sid,
-                                                float* sd) {
+                                                float* ss) {
     const int lane = threadIdx.x & 31;
     const float c = 1.4426950408889634f / a.tau;  // log2(e) / tau
     float m = -INFINITY;
@@ -155,10 +172,10 @@ __device__ __forceinline__ bool distill_teacher(const DistillArgs& a, int64_t ro
         const bool ok = distill_entry<TT>(a, row, j, id, t, bad);
         bad_any |= bad;
         sid[j] = ok ? id : -1;
-        sp[j] = ok ? t * c : -INFINITY;
-        if (want_loss) sd[j] = ok ? as_float(static_cast<const T*>(a.s)[row * a.lds + id]) * c : 0.0f;
+        sp[j] = ok ? t : -INFINITY;
+        if (want_loss) ss[j] = ok ? as_float(static_cast<const T*>(a.s)[row * a.lds + id]) : 0.0f;
         live |= ok;
-        if (ok) m = fmaxf(m, t * c);
+        if (ok) m = fmaxf(m, t);
     }
     if (bad_any) atomicOr(a.err, RAVEL_DEVERR_INDEX);
     live = __any_sync(0xffffffffu, live);
@@ -166,30 +183,34 @@ __device__ __forceinline__ bool distill_teacher(const DistillArgs& a, int64_t ro
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     float z = 0.0f;
     for (int j = lane; j < a.k; j += 32)
-        if (sid[j] >= 0) z += ex2(sp[j] - m);
+        if (sid[j] >= 0) z += ex2((sp[j] - m) * c);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-    const float lz = m + __log2f(z), iz = 1.0f / z;
+    const float lz = log2f(z);
     for (int j = lane; j < a.k; j += 32) {
-        const bool ok = sid[j] >= 0;
-        if (want_loss) sd[j] = sp[j] - lz - sd[j];
-        sp[j] = ok ? ex2(sp[j] - m) * iz : 0.0f;
+        const float lp = sid[j] >= 0 ? fmaf(sp[j] - m, c, -lz) : -INFINITY;
+        sp[j] = want_loss ? lp : ex2(lp);
     }
     return live;
 }
 
-// The row's loss from those and the student's (m, l), by the same warp.
-__device__ __forceinline__ float distill_loss(const DistillArgs& a, MaxSum st, const float* sp, const float* sd) {
-    const float lse = st.m + __log2f(st.l);
+// The row's loss from those and the student's (m, l), by the same warp; leaves p_j in the place of log2 p_j.
+// An entry's term is p (log p - (s - m) / tau + log l): natural units, which hold a student's logit of the type's
+// lowest value for tau >= 1.
+__device__ __forceinline__ float distill_loss(const DistillArgs& a, MaxSum st, float* sp, const float* ss) {
+    const float ll = log2f(st.l), it = 1.0f / a.tau;
     float acc = 0.0f;
-    for (int j = threadIdx.x & 31; j < a.k; j += 32)
-        if (sp[j] != 0.0f) acc += sp[j] * (sd[j] + lse);  // base 2; p = 0 contributes nothing
+    for (int j = threadIdx.x & 31; j < a.k; j += 32) {
+        const float lp = sp[j], p = ex2(lp);
+        if (p != 0.0f) acc += p * fmaf(lp + ll, 0.6931471805599453f, (st.m - ss[j]) * it);  // p = 0 contributes nothing
+        sp[j] = p;
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-    return acc * 0.6931471805599453f * a.tau * a.tau * a.weight;
+    return acc * a.tau * a.tau * a.weight;
 }
 
-// grad row = gs * (2^(s c - m) / l - p at the entries); a row without a live entry gets zeros.  The row's vectors are
+// grad row = gs * (2^((s - m) c) / l - p at the entries); a row without a live entry gets zeros.  The row's vectors are
 // in v (NV > 0: vector i * TH + thread in v[i]) or read again.
 template <typename T, int TH, int NV>
 __device__ __forceinline__ void distill_grad_row(const DistillArgs& a, int64_t row, MaxSum st, float gs, bool live,
@@ -210,13 +231,14 @@ __device__ __forceinline__ void distill_grad_row(const DistillArgs& a, int64_t r
         return;
     }
     const float gl = gs / st.l;
-    auto one = [&](T x) { return round_to<T>(gl * ex2(fmaf(as_float(x), c, -st.m))); };
+    auto one = [&](T x) { return round_to<T>(gl * ex2((as_float(x) - st.m) * c)); };
     if (same) {
         auto put = [&](int i, const Pack<T, E>& x) {
             float f[E];
             to_floats<T, E>(x, f);
+            sub_scale<E>(f, st.m, c);
 #pragma unroll
-            for (int e = 0; e < E; ++e) f[e] = gl * ex2(fmaf(f[e], c, -st.m));
+            for (int e = 0; e < E; ++e) f[e] = gl * ex2(f[e]);
             store_pack_stream<T, E>(d + rs.head + i * E, from_floats<T, E>(f));
         };
         if constexpr (NV > 0) {
@@ -246,7 +268,7 @@ __device__ __forceinline__ void distill_grad_row(const DistillArgs& a, int64_t r
             if (i < j) first = false;
             p += sp[i];
         }
-        if (first) d[id] = round_to<T>(gl * ex2(fmaf(as_float(s[id]), c, -st.m)) - gs * p);
+        if (first) d[id] = round_to<T>(gl * ex2((as_float(s[id]) - st.m) * c) - gs * p);
     }
 }
 
@@ -254,12 +276,12 @@ __device__ __forceinline__ void distill_grad_row(const DistillArgs& a, int64_t r
 template <typename T, typename TT, int TH, int NV, bool GRAD>
 __global__ void __launch_bounds__(TH) k_distill(const DistillArgs a) {
     constexpr int E = 16 / sizeof(T);
-    extern __shared__ float dyn[];  // p [k], ids [k], d [k]
+    extern __shared__ float dyn[];  // p [k], ids [k], the entries' logits [k]
     __shared__ MaxSum red[TH / 32];
     __shared__ float s_live, s_count;
     float* const sp = dyn;
     int* const sid = reinterpret_cast<int*>(dyn + a.k);
-    float* const sd = dyn + 2 * a.k;
+    float* const ss = dyn + 2 * a.k;
     grid_wait();
     grid_trigger();
     const int64_t row = blockIdx.x;
@@ -274,7 +296,7 @@ __global__ void __launch_bounds__(TH) k_distill(const DistillArgs a) {
     }
     // the teacher's part first: its chain of loads runs under the other warps' pass over the logits
     if (threadIdx.x < 32) {
-        const bool live = distill_teacher<T, TT>(a, row, true, sp, sid, sd);
+        const bool live = distill_teacher<T, TT>(a, row, true, sp, sid, ss);
         if (threadIdx.x == 0) s_live = live ? 1.0f : 0.0f;
     } else if (GRAD && threadIdx.x < 64) {
         const float n = distill_counted(a);
@@ -286,22 +308,20 @@ __global__ void __launch_bounds__(TH) k_distill(const DistillArgs a) {
         to_floats<T, E>(p, x);
 #pragma unroll
         for (int e = 0; e < E; ++e) m = fmaxf(m, x[e]);
-        m *= c;
         if (m > v.m) {
-            v.l *= ex2(v.m - m);
+            v.l *= ex2((v.m - m) * c);
             v.m = m;
         }
-        const float r = finite_ref(v.m);
+        sub_scale<E>(x, finite_ref(v.m), c);
 #pragma unroll
-        for (int e = 0; e < E; ++e) v.l += ex2(fmaf(x[e], c, -r));
+        for (int e = 0; e < E; ++e) v.l += ex2(x[e]);
     };
     auto take = [&](float x) {
-        const float x2 = x * c;
-        if (x2 > v.m) {
-            v.l *= ex2(v.m - x2);
-            v.m = x2;
+        if (x > v.m) {
+            v.l *= ex2((v.m - x) * c);
+            v.m = x;
         }
-        v.l += ex2(fmaf(x, c, -finite_ref(v.m)));
+        v.l += ex2((x - finite_ref(v.m)) * c);
     };
     if constexpr (NV > 0) {
 #pragma unroll
@@ -313,10 +333,10 @@ __global__ void __launch_bounds__(TH) k_distill(const DistillArgs a) {
     }
     for (int i = threadIdx.x; i < rs.head; i += TH) take(as_float(s[i]));
     for (int i = rs.head + rs.vecs * E + threadIdx.x; i < a.V; i += TH) take(as_float(s[i]));
-    v = block_join<TH>(v, red);
+    v = block_join<TH>(v, c, red);
     const bool live = s_live != 0.0f;
     if (threadIdx.x < 32) {
-        const float loss = live ? distill_loss(a, v, sp, sd) : 0.0f;
+        const float loss = live ? distill_loss(a, v, sp, ss) : 0.0f;
         if (threadIdx.x == 0) {
             a.losses[row] = loss;
             if (a.live != nullptr) a.live[row] = live;
@@ -326,8 +346,9 @@ __global__ void __launch_bounds__(TH) k_distill(const DistillArgs a) {
     if constexpr (GRAD) distill_grad_row<T, TH, NV>(a, row, v, a.weight * a.tau / s_count, live, sp, sid, held);
 }
 
+// 32 registers, so that an SM is full: 16384 x 8192 bf16 125 us without the bound, 98 with it.
 template <typename T, typename TT, int TH>
-__global__ void __launch_bounds__(TH) k_distill_bwd(const DistillArgs a) {
+__global__ void __launch_bounds__(TH, 2048 / TH) k_distill_bwd(const DistillArgs a) {
     extern __shared__ float dyn[];
     __shared__ float s_live, s_count;
     float* const sp = dyn;
