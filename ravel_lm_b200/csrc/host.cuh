@@ -19,7 +19,8 @@ int sm_count();
 // RAVEL_OK or RAVEL_ERR_CUDA.
 int check_launch();
 
-// Raise a kernel's dynamic shared-memory limit to `bytes` (once per kernel and device).
+// Let a kernel be launched with `bytes` of dynamic shared memory beside its static shared memory (the limit is raised
+// once per kernel and device where the two pass 48 KB).
 int raise_smem(const void* kernel, size_t bytes);
 
 template <typename K>

@@ -305,7 +305,10 @@ std::atomic<uint64_t> g_launches{0};
 // Per-(kernel, device) results of CUDA attribute calls, so that a launch pays for
 // them once per process instead of on every call.
 std::mutex g_attr_mu;
-std::map<std::pair<const void*, int>, size_t> g_smem_set;            // dynamic smem limit raised to
+struct SmemLimit {
+    size_t own, dynamic;  // the kernel's static shared memory; what a launch may ask for beside it
+};
+std::map<std::pair<const void*, int>, SmemLimit> g_smem;
 std::map<std::tuple<const void*, int, int, size_t>, int> g_occupancy;  // blocks per SM
 
 int current_device() {
@@ -322,16 +325,24 @@ int check_launch() {
 }
 
 int raise_smem(const void* kernel, size_t bytes) {
-    if (bytes <= 48 * 1024) return RAVEL_OK;
-    if (bytes > 227 * 1024) return RAVEL_ERR_UNSUPPORTED;
+    if (bytes == 0) return RAVEL_OK;
     const auto key = std::make_pair(kernel, current_device());
     std::lock_guard<std::mutex> lock(g_attr_mu);
-    auto it = g_smem_set.find(key);
-    if (it != g_smem_set.end() && it->second >= bytes) return RAVEL_OK;
+    auto it = g_smem.find(key);
+    if (it == g_smem.end()) {
+        cudaFuncAttributes at;
+        if (cudaFuncGetAttributes(&at, kernel) != cudaSuccess) return RAVEL_ERR_CUDA;
+        // 48 KB in all unless asked for
+        const size_t own = at.sharedSizeBytes;
+        it = g_smem.emplace(key, SmemLimit{own, own < 48 * 1024 ? 48 * 1024 - own : 0}).first;
+    }
+    SmemLimit& limit = it->second;
+    if (bytes <= limit.dynamic) return RAVEL_OK;
+    if (bytes + limit.own > 227 * 1024) return RAVEL_ERR_UNSUPPORTED;
     const cudaError_t e =
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
     if (e != cudaSuccess) return RAVEL_ERR_CUDA;
-    g_smem_set[key] = bytes;
+    limit.dynamic = bytes;
     return RAVEL_OK;
 }
 

@@ -10,7 +10,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from test_gpu_distill import DTYPES, E, make, reference, within
+from test_gpu_distill import DTYPES, E, check, make, reference, within
 
 pytestmark = pytest.mark.gpu
 
@@ -101,3 +101,13 @@ def test_a_common_offset_does_not_matter():
         s.copy_((s * 8).round() / 8 + 2.0 ** 20)
         t = (t * 8).round() / 8 - 2.0 ** 20
     check_ends(s, ids, t, 1.0)
+
+
+# the forward keeps 12 bytes an entry in shared memory, beside what the kernel has of its own: around and at the
+# largest k, for blocks of 128, 256 and 512 threads
+@pytest.mark.parametrize("R,V,dtype", [(160, 1000, torch.bfloat16), (160, 9001, torch.float16), (3, 20000, torch.float32)])
+@pytest.mark.parametrize("k", [4084, 4085, 4090, 4093, 4096])
+def test_the_largest_k(R, V, dtype, k):
+    s, ids, t = make(R, V, k, dtype, seed=k)
+    for reduction in ("mean", "none"):
+        check(s, ids, t, 2.0, reduction)
