@@ -520,6 +520,8 @@ int ravel_distill_topk_fwd(const void* logits, int64_t ld, const void* ids, int 
                            int reduction, float* losses, float* stat, float* out, void* grad, int dtype, void* scratch,
                            size_t scratch_bytes, void* stream) {
     RAVEL_TIMED("ravel_distill_topk_fwd", stream);
+    // the gradient divides by the count of rows, which is made with stat only
+    if (grad != nullptr && stat == nullptr) return RAVEL_ERR_INVALID_ARG;
     DistillArgs a;
     if (int e = distill_args(a, logits, ld, ids, ids_dtype, teacher, R, V, k, temperature, dtype, teacher_dtype))
         return e;

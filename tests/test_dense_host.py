@@ -99,3 +99,12 @@ def test_python_refusals_without_a_gpu():
         distill_topk_loss(x, ids, torch.zeros(2, 3), reduction="max")
     with pytest.raises(ValueError, match="temperature"):
         distill_topk_loss(x, ids, torch.zeros(2, 3), temperature=0.0)
+
+
+def test_distill_refuses_a_gradient_without_the_statistics(lib):
+    """grad needs stat, with which the count that the mean's gradient divides by is made."""
+    for reduction in (1, 2):
+        for args in ((2, 8, 2), (0, 8, 2)):
+            R, V, k = args
+            rc = lib.ravel_distill_topk_fwd(P, V, P, 1, P, 0, R, V, k, 1.0, 1.0, reduction, P, None, P, P, 0, P, 1 << 20, None)
+            assert rc == INVALID
