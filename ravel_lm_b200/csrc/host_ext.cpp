@@ -216,6 +216,13 @@ void once_differentiable(const char* op) {
         throw std::runtime_error(std::string(op) + ": the backward pass is not differentiable (create_graph=True)");
 }
 
+// Nor is there a forward-mode derivative: refuse a tangent rather than drop it.
+void no_tangents(const char* op, std::initializer_list<const OptTensor*> tensors) {
+    for (const OptTensor* t : tensors)
+        if (t->has_value() && (*t)->_fw_grad(/*level=*/0).defined())
+            throw std::runtime_error(std::string(op) + " has no forward-mode derivative");
+}
+
 int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 
 // A row-major matrix as the kernels take it: elements of a row adjacent, rows `ld` apart.
@@ -371,7 +378,8 @@ at::Tensor fused_linear(const at::Tensor& x, const at::Tensor& weight, const Opt
     shape.back() = N;
     if (residual && residual->sizes() != at::IntArrayRef(shape))
         throw py::value_error("residual must have the output's shape [..., N]");
-    const OptTensor w(weight);
+    const OptTensor in(x), w(weight);
+    no_tangents("fused_linear", {&in, &w, &bias, &residual});
     require_cuda(x, {&w, &bias, &residual});
     const c10::cuda::CUDAGuard guard(x.device());
     const bool grad = at::GradMode::is_enabled() &&
@@ -469,6 +477,8 @@ at::Tensor layer_norm(const at::Tensor& x, const OptTensor& weight, const OptTen
     for (const OptTensor* t : {&weight, &bias})
         if (t->has_value() && (*t)->scalar_type() != x.scalar_type())
             throw py::type_error("layer_norm expects x, weight and bias of one dtype");
+    const OptTensor in(x);
+    no_tangents("layer_norm", {&in, &weight, &bias});
     require_cuda(x, {&weight, &bias});
     const c10::cuda::CUDAGuard guard(x.device());
     if (at::GradMode::is_enabled() &&
@@ -583,7 +593,8 @@ at::Tensor distill_topk_loss(const at::Tensor& logits, const at::Tensor& ids, co
     if (!(tau > 0.0) || !std::isfinite(tau)) throw py::value_error("temperature must be positive and finite");
     if (teacher.requires_grad() && at::GradMode::is_enabled())
         throw py::value_error("teacher_logits must not require a gradient (detach them)");
-    const OptTensor i(ids), t(teacher);
+    const OptTensor s(logits), i(ids), t(teacher);
+    no_tangents("distill_topk_loss", {&s, &t});
     require_cuda(logits, {&i, &t});
     const c10::cuda::CUDAGuard guard(logits.device());
     if (at::GradMode::is_enabled() && logits.requires_grad())

@@ -108,3 +108,25 @@ def test_distill_refuses_a_gradient_without_the_statistics(lib):
             R, V, k = args
             rc = lib.ravel_distill_topk_fwd(P, V, P, 1, P, 0, R, V, k, 1.0, 1.0, reduction, P, None, P, P, 0, P, 1 << 20, None)
             assert rc == INVALID
+
+
+def test_forward_mode_tangents_are_refused():
+    """There is no forward-mode derivative; a tangent on any tensor raises instead of being lost."""
+    import torch.autograd.forward_ad as fw
+    from ravel_lm_b200.dense import fused_linear
+    from ravel_lm_b200.distill import distill_topk_loss
+    from ravel_lm_b200.glue import layer_norm
+    x, w, b = torch.zeros(2, 8, dtype=torch.bfloat16), torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(4, dtype=torch.bfloat16)
+    r, g, ids, t = torch.zeros(2, 4, dtype=torch.bfloat16), torch.ones(8, dtype=torch.bfloat16), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3)
+    with fw.dual_level():
+        def dual(v):
+            return fw.make_dual(v, torch.ones_like(v))
+        calls = [lambda: fused_linear(dual(x), w), lambda: fused_linear(x, dual(w)), lambda: fused_linear(x, w, dual(b)),
+                 lambda: fused_linear(x, w, b, activation="silu", residual=dual(r)), lambda: layer_norm(dual(x)),
+                 lambda: layer_norm(x, dual(g)), lambda: layer_norm(x, g, dual(g)), lambda: distill_topk_loss(dual(x), ids, t),
+                 lambda: distill_topk_loss(x, ids, dual(t))]
+        for call in calls:
+            with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                call()
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        fused_linear(x, w)
