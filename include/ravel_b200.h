@@ -349,6 +349,14 @@ int ravel_matmul(const void* A, int64_t lda, int a_mn, const void* B, int64_t ld
                  int64_t K, const void* bias, const void* residual, int64_t ldr, int act, void* y, int64_t ldy,
                  void* z, int64_t ldz, int dtype, void* stream);
 
+/*
+ * The launch shape ravel_matmul takes for these sizes (all positive) on the
+ * current device: plan[0] CTAs per product (1, or 2: a pair), plan[1] columns of
+ * a tile, plan[2] CTAs that divide k (1, 2 or 4).  One row with both operands
+ * K-major: 0, the warps per weight row, 1.
+ */
+int ravel_matmul_plan(int64_t M, int64_t N, int64_t K, int b_mn, int* plan);
+
 /* Scratch bytes of ravel_linear_dz (per-block column sums). */
 size_t ravel_linear_dz_scratch_bytes(int64_t M, int64_t N);
 

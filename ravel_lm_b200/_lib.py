@@ -77,6 +77,7 @@ SIGNATURES = {
     "ravel_rms_norm_bwd": (_c_int, [_c_vp] * 6 + [_c_i64, _c_i64, _c_int, _c_vp, _c_sz, _c_vp]),
     "ravel_matmul": (_c_int, [_c_vp, _c_i64, _c_int, _c_vp, _c_i64, _c_int] + [_c_i64] * 3 +
                      [_c_vp, _c_vp, _c_i64, _c_int, _c_vp, _c_i64, _c_vp, _c_i64, _c_int, _c_vp]),
+    "ravel_matmul_plan": (_c_int, [_c_i64] * 3 + [_c_int, ctypes.POINTER(_c_int)]),
     "ravel_linear_dz_scratch_bytes": (_c_sz, [_c_i64, _c_i64]),
     "ravel_linear_dz": (_c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_int, _c_vp, _c_i64, _c_vp, _c_i64, _c_i64] +
                         [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_int, _c_vp, _c_sz, _c_vp]),

@@ -148,14 +148,19 @@ int launch_matmul(const Operand& A, const Operand& B, int64_t K, MatmulArgs a, c
 }
 
 // One row.  Warps per weight row: at least 16 warps an SM in all while every lane keeps a few loads of its row.
+int gemv_warps(int64_t N, int64_t K) {
+    int s = 1;
+    while (s < GV_WARPS && N * s < static_cast<int64_t>(sm_count()) * 16 && K >= 512 * s) s *= 2;
+    return s;
+}
+
 template <typename T>
 int launch_gemv(const Operand& X, const Operand& W, int64_t K, int act, const MatmulArgs& e, cudaStream_t st) {
     GemvArgs a;
     a.x = X.p; a.w = W.p; a.ldw = W.ld; a.K = K;
     a.act = act;
     a.e = e;
-    int s = 1;
-    while (s < GV_WARPS && e.N * s < static_cast<int64_t>(sm_count()) * 16 && K >= 512 * s) s *= 2;
+    const int s = gemv_warps(e.N, K);
     const dim3 grid(static_cast<unsigned>((e.N + GV_WARPS / s - 1) / (GV_WARPS / s)));
     const auto kern = s == 1 ? k_gemv<T, 1> : (s == 2 ? k_gemv<T, 2> : (s == 4 ? k_gemv<T, 4> : k_gemv<T, 8>));
     return launch(kern, grid, 32 * GV_WARPS, 0, st, 1, a);
@@ -365,6 +370,18 @@ int ravel_matmul(const void* A, int64_t lda, int a_mn, const void* B, int64_t ld
             return matmul_shape<T, false, false, true, ACT>(oa, ob, K, a, st);
         });
     });
+}
+
+int ravel_matmul_plan(int64_t M, int64_t N, int64_t K, int b_mn, int* plan) {
+    if (plan == nullptr || M <= 0 || N <= 0 || K <= 0 || M > kMaxDim || N > kMaxDim || K > kMaxDim)
+        return RAVEL_ERR_INVALID_ARG;
+    if (M == 1 && !b_mn) {
+        plan[0] = 0, plan[1] = gemv_warps(N, K), plan[2] = 1;
+    } else {
+        const Plan p = plan_matmul(M, N, K, b_mn != 0);
+        plan[0] = p.cg, plan[1] = p.bn, plan[2] = p.splits;
+    }
+    return RAVEL_OK;
 }
 
 size_t ravel_linear_dz_scratch_bytes(int64_t M, int64_t N) {

@@ -130,3 +130,19 @@ def test_forward_mode_tangents_are_refused():
                 call()
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         fused_linear(x, w)
+
+
+def test_the_launch_shapes_are_all_tested(lib):
+    """The sizes of the GPU tests reach every launch shape in every direction (on 148 SMs, which a machine without a
+    GPU is taken to have), and every number of warps per row."""
+    from dense_shapes import CASES, ONE32, ONE64, ONE128, PAIR128, PAIR256, ROWS, SPLIT2, SPLIT4, plan, plans
+    every = {PAIR256, PAIR128, ONE128, ONE64, SPLIT2, SPLIT4}
+    got = [plans(lib, *sizes) for sizes, *_ in CASES]
+    assert got == [tuple(case[1:]) for case in CASES]
+    assert {p[0] for p in got} == every | {ONE32}
+    assert {p[1] for p in got} == {p[2] for p in got} == every
+    assert [plan(lib, 1, N, K, 0) for K, N, _ in ROWS] == [(0, warps, 1) for *_, warps in ROWS]
+    assert {warps for *_, warps in ROWS} == {1, 2, 4, 8}
+    out = (ctypes.c_int * 3)()
+    assert lib.ravel_matmul_plan(0, 8, 8, 0, out) == INVALID
+    assert lib.ravel_matmul_plan(8, 8, 8, 0, None) == INVALID

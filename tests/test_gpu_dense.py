@@ -133,7 +133,7 @@ def step(x, w, b, r, act, gy):
     return y, dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), gy)))
 
 
-# every launch shape (pairs, single, clusters of 2, 4 and 8), its edges, and widths that need the padded copies
+# small and odd sizes, tile edges, and widths that need the padded copies (the launch shapes: test_gpu_dense_shapes.py)
 SHAPES = [(1, 64, 128), (1, 4096, 256), (2, 512, 1000), (7, 8, 8), (24, 2048, 512), (33, 100, 60), (127, 65, 129),
           (128, 1024, 128), (129, 1000, 257), (300, 333, 515), (512, 256, 768), (1000, 128, 2056), (2049, 64, 511),
           (4096, 192, 1024), (3000, 520, 2304)]
