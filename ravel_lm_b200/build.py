@@ -68,12 +68,27 @@ def obj_path(unit: Path) -> Path:
     return OBJ / (unit.stem + ".o")
 
 
+def flags_path(unit: Path) -> Path:
+    return OBJ / (unit.stem + ".flags")
+
+
+def compiled_with(unit: Path) -> str | None:
+    """The flags of the unit's object file (None: not known)."""
+    path = flags_path(unit)
+    return path.read_text() if path.exists() and obj_path(unit).exists() else None
+
+
 def stale(unit: Path, target: Path) -> bool:
     return not target.exists() or any(p.stat().st_mtime > target.stat().st_mtime for p in includes(unit))
 
 
-def needs_build() -> bool:
-    return any(stale(u, LIB) for u in units())
+def needs_build(flags: str = " ".join(NVCC_FLAGS)) -> bool:
+    """Whether a source or an object is newer than the library, or an object was compiled with other flags."""
+    def changed(unit: Path) -> bool:
+        obj = obj_path(unit)
+        unlinked = LIB.exists() and obj.exists() and obj.stat().st_mtime > LIB.stat().st_mtime
+        return stale(unit, LIB) or unlinked or compiled_with(unit) not in (None, flags)
+    return any(changed(u) for u in units())
 
 
 def build_host(force: bool = False, verbose: bool = False) -> Path:
@@ -100,7 +115,8 @@ def build_host(force: bool = False, verbose: bool = False) -> Path:
 def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | None = None) -> Path:
     """Compile the stale translation units of ``csrc`` (in parallel) and link ``libravel_b200.so``, then build
     the host extension."""
-    if not force and not needs_build():
+    flags = " ".join([*NVCC_FLAGS, *(extra_flags or [])])
+    if not force and not needs_build(flags):
         build_host(force=force, verbose=verbose)
         return LIB
     OBJ.mkdir(exist_ok=True)
@@ -111,10 +127,12 @@ def build(force: bool = False, verbose: bool = False, extra_flags: list[str] | N
         cmd = [nvcc_path(), *NVCC_FLAGS, *(extra_flags or []), "-c", "-o", str(tmp), str(unit)]
         if verbose:
             print(" ".join(cmd), flush=True)
+        flags_path(unit).unlink(missing_ok=True)
         subprocess.run(cmd, check=True)
         os.replace(tmp, obj)
+        flags_path(unit).write_text(flags)
 
-    todo = [u for u in units() if force or extra_flags or stale(u, obj_path(u))]
+    todo = [u for u in units() if force or stale(u, obj_path(u)) or compiled_with(u) != flags]
     with ThreadPoolExecutor(max_workers=max(1, len(todo))) as pool:
         list(pool.map(compile_unit, todo))
     tmp = LIB.with_suffix(".so.tmp")
