@@ -426,7 +426,11 @@ int ravel_linear_dz(const void* grad_y, int64_t ldg, const void* z, int64_t ldz,
         const int rc = with_act(act, [&](auto av) -> int {
             return launch(k_linear_dz<T, decltype(av)::value>, grid, 32 * DZ_WARPS, 0, st, 1, a);
         });
-        if (rc != RAVEL_OK || grad_bias == nullptr) return rc;
+        if (rc != RAVEL_OK) return rc;
+        if (a.x != nullptr && M > 0) {
+            if (int e = launch(k_relu_settle<T>, grid, 32 * DZ_WARPS, 0, st, 1, a)) return e;
+        }
+        if (grad_bias == nullptr) return RAVEL_OK;
         return launch(k_col_reduce<T>, dim3(static_cast<unsigned>((N + CR_COLS - 1) / CR_COLS)), CR_COLS * CR_ROWS, 0,
                       st, 1, a.part, static_cast<int>(blocks), N, N, static_cast<T*>(grad_bias),
                       static_cast<T*>(nullptr));

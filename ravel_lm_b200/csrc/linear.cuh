@@ -26,8 +26,8 @@
 //   k_gemv          the forward of one row: a warp (or 2, 4, 8 warps) per weight row, plain 16-byte
 //                   loads, one multiply-add per weight.
 //   k_linear_dz     dz = dy * act'(z) in 16 bits (the operand of the two gradient products) and
-//                   per-block column sums of dz in float32 (the bias gradient) in one pass; for relu
-//                   it adds up again in float32 the few sums whose sign is in doubt.
+//                   per-block column sums of dz in float32 (the bias gradient) in one pass.
+//   k_relu_settle   adds up again in float32 the few of relu's sums whose sign is in doubt, and mends both.
 //   k_col_reduce    those partial sums added in block order: deterministic, no atomics.
 //   k_pad_rows      rows copied to a 16-byte pitch, for operands that TMA cannot read in place.
 //
@@ -646,6 +646,8 @@ __global__ void __launch_bounds__(32 * GV_WARPS) k_gemv(const GemvArgs a) {
 constexpr int DZ_COLS = 256;   // columns per block: 32 lanes x 8
 constexpr int DZ_WARPS = 8;    // rows per block at a time
 constexpr int DZ_ROWS = 2;     // rows per warp whose loads are in flight together
+constexpr int RS_ROWS = 4;     // the same of the pass over relu's sums
+constexpr int RS_SEGMENT = 32; // rows per warp between two looks at those in doubt (a bit each)
 
 struct DzArgs {
     int64_t M, N, ldg, ldz, ldd;
@@ -662,64 +664,6 @@ struct DzArgs {
     int64_t ldx, ldw, K;
 };
 
-// relu's derivative jumps where z changes sign, and a long sum on the tensor cores is off by some K 2^-31 of its
-// terms' size (rms 0.9e-6 at K 2048 and 2e-6 at 4096 for sums of size 1, ten times float32's own): enough to
-// turn one derivative in a million. Sums nearer to zero than ten times that, K 2^-28 of the largest of the row's sums in
-// a window of 256 columns, are added up again in float32, by the whole warp; one in some 10^5 is.  So are all that
-// float16 keeps as its smallest subnormal, whose size is not known (one in 10^3 of sums of size 1e-4), and every sum
-// of a row of fewer than 8, which tell nothing about size.  Exact zeros keep the derivative 0: rows of zeros (padding)
-// and columns of zeros would otherwise be added up for nothing.
-//
-// z: the sums of columns c .. c + 7 where `mine`, else (past the last column) those of the strip before, which only
-// count for the size.
-template <typename T>
-__device__ __forceinline__ void relu_settle(const DzArgs& a, int64_t row, int64_t c, bool mine, float (&z)[8]) {
-    constexpr bool HALF = std::is_same<T, __half>::value;
-    float most = 0.0f, least = INFINITY;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        // a float16 sum that is infinite is of size 65504 at least; an infinite bfloat16 one tells no size
-        const float v = HALF ? fminf(fabsf(z[e]), 65504.0f) : (fabsf(z[e]) < INFINITY ? fabsf(z[e]) : 0.0f);
-        most = fmaxf(most, v);
-        least = fminf(least, fabsf(z[e]));
-    }
-    most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));  // of positive floats
-    float limit = most * static_cast<float>(a.K) * 3.7252903e-9f;
-    if (HALF) limit = fmaxf(limit, 1.5f * F16_TINY);
-    if (a.N < 8) limit = INFINITY;
-    if (most == 0.0f) limit = 0.0f;
-    if (!__any_sync(0xffffffffu, mine && least < limit)) return;
-    unsigned near = 0u;
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-        if (mine && c + e < a.N && z[e] != 0.0f && fabsf(z[e]) < limit) near |= 1u << e;
-    const int lane = threadIdx.x & 31;
-    for (unsigned who = __ballot_sync(0xffffffffu, near != 0u); who != 0u; who &= who - 1u) {
-        const int src = __ffs(static_cast<int>(who)) - 1;
-        const int64_t cs = __shfl_sync(0xffffffffu, c, src);
-        for (unsigned bits = __shfl_sync(0xffffffffu, near, src); bits != 0u; bits &= bits - 1u) {
-            const int e = __ffs(static_cast<int>(bits)) - 1;
-            const T* const x = static_cast<const T*>(a.x) + row * a.ldx;
-            const T* const w = static_cast<const T*>(a.w) + (cs + e) * a.ldw;
-            float acc = 0.0f;
-#pragma unroll 4
-            for (int64_t k = lane * 8; k < a.K; k += 256) {
-                float xf[8], wf[8];
-                unpack8<T>(load8(x, k, a.K, true), xf);
-                unpack8<T>(load8(w, k, a.K, true), wf);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) acc = fmaf(xf[i], wf[i], acc);
-            }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-            if (a.bias != nullptr) acc += static_cast<float>(static_cast<const T*>(a.bias)[cs + e]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (lane == src && i == e) z[i] = acc;
-        }
-    }
-}
-
 // Reads dy and z, writes dz, 6 bytes an element: 16384 x 8192 with gelu in 153 us, 80% of the copy rate (two rows in
 // flight and four blocks an SM; four rows and three blocks were 6 us slower).  The derivative's 20 instructions an element keep the
 // issue slots half busy.
@@ -733,10 +677,7 @@ __global__ void __launch_bounds__(32 * DZ_WARPS, 4) k_linear_dz(const DzArgs a) 
     const int64_t r0 = static_cast<int64_t>(blockIdx.y) * a.rows;
     const int64_t r1 = (r0 + a.rows) < a.M ? (r0 + a.rows) : a.M;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    const bool settle = ACT == RAVEL_ACT_RELU && a.x != nullptr;
-    const bool mine = c < a.N;
-    const bool look = settle && !mine && c >= DZ_COLS;  // lanes past the last column: the strip before, for its size
-    if (mine || settle) {  // settling takes the whole warp
+    if (c < a.N) {
         const T* const gy = static_cast<const T*>(a.gy);
         const T* const zz = static_cast<const T*>(a.z);
         T* const dz = static_cast<T*>(a.dz);
@@ -745,12 +686,9 @@ __global__ void __launch_bounds__(32 * DZ_WARPS, 4) k_linear_dz(const DzArgs a) 
 #pragma unroll
             for (int i = 0; i < DZ_ROWS; ++i) {
                 const int64_t row = r + i * DZ_WARPS;
-                if (row < r1 && mine) {
+                if (row < r1) {
                     gv[i] = load8(gy + row * a.ldg, c, a.N, a.vec_g);
                     if constexpr (ACT != RAVEL_ACT_NONE) zv[i] = load8(zz + row * a.ldz, c, a.N, a.vec_z);
-                } else if constexpr (ACT == RAVEL_ACT_RELU) {
-                    zv[i] = make_uint4(0u, 0u, 0u, 0u);
-                    if (row < r1 && look) zv[i] = load8(zz + row * a.ldz, c - DZ_COLS, a.N, a.vec_z);
                 }
             }
 #pragma unroll
@@ -759,10 +697,6 @@ __global__ void __launch_bounds__(32 * DZ_WARPS, 4) k_linear_dz(const DzArgs a) 
                 if (row < r1) {
                     float g[8], z[8];
                     if constexpr (ACT != RAVEL_ACT_NONE) unpack8<T>(zv[i], z);
-                    if constexpr (ACT == RAVEL_ACT_RELU) {
-                        if (settle) relu_settle<T>(a, row, c, mine, z);
-                    }
-                    if (!mine) continue;
                     unpack8<T>(gv[i], g);
                     if constexpr (ACT != RAVEL_ACT_NONE) {
 #pragma unroll
@@ -785,6 +719,213 @@ __global__ void __launch_bounds__(32 * DZ_WARPS, 4) k_linear_dz(const DzArgs a) 
 #pragma unroll
         for (int w = 0; w < DZ_WARPS; ++w) s += sums[w][threadIdx.x];
         a.part[static_cast<int64_t>(blockIdx.y) * a.N + col] = s;
+    }
+}
+
+// relu's derivative jumps where z changes sign, and a long sum on the tensor cores is off by some K 2^-31 of its
+// terms' size (rms 0.9e-6 at K 2048 and 2e-6 at 4096 for sums of size 1, ten times float32's own): enough to
+// turn one derivative in a million. Sums nearer to zero than ten times that, K 2^-28 of the largest of the row's sums in
+// a window of 256 columns, are added up again in float32, by the whole warp; one in some 10^5 is.  So are all that
+// float16 keeps as its smallest subnormal, whose size is not known (one in 10^3 of sums of size 1e-4), and every sum
+// of a row of fewer than 8, which tell nothing about size.  A sum of exactly 0 may be one that the accumulator's last
+// bit swallowed (one in 10^7 was), so it is added up too, but rows of x (padding) and columns of weights that are zero
+// throughout only once: such a row for the strip, such a column for the block.
+//
+// A pass of its own over z after k_linear_dz, which takes the derivatives from the signs as they stand: within that
+// kernel the whole warp's work took the registers of the loads (16384 x 8192 sums over k 2048, us: 255 inlined, 313 and
+// more as a call, 148 + 93 apart; with one column of weights in ten dead 473, 510, 148 + 178).
+
+// The size below which a sum of the row is in doubt, by the whole warp, and the lane's smallest |z|.  zv: 8 sums of the
+// row a lane; skip: ones in the place of those that need no look (the pairs' minimum takes them for NaN and passes over).
+template <typename T>
+__device__ __forceinline__ float relu_limit(const uint4& zv, const uint32_t (&skip)[4], const DzArgs& a, float& least) {
+    constexpr bool HALF = std::is_same<T, __half>::value;
+    using Two = typename std::conditional<HALF, __half2, __nv_bfloat162>::type;
+    const uint32_t word[4] = {zv.x, zv.y, zv.z, zv.w};
+    auto two = [](uint32_t w) { return __habs2(*reinterpret_cast<const Two*>(&w)); };
+    Two hi = two(word[0]), lo = two(word[0] | skip[0]);
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+        hi = __hmax2(hi, two(word[i]));
+        lo = __hmin2(lo, two(word[i] | skip[i]));
+    }
+    float most = fmaxf(fmaxf(as_float(hi.x), as_float(hi.y)), 0.0f);
+    least = fminf(as_float(lo.x), as_float(lo.y));
+    if (most == INFINITY) {  // in float16 of size 65504 at least; in bfloat16 it tells no size
+        most = HALF ? 65504.0f : 0.0f;
+        float z[8];
+        unpack8<T>(zv, z);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (fabsf(z[e]) < INFINITY) most = fmaxf(most, fabsf(z[e]));
+    }
+    most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));  // of positive floats
+    float limit = most * static_cast<float>(a.K) * 3.7252903e-9f;
+    if (HALF) limit = fmaxf(limit, 1.5f * F16_TINY);
+    if (most == 0.0f) limit = 0.0f;
+    return a.N < 8 ? INFINITY : limit;
+}
+
+// The columns that need no look: those past the last, and the dead ones (a bit for each of the strip's 256).
+__device__ __forceinline__ void relu_skip(uint32_t (&skip)[4], int64_t left, const unsigned* dead) {
+    const int lane = threadIdx.x & 31;
+    const unsigned known = *const_cast<const volatile unsigned*>(dead + (lane >> 2)) >> (8 * (lane & 3));
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if ((known >> e & 1u) != 0u || e >= left) skip[e >> 1] |= 0x7fffu << (16 * (e & 1));
+}
+
+// The signs of the sums in `near` (bits e of lane l: column 8 l + e of the strip whose weights and bias are given) over a
+// row of x, each by the whole warp: a bit for those above 0.  zero: those kept as 0.  The warps start at different
+// columns, so that the block scans a dead column once, not once a warp.
+template <typename T>
+__device__ __forceinline__ unsigned relu_signs(const T* x, const T* weight, int64_t ldw, const T* bias, int64_t K,
+                                            unsigned near, unsigned zero, unsigned* dead) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    unsigned above = 0u;
+    bool blank = false;  // the row of x is zero throughout
+    for (int i = 0; i < 8; ++i) {
+        const int e = (warp + i) & 7;
+        for (unsigned who = __ballot_sync(0xffffffffu, near >> e & 1u); who != 0u; who &= who - 1u) {
+            const int src = __ffs(static_cast<int>(who)) - 1;
+            const bool was_zero = (__shfl_sync(0xffffffffu, zero, src) >> e & 1u) != 0u;
+            unsigned* const mark = dead + (src >> 2);
+            const int bit = 8 * (src & 3) + e;
+            if (was_zero) {
+                const unsigned known = __shfl_sync(0xffffffffu, *const_cast<volatile unsigned*>(mark), 0);
+                if (blank || (known >> bit & 1u) != 0u) continue;
+            }
+            const T* const w = weight + static_cast<int64_t>(src * 8 + e) * ldw;
+            float acc = 0.0f;
+            unsigned xb = 0u, wb = 0u;
+#pragma unroll 4
+            for (int64_t k = lane * 8; k < K; k += 256) {
+                float xf[8], wf[8];
+                const uint4 xv = load8(x, k, K, true), wv = load8(w, k, K, true);
+                xb |= xv.x | xv.y | xv.z | xv.w;
+                wb |= wv.x | wv.y | wv.z | wv.w;
+                unpack8<T>(xv, xf);
+                unpack8<T>(wv, wf);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) acc = fmaf(xf[j], wf[j], acc);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+            if (was_zero) {  // the words' sign bits aside: -0 is zero
+                blank = !__any_sync(0xffffffffu, (xb & 0x7fff7fffu) != 0u);
+                const bool none = !__any_sync(0xffffffffu, (wb & 0x7fff7fffu) != 0u);
+                if (none && lane == 0) atomicOr(mark, 1u << bit);
+            }
+            if (bias != nullptr) acc += static_cast<float>(bias[src * 8 + e]);
+            if (lane == src && acc > 0.0f) above |= 1u << e;
+        }
+    }
+    return above;
+}
+
+// The rows first + 8 i for the bits i of `doubt`: their sums in doubt added up, dz mended where a sign turns, and what
+// that adds to the lane's column sums.
+template <typename T>
+__device__ __noinline__ void relu_rows(const DzArgs& a, int64_t first, unsigned doubt, int64_t c, unsigned* dead,
+                                       float* delta) {
+    const int64_t c0 = c - (threadIdx.x & 31) * 8;
+    const int64_t cw = c < a.N ? c : c - DZ_COLS;
+    for (; doubt != 0u; doubt &= doubt - 1u) {
+        const int64_t row = first + (__ffs(static_cast<int>(doubt)) - 1) * DZ_WARPS;
+        uint4 zv = make_uint4(0u, 0u, 0u, 0u);
+        if (cw >= 0) zv = load8(static_cast<const T*>(a.z) + row * a.ldz, cw, a.N, a.vec_z);
+        uint32_t skip[4] = {0u, 0u, 0u, 0u};
+        relu_skip(skip, a.N - c, dead);
+        float z[8], g[8], least;
+        const float limit = relu_limit<T>(zv, skip, a, least);
+        unpack8<T>(zv, z);
+        unsigned near = 0u, zero = 0u;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if ((skip[e >> 1] >> (16 * (e & 1)) & 0x7fffu) == 0u && fabsf(z[e]) < limit) {
+                near |= 1u << e;
+                if (z[e] == 0.0f) zero |= 1u << e;
+            }
+        }
+        const unsigned above =
+            relu_signs<T>(static_cast<const T*>(a.x) + row * a.ldx, static_cast<const T*>(a.w) + c0 * a.ldw, a.ldw,
+                          a.bias != nullptr ? static_cast<const T*>(a.bias) + c0 : nullptr, a.K, near, zero, dead);
+        if (near == 0u) continue;
+        unpack8<T>(load8(static_cast<const T*>(a.gy) + row * a.ldg, c, a.N, a.vec_g), g);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool was = z[e] > 0.0f, is = (above >> e & 1u) != 0u;
+            if ((near >> e & 1u) == 0u || was == is) continue;
+            const float d = g[e] * (is ? 1.0f : 0.0f);
+            if (a.dz != nullptr) static_cast<T*>(a.dz)[row * a.ldd + c + e] = round_to<T>(d);
+            delta[e] += d - g[e] * (was ? 1.0f : 0.0f);
+        }
+    }
+}
+
+// k_linear_dz's grid and rows.  A lane looks at its 8 columns or, past the last, at those of the strip before, which only
+// count for the size.  The rows with a sum in doubt are noted, RS_SEGMENT of a warp at a time, and gone over then: the
+// call's registers stay out of the loop.  Reads z once: 16384 x 8192 in 64 us where next to none is in doubt (k 256), 64% of
+// the copy rate.
+template <typename T>
+__global__ void __launch_bounds__(32 * DZ_WARPS, 4) k_relu_settle(const __grid_constant__ DzArgs a) {
+    __shared__ float delta[DZ_WARPS][DZ_COLS];  // to add to the block's column sums
+    __shared__ unsigned dead[DZ_COLS / 32];
+    grid_wait();
+    grid_trigger();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * DZ_COLS + lane * 8;
+    const int64_t r0 = static_cast<int64_t>(blockIdx.y) * a.rows;
+    const int64_t r1 = (r0 + a.rows) < a.M ? (r0 + a.rows) : a.M;
+    float* const mine = &delta[warp][lane * 8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) mine[e] = 0.0f;
+    if (threadIdx.x < DZ_COLS / 32) dead[threadIdx.x] = 0u;
+    __syncthreads();
+    bool any = false;
+    const int64_t cw = c < a.N ? c : c - DZ_COLS;
+    const bool wide = a.vec_z && cw >= 0 && cw + 8 <= a.N;
+    const T* const zc = static_cast<const T*>(a.z) + cw;
+    int rows = RS_ROWS;  // the first few find most of the dead columns
+    for (int64_t first = r0 + warp; first < r1; first += static_cast<int64_t>(DZ_WARPS) * rows, rows = RS_SEGMENT) {
+        uint32_t skip[4] = {0u, 0u, 0u, 0u};
+        relu_skip(skip, a.N - c, dead);
+        const int64_t left = (r1 - first + DZ_WARPS - 1) / DZ_WARPS;
+        const int n = left < rows ? static_cast<int>(left) : rows;
+        unsigned doubt = 0u;
+#pragma unroll 1
+        for (int j = 0; j < n; j += RS_ROWS) {
+            const T* const p = zc + (first + static_cast<int64_t>(j) * DZ_WARPS) * a.ldz;
+            uint4 zv[RS_ROWS];
+#pragma unroll
+            for (int i = 0; i < RS_ROWS; ++i) {
+                zv[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (wide && j + i < n) zv[i] = __ldg(reinterpret_cast<const uint4*>(p + i * DZ_WARPS * a.ldz));
+            }
+            if (!wide && cw >= 0) {
+#pragma unroll
+                for (int i = 0; i < RS_ROWS; ++i)
+                    if (j + i < n) zv[i] = load8(p + i * DZ_WARPS * a.ldz, 0, a.N - cw, false);
+            }
+#pragma unroll
+            for (int i = 0; i < RS_ROWS; ++i) {  // rows past the last are zeros, without a limit but where N < 8
+                float least;
+                const float limit = relu_limit<T>(zv[i], skip, a, least);
+                if (__any_sync(0xffffffffu, least < limit) && j + i < n) doubt |= 1u << (j + i);
+            }
+        }
+        if (doubt != 0u) {
+            relu_rows<T>(a, first, doubt, c, dead, mine);
+            any = true;
+        }
+    }
+    if (a.part == nullptr || !__syncthreads_or(any)) return;
+    const int64_t col = static_cast<int64_t>(blockIdx.x) * DZ_COLS + threadIdx.x;
+    if (col < a.N) {
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < DZ_WARPS; ++w) s += delta[w][threadIdx.x];
+        a.part[static_cast<int64_t>(blockIdx.y) * a.N + col] += s;
     }
 }
 

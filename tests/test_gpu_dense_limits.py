@@ -146,3 +146,44 @@ def test_relu_sign_of_a_sum_that_underflows():
             want = torch.full((72,), float(M), device="cuda")
             want[30] = M if sign > 0 else 0
             assert torch.equal(db.float(), want), (M, sign, db[30])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("N,col", [(72, 30), (257, 256), (1, 0)])
+def test_relu_sign_of_a_sum_swallowed_whole(N, col, dtype):
+    """The same without the 2^-20: what an accumulator of some 25 bits leaves of 1 + 255 2^-26 - 1 may be 0."""
+    from ravel_lm_b200.dense import fused_linear
+    for M in (2, 40, 300):
+        for sign in (1.0, -1.0):
+            x, w = near_zero(M, 512, N, col, dtype, sign=sign)
+            w[col, 300] = 0.0
+            assert float(x[0].double() @ w[col].double()) == sign * 255 * 2.0 ** -26
+            b = torch.zeros(N, device="cuda", dtype=dtype).requires_grad_(True)
+            db, = torch.autograd.grad(fused_linear(x, w, b, activation="relu"), b, torch.ones(M, N, device="cuda", dtype=dtype))
+            want = torch.full((N,), float(M), device="cuda", dtype=torch.float64)
+            want[col] = M if sign > 0 else 0
+            assert bool(((db.double() - want).abs() <= U[dtype] * want).all()), (M, sign, db[col])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_relu_of_rows_and_columns_of_zeros(dtype):
+    """Rows of x and columns of weights that are zero throughout (-0 among them) leave the bias; where that is 0 too the
+    derivative is 0.  Beside them the other sums, and in a zero column of weights the sums that a zero bias leaves."""
+    from ravel_lm_b200.dense import fused_linear
+    M, K, N = 700, 1000, 520
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(M, K, generator=g, device="cuda").to(dtype)
+    w = (torch.randn(N, K, generator=g, device="cuda") * K ** -0.5).to(dtype)
+    b = torch.randn(N, generator=g, device="cuda").to(dtype)
+    x[::5] = 0.0
+    x[::10] = -0.0
+    w[::7] = -0.0
+    b[::3] = 0.0
+    z = x.double() @ w.double().t() + b.double()
+    gy = torch.randn(M, N, generator=g, device="cuda").to(dtype)
+    b.requires_grad_(True)
+    db, = torch.autograd.grad(fused_linear(x, w, b, activation="relu"), b, gy)
+    sure = (z == 0) | (z.abs() > (K / 32 + 16) * 2.0 ** -24 * 4)  # as in the general test of signs
+    dz = gy.double() * (z > 0)
+    tol = (M + 8) * 2.0 ** -23 * dz.abs().sum(0) + U[dtype] * dz.sum(0).abs() + (gy.double().abs() * ~sure).sum(0)
+    assert bool(((db.double() - dz.sum(0)).abs() <= tol).all())
