@@ -86,6 +86,8 @@ struct Plan {
 //   single 32: 3.5 / 5.3 / 11.6 / 21.3    single 64: 3.5 / 5.5 / 12.2 / 21.2    single 128: 4.4 / 6.8 / 14.6 / 31.6
 //   pairs 128: 4.4 / 6.7 / 13.7 / 23.8    pairs 256: 6.0 / 10.3 / 23.6 / 41.8
 //   split 2: - / 8.4 / 12.5 / 19.7        split 4: - / 10.7 / 13.5 / 17.4
+// The formula gives split 4 less than that there (- / 8.8 / 10.8 / 13.3), so that it takes 32 tiles over k 4096 from the
+// single CTAs that measured faster.
 Plan plan_matmul(int64_t M, int64_t N, int64_t K, bool b_mn) {
 #ifdef RAVEL_MM_FORCE_SHAPE  // build-time tuning knob (sweeps): cg * 10000 + bn * 10 + splits
     return {RAVEL_MM_FORCE_SHAPE / 10000, RAVEL_MM_FORCE_SHAPE / 10 % 1000, RAVEL_MM_FORCE_SHAPE % 10};

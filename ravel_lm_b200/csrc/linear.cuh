@@ -587,7 +587,7 @@ struct GemvArgs {
 // S warps share a weight row's K, each lane taking 16 bytes of it at a time; the warp's (then the block's, in warp
 // order) partial sums are added and one lane finishes the element.  Bound by HBM: 8192 x 8192 in 24.9 us (82% of the
 // copy rate), 4096 x 4096 in 8.5 (the launch and the first loads' latency are 3).  Two rows and more repeat the
-// loads and conversions of x per weight (4 rows: 24.6 us at 4096 x 4096) and go to the tensor cores (9 us).
+// loads and conversions of x per weight (4 rows: 24.6 us at 4096 x 4096) and go to the tensor cores (11 us).
 template <typename T, int S>
 __global__ void __launch_bounds__(32 * GV_WARPS) k_gemv(const GemvArgs a) {
     __shared__ float part[GV_WARPS];

@@ -18,7 +18,8 @@ divide the contraction over a cluster of CTAs.
 Leading dimensions are arbitrary and may be strided or empty.  Rows that TMA
 cannot read in place (a pitch or an address that is no multiple of 16 bytes)
 are copied once to a padded pitch.  Every result is deterministic.  There is no
-CPU path, no second derivative (``create_graph`` is refused) and no forward-mode
+CPU path, no float32 form (parameters kept in float32, as under autocast, are cast by
+the caller), no second derivative (``create_graph`` is refused) and no forward-mode
 one (tangents are refused).
 """
 from __future__ import annotations

@@ -18,7 +18,10 @@ for an upstream gradient of 1 (``loss.backward()``; ``weight`` scales the loss w
 it is one term of several, so that its upstream gradient stays 1); with any other
 upstream gradient the backward computes it from the logits again, as it does for
 float16 logits and for ``reduction="none"``.  The gradient's memory is thus held from
-the forward on.  Sums are float32; results are deterministic.  There is no CPU path.
+the forward on, until the backward takes it or the graph goes; saved-tensor hooks do not see it.
+The search for entries of the same id costs k^2 a row: some hundreds of entries are cheap, thousands
+take longer than the logits.  Sums are float32, of exponentials of differences from the row's
+largest logit; results are deterministic.  There is no CPU path.
 """
 from __future__ import annotations
 
