@@ -648,6 +648,7 @@ constexpr int DZ_WARPS = 8;    // rows per block at a time
 constexpr int DZ_ROWS = 2;     // rows per warp whose loads are in flight together
 constexpr int RS_ROWS = 4;     // the same of the pass over relu's sums
 constexpr int RS_SEGMENT = 32; // rows per warp between two looks at those in doubt (a bit each)
+constexpr int RS_ZEROS = 4;
 
 struct DzArgs {
     int64_t M, N, ldg, ldz, ldd;
@@ -665,8 +666,8 @@ struct DzArgs {
 };
 
 // Reads dy and z, writes dz, 6 bytes an element: 16384 x 8192 with gelu in 153 us, 80% of the copy rate (two rows in
-// flight and four blocks an SM; four rows and three blocks were 6 us slower).  The derivative's 20 instructions an element keep the
-// issue slots half busy.
+// flight and four blocks an SM; four rows and three blocks were 6 us slower).  The derivative's 20 instructions an
+// element keep the issue slots busy.
 template <typename T, int ACT>
 __global__ void __launch_bounds__(32 * DZ_WARPS, 4) k_linear_dz(const DzArgs a) {
     __shared__ float sums[DZ_WARPS][DZ_COLS];
@@ -729,7 +730,8 @@ __global__ void __launch_bounds__(32 * DZ_WARPS, 4) k_linear_dz(const DzArgs a) 
 // float16 keeps as its smallest subnormal, whose size is not known (one in 10^3 of sums of size 1e-4), and every sum
 // of a row of fewer than 8, which tell nothing about size.  A sum of exactly 0 may be one that the accumulator's last
 // bit swallowed (one in 10^7 was), so it is added up too, but rows of x (padding) and columns of weights that are zero
-// throughout only once: such a row for the strip, such a column for the block.
+// throughout only once: such a row for the strip, such a column for the block.  Where a row still has more than RS_ZEROS
+// zeros among 256 columns they are no accidents (sparse inputs) and stand; only a warp's first row looks at them all.
 //
 // A pass of its own over z after k_linear_dz, which takes the derivatives from the signs as they stand: within that
 // kernel the whole warp's work took the registers of the loads (16384 x 8192 sums over k 2048, us: 255 inlined, 313 and
@@ -824,10 +826,10 @@ __device__ __forceinline__ unsigned relu_signs(const T* x, const T* weight, int6
 }
 
 // The rows first + 8 i for the bits i of `doubt`: their sums in doubt added up, dz mended where a sign turns, and what
-// that adds to the lane's column sums.
+// that adds to the lane's column sums.  opening: `first` is the warp's first row.
 template <typename T>
-__device__ __noinline__ void relu_rows(const DzArgs& a, int64_t first, unsigned doubt, int64_t c, unsigned* dead,
-                                       float* delta) {
+__device__ __noinline__ void relu_rows(const DzArgs& a, int64_t first, unsigned doubt, bool opening, int64_t c,
+                                       unsigned* dead, float* delta) {
     const int64_t c0 = c - (threadIdx.x & 31) * 8;
     const int64_t cw = c < a.N ? c : c - DZ_COLS;
     for (; doubt != 0u; doubt &= doubt - 1u) {
@@ -847,6 +849,7 @@ __device__ __noinline__ void relu_rows(const DzArgs& a, int64_t first, unsigned 
                 if (z[e] == 0.0f) zero |= 1u << e;
             }
         }
+        if (!(opening && row == first) && __reduce_add_sync(0xffffffffu, __popc(zero)) > RS_ZEROS) near &= ~zero;
         const unsigned above =
             relu_signs<T>(static_cast<const T*>(a.x) + row * a.ldx, static_cast<const T*>(a.w) + c0 * a.ldw, a.ldw,
                           a.bias != nullptr ? static_cast<const T*>(a.bias) + c0 : nullptr, a.K, near, zero, dead);
@@ -915,7 +918,7 @@ __global__ void __launch_bounds__(32 * DZ_WARPS, 4) k_relu_settle(const __grid_c
             }
         }
         if (doubt != 0u) {
-            relu_rows<T>(a, first, doubt, c, dead, mine);
+            relu_rows<T>(a, first, doubt, rows == RS_ROWS, c, dead, mine);
             any = true;
         }
     }

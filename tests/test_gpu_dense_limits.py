@@ -187,3 +187,27 @@ def test_relu_of_rows_and_columns_of_zeros(dtype):
     dz = gy.double() * (z > 0)
     tol = (M + 8) * 2.0 ** -23 * dz.abs().sum(0) + U[dtype] * dz.sum(0).abs() + (gy.double().abs() * ~sure).sum(0)
     assert bool(((db.double() - dz.sum(0)).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("density", [0.02, 0.3])
+def test_relu_of_sparse_inputs(density, dtype):
+    """Ones, minus ones and zeros: sums are small whole numbers, many of them 0, and every derivative is known."""
+    from ravel_lm_b200.dense import fused_linear
+    M, K, N = 900, 512, 600
+    g = torch.Generator(device="cuda").manual_seed(2)
+
+    def sparse(*shape):
+        keep = torch.rand(*shape, generator=g, device="cuda") < density
+        sign = torch.where(torch.rand(*shape, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+        return (keep * sign).to(dtype)
+    x, w, b = sparse(M, K), sparse(N, K), sparse(N)
+    z = x.double() @ w.double().t() + b.double()
+    assert float((z == 0).double().mean()) > 0.02
+    for t in (x, w, b):
+        t.requires_grad_(True)
+    gy = torch.ones(M, N, device="cuda", dtype=dtype)
+    dx, dw, db = torch.autograd.grad(fused_linear(x, w, b, activation="relu"), [x, w, b], gy)
+    dz = (z > 0).double()
+    for got, want in ((dx, dz @ w.detach().double()), (dw, dz.t() @ x.detach().double()), (db, dz.sum(0))):
+        assert bool(((got.double() - want).abs() <= U[dtype] * want.abs()).all())  # whole numbers, rounded once
