@@ -436,6 +436,102 @@ int ravel_distill_topk_bwd(const void* logits, int64_t ld, const void* ids, int 
                            int grad_is_unit, void* grad, int dtype, void* stream);
 
 /*
+ * Token embedding: y[i] = scale weight[ids[i]], N rows of K elements (weight's
+ * rows ldw apart, y contiguous), float32, bfloat16 or float16.  An id outside
+ * [0, V) gives a row of zeros and sets RAVEL_DEVERR_INDEX.
+ */
+int ravel_embedding_fwd(const void* ids, int ids_dtype, const void* weight, int64_t ldw, int64_t N, int64_t V, int64_t K,
+                        float scale, void* y, int dtype, void* stream);
+
+/*
+ * Its gradient: grad_weight[v] = scale sum over the i with ids[i] = v of grad_y[i], all V rows
+ * written (contiguous); none from rows whose id is padding_idx or outside [0, V).
+ * Sums in float32 in a fixed order of the sorted positions, without atomics.
+ */
+size_t ravel_embedding_scratch_bytes(int64_t N, int64_t V, int64_t K);
+int ravel_embedding_bwd(const void* ids, int ids_dtype, const void* grad_y, int64_t ldg, int64_t N, int64_t V, int64_t K,
+                        float scale, int64_t padding_idx, void* grad_weight, int dtype, void* scratch,
+                        size_t scratch_bytes, void* stream);
+
+/*
+ * Softmax cross entropy of z = x weight^T (x [M, K], rows ldx apart; weight [V, K],
+ * 16-byte rows; bfloat16 or float16) against targets [M], without keeping z:
+ *   losses[i] = log sum_v exp z_iv - z_i,t;  0 where targets[i] is ignore_index
+ * A target outside [0, V) that is not ignore_index counts as ignored and sets
+ * RAVEL_DEVERR_INDEX.  out: their sum (RAVEL_REDUCE_SUM) or mean over the rows with a target (_MEAN).
+ *
+ * A training step gives slabs_x and slabs_w (either may be NULL): float32
+ * sums of the gradients for an upstream gradient of 1, sizes[0] slabs of M rows and
+ * sizes[1] slabs of V rows, rows sizes[2] floats apart (ravel_linear_ce_slabs);
+ * factor (one float) goes with them.  ravel_linear_ce_bwd adds the slabs up, scales
+ * them by *up (device) and rounds: grad_x [M, K], grad_w [V, K], contiguous.
+ * Single rows' losses (RAVEL_REDUCE_NONE) get their gradients from
+ * ravel_linear_ce_grad, given the forward's scratch and up [M]; then ravel_linear_ce_bwd
+ * with up NULL.  work is needed during a call only.
+ */
+size_t ravel_linear_ce_scratch_bytes(int64_t M, int64_t K, int64_t V);
+size_t ravel_linear_ce_work_bytes(int64_t M, int64_t K, int64_t V, int grads);
+int ravel_linear_ce_slabs(int64_t M, int64_t K, int64_t V, int64_t* sizes);
+int ravel_linear_ce_fwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* targets,
+                        int target_dtype, int64_t M, int64_t K, int64_t V, int64_t ignore_index, int reduction,
+                        float* losses, float* out, float* factor, float* slabs_x, float* slabs_w, int dtype,
+                        void* scratch, size_t scratch_bytes, void* work, size_t work_bytes, void* stream);
+int ravel_linear_ce_grad(const void* weight, int64_t ldw, const float* up, int64_t M, int64_t K, int64_t V, float* factor,
+                         float* slabs_x, float* slabs_w, int dtype, void* scratch, size_t scratch_bytes, void* work,
+                         size_t work_bytes, void* stream);
+int ravel_linear_ce_bwd(const float* slabs_x, const float* slabs_w, const float* up, const float* factor, int64_t M,
+                        int64_t K, int64_t V, void* grad_x, void* grad_w, int dtype, void* stream);
+
+/*
+ * ---- the optimizer step -------------------------------------------------
+ * One tensor of a list (host memory; the pointers are device pointers): n
+ * elements each, adjacent.  param and grad have the list's type; master (float32)
+ * is what a 16-bit parameter is rounded from, NULL for float32 parameters.  With
+ * 32-bit states exp_avg and exp_avg_sq are float32 and the exponents NULL; with
+ * 8-bit states they are one byte an element, and the exponents one a block of 256
+ * elements, (n + 255) / 256 of them: exp_avg sign, 4 bits of exponent and 3 of mantissa,
+ * exp_avg_sq 5 and 3, below 2^exponent (code c of exponent field f > 0 is
+ * (1 + (c & 7) / 8) 2^(f - 15), 31 for exp_avg_sq, and (c & 7) 2^-17, 2^-33 for
+ * f = 0, times 2^exponent; exponent -128: NaN).
+ */
+typedef struct {
+    void* param;
+    const void* grad;
+    float* master;
+    void* exp_avg;
+    void* exp_avg_sq;
+    signed char* exp_avg_exponents;
+    signed char* exp_avg_sq_exponents;
+    int64_t n;
+} ravel_adamw_tensor;
+
+/* *norm (float64, device) = the 2-norm over every tensor's gradient; param and
+ * states are not read.  Deterministic: a part per block, added in order. */
+size_t ravel_grad_norm_scratch_bytes(const ravel_adamw_tensor* tensors, int64_t count);
+int ravel_grad_norm(const ravel_adamw_tensor* tensors, int64_t count, int dtype, double* norm, void* scratch,
+                    size_t scratch_bytes, void* stream);
+
+/*
+ * One AdamW step (decoupled weight decay; the reference's optimizer is FlatAdamW,
+ * ravel_lm/runtime.py:44): *step (device) counts up by one, then for every element in float32
+ *   g' = g min(1, max_norm / (*norm + 1e-6))   (norm, from ravel_grad_norm, NULL: g)
+ *   m = beta1 m + (1 - beta1) g',  v = beta2 v + (1 - beta2) g'^2
+ *   p = p (1 - lr wd) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * lr_device (one float32 on the device) is taken in place of lr where given.
+ * norm_out (NULL: not wanted) receives the norm in float32.  8-bit states are
+ * rounded stochastically by a hash of the step, the tensor's place in the list and
+ * the element: the same call gives the same bits.  No tensor may appear twice.
+ */
+size_t ravel_adamw_scratch_bytes(void);
+int ravel_adamw(const ravel_adamw_tensor* tensors, int64_t count, int dtype, int state_bits, int64_t* step, double lr,
+                const float* lr_device, double beta1, double beta2, double eps, double weight_decay, double max_norm,
+                const double* norm, float* norm_out, void* scratch, size_t scratch_bytes, void* stream);
+
+/* The values of n 8-bit codes (is_signed: exp_avg's, else exp_avg_sq's) as float32 or bfloat16. */
+int ravel_state_values(const void* codes, const signed char* exponents, int64_t n, int is_signed, void* out, int dtype,
+                       void* stream);
+
+/*
  * Poll limit of every wait on another block, on the current device (default
  * 2^22 polls, about a second of waiting; 1 .. 2^28).  A copy to device memory:
  * call it between steps, not while a stream is being captured.

@@ -35,6 +35,12 @@ _c_int = ctypes.c_int
 _c_vp = ctypes.c_void_p
 _c_sz = ctypes.c_size_t
 
+class AdamTensor(ctypes.Structure):
+    """``ravel_adamw_tensor``."""
+    _fields_ = [(n, _c_vp) for n in ("param", "grad", "master", "exp_avg", "exp_avg_sq", "exp_avg_exponents",
+                                     "exp_avg_sq_exponents")] + [("n", _c_i64)]
+
+
 # name -> (restype, argtypes); the order follows include/ravel_b200.h
 SIGNATURES = {
     "ravel_tape_bytes": (_c_sz, [_c_i64, _c_i64, _c_i64, _c_i64, _c_int]),
@@ -92,6 +98,24 @@ SIGNATURES = {
                                [ctypes.c_float, ctypes.c_float, _c_int] + [_c_vp] * 4 + [_c_int, _c_vp, _c_sz, _c_vp]),
     "ravel_distill_topk_bwd": (_c_int, [_c_vp, _c_i64, _c_vp, _c_int, _c_vp, _c_int] + [_c_i64] * 3 +
                                [ctypes.c_float, ctypes.c_float, _c_int] + [_c_vp] * 3 + [_c_int, _c_vp, _c_int, _c_vp]),
+    "ravel_embedding_fwd": (_c_int, [_c_vp, _c_int, _c_vp] + [_c_i64] * 4 + [ctypes.c_float, _c_vp, _c_int, _c_vp]),
+    "ravel_embedding_scratch_bytes": (_c_sz, [_c_i64] * 3),
+    "ravel_embedding_bwd": (_c_int, [_c_vp, _c_int, _c_vp] + [_c_i64] * 4 + [ctypes.c_float, _c_i64, _c_vp, _c_int, _c_vp,
+                                     _c_sz, _c_vp]),
+    "ravel_linear_ce_scratch_bytes": (_c_sz, [_c_i64] * 3),
+    "ravel_linear_ce_work_bytes": (_c_sz, [_c_i64] * 3 + [_c_int]),
+    "ravel_linear_ce_slabs": (_c_int, [_c_i64] * 3 + [ctypes.POINTER(_c_i64)]),
+    "ravel_linear_ce_fwd": (_c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_int] + [_c_i64] * 4 + [_c_int] + [_c_vp] * 5 +
+                            [_c_int, _c_vp, _c_sz, _c_vp, _c_sz, _c_vp]),
+    "ravel_linear_ce_grad": (_c_int, [_c_vp, _c_i64, _c_vp] + [_c_i64] * 3 + [_c_vp] * 3 +
+                             [_c_int, _c_vp, _c_sz, _c_vp, _c_sz, _c_vp]),
+    "ravel_linear_ce_bwd": (_c_int, [_c_vp] * 4 + [_c_i64] * 3 + [_c_vp, _c_vp, _c_int, _c_vp]),
+    "ravel_grad_norm_scratch_bytes": (_c_sz, [ctypes.POINTER(AdamTensor), _c_i64]),
+    "ravel_grad_norm": (_c_int, [ctypes.POINTER(AdamTensor), _c_i64, _c_int, _c_vp, _c_vp, _c_sz, _c_vp]),
+    "ravel_adamw_scratch_bytes": (_c_sz, []),
+    "ravel_adamw": (_c_int, [ctypes.POINTER(AdamTensor), _c_i64, _c_int, _c_int, _c_vp, ctypes.c_double, _c_vp] +
+                    [ctypes.c_double] * 5 + [_c_vp, _c_vp, _c_vp, _c_sz, _c_vp]),
+    "ravel_state_values": (_c_int, [_c_vp, _c_vp, _c_i64, _c_int, _c_vp, _c_int, _c_vp]),
     "ravel_set_wait_limit": (_c_int, [ctypes.c_uint32]),
     "ravel_wait_selftest": (_c_int, [_c_vp, _c_vp]),
     "ravel_device_error": (_c_int, [ctypes.POINTER(_c_int), _c_vp]),

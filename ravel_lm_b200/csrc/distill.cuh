@@ -25,6 +25,7 @@
 #include "colsum.cuh"
 #include "host.cuh"
 #include "norm.cuh"
+#include "softmax.cuh"
 
 namespace ravel {
 
@@ -96,41 +97,6 @@ __device__ __forceinline__ float distill_counted(const DistillArgs& a) {
     return fmaxf(static_cast<float>(n), 1.0f);
 }
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// x[i] = (x[i] - m) c for an even number of elements, two an instruction.
-template <int E>
-__device__ __forceinline__ void sub_scale(float (&x)[E], float m, float c) {
-    uint64_t m2, c2;
-    asm("mov.b64 %0, {%1, %1};" : "=l"(m2) : "f"(-m));
-    asm("mov.b64 %0, {%1, %1};" : "=l"(c2) : "f"(c));
-#pragma unroll
-    for (int e = 0; e < E; e += 2)
-        asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%0, %1};\n\tadd.rn.f32x2 t, t, %2;\n\tmul.rn.f32x2 t, t, %3;\n\t"
-            "mov.b64 {%0, %1}, t;\n\t}"
-            : "+f"(x[e]), "+f"(x[e + 1])
-            : "l"(m2), "l"(c2));
-}
-
-// Running (maximum, sum of 2^((x - maximum) c)); an empty one is (-inf, 0).
-struct MaxSum {
-    float m, l;
-};
-__device__ __forceinline__ float finite_ref(float m) { return m == -INFINITY ? 0.0f : m; }
-// The warp's (maximum, sum): the maxima first, then one rescaling of each lane's sum.
-__device__ __forceinline__ MaxSum warp_join(MaxSum v, float c) {
-    float m = v.m;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float l = v.l * ex2((v.m - finite_ref(m)) * c);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    return {m, l};
-}
 template <int TH>
 __device__ __forceinline__ MaxSum block_join(MaxSum v, float c, MaxSum* red) {
     v = warp_join(v, c);

@@ -1,0 +1,494 @@
+// head.cuh -- softmax cross entropy of a Linear's outputs over a vocabulary, without keeping those outputs.
+//
+// Row i of x [M, K] has the logits z_v = x_i . W_v (bfloat16 or float16 operands, float32 sums) and a target t:
+//
+//   loss_i = log sum_v exp z_v - z_t
+//   d z_v  = u_i (exp(z_v) / sum - [v = t]),   d x = d z W,   d W = d z^T x
+//
+// A row without a target (the ignored index) has loss 0 and gradient 0, whatever its x holds.
+//
+//   k_head_prep    targets as int32 (-1: none), and x with the rows that have none zeroed.
+//   k_head_logits  the logits' product, on the pairs and single CTAs of k_matmul.  The logits never leave the SM:
+//     HEAD_STATS   a thread owns a row of the tile and keeps the maximum and the sum of 2^((z - max) log2 e) over its
+//                  columns, the target's column apart (so that a confident row's 1 - p_t is no difference), a
+//                  part per row and half tile in memory; the target's logit is kept.
+//     HEAD_EXP     with the row's maximum and sum known: d z in 16 bits (the tensor cores' operand), for a piece
+//                  of the rows.
+//   k_head_rows    the parts of a row joined: loss, maximum, log2 of the sum, 1 - p_t.
+//   k_head_grad    d x and d W of a piece as float32 products, k divided over splits whose sums lie in slabs of their
+//                  own; d W adds up over the pieces.
+//   k_head_out     slabs added in order, scaled by the upstream gradient, rounded once.
+//   k_head_total   losses added in a fixed order, rows counted.
+// float16: d z is kept times 2^15, so that probabilities down to 2^-29 stay normal numbers.
+// Every wait is bounded, as k_matmul's.
+#pragma once
+
+#include "mma.cuh"
+#include "softmax.cuh"
+
+namespace ravel {
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+enum HeadMode { HEAD_STATS = 0, HEAD_EXP = 1 };
+
+struct HeadLogitsArgs : MmShape {
+    int64_t M;                 // rows of the piece
+    int V;
+    const int32_t* target;     // [M], -1: none
+    float2* part;              // STATS: [2 ntiles][M]
+    float* zt;                 // STATS: [M] the target's logit
+    const float4* stat;        // EXP: [M] (max, log2 sum, 1 - p_t, live)
+    const float* up;           // EXP: a row's upstream gradient, or null
+    const float* up_max;       //   and the largest of them
+    float unit_log2;           // EXP: log2 of what d z is kept times
+    void* dz;                  // EXP: [M], rows ldz apart
+    int64_t ldz;
+    unsigned int* err;
+    const unsigned int* wait_limit;
+};
+
+struct HeadGradArgs : MmShape {
+    int64_t M, N;              // outputs; N without its padding
+    int splits;
+    float* out;                // [splits][M], rows ldo apart (a multiple of 4)
+    int64_t ldo, slab;
+    int add;                   // to what is there
+    unsigned int* err;
+    const unsigned int* wait_limit;
+};
+
+// ------------------------------------------------------------------ a product's CTA
+struct MmCta {
+    uint32_t base, sbar, tmem, rank, limit;
+    unsigned char* gen;        // base as a generic address
+    volatile int* abort;
+    int warp, lane;
+};
+// Barriers, tensor memory and (pairs) the other CTA; returns with the previous kernel's writes visible.
+template <int CG, uint32_t COLS>
+__device__ __forceinline__ MmCta mm_begin(unsigned char* smem_raw, int stages, const CUtensorMap* map_a,
+                                          const CUtensorMap* map_b, const unsigned int* wait_limit) {
+    MmCta c;
+    const uint32_t raw = static_cast<uint32_t>(__cvta_generic_to_shared(smem_raw));
+    c.base = (raw + 1023u) & ~1023u;  // swizzled tiles need 1024-byte alignment
+    c.gen = smem_raw + (c.base - raw);
+    c.sbar = c.base + MM_RING + MM_EPI_WARPS * MM_EPI_BYTES;
+    const uint32_t bar_tfull = c.sbar + 16 * MM_MAX_STAGES, bar_tempty = bar_tfull + 16;
+    unsigned char* const tail = c.gen + (bar_tempty + 16 - c.base);
+    c.abort = reinterpret_cast<volatile int*>(tail + 4);
+    c.warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+    c.lane = threadIdx.x & 31;
+    c.rank = CG == 2 ? cluster_rank() : 0u;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(c.sbar + 8 * s, 1);
+            mbar_init(c.sbar + 8 * MM_MAX_STAGES + 8 * s, 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(bar_tfull + 8 * b, 1);
+            mbar_init(bar_tempty + 8 * b, CG * MM_EPI_WARPS);
+        }
+        *c.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (threadIdx.x == 32) {
+        prefetch_map(map_a);
+        prefetch_map(map_b);
+    }
+    if (c.warp == 2) tmem_alloc<CG>(bar_tempty + 16, COLS);
+    tc_fence_before();
+    __syncthreads();
+    if (CG == 2) cluster_sync_all();
+    tc_fence_after();
+    c.tmem = *reinterpret_cast<volatile uint32_t*>(tail);
+    grid_wait();
+    grid_trigger();
+    c.limit = 4u * *const_cast<volatile const unsigned int*>(wait_limit);
+    return c;
+}
+// Nobody leaves while its shared memory, barriers or TMEM may still be used by the other CTA.
+template <int CG, uint32_t COLS>
+__device__ __forceinline__ void mm_end(const MmCta& c, unsigned int* err) {
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (CG == 2) cluster_sync_all();
+    tc_fence_after();
+    if (*c.abort && threadIdx.x == 0) atomicOr(err, RAVEL_DEVERR_SPIN);
+    if (c.warp == 2) tmem_free<CG>(c.tmem, COLS);
+}
+
+// ------------------------------------------------------------------ the logits
+// T: element type.  CG, BN as k_matmul's: CTAs per product and a tile's columns.
+template <typename T, int CG, int BN, int MODE>
+__global__ void __launch_bounds__(MM_THREADS, 1)
+    k_head_logits(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                  const __grid_constant__ HeadLogitsArgs a) {
+    constexpr uint32_t COLS = 2 * BN;
+    constexpr int UNITS = BN / 64;  // 32-column units of an epilogue warp
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    extern __shared__ unsigned char smem_raw[];
+    const MmCta c = mm_begin<CG, COLS>(smem_raw, a.stages, &map_a, &map_b, a.wait_limit);
+    const int tiles = a.mtiles * a.ntiles;
+    const int t0 = static_cast<int>(blockIdx.x) / CG, tstep = static_cast<int>(gridDim.x) / CG;
+    const auto unit = [&](int j, int& mt, int& nt, int& c0, int& c1) {
+        const int t = t0 + j * tstep;
+        if (t >= tiles) return false;
+        mm_tile(a, t, mt, nt);
+        c0 = 0;
+        c1 = a.ksteps;
+        return true;
+    };
+    if (c.warp == 0 && elect_one()) {
+        mm_load<CG, BN, false, false>(a, &map_a, &map_b, c.base, c.sbar, c.rank, c.limit, c.abort, unit);
+    } else if (c.warp == 1 && (CG == 1 || c.rank == 0) && elect_one()) {
+        mm_issue<CG, BN, false, false, 2, BF16>(a, c.base, c.sbar, c.tmem, c.limit, c.abort, unit);
+    } else if (c.warp >= 4) {
+        const int q = c.warp & 3, half = (c.warp - 4) >> 2, lane = c.lane;
+        unsigned char* const st = c.gen + MM_RING + (c.warp - 4) * MM_EPI_BYTES;
+        const uint32_t bar_tfull = c.sbar + 16 * MM_MAX_STAGES, bar_tempty = bar_tfull + 16;
+        const uint32_t done_bar = map_to_rank(bar_tempty, 0u);
+        int mt, nt, k0, k1;
+        for (uint32_t j = 0; unit(static_cast<int>(j), mt, nt, k0, k1); ++j) {
+            const uint32_t buf = j % 2;
+            const int64_t m0 = static_cast<int64_t>(mt) * (MM_BM * CG) + c.rank * MM_BM + q * 32, row = m0 + lane;
+            const int n0 = nt * BN + half * UNITS * 32;
+            const bool rows = m0 < a.M;  // the same for the whole warp
+            int t = -1;
+            MaxSum v = {-INFINITY, 0.0f};
+            float zt = 0.0f;
+            // EXP: d z = +- 2^((z - max) log2 e + e0), the target's column, and which bits of a packed pair live
+            float top = 0.0f, e0 = 0.0f, tv = 0.0f;
+            uint32_t keep = 0u, sign = 0u;
+            if (row < a.M) {
+                t = a.target[row];
+                if constexpr (MODE == HEAD_EXP) {
+                    const float4 s = a.stat[row];
+                    float u = 1.0f;
+                    if (a.up != nullptr) u = a.up[row] / *a.up_max;
+                    const bool live = s.w != 0.0f && u != 0.0f;
+                    top = s.x;
+                    e0 = a.unit_log2 - s.y + log2f(fabsf(u));
+                    tv = -s.z * ex2(a.unit_log2) * fabsf(u);
+                    keep = live ? 0xffffffffu : 0u;
+                    sign = u < 0.0f ? 0x80008000u : 0u;
+                }
+            }
+            const bool ok = __all_sync(0xffffffffu, mm_wait(bar_tfull + 8 * buf, (j / 2) & 1, c.limit, c.abort));
+            tc_fence_after();
+            if (!ok) break;
+            const uint32_t tm = c.tmem + buf * BN + (static_cast<uint32_t>(q * 32) << 16) + half * UNITS * 32;
+#pragma unroll 1
+            for (int u = 0; u < UNITS; ++u) {
+                const int col = n0 + u * 32;
+                uint32_t r[32];
+                tmem_ld32(tm + u * 32, r);
+                if (u == UNITS - 1) {  // this warp has read its part of the accumulator
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(done_bar + 8 * buf);
+                }
+                if (!rows || col >= a.V) continue;
+                float x[32];
+#pragma unroll
+                for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(r[e]);
+                const bool here = __any_sync(0xffffffffu, t >= col && t < col + 32);
+                if constexpr (MODE == HEAD_STATS) {
+                    if (here) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (col + e == t) {
+                                zt = x[e];
+                                x[e] = -INFINITY;
+                            }
+                    }
+                    if (col + 32 > a.V) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (col + e >= a.V) x[e] = -INFINITY;
+                    }
+                    if (here && t >= col && t < col + 32) a.zt[row] = zt;
+                    float m = -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) m = fmaxf(m, x[e]);
+                    if (m > v.m) {
+                        v.l *= ex2((v.m - m) * LOG2E);
+                        v.m = m;
+                    }
+                    sub_scale<32>(x, finite_ref(v.m), LOG2E);
+                    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) s[e & 3] += ex2(x[e]);
+                    v.l += (s[0] + s[1]) + (s[2] + s[3]);
+                } else {
+                    sub_fma<32>(x, top, LOG2E, e0);
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) x[e] = ex2(x[e]);
+                    if (here) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (col + e == t) x[e] = tv;
+                    }
+#pragma unroll
+                    for (int p = 0; p < 4; ++p) {
+                        uint4 w;
+                        uint32_t* const wp = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            wp[e] = (pack2<T>(x[p * 8 + 2 * e], x[p * 8 + 2 * e + 1]) ^ sign) & keep;
+                        *reinterpret_cast<uint4*>(st + epi_piece(lane, p)) = w;
+                    }
+                    __syncwarp();
+                    epi_store(st, static_cast<T*>(a.dz), a.ldz, m0, a.M, col, a.V, true, lane);
+                    __syncwarp();
+                }
+            }
+            if constexpr (MODE == HEAD_STATS) {
+                if (row < a.M) a.part[static_cast<int64_t>(nt * 2 + half) * a.M + row] = make_float2(v.m, v.l);
+            }
+        }
+    }
+    mm_end<CG, COLS>(c, a.err);
+}
+
+// ------------------------------------------------------------------ the gradients' products
+// A: d z [rows][V] (A_MN false: d x, k over the vocabulary) or its transpose (true: d W, k over the rows); B [k][N].
+template <typename T, int CG, int BN, bool A_MN>
+__global__ void __launch_bounds__(MM_THREADS, 1)
+    k_head_grad(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                const __grid_constant__ HeadGradArgs a) {
+    constexpr uint32_t COLS = 2 * BN;
+    constexpr int UNITS = BN / 64;
+    constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
+    static_assert(BN / CG % 64 == 0, "MN-major tiles come in blocks of 64");
+    extern __shared__ unsigned char smem_raw[];
+    const MmCta c = mm_begin<CG, COLS>(smem_raw, a.stages, &map_a, &map_b, a.wait_limit);
+    const int units = a.mtiles * a.ntiles * a.splits;
+    const int t0 = static_cast<int>(blockIdx.x) / CG, tstep = static_cast<int>(gridDim.x) / CG;
+    int split = 0;
+    const auto unit = [&](int j, int& mt, int& nt, int& c0, int& c1) {
+        const int t = t0 + j * tstep;
+        if (t >= units) return false;
+        const int tile = t / a.splits;
+        split = t - tile * a.splits;
+        mm_tile(a, tile, mt, nt);
+        c0 = static_cast<int>(static_cast<int64_t>(a.ksteps) * split / a.splits);
+        c1 = static_cast<int>(static_cast<int64_t>(a.ksteps) * (split + 1) / a.splits);
+        return true;
+    };
+    if (c.warp == 0 && elect_one()) {
+        mm_load<CG, BN, A_MN, true>(a, &map_a, &map_b, c.base, c.sbar, c.rank, c.limit, c.abort, unit);
+    } else if (c.warp == 1 && (CG == 1 || c.rank == 0) && elect_one()) {
+        mm_issue<CG, BN, A_MN, true, 2, BF16>(a, c.base, c.sbar, c.tmem, c.limit, c.abort, unit);
+    } else if (c.warp >= 4) {
+        const int q = c.warp & 3, half = (c.warp - 4) >> 2, lane = c.lane;
+        unsigned char* const st = c.gen + MM_RING + (c.warp - 4) * MM_EPI_BYTES;
+        const uint32_t bar_tfull = c.sbar + 16 * MM_MAX_STAGES, bar_tempty = bar_tfull + 16;
+        const uint32_t done_bar = map_to_rank(bar_tempty, 0u);
+        int mt, nt, k0, k1;
+        for (uint32_t j = 0; unit(static_cast<int>(j), mt, nt, k0, k1); ++j) {
+            const uint32_t buf = j % 2;
+            const int64_t m0 = static_cast<int64_t>(mt) * (MM_BM * CG) + c.rank * MM_BM + q * 32;
+            const int64_t n0 = static_cast<int64_t>(nt) * BN + half * UNITS * 32;
+            float* const out = a.out + split * a.slab;
+            const bool ok = __all_sync(0xffffffffu, mm_wait(bar_tfull + 8 * buf, (j / 2) & 1, c.limit, c.abort));
+            tc_fence_after();
+            if (!ok) break;
+            const uint32_t tm = c.tmem + buf * BN + (static_cast<uint32_t>(q * 32) << 16) + half * UNITS * 32;
+#pragma unroll 1
+            for (int u = 0; u < UNITS; ++u) {
+                const int64_t col = n0 + u * 32;
+                uint32_t r[32];
+                tmem_ld32(tm + u * 32, r);
+                if (u == UNITS - 1) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(done_bar + 8 * buf);
+                }
+                if (m0 >= a.M || col >= a.N) continue;
+                // 32 rows of 128 bytes, their 16-byte pieces rotated against bank conflicts, then whole rows out
+#pragma unroll
+                for (int p = 0; p < 8; ++p)
+                    *reinterpret_cast<uint4*>(st + lane * 128 + ((p ^ (lane & 7)) << 4)) =
+                        make_uint4(r[4 * p], r[4 * p + 1], r[4 * p + 2], r[4 * p + 3]);
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int rw = i * 4 + (lane >> 3), p = lane & 7;
+                    if (m0 + rw < a.M && col + p * 4 < a.ldo) {  // rows are padded to 4: what B lacks there is zero
+                        float4 v = *reinterpret_cast<const float4*>(st + rw * 128 + ((p ^ (rw & 7)) << 4));
+                        float4* const o = reinterpret_cast<float4*>(out + (m0 + rw) * a.ldo + col + p * 4);
+                        if (a.add) {
+                            const float4 w = *o;
+                            v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+                        }
+                        *o = v;
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    }
+    mm_end<CG, COLS>(c, a.err);
+}
+
+// ------------------------------------------------------------------ around the products
+struct HeadPrepArgs {
+    const void* targets;   // [M]
+    int targets64;
+    int64_t M, V, ignore;
+    int32_t* target;       // [M]
+    const void* x;         // [M, K], rows ldx apart
+    void* clean;           // [M, K], rows ldc apart (16 bytes), or null
+    int64_t K, ldx, ldc;
+    int vec;               // x has 16-byte rows
+    unsigned int* err;
+};
+// A warp per row.
+template <typename T>
+__global__ void __launch_bounds__(256) k_head_prep(const HeadPrepArgs a) {
+    grid_wait();
+    grid_trigger();
+    const int lane = threadIdx.x & 31;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); i < a.M;
+         i += static_cast<int64_t>(gridDim.x) * 8) {
+        const int64_t t = a.targets64 ? static_cast<const int64_t*>(a.targets)[i] : static_cast<const int32_t*>(a.targets)[i];
+        const bool in = t >= 0 && t < a.V, live = in && t != a.ignore;
+        if (lane == 0) {
+            if (!in && t != a.ignore) atomicOr(a.err, RAVEL_DEVERR_INDEX);
+            a.target[i] = live ? static_cast<int32_t>(t) : -1;
+        }
+        if (a.clean == nullptr) continue;
+        const T* const x = static_cast<const T*>(a.x) + i * a.ldx;
+        T* const d = static_cast<T*>(a.clean) + i * a.ldc;
+#pragma unroll 4
+        for (int64_t c = lane * 8; c < a.K; c += 256)
+            store8(d, c, a.K, true, live ? load8(x, c, a.K, a.vec) : make_uint4(0u, 0u, 0u, 0u));
+    }
+}
+
+constexpr int HR_ROWS = 32, HR_GROUPS = 16;
+// loss, and stat = (max, log2 sum, 1 - p_t, live); HR_GROUPS groups of threads share a row's parts.
+__global__ void __launch_bounds__(HR_ROWS* HR_GROUPS) k_head_rows(const float2* __restrict__ part, int parts, int64_t M,
+                                                                  const int32_t* __restrict__ target,
+                                                                  const float* __restrict__ zt, float* __restrict__ losses,
+                                                                  float4* __restrict__ stat) {
+    __shared__ MaxSum red[HR_GROUPS][HR_ROWS];
+    grid_wait();
+    grid_trigger();
+    const int x = threadIdx.x % HR_ROWS, y = threadIdx.x / HR_ROWS;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * HR_ROWS + x;
+    auto join = [](MaxSum& v, float m, float l) {
+        const float t = fmaxf(v.m, m), f = finite_ref(t);
+        v.l = v.l * ex2((v.m - f) * LOG2E) + l * ex2((m - f) * LOG2E);
+        v.m = t;
+    };
+    MaxSum v = {-INFINITY, 0.0f};
+    if (row < M) {
+#pragma unroll 4
+        for (int p = y; p < parts; p += HR_GROUPS) {
+            const float2 w = part[static_cast<int64_t>(p) * M + row];
+            join(v, w.x, w.y);
+        }
+    }
+    red[y][x] = v;
+    __syncthreads();
+    if (y != 0 || row >= M) return;
+#pragma unroll
+    for (int g = 1; g < HR_GROUPS; ++g) join(v, red[g][x].m, red[g][x].l);
+    if (target[row] < 0) {
+        losses[row] = 0.0f;
+        if (stat != nullptr) stat[row] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        return;
+    }
+    // the others' sum and the target's term under one maximum
+    const float z = zt[row], m = fmaxf(v.m, z);
+    const float others = v.l * ex2((v.m - finite_ref(m)) * LOG2E), mine = ex2((z - m) * LOG2E), l = others + mine;
+    losses[row] = (m - z) + (mine == 1.0f ? log1pf(others) : logf(l));
+    if (stat != nullptr) stat[row] = make_float4(m, log2f(l), others / l, 1.0f);
+}
+
+// out = the losses' sum (MEAN: over the rows with a target), *factor = 1 or 1 / rows: one block, a fixed order.
+template <bool MEAN>
+__global__ void __launch_bounds__(1024) k_head_total(const float* __restrict__ losses, const int32_t* __restrict__ target,
+                                                     int64_t M, float* __restrict__ out, float* __restrict__ factor) {
+    __shared__ float rs[32];
+    __shared__ int rn[32];
+    grid_wait();
+    grid_trigger();
+    float s = 0.0f;
+    int n = 0;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < M; i += 1024) {
+        s += losses[i];
+        if (MEAN) n += target[i] >= 0;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    n = __reduce_add_sync(0xffffffffu, n);
+    if ((threadIdx.x & 31) == 0) {
+        rs[threadIdx.x >> 5] = s;
+        rn[threadIdx.x >> 5] = n;
+    }
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int w = 1; w < 32; ++w) {
+        s += rs[w];
+        n += rn[w];
+    }
+    const float rows = MEAN ? fmaxf(static_cast<float>(n), 1.0f) : 1.0f;
+    *out = s / rows;
+    if (factor != nullptr) *factor = 1.0f / rows;
+}
+
+// *up_max = the largest |up| of a row with a target (1 where that is 0): one block.
+__global__ void __launch_bounds__(1024) k_head_up_max(const float* __restrict__ up, const int32_t* __restrict__ target,
+                                                      int64_t M, float* __restrict__ up_max) {
+    __shared__ float red[32];
+    grid_wait();
+    grid_trigger();
+    float m = 0.0f;
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < M; i += 1024)
+        if (target[i] >= 0) m = fmaxf(m, fabsf(up[i]));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int w = 1; w < 32; ++w) m = fmaxf(m, red[w]);
+    *up_max = m > 0.0f ? m : 1.0f;
+}
+
+// out[r][c] = (sum of the slabs) up factor unit, rows of N; a thread per 4 columns.
+template <typename T>
+__global__ void __launch_bounds__(256) k_head_out(const float* __restrict__ slabs, int splits, int64_t slab, int64_t ldo,
+                                                  int64_t M, int64_t N, int vec, const float* __restrict__ up,
+                                                  const float* __restrict__ factor, float unit, T* __restrict__ out) {
+    grid_wait();
+    grid_trigger();
+    const float f = (up != nullptr ? *up : 1.0f) * *factor * unit;
+    const int64_t per = (N + 3) / 4, total = M * per;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
+         i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t r = i / per, c = (i - r * per) * 4;
+        const float* p = slabs + r * ldo + c;
+        float4 v = __ldcs(reinterpret_cast<const float4*>(p));
+        for (int s = 1; s < splits; ++s) {
+            const float4 w = __ldcs(reinterpret_cast<const float4*>(p + s * slab));
+            v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+        }
+        T* const o = out + r * N + c;
+        if (vec) {
+            *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(v.x * f, v.y * f), pack2<T>(v.z * f, v.w * f));
+        } else {
+            const float e[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (c + k < N) o[k] = round_to<T>(e[k] * f);
+        }
+    }
+}
+
+}  // namespace ravel

@@ -15,7 +15,8 @@
 // returns None when its arguments are not the common case (the caller then
 // takes the fully checked Python path, with its error messages).
 //
-// The dense operators (fused_linear, layer_norm, distill_topk_loss) live here whole: argument checks, outputs and
+// The dense operators (fused_linear, layer_norm, distill_topk_loss), the vocabulary's (token_embedding,
+// linear_cross_entropy) and the optimizer step (adamw_step) live here whole: argument checks, outputs and
 // workspaces, and the autograd node, so that a decoded token's call or a small
 // training step is not bound by Python.  Workspaces come from the caching
 // allocator on the current stream of the tensors' device.
@@ -27,6 +28,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 #include <string>
@@ -603,6 +605,382 @@ at::Tensor distill_topk_loss(const at::Tensor& logits, const at::Tensor& ids, co
     return c.forward(logits.sizes().slice(0, logits.dim() - 1), false, at::Tensor());
 }
 
+// ------------------------------------------------------------------ the vocabulary's two ends
+int index_code(const at::Tensor& t, const char* what) {
+    if (t.scalar_type() == at::kLong) return RAVEL_I64;
+    if (t.scalar_type() == at::kInt) return RAVEL_I32;
+    throw py::type_error(std::string(what) + " must be int32 or int64");
+}
+
+at::Tensor embedding_forward(const at::Tensor& ids, const Rows& w, double scale) {
+    std::vector<int64_t> shape = ids.sizes().vec();
+    const int64_t V = w.t.size(0), K = w.t.size(1);
+    shape.push_back(K);
+    at::Tensor y = at::empty(shape, w.t.options());
+    check_status("ravel_embedding_fwd",
+                 ravel_embedding_fwd(ids.data_ptr(), index_code(ids, "ids"), w.t.data_ptr(), w.ld, ids.numel(), V, K,
+                                     static_cast<float>(scale), y.data_ptr(), payload_code(y.scalar_type()),
+                                     stream_of(y)));
+    return y;
+}
+
+struct TokenEmbedding : public torch::autograd::Function<TokenEmbedding> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& ids, const at::Tensor& weight, double scale,
+                              int64_t padding) {
+        at::Tensor y = embedding_forward(ids, rows_of(weight), scale);
+        ctx->save_for_backward({ids});
+        ctx->saved_data["V"] = weight.size(0);
+        ctx->saved_data["K"] = weight.size(1);
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["padding"] = padding;
+        return y;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor& ids = saved[0];
+        variable_list out(4);
+        if (!grads[0].defined()) return out;
+        once_differentiable("token_embedding");
+        const c10::cuda::CUDAGuard guard(ids.device());
+        const int64_t V = ctx->saved_data["V"].toInt(), K = ctx->saved_data["K"].toInt(), N = ids.numel();
+        const Rows gy = rows_of(grads[0]);
+        at::Tensor dw = at::empty({V, K}, gy.t.options());
+        const size_t sb = ravel_embedding_scratch_bytes(N, V, K);
+        at::Tensor scratch = bytes(sb, gy.t);
+        check_status("ravel_embedding_bwd",
+                     ravel_embedding_bwd(ids.data_ptr(), index_code(ids, "ids"), gy.t.data_ptr(), gy.ld, N, V, K,
+                                         static_cast<float>(ctx->saved_data["scale"].toDouble()),
+                                         ctx->saved_data["padding"].toInt(), dw.data_ptr(),
+                                         payload_code(dw.scalar_type()), scratch.data_ptr(), sb, stream_of(gy.t)));
+        out[1] = dw;
+        return out;
+    }
+};
+
+at::Tensor token_embedding(const at::Tensor& ids, const at::Tensor& weight, double scale,
+                           std::optional<int64_t> padding_idx) {
+    if (weight.dim() != 2 || weight.size(0) < 1)
+        throw py::value_error("token_embedding expects a weight [V, K] with V >= 1");
+    index_code(ids, "ids");
+    float_code(weight, "token_embedding");
+    if (!std::isfinite(scale)) throw py::value_error("scale must be finite");
+    const int64_t V = weight.size(0);
+    int64_t padding = -1;
+    if (padding_idx) {
+        padding = *padding_idx < 0 ? *padding_idx + V : *padding_idx;
+        if (padding < 0 || padding >= V) throw py::value_error("padding_idx must lie in the vocabulary");
+    }
+    const OptTensor i(ids), w(weight);
+    no_tangents("token_embedding", {&w});
+    require_cuda(ids, {&w});
+    const c10::cuda::CUDAGuard guard(weight.device());
+    const at::Tensor idc = ids.contiguous();
+    if (at::GradMode::is_enabled() && weight.requires_grad())
+        return TokenEmbedding::apply(idc, weight, scale, padding);
+    return embedding_forward(idc, rows_of(weight), scale);
+}
+
+// The tensors of a cross entropy call, its forward, and the gradients' float32 sums.
+struct CrossEntropyCall {
+    Rows w;
+    int64_t M, K, V;
+    int dtype;
+    at::Tensor losses, out, factor, scratch, slabs_x, slabs_w;
+
+    // w: rows that TMA can read, of K elements and perhaps padding
+    CrossEntropyCall(const Rows& w_, int64_t M_, int64_t K_, int64_t V_)
+        : w(w_), M(M_), K(K_), V(V_), dtype(payload_code(w_.t.scalar_type())) {}
+
+    void make_slabs(bool need_x, bool need_w) {
+        int64_t sizes[3];
+        check_status("ravel_linear_ce_slabs", ravel_linear_ce_slabs(M, K, V, sizes));
+        const auto f32 = w.t.options().dtype(at::kFloat);
+        if (need_x) slabs_x = at::empty({sizes[0], M, sizes[2]}, f32);
+        if (need_w) slabs_w = at::empty({sizes[1], V, sizes[2]}, f32);
+        factor = at::empty({}, f32);
+    }
+    float* slab(at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+
+    at::Tensor forward(const Rows& x, const at::Tensor& targets, int64_t ignore, int reduction, bool need_x, bool need_w,
+                       at::IntArrayRef rows_shape) {
+        const auto f32 = w.t.options().dtype(at::kFloat);
+        const bool reduced = reduction != RAVEL_REDUCE_NONE, grads = reduced && (need_x || need_w);
+        losses = at::empty(rows_shape, f32);
+        if (reduced) out = at::empty({}, f32);
+        if (grads) make_slabs(need_x, need_w);
+        const size_t sb = ravel_linear_ce_scratch_bytes(M, K, V), wb = ravel_linear_ce_work_bytes(M, K, V, grads);
+        scratch = bytes(sb, w.t);
+        at::Tensor work = bytes(wb, w.t);
+        check_status("ravel_linear_ce_fwd",
+                     ravel_linear_ce_fwd(x.t.data_ptr(), x.ld, w.t.data_ptr(), w.ld, targets.data_ptr(),
+                                         index_code(targets, "targets"), M, K, V, ignore, reduction,
+                                         losses.data_ptr<float>(), reduced ? out.data_ptr<float>() : nullptr,
+                                         grads ? factor.data_ptr<float>() : nullptr, slab(slabs_x), slab(slabs_w), dtype,
+                                         scratch.data_ptr(), sb, work.data_ptr(), wb, stream_of(w.t)));
+        return reduced ? out : losses;
+    }
+};
+
+struct LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy> {
+    static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& weight,
+                              const at::Tensor& targets, int64_t ignore, int64_t reduction) {
+        // A reduced loss's gradients are made here, a piece of the rows at a time, while their logits exist, up to a
+        // factor that the backward applies: float32 sums, so that nothing depends on the size of the upstream gradient.
+        CrossEntropyCall c(tma_rows(weight), leading(x), weight.size(1), weight.size(0));
+        at::Tensor loss = c.forward(rows_of(x), targets, ignore, static_cast<int>(reduction), x.requires_grad(),
+                                    weight.requires_grad(), targets.sizes());
+        const bool reduced = reduction != RAVEL_REDUCE_NONE;
+        ctx->save_for_backward({c.slabs_x, c.slabs_w, c.factor, reduced ? at::Tensor() : c.w.t,
+                                reduced ? at::Tensor() : c.scratch});
+        ctx->saved_data["ld"] = c.w.ld;
+        ctx->saved_data["M"] = c.M;
+        ctx->saved_data["K"] = c.K;
+        ctx->saved_data["V"] = c.V;
+        ctx->saved_data["dtype"] = static_cast<int64_t>(c.dtype);
+        ctx->saved_data["x_shape"] = x.sizes().vec();
+        return loss;
+    }
+
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        variable_list out(5);
+        if (!grads[0].defined()) return out;
+        once_differentiable("linear_cross_entropy");
+        const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+        if (!need_x && !need_w) return out;
+        const at::Tensor up = grads[0].contiguous();
+        const c10::cuda::CUDAGuard guard(up.device());
+        const int64_t M = ctx->saved_data["M"].toInt(), K = ctx->saved_data["K"].toInt(), V = ctx->saved_data["V"].toInt();
+        const int dtype = static_cast<int>(ctx->saved_data["dtype"].toInt());
+        at::Tensor slabs_x = saved[0], slabs_w = saved[1], factor = saved[2];
+        void* const st = stream_of(up);
+        const bool reduced = factor.defined();
+        if (!reduced) {
+            CrossEntropyCall c(Rows{saved[3], ctx->saved_data["ld"].toInt()}, M, K, V);
+            c.make_slabs(need_x, need_w);
+            at::Tensor scratch = saved[4];
+            const size_t wb = ravel_linear_ce_work_bytes(M, K, V, 1);
+            at::Tensor work = bytes(wb, up);
+            check_status("ravel_linear_ce_grad",
+                         ravel_linear_ce_grad(c.w.t.data_ptr(), c.w.ld, up.data_ptr<float>(), M, K, V,
+                                              c.factor.data_ptr<float>(), c.slab(c.slabs_x), c.slab(c.slabs_w), dtype,
+                                              scratch.data_ptr(), static_cast<size_t>(scratch.numel()), work.data_ptr(),
+                                              wb, st));
+            slabs_x = c.slabs_x;
+            slabs_w = c.slabs_w;
+            factor = c.factor;
+        }
+        const auto like = up.options().dtype(dtype == RAVEL_F16 ? at::kHalf : at::kBFloat16);
+        if (need_x) out[0] = at::empty(ctx->saved_data["x_shape"].toIntVector(), like);
+        if (need_w) out[1] = at::empty({V, K}, like);
+        check_status("ravel_linear_ce_bwd",
+                     ravel_linear_ce_bwd(need_x ? slabs_x.data_ptr<float>() : nullptr,
+                                         need_w ? slabs_w.data_ptr<float>() : nullptr,
+                                         reduced ? up.data_ptr<float>() : nullptr, factor.data_ptr<float>(), M, K, V,
+                                         need_x ? out[0].data_ptr() : nullptr, need_w ? out[1].data_ptr() : nullptr,
+                                         dtype, st));
+        return out;
+    }
+};
+
+at::Tensor linear_cross_entropy(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& targets, int64_t ignore,
+                                int64_t reduction) {
+    if (x.dim() < 1 || weight.dim() != 2 || weight.size(1) != x.size(-1) || weight.size(0) < 1 || weight.size(1) < 1)
+        throw py::value_error("linear_cross_entropy expects x [..., K] and a weight [V, K], V and K at least 1");
+    if (targets.sizes() != x.sizes().slice(0, x.dim() - 1))
+        throw py::value_error("targets must have x's leading dimensions");
+    const auto dt = x.scalar_type();
+    if (dt != at::kBFloat16 && dt != at::kHalf)
+        throw py::type_error(std::string("linear_cross_entropy takes bfloat16 or float16 tensors, got ") + toString(dt));
+    if (weight.scalar_type() != dt) throw py::type_error("linear_cross_entropy expects x and weight of one dtype");
+    index_code(targets, "targets");
+    const OptTensor in(x), w(weight), t(targets);
+    no_tangents("linear_cross_entropy", {&in, &w});
+    require_cuda(x, {&w, &t});
+    const c10::cuda::CUDAGuard guard(x.device());
+    const at::Tensor tc = targets.contiguous();
+    if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad()))
+        return LinearCrossEntropy::apply(x, weight, tc, ignore, reduction);
+    CrossEntropyCall c(tma_rows(weight), leading(x), weight.size(1), weight.size(0));
+    return c.forward(rows_of(x), tc, ignore, static_cast<int>(reduction), false, false, tc.sizes());
+}
+
+// ------------------------------------------------------------------ the optimizer step
+using TensorList = std::vector<at::Tensor>;
+using OptTensorList = std::optional<TensorList>;
+
+void written(const at::Tensor& t) {  // autograd counts writes in place
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
+std::string at_place(const char* what, size_t i) { return std::string(what) + "[" + std::to_string(i) + "]"; }
+
+// A list's 2-norm (float64, 0-dim) of tensors of one dtype, as the library takes them.
+void list_norm(const std::vector<ravel_adamw_tensor>& list, const at::Tensor& like, double* norm) {
+    const size_t sb = ravel_grad_norm_scratch_bytes(list.data(), static_cast<int64_t>(list.size()));
+    at::Tensor scratch = bytes(sb, like);
+    check_status("ravel_grad_norm",
+                 ravel_grad_norm(list.data(), static_cast<int64_t>(list.size()), payload_code(like.scalar_type()), norm,
+                                 scratch.data_ptr(), sb, stream_of(like)));
+}
+
+at::Tensor global_norm(const TensorList& tensors) {
+    if (tensors.empty()) throw py::value_error("global_norm expects at least one tensor");
+    for (const at::Tensor& t : tensors) float_code(t, "global_norm");
+    for (const at::Tensor& t : tensors) {
+        const OptTensor o(t);
+        require_cuda(tensors[0], {&o});
+    }
+    const c10::cuda::CUDAGuard guard(tensors[0].device());
+    std::vector<at::ScalarType> types;
+    for (const at::Tensor& t : tensors)
+        if (std::find(types.begin(), types.end(), t.scalar_type()) == types.end()) types.push_back(t.scalar_type());
+    at::Tensor norms = at::empty({static_cast<int64_t>(types.size())}, tensors[0].options().dtype(at::kDouble));
+    TensorList held;
+    for (size_t k = 0; k < types.size(); ++k) {
+        std::vector<ravel_adamw_tensor> list;
+        const at::Tensor* first = nullptr;
+        for (const at::Tensor& t : tensors) {
+            if (t.scalar_type() != types[k]) continue;
+            held.push_back(t.contiguous());
+            if (first == nullptr) first = &t;
+            list.push_back({nullptr, held.back().data_ptr(), nullptr, nullptr, nullptr, nullptr, nullptr, t.numel()});
+        }
+        list_norm(list, *first, norms.data_ptr<double>() + k);
+    }
+    return types.size() == 1 ? norms[0] : at::norm(norms);
+}
+
+OptTensor adamw_step(const TensorList& params, const TensorList& grads, const TensorList& avgs, const TensorList& sqs,
+                     const at::Tensor& step, const OptTensorList& masters, const OptTensorList& avg_exps,
+                     const OptTensorList& sq_exps, double lr, const OptTensor& lr_tensor, double beta1, double beta2,
+                     double eps, double weight_decay, std::optional<double> max_norm, const OptTensor& norm) {
+    const size_t n = params.size();
+    if (n == 0) throw py::value_error("adamw_step expects at least one tensor");
+    if (grads.size() != n || avgs.size() != n || sqs.size() != n || (masters && masters->size() != n) ||
+        (avg_exps && avg_exps->size() != n) || (sq_exps && sq_exps->size() != n))
+        throw py::value_error("adamw_step expects lists of one length");
+    if (avg_exps.has_value() != sq_exps.has_value())
+        throw py::value_error("exp_avg_exponents and exp_avg_sq_exponents come together (8-bit states)");
+    if (!(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0))
+        throw py::value_error("betas must lie in [0, 1)");
+    if (!(eps >= 0.0) || !(weight_decay >= 0.0) || (!lr_tensor && !(lr >= 0.0)))
+        throw py::value_error("lr, eps and weight_decay must not be negative");
+    if (max_norm && !(*max_norm > 0.0)) throw py::value_error("max_norm must be positive");
+    if (norm && !max_norm) throw py::value_error("norm is used with max_norm only");
+    const at::Tensor& first = params[0];
+    const auto dt = first.scalar_type();
+    const bool eight = avg_exps.has_value(), half = dt != at::kFloat;
+    float_code(first, "adamw_step");
+    if (half != masters.has_value())
+        throw py::value_error("16-bit parameters need float32 masters, and float32 parameters take none");
+    if (step.scalar_type() != at::kLong || step.numel() != 1) throw py::type_error("step must be one int64");
+    if (lr_tensor && (lr_tensor->scalar_type() != at::kFloat || lr_tensor->numel() != 1))
+        throw py::type_error("an lr tensor must be one float32");
+    if (norm && (norm->scalar_type() != at::kDouble || norm->numel() != 1))
+        throw py::type_error("norm must be one float64 (global_norm's)");
+    auto check = [&](const char* what, size_t i, const at::Tensor& t, at::ScalarType type, int64_t size) {
+        if (t.numel() != size) throw py::value_error(at_place(what, i) + " has the wrong number of elements");
+        if (t.scalar_type() != type)
+            throw py::type_error(at_place(what, i) + " must be " + toString(type) + ", got " + toString(t.scalar_type()));
+        if (!t.is_contiguous()) throw py::value_error(at_place(what, i) + " must be contiguous");
+    };
+    const auto state = eight ? at::kByte : at::kFloat;
+    for (size_t i = 0; i < n; ++i) {
+        const int64_t size = params[i].numel();
+        check("params", i, params[i], dt, size);
+        if (grads[i].sizes() != params[i].sizes()) throw py::value_error(at_place("grads", i) + " must have its parameter's shape");
+        if (grads[i].is_sparse()) throw py::value_error(at_place("grads", i) + " must be dense");
+        if (grads[i].scalar_type() != dt) throw py::type_error(at_place("grads", i) + " must have its parameter's dtype");
+        check("exp_avgs", i, avgs[i], state, size);
+        check("exp_avg_sqs", i, sqs[i], state, size);
+        if (half) check("masters", i, (*masters)[i], at::kFloat, size);
+        if (eight) {
+            check("exp_avg_exponents", i, (*avg_exps)[i], at::kChar, (size + 255) / 256);
+            check("exp_avg_sq_exponents", i, (*sq_exps)[i], at::kChar, (size + 255) / 256);
+        }
+    }
+    {
+        std::vector<const void*> seen;
+        for (const at::Tensor& t : params)
+            if (t.numel() > 0) seen.push_back(t.data_ptr());
+        std::sort(seen.begin(), seen.end());
+        if (std::adjacent_find(seen.begin(), seen.end()) != seen.end())
+            throw py::value_error("adamw_step: a parameter appears twice");
+    }
+    const OptTensor st(step);
+    require_cuda(first, {&st, &lr_tensor, &norm});
+    auto same_device = [&](const TensorList& l) {
+        for (const at::Tensor& t : l)
+            if (t.device() != first.device()) {
+                const OptTensor o(t);
+                require_cuda(first, {&o});
+            }
+    };
+    for (const TensorList* l : {&params, &grads, &avgs, &sqs}) same_device(*l);
+    for (const OptTensorList* l : {&masters, &avg_exps, &sq_exps})
+        if (l->has_value()) same_device(**l);
+    const c10::cuda::CUDAGuard guard(first.device());
+    TensorList held;  // gradients laid out otherwise
+    std::vector<ravel_adamw_tensor> list(n);
+    for (size_t i = 0; i < n; ++i) {
+        const at::Tensor* g = &grads[i];
+        if (!g->is_contiguous()) {
+            held.push_back(g->contiguous());
+            g = &held.back();
+        }
+        list[i] = {params[i].data_ptr(), g->data_ptr(), half ? (*masters)[i].data_ptr<float>() : nullptr,
+                   avgs[i].data_ptr(), sqs[i].data_ptr(),
+                   eight ? static_cast<signed char*>((*avg_exps)[i].data_ptr()) : nullptr,
+                   eight ? static_cast<signed char*>((*sq_exps)[i].data_ptr()) : nullptr, params[i].numel()};
+    }
+    at::Tensor own_norm, norm32;
+    const double* norm_ptr = nullptr;
+    if (max_norm) {
+        if (norm) {
+            norm_ptr = norm->data_ptr<double>();
+        } else {
+            own_norm = at::empty({}, first.options().dtype(at::kDouble).requires_grad(false));
+            list_norm(list, first, own_norm.data_ptr<double>());
+            norm_ptr = own_norm.data_ptr<double>();
+        }
+        norm32 = at::empty({}, first.options().dtype(at::kFloat));
+    }
+    const size_t sb = ravel_adamw_scratch_bytes();
+    at::Tensor scratch = bytes(sb, first);
+    check_status("ravel_adamw",
+                 ravel_adamw(list.data(), static_cast<int64_t>(n), payload_code(dt), eight ? 8 : 32,
+                             step.data_ptr<int64_t>(), lr, lr_tensor ? lr_tensor->data_ptr<float>() : nullptr, beta1,
+                             beta2, eps, weight_decay, max_norm.value_or(0.0), norm_ptr,
+                             max_norm ? norm32.data_ptr<float>() : nullptr, scratch.data_ptr(), sb, stream_of(first)));
+    written(step);
+    for (size_t i = 0; i < n; ++i) {
+        written(params[i]);
+        written(avgs[i]);
+        written(sqs[i]);
+        if (half) written((*masters)[i]);
+        if (eight) written((*avg_exps)[i]), written((*sq_exps)[i]);
+    }
+    return max_norm ? OptTensor(norm32) : std::nullopt;
+}
+
+at::Tensor state_values(const at::Tensor& codes, const at::Tensor& exponents, bool is_signed, bool half) {
+    if (codes.scalar_type() != at::kByte || exponents.scalar_type() != at::kChar)
+        throw py::type_error("state_values expects uint8 codes and int8 exponents");
+    if (exponents.numel() != (codes.numel() + 255) / 256)
+        throw py::value_error("state_values expects one exponent per block of 256 codes");
+    const OptTensor e(exponents);
+    require_cuda(codes, {&e});
+    const c10::cuda::CUDAGuard guard(codes.device());
+    const at::Tensor c = codes.contiguous(), x = exponents.contiguous();
+    at::Tensor out = at::empty(codes.sizes(), codes.options().dtype(half ? at::kBFloat16 : at::kFloat));
+    check_status("ravel_state_values",
+                 ravel_state_values(c.data_ptr(), static_cast<const signed char*>(x.data_ptr()), c.numel(),
+                                    is_signed ? 1 : 0, out.data_ptr(), half ? RAVEL_BF16 : RAVEL_F32, stream_of(out)));
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_ravel_host, m) {
@@ -616,4 +994,9 @@ PYBIND11_MODULE(_ravel_host, m) {
     m.def("fused_linear", &fused_linear);
     m.def("layer_norm", &layer_norm);
     m.def("distill_topk_loss", &distill_topk_loss);
+    m.def("token_embedding", &token_embedding);
+    m.def("linear_cross_entropy", &linear_cross_entropy);
+    m.def("global_norm", &global_norm);
+    m.def("adamw_step", &adamw_step);
+    m.def("state_values", &state_values);
 }

@@ -1,0 +1,544 @@
+// vocab.cu -- C ABI of the vocabulary's two ends: the token embedding, and the cross entropy of a Linear's outputs.
+// Argument validation and launch plumbing; the kernels live in embedding.cuh and head.cuh.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <map>
+#include <mutex>
+
+#include "embedding.cuh"
+#include "head.cuh"
+#include "host.cuh"
+
+namespace ravel {
+namespace {
+
+constexpr int64_t kMaxRows = int64_t{1} << 30;  // tokens, vocabulary, width
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+int esize(int dtype) { return dtype == RAVEL_F32 ? 4 : 2; }
+size_t up256(size_t n) { return (n + 255) / 256 * 256; }
+int64_t up_to(int64_t n, int64_t m) { return (n + m - 1) / m * m; }
+
+template <typename F>
+int with_half_type(int dtype, F&& f) {
+    if (dtype == RAVEL_BF16) return f(__nv_bfloat16());
+    if (dtype == RAVEL_F16) return f(__half());
+    return RAVEL_ERR_UNSUPPORTED;
+}
+template <typename F>
+int with_float_type(int dtype, F&& f) {
+    if (dtype == RAVEL_F32) return f(float());
+    return with_half_type(dtype, f);
+}
+
+// ------------------------------------------------------------------ embedding
+// Threads per row: the least power of two from 32 on that holds the row's units, at most a block.
+int embed_tx(int64_t units) {
+    int tx = 32;
+    while (tx < EM_THREADS && tx < units) tx *= 2;
+    return tx;
+}
+
+// Positions per range of the backward's sums: at least two waves of groups, and no range under 16 positions (a piece
+// costs as much memory traffic as four 16-bit rows).
+int embed_range(int64_t N, int tx) {
+    const int64_t groups = static_cast<int64_t>(sm_count()) * 8 * (EM_THREADS / tx);
+    int64_t r = 128;
+    while (r > 16 && N / r < groups * 2) r /= 2;
+    return static_cast<int>(r);
+}
+
+struct EmbedLayout {
+    size_t off_clean, off_present, off_part, off_tape, off_sort, total, tape_bytes, sort_bytes;
+    int64_t ranges;
+};
+// Ranges as if each row took a whole block: the most there can be.
+EmbedLayout embed_layout(int64_t N, int64_t V, int64_t K) {
+    EmbedLayout l;
+    l.ranges = (N + 15) / 16;
+    l.tape_bytes = ravel_tape_bytes(1, N, 1, V + 1, 0);
+    l.sort_bytes = ravel_scratch_bytes(1, N, 1, 1, V + 1, 1, RAVEL_F32, 0);
+    l.off_clean = 0;
+    l.off_present = up256(static_cast<size_t>(N) * 4);
+    l.off_part = l.off_present + up256(static_cast<size_t>(V));
+    l.off_tape = l.off_part + up256(static_cast<size_t>(l.ranges) * 2 * static_cast<size_t>(K) * sizeof(float));
+    l.off_sort = l.off_tape + up256(l.tape_bytes);
+    l.total = l.off_sort + up256(l.sort_bytes);
+    return l;
+}
+
+int embed_check(int64_t N, int64_t V, int64_t K, int ids_dtype, int dtype) {
+    if (N < 0 || V <= 0 || K < 0 || (ids_dtype != RAVEL_I32 && ids_dtype != RAVEL_I64)) return RAVEL_ERR_INVALID_ARG;
+    if (dtype != RAVEL_F32 && dtype != RAVEL_BF16 && dtype != RAVEL_F16) return RAVEL_ERR_UNSUPPORTED;
+    if (N > kMaxRows || V >= kMaxRows || K > kMaxRows) return RAVEL_ERR_UNSUPPORTED;
+    return RAVEL_OK;
+}
+
+// ------------------------------------------------------------------ cross entropy
+constexpr size_t kHeadPieceBytes = size_t{512} << 20;  // of d z: rows go in pieces of this, or of 1024 rows
+
+struct HeadLayout {
+    int64_t piece, parts;  // rows of a piece
+    int64_t ldz, ldc, ldo;
+    size_t off_target, off_zt, off_stat, off_up, off_clean, total;  // scratch: what the backward of single losses needs again
+    size_t work, work_grads;  // the parts, and d z in their place
+};
+
+// Rows of a piece: whole tiles of 256.  d W is read and written once more for every piece after the first, which at 1024
+// rows takes about as long as the piece's products.
+int64_t head_piece(int64_t M, int64_t V) {
+    const int64_t most = std::max<int64_t>(1024, static_cast<int64_t>(kHeadPieceBytes / 2) / up_to(V, 8) / 256 * 256);
+    if (M <= most) return std::max<int64_t>(M, 1);
+    const int64_t pieces = (M + most - 1) / most;
+    return up_to((M + pieces - 1) / pieces, 256);
+}
+
+HeadLayout head_layout(int64_t M, int64_t K, int64_t V) {
+    HeadLayout l;
+    l.piece = head_piece(M, V);
+    l.ldz = up_to(V, 8);
+    l.ldc = up_to(K, 8);
+    l.ldo = up_to(K, 4);
+    l.parts = 2 * ((V + 127) / 128);
+    l.off_target = 0;
+    l.off_zt = up256(static_cast<size_t>(M) * 4);
+    l.off_stat = l.off_zt + up256(static_cast<size_t>(l.piece) * 4);
+    l.off_up = l.off_stat + up256(static_cast<size_t>(M) * 16);
+    l.off_clean = l.off_up + 256;
+    l.total = l.off_clean + up256(static_cast<size_t>(M) * static_cast<size_t>(l.ldc) * 2);
+    l.work = static_cast<size_t>(l.parts) * static_cast<size_t>(l.piece) * 8;
+    l.work_grads = std::max(l.work, static_cast<size_t>(l.piece) * static_cast<size_t>(l.ldz) * 2);
+    return l;
+}
+
+// Clusters of two product CTAs that fit the device at once (queried once per kernel and device).
+int resident_pairs(const void* kernel) {
+    static std::mutex mu;
+    static std::map<std::pair<const void*, int>, int> known;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return sm_count() / 2;
+    std::lock_guard<std::mutex> lock(mu);
+    const auto key = std::make_pair(kernel, dev);
+    const auto it = known.find(key);
+    if (it != known.end()) return it->second;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at = {};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = 2;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(static_cast<unsigned>(sm_count() / 2 * 2));
+    cfg.blockDim = dim3(MM_THREADS);
+    cfg.dynamicSmemBytes = MM_SMEM;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n <= 0) {
+        (void)cudaGetLastError();
+        n = sm_count() / 2;
+    }
+    known[key] = n;
+    return n;
+}
+
+// A product's operand: rows x k (K-major) or k x rows (MN-major), 16-byte rows.
+struct HeadOperand {
+    const void* p;
+    int64_t ld;
+};
+
+// The ring and the tiles of a product of M x N outputs over k.
+template <int CG, int BN, bool A_MN, typename Args>
+void head_shape(Args& a, int64_t M, int64_t N, int64_t k) {
+    constexpr int B_ROWS = BN / CG, KS = mm_ksub(CG);
+    a.mtiles = static_cast<int>((M + 128 * CG - 1) / (128 * CG));
+    a.ntiles = static_cast<int>((N + BN - 1) / BN);
+    a.a_rows = A_MN || M >= 128 ? 128 : static_cast<int>((M + 7) / 8 * 8);
+    a.a_bytes = static_cast<uint32_t>(a.a_rows) * 128u;
+    a.stage_bytes = KS * (a.a_bytes + B_ROWS * 128u);
+    a.ksteps = static_cast<int>((k + KS * MM_BK - 1) / (KS * MM_BK));
+    a.stages = static_cast<int>(std::min<uint32_t>(MM_MAX_STAGES, MM_RING / a.stage_bytes));
+}
+
+template <typename T, bool MN>
+int head_map(CUtensorMap* map, const HeadOperand& o, int64_t rows, int64_t k, int box_rows) {
+    constexpr CUtensorMapDataType TY =
+        std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return MN ? encode_map_2d(map, TY, o.p, rows, k, o.ld * 2, 64, MM_BK)
+              : encode_map_2d(map, TY, o.p, k, rows, o.ld * 2, MM_BK, box_rows);
+}
+
+template <typename T, int CG, int BN, int MODE>
+int launch_logits(const HeadOperand& X, const HeadOperand& W, int64_t K, HeadLogitsArgs a, cudaStream_t st) {
+    const auto kern = k_head_logits<T, CG, BN, MODE>;
+    head_shape<CG, BN, false>(a, a.M, a.V, K);
+    CUtensorMap ma, mb;
+    if (int e = head_map<T, false>(&ma, X, a.M, K, a.a_rows)) return e;
+    if (int e = head_map<T, false>(&mb, W, a.V, K, BN / CG)) return e;
+    if (int e = set_smem(kern, MM_SMEM)) return e;
+    const int64_t tiles = static_cast<int64_t>(a.mtiles) * a.ntiles;
+    const int64_t fit = CG == 2 ? resident_pairs(reinterpret_cast<const void*>(kern)) : sm_count();
+    return launch(kern, dim3(static_cast<unsigned>(std::min(tiles, fit) * CG)), MM_THREADS, MM_SMEM, st, CG, ma, mb, a);
+}
+
+// Pairs where two row tiles exist, single CTAs for fewer rows.
+bool head_pairs(int64_t M) { return M > 128; }
+
+template <typename T, int MODE>
+int head_logits(const HeadOperand& X, const HeadOperand& W, int64_t K, const HeadLogitsArgs& a, cudaStream_t st) {
+    if (head_pairs(a.M)) return launch_logits<T, 2, 256, MODE>(X, W, K, a, st);
+    return launch_logits<T, 1, 128, MODE>(X, W, K, a, st);
+}
+
+struct HeadPlan {
+    int cg, splits;
+};
+// A gradient's launch shape and the CTAs (or pairs) that share its k, by an estimate in microseconds: waves of units, each
+// the larger of its chunks and its epilogue, and the slabs' traffic.
+HeadPlan plan_grad(int64_t M, int64_t N, int64_t k) {
+    const double sms = sm_count(), kc = static_cast<double>((k + MM_BK - 1) / MM_BK);
+    struct Kind {
+        int cg, bn;
+        double chunk, epilogue;
+    };
+    const Kind kinds[] = {{2, 256, 0.280, 3.0}, {1, 128, 0.160, 1.6}};
+    HeadPlan best = {1, 1};
+    double cost = 1e30;
+    for (const Kind& q : kinds) {
+        const double tiles = std::ceil(M / (128.0 * q.cg)) * std::ceil(static_cast<double>(N) / q.bn);
+        for (int s = 1; s <= 32 && kc >= 4 * s; s *= 2) {
+            const double waves = std::ceil(tiles * s / std::floor(sms / q.cg));
+            const double us = waves * std::max(std::ceil(kc / s) * q.chunk, q.epilogue) + (s - 1) * (M * N) * 8.0 / 5e6;
+            if (us < cost) cost = us, best = {q.cg, s};
+        }
+    }
+    return best;
+}
+
+template <typename T, int CG, int BN, bool A_MN>
+int launch_grad(const HeadOperand& A, const HeadOperand& B, int64_t k, HeadGradArgs a, cudaStream_t st) {
+    const auto kern = k_head_grad<T, CG, BN, A_MN>;
+    head_shape<CG, BN, A_MN>(a, a.M, a.N, k);
+    CUtensorMap ma, mb;
+    if (int e = head_map<T, A_MN>(&ma, A, a.M, k, a.a_rows)) return e;
+    if (int e = head_map<T, true>(&mb, B, a.N, k, 0)) return e;
+    if (int e = set_smem(kern, MM_SMEM)) return e;
+    const int64_t units = static_cast<int64_t>(a.mtiles) * a.ntiles * a.splits;
+    const int64_t fit = CG == 2 ? resident_pairs(reinterpret_cast<const void*>(kern)) : sm_count();
+    return launch(kern, dim3(static_cast<unsigned>(std::min(units, fit) * CG)), MM_THREADS, MM_SMEM, st, CG, ma, mb, a);
+}
+
+// The split counts of a whole call: of its full pieces for d W and of the first piece for d x.
+struct HeadSplits {
+    HeadPlan x, w;
+};
+HeadSplits head_splits(int64_t M, int64_t K, int64_t V) {
+    const int64_t piece = head_piece(M, V);
+    // the last piece may have fewer rows: its k must still hold every split
+    const int64_t last = M - (std::max<int64_t>(M, 1) - 1) / piece * piece;
+    HeadSplits s = {plan_grad(piece, K, V), plan_grad(V, K, std::max<int64_t>(1, std::min(piece, last)))};
+    return s;
+}
+
+int head_check(int64_t M, int64_t K, int64_t V, int t_dtype, int dtype) {
+    if (M < 0 || K <= 0 || V <= 0 || (t_dtype != RAVEL_I32 && t_dtype != RAVEL_I64)) return RAVEL_ERR_INVALID_ARG;
+    if (dtype != RAVEL_BF16 && dtype != RAVEL_F16) return RAVEL_ERR_UNSUPPORTED;
+    if (M > kMaxRows || K > kMaxRows || V >= kMaxRows) return RAVEL_ERR_UNSUPPORTED;
+    const int64_t piece = head_piece(M, V);
+    if (((piece + 127) / 128) * ((V + 127) / 128) >= (int64_t{1} << 27) ||
+        ((std::max(piece, V) + 127) / 128) * ((K + 127) / 128) >= (int64_t{1} << 24))
+        return RAVEL_ERR_UNSUPPORTED;  // tiles are counted in 32 bits
+    return RAVEL_OK;
+}
+
+struct HeadCall {
+    const void *x, *w;
+    int64_t ldx, ldw, M, K, V;
+    float* losses;     // null: the statistics are there (the gradient of given upstream values)
+    const float* up;   // [M] or null
+    float *gx, *gw;    // null: not wanted
+    char* scratch;
+    void* work;
+    HeadLayout l;
+    DeviceWords words;
+    cudaStream_t st;
+};
+
+// Statistics and losses, and the gradients' float32 sums, a piece of the rows at a time.
+template <typename T>
+int head_run(const HeadCall& c, bool stats) {
+    const bool half = std::is_same<T, __half>::value;
+    int32_t* const target = reinterpret_cast<int32_t*>(c.scratch + c.l.off_target);
+    float* const zt = reinterpret_cast<float*>(c.scratch + c.l.off_zt);
+    float4* const stat = reinterpret_cast<float4*>(c.scratch + c.l.off_stat);
+    float2* const part = static_cast<float2*>(c.work);
+    float* const up_max = reinterpret_cast<float*>(c.scratch + c.l.off_up);
+    char* const clean = c.scratch + c.l.off_clean;
+    void* const dz = c.work;  // the parts are read before it is written
+    const bool grads = c.gx != nullptr || c.gw != nullptr;
+    const HeadOperand W{c.w, c.ldw};
+    const HeadSplits sp = head_splits(c.M, c.K, c.V);
+    if (grads && c.up != nullptr) {
+        if (int e = launch(k_head_up_max, dim3(1), 1024, 0, c.st, 1, c.up, target, c.M, up_max)) return e;
+    }
+    if (c.M == 0 && c.gw != nullptr &&
+        cudaMemsetAsync(c.gw, 0, static_cast<size_t>(sp.w.splits) * c.V * c.l.ldo * sizeof(float), c.st) != cudaSuccess)
+        return RAVEL_ERR_CUDA;
+    for (int64_t r0 = 0; r0 < c.M; r0 += c.l.piece) {
+        const int64_t rows = std::min(c.l.piece, c.M - r0);
+        const HeadOperand X{clean + static_cast<size_t>(r0) * c.l.ldc * 2, c.l.ldc};
+        HeadLogitsArgs a;
+        std::memset(&a, 0, sizeof(a));
+        a.M = rows; a.V = static_cast<int>(c.V);
+        a.target = target + r0;
+        a.err = c.words.error; a.wait_limit = c.words.wait_limit;
+        if (stats) {
+            a.part = part; a.zt = zt;
+            if (int e = head_logits<T, HEAD_STATS>(X, W, c.K, a, c.st)) return e;
+            const int tile = head_pairs(rows) ? 256 : 128;
+            const int parts = static_cast<int>((c.V + tile - 1) / tile) * 2;
+            if (int e = launch(k_head_rows, dim3(static_cast<unsigned>((rows + HR_ROWS - 1) / HR_ROWS)),
+                               HR_ROWS * HR_GROUPS, 0, c.st, 1, part, parts, rows, target + r0, zt, c.losses + r0,
+                               stat + r0))
+                return e;
+        }
+        if (!grads) continue;
+        a.stat = stat + r0;
+        a.up = c.up != nullptr ? c.up + r0 : nullptr;
+        a.up_max = up_max;
+        a.unit_log2 = half ? 15.0f : 0.0f;
+        a.dz = dz; a.ldz = c.l.ldz;
+        if (int e = head_logits<T, HEAD_EXP>(X, W, c.K, a, c.st)) return e;
+        const HeadOperand Z{dz, c.l.ldz};
+        HeadGradArgs g;
+        std::memset(&g, 0, sizeof(g));
+        g.N = c.K; g.ldo = c.l.ldo;
+        g.err = c.words.error; g.wait_limit = c.words.wait_limit;
+        if (c.gx != nullptr) {
+            g.M = rows; g.splits = sp.x.splits;
+            g.out = c.gx + r0 * c.l.ldo; g.slab = c.M * c.l.ldo; g.add = 0;
+            if (int e = sp.x.cg == 2 ? launch_grad<T, 2, 256, false>(Z, W, c.V, g, c.st)
+                                     : launch_grad<T, 1, 128, false>(Z, W, c.V, g, c.st))
+                return e;
+        }
+        if (c.gw != nullptr) {
+            g.M = c.V; g.splits = sp.w.splits;
+            g.out = c.gw; g.slab = c.V * c.l.ldo; g.add = r0 > 0;
+            if (int e = sp.w.cg == 2 ? launch_grad<T, 2, 256, true>(Z, X, rows, g, c.st)
+                                     : launch_grad<T, 1, 128, true>(Z, X, rows, g, c.st))
+                return e;
+        }
+    }
+    return RAVEL_OK;
+}
+
+}  // namespace
+}  // namespace ravel
+
+using namespace ravel;
+
+extern "C" {
+
+int ravel_embedding_fwd(const void* ids, int ids_dtype, const void* weight, int64_t ldw, int64_t N, int64_t V, int64_t K,
+                        float scale, void* y, int dtype, void* stream) {
+    RAVEL_TIMED("ravel_embedding_fwd", stream);
+    if (int e = embed_check(N, V, K, ids_dtype, dtype)) return e;
+    if (N == 0 || K == 0) return RAVEL_OK;
+    if (ids == nullptr || weight == nullptr || y == nullptr || (V > 1 && ldw < K)) return RAVEL_ERR_INVALID_ARG;
+    EmbedArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.ids = ids; a.ids64 = ids_dtype == RAVEL_I64;
+    a.w = weight; a.out = y;
+    a.N = N; a.V = V; a.K = K; a.ldw = ldw; a.scale = scale;
+    DeviceWords words;
+    if (int e = device_words(&words)) return e;
+    a.err = words.error;
+    const int es = esize(dtype);
+    const bool vec = (K * es) % 16 == 0 && aligned16(weight) && (V == 1 || ldw * es % 16 == 0) && aligned16(y);
+    const int64_t units = vec ? K * es / 16 : K;
+    a.tx = embed_tx(units);
+    const int64_t blocks = (N + EM_THREADS / a.tx - 1) / (EM_THREADS / a.tx);
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, int64_t{sm_count()} * 64)));
+    return with_float_type(dtype, [&](auto tv) -> int {
+        using T = decltype(tv);
+        const auto kern = vec ? k_embed<T, 16 / sizeof(T)> : k_embed<T, 1>;
+        return launch(kern, grid, EM_THREADS, 0, static_cast<cudaStream_t>(stream), 1, a);
+    });
+}
+
+size_t ravel_embedding_scratch_bytes(int64_t N, int64_t V, int64_t K) {
+    if (N < 0 || V <= 0 || K < 0 || N > kMaxRows || V >= kMaxRows || K > kMaxRows) return 0;
+    return embed_layout(N, V, K).total;
+}
+
+int ravel_embedding_bwd(const void* ids, int ids_dtype, const void* grad_y, int64_t ldg, int64_t N, int64_t V, int64_t K,
+                        float scale, int64_t padding_idx, void* grad_weight, int dtype, void* scratch,
+                        size_t scratch_bytes, void* stream) {
+    RAVEL_TIMED("ravel_embedding_bwd", stream);
+    if (int e = embed_check(N, V, K, ids_dtype, dtype)) return e;
+    if (K == 0) return RAVEL_OK;
+    if (grad_weight == nullptr || (N > 0 && (ids == nullptr || grad_y == nullptr || (N > 1 && ldg < K))))
+        return RAVEL_ERR_INVALID_ARG;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int es = esize(dtype);
+    if (N == 0)
+        return cudaMemsetAsync(grad_weight, 0, static_cast<size_t>(V) * K * es, st) == cudaSuccess ? RAVEL_OK
+                                                                                                     : RAVEL_ERR_CUDA;
+    const EmbedLayout l = embed_layout(N, V, K);
+    if (scratch == nullptr || scratch_bytes < l.total) return RAVEL_ERR_WORKSPACE;
+    char* const s = static_cast<char*>(scratch);
+    EmbedArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.ids = ids; a.ids64 = ids_dtype == RAVEL_I64;
+    a.g = grad_y; a.out = grad_weight;
+    a.N = N; a.V = V; a.K = K; a.ldg = ldg; a.pad = padding_idx; a.scale = scale;
+    DeviceWords words;
+    if (int e = device_words(&words)) return e;
+    a.err = words.error;
+    a.clean = reinterpret_cast<int32_t*>(s + l.off_clean);
+    a.present = reinterpret_cast<unsigned char*>(s + l.off_present);
+    a.part = reinterpret_cast<float*>(s + l.off_part);
+    a.keys = s + l.off_tape;
+    event_keys(N, V + 1, &a.tbits, &a.key64);  // token above position
+    if (cudaMemsetAsync(a.present, 0, static_cast<size_t>(V), st) != cudaSuccess) return RAVEL_ERR_CUDA;
+    if (int e = launch(k_embed_ids, dim3(static_cast<unsigned>((N + 255) / 256)), 256, 0, st, 1, a)) return e;
+    if (int e = ravel_tape_build(a.clean, nullptr, RAVEL_I32, nullptr, 1, N, 1, V + 1, 0, s + l.off_tape, l.tape_bytes,
+                                 s + l.off_sort, l.sort_bytes, stream))
+        return e;
+    const bool vec = (K * es) % 16 == 0 && aligned16(grad_y) && (N == 1 || ldg * es % 16 == 0) && aligned16(grad_weight);
+    a.tx = embed_tx(vec ? K * es / 16 : K);
+    a.range = embed_range(N, a.tx);
+    a.ranges = (N + a.range - 1) / a.range;
+    const int groups = EM_THREADS / a.tx;
+    a.sum_blocks = (a.ranges + groups - 1) / groups;
+    const int64_t zero_blocks = (V + EM_ZERO_ROWS - 1) / EM_ZERO_ROWS;
+    return with_float_type(dtype, [&](auto tv) -> int {
+        using T = decltype(tv);
+        const auto kern = vec ? k_embed_sum<T, 16 / sizeof(T)> : k_embed_sum<T, 1>;
+        if (int e = launch(kern, dim3(static_cast<unsigned>(a.sum_blocks + zero_blocks)), EM_THREADS, 0, st, 1, a)) return e;
+        if (a.ranges < 2) return RAVEL_OK;
+        const unsigned cols = static_cast<unsigned>(std::min<int64_t>((K + 31) / 32, 32));
+        return launch(k_embed_join<T>, dim3(static_cast<unsigned>(a.ranges - 1), cols), EM_THREADS, 0, st, 1, a);
+    });
+}
+
+size_t ravel_linear_ce_scratch_bytes(int64_t M, int64_t K, int64_t V) {
+    if (head_check(M, K, V, RAVEL_I64, RAVEL_BF16) != RAVEL_OK) return 0;
+    return head_layout(M, K, V).total;
+}
+
+size_t ravel_linear_ce_work_bytes(int64_t M, int64_t K, int64_t V, int grads) {
+    if (head_check(M, K, V, RAVEL_I64, RAVEL_BF16) != RAVEL_OK) return 0;
+    const HeadLayout l = head_layout(M, K, V);
+    return grads ? l.work_grads : l.work;
+}
+
+int ravel_linear_ce_slabs(int64_t M, int64_t K, int64_t V, int64_t* sizes) {
+    if (sizes == nullptr) return RAVEL_ERR_INVALID_ARG;
+    if (int e = head_check(M, K, V, RAVEL_I64, RAVEL_BF16)) return e;
+    const HeadSplits s = head_splits(M, K, V);
+    sizes[0] = s.x.splits;
+    sizes[1] = s.w.splits;
+    sizes[2] = up_to(K, 4);
+    return RAVEL_OK;
+}
+
+int ravel_linear_ce_fwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* targets,
+                        int target_dtype, int64_t M, int64_t K, int64_t V, int64_t ignore_index, int reduction,
+                        float* losses, float* out, float* factor, float* slabs_x, float* slabs_w, int dtype,
+                        void* scratch, size_t scratch_bytes, void* work, size_t work_bytes, void* stream) {
+    RAVEL_TIMED("ravel_linear_ce_fwd", stream);
+    if (int e = head_check(M, K, V, target_dtype, dtype)) return e;
+    const bool grads = slabs_x != nullptr || slabs_w != nullptr;
+    if (reduction < RAVEL_REDUCE_NONE || reduction > RAVEL_REDUCE_MEAN || weight == nullptr || ldw < K ||
+        (M > 0 && (x == nullptr || targets == nullptr || losses == nullptr || (M > 1 && ldx < K))) ||
+        (reduction == RAVEL_REDUCE_NONE ? grads : out == nullptr) || (grads && factor == nullptr) ||
+        !aligned16(weight) || ldw % 8 != 0 || !aligned16(slabs_x) || !aligned16(slabs_w))
+        return RAVEL_ERR_INVALID_ARG;
+    HeadCall c;
+    c.l = head_layout(M, K, V);
+    if (scratch == nullptr || scratch_bytes < c.l.total || work == nullptr ||
+        work_bytes < (grads ? c.l.work_grads : c.l.work) || !aligned16(scratch) || !aligned16(work))
+        return RAVEL_ERR_WORKSPACE;
+    if (int e = device_words(&c.words)) return e;
+    c.x = x; c.w = weight; c.ldx = ldx; c.ldw = ldw;
+    c.M = M; c.K = K; c.V = V;
+    c.losses = losses; c.up = nullptr; c.gx = slabs_x; c.gw = slabs_w;
+    c.scratch = static_cast<char*>(scratch);
+    c.work = work;
+    c.st = static_cast<cudaStream_t>(stream);
+    int32_t* const target = reinterpret_cast<int32_t*>(c.scratch + c.l.off_target);
+    return with_half_type(dtype, [&](auto tv) -> int {
+        using T = decltype(tv);
+        if (M > 0) {
+            HeadPrepArgs p;
+            std::memset(&p, 0, sizeof(p));
+            p.targets = targets; p.targets64 = target_dtype == RAVEL_I64;
+            p.M = M; p.V = V; p.ignore = ignore_index; p.target = target;
+            p.x = x; p.clean = c.scratch + c.l.off_clean;
+            p.K = K; p.ldx = ldx; p.ldc = c.l.ldc;
+            p.vec = aligned16(x) && (M == 1 || ldx % 8 == 0);
+            p.err = c.words.error;
+            const dim3 grid(static_cast<unsigned>(std::min<int64_t>((M + 7) / 8, int64_t{sm_count()} * 32)));
+            if (int e = launch(k_head_prep<T>, grid, 256, 0, c.st, 1, p)) return e;
+        }
+        if (int e = head_run<T>(c, true)) return e;
+        if (reduction == RAVEL_REDUCE_NONE) return RAVEL_OK;
+        return launch(reduction == RAVEL_REDUCE_MEAN ? k_head_total<true> : k_head_total<false>, dim3(1), 1024, 0, c.st, 1,
+                      losses, target, M, out, factor);
+    });
+}
+
+int ravel_linear_ce_grad(const void* weight, int64_t ldw, const float* up, int64_t M, int64_t K, int64_t V, float* factor,
+                         float* slabs_x, float* slabs_w, int dtype, void* scratch, size_t scratch_bytes, void* work,
+                         size_t work_bytes, void* stream) {
+    RAVEL_TIMED("ravel_linear_ce_grad", stream);
+    if (int e = head_check(M, K, V, RAVEL_I64, dtype)) return e;
+    if (weight == nullptr || ldw < K || !aligned16(weight) || ldw % 8 != 0 || factor == nullptr ||
+        (M > 0 && up == nullptr) || !aligned16(slabs_x) || !aligned16(slabs_w))
+        return RAVEL_ERR_INVALID_ARG;
+    HeadCall c;
+    c.l = head_layout(M, K, V);
+    if (scratch == nullptr || scratch_bytes < c.l.total || work == nullptr || work_bytes < c.l.work_grads ||
+        !aligned16(scratch) || !aligned16(work))
+        return RAVEL_ERR_WORKSPACE;
+    if (int e = device_words(&c.words)) return e;
+    c.x = nullptr; c.w = weight; c.ldx = 0; c.ldw = ldw;
+    c.M = M; c.K = K; c.V = V;
+    c.losses = nullptr; c.up = up; c.gx = slabs_x; c.gw = slabs_w;
+    c.scratch = static_cast<char*>(scratch);
+    c.work = work;
+    c.st = static_cast<cudaStream_t>(stream);
+    const int rc = with_half_type(dtype, [&](auto tv) -> int { return head_run<decltype(tv)>(c, false); });
+    if (rc != RAVEL_OK) return rc;
+    return cudaMemcpyAsync(factor, c.scratch + c.l.off_up, sizeof(float), cudaMemcpyDeviceToDevice, c.st) == cudaSuccess
+               ? RAVEL_OK
+               : RAVEL_ERR_CUDA;
+}
+
+int ravel_linear_ce_bwd(const float* slabs_x, const float* slabs_w, const float* up, const float* factor, int64_t M,
+                        int64_t K, int64_t V, void* grad_x, void* grad_w, int dtype, void* stream) {
+    RAVEL_TIMED("ravel_linear_ce_bwd", stream);
+    if (int e = head_check(M, K, V, RAVEL_I64, dtype)) return e;
+    if (factor == nullptr || (grad_x != nullptr && M > 0 && slabs_x == nullptr) || (grad_w != nullptr && slabs_w == nullptr))
+        return RAVEL_ERR_INVALID_ARG;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const HeadSplits s = head_splits(M, K, V);
+    const int64_t ldo = up_to(K, 4);
+    return with_half_type(dtype, [&](auto tv) -> int {
+        using T = decltype(tv);
+        const float unit = std::is_same<T, __half>::value ? 1.0f / 32768.0f : 1.0f;
+        auto out = [&](const float* slabs, int splits, int64_t rows, void* g) -> int {
+            if (g == nullptr || rows == 0) return RAVEL_OK;
+            const int64_t units = rows * ((K + 3) / 4);
+            const dim3 grid(static_cast<unsigned>(std::min<int64_t>((units + 255) / 256, int64_t{sm_count()} * 32)));
+            const int vec = K % 4 == 0 && reinterpret_cast<uintptr_t>(g) % 8 == 0;
+            return launch(k_head_out<T>, grid, 256, 0, st, 1, slabs, splits, rows * ldo, ldo, rows, K, vec, up, factor, unit,
+                          static_cast<T*>(g));
+        };
+        if (int e = out(slabs_x, s.x.splits, M, grad_x)) return e;
+        return out(slabs_w, s.w.splits, V, grad_w);
+    });
+}
+
+}  // extern "C"
