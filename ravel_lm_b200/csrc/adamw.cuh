@@ -4,8 +4,9 @@
 //   m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2
 //   p = p (1 - lr wd) - lr / (1 - b1^t)  m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
-// in float32 (p: the float32 master of a 16-bit parameter, which gets its rounding in the same pass), every operation
-// rounded by itself, so that the result does not depend on what a compiler contracts.
+// in float32 (p: the float32 master of a 16-bit parameter, which gets its rounding in the same pass).  The states'
+// operations are rounded one by one, so that a state does not depend on what a compiler contracts; the root and
+// the reciprocal are the hardware's approximations (2^-22 of a step that is a small part of p).
 //
 //   k_grad_norm      sums of squares in float64, a part per block (any float32 gradient's square is finite there, and the
 //                    sum is the same to float32 whatever its order).
@@ -126,40 +127,56 @@ __device__ __forceinline__ void adam_put_codes(unsigned char* p, int64_t i, int6
 
 // ------------------------------------------------------------------ 8-bit values
 // BIAS 15: sign, 4, 3 (the first moment).  BIAS 31: 5, 3, no sign (the second).
+//
+// A code's exponent and mantissa put in place of float32's stand for its value times 2^(BIAS - 127), the smallest exponent
+// field for float32's subnormal numbers: two multiplications by powers of two decode every code, and
+// encode with 20 bits to spare, without a case apart.  The first form, which told the cases apart by integers
+// and comparisons, made the 8-bit step issue-bound (118 M bfloat16 elements: 643 us).
 constexpr int AW_NAN = -128;  // the exponent of a block that stands for NaN
 
 __device__ __forceinline__ float pow2_of(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
-
-template <int BIAS>
-__device__ __forceinline__ float value8(uint32_t code, float scale) {
-    const uint32_t a = BIAS == 15 ? code & 0x7Fu : code;
-    const float y = a < 8u ? static_cast<float>(a) * pow2_of(-BIAS - 2)
-                           : __uint_as_float((a + ((127u - BIAS) << 3)) << 20);
-    const float x = __fmul_rn(y, scale);
-    return BIAS == 15 && code > 127u ? -x : x;
-}
 __device__ __forceinline__ float scale8(int e) { return e == AW_NAN ? __int_as_float(0x7fc00000) : pow2_of(e); }
 
-// The warp's block exponent of its values' largest magnitude (a NaN or infinity in it: AW_NAN).
-__device__ __forceinline__ int block_exponent(float top, bool bad) {
-    const unsigned t = __reduce_max_sync(0xffffffffu, __float_as_uint(top));  // magnitudes order as their bits
-    if (__any_sync(0xffffffffu, bad)) return AW_NAN;
+// The value of byte k of c (its block's scale: scale8 of the exponent).
+template <int BIAS>
+__device__ __forceinline__ float value8(uint32_t c, int k, float scale) {
+    uint32_t b;
+    if constexpr (BIAS == 15) {
+        const uint32_t t = c << (24 - 8 * k);  // the byte on top: its sign is float32's
+        b = ((t >> 4) & 0x07f00000u) | (t & 0x80000000u);
+    } else {
+        b = (k < 3 ? c << (k < 3 ? 20 - 8 * k : 0) : c >> 4) & 0x0ff00000u;
+    }
+    return __fmul_rn(__fmul_rn(__uint_as_float(b), pow2_of(127 - BIAS)), scale);
+}
+
+// A block's exponent from its values' largest magnitude, as bits (a NaN's are above infinity's): AW_NAN for no number.
+__device__ __forceinline__ int block_exponent(uint32_t top) {
+    const uint32_t t = __reduce_max_sync(0xffffffffu, top);
+    if (t >= 0x7f800000u) return AW_NAN;
     int e = static_cast<int>(t >> 23) - 127;
     e = e < -126 ? -126 : e;
     if (__uint_as_float(t) > __fmul_rn(pow2_of(e), 1.875f)) ++e;
     return e > 127 ? 127 : e;
 }
 
-// x rounded to a code, up or down by 16 random bits.
+// x rounded to a code, up or down by 16 random bits (r: those above bit 4, and 8).
 template <int BIAS>
 __device__ __forceinline__ uint32_t code8(float x, float down1, float down2, uint32_t r) {
-    const float y = __fmul_rn(__fmul_rn(fabsf(x), down1), down2);
-    const uint32_t normal = ((__float_as_uint(y) + (r << 4) + 8u) >> 20) - ((127u - BIAS) << 3);
-    const float tiny = __fadd_rn(__fmul_rn(y, pow2_of(BIAS + 2)),
-                                 __fmul_rn(__fadd_rn(static_cast<float>(r), 0.5f), pow2_of(-16)));
-    uint32_t c = y < pow2_of(1 - BIAS) ? static_cast<uint32_t>(tiny) : normal;
+    const uint32_t c = (__float_as_uint(__fmul_rn(__fmul_rn(fabsf(x), down1), down2)) + r) >> 20;
     if (BIAS == 31) return c > 255u ? 255u : c;
     return (c > 127u ? 127u : c) | (x < 0.0f ? 0x80u : 0u);
+}
+
+__device__ __forceinline__ float sqrt_approx(float x) {
+    float y;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 // Well-mixed bits of 32: two multiplications between shifted exclusive ors.
@@ -169,26 +186,26 @@ __device__ __forceinline__ uint32_t mix32(uint32_t i) {
     return i ^ (i >> 16);
 }
 
-// 8 values of a lane as codes, their block's exponent into *e.
+// 8 values of a lane as codes, their block's exponent into *e; the random bits are h's low or high halves.
 template <int BIAS>
-__device__ __forceinline__ uint64_t quantise8(const float (&x)[8], const uint32_t (&r)[8], signed char* e, int lane) {
-    float top = 0.0f;
-    bool bad = false;
+__device__ __forceinline__ uint64_t quantise8(const float (&x)[8], const uint32_t (&h)[8], signed char* e, int lane) {
+    uint32_t top = 0u;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const float a = fabsf(x[k]);
-        bad |= !(a <= 3.402823466e38f);
-        top = fmaxf(top, a);
-    }
-    const int b = block_exponent(top, bad);
+    for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(x[k]) & 0x7fffffffu);
+    const int b = block_exponent(top);
     if (lane == 0) *e = static_cast<signed char>(b);
     if (b == AW_NAN) return 0;
-    const int h = b >> 1;
-    const float d1 = pow2_of(-h), d2 = pow2_of(h - b);
-    uint64_t c = 0;
+    const int s = BIAS - 127 - b, s1 = s >> 1;  // -239 <= s <= 30, in two steps
+    const float d1 = pow2_of(s1), d2 = pow2_of(s - s1);
+    uint32_t c[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) c |= static_cast<uint64_t>(code8<BIAS>(x[k], d1, d2, r[k])) << (8 * k);
-    return c;
+    for (int k = 0; k < 8; ++k) {
+        const uint32_t r = BIAS == 15 ? (h[k] & 0xFFFFu) * 16u + 8u : ((h[k] >> 12) & 0xFFFF0u) + 8u;
+        c[k] = code8<BIAS>(x[k], d1, d2, r);
+    }
+    const uint32_t lo = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
+    const uint32_t hi = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
+    return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
 // ------------------------------------------------------------------ the norm
@@ -296,8 +313,8 @@ __global__ void __launch_bounds__(32 * AW_WARPS) k_adamw(const __grid_constant__
         const float ms = scale8(me), vs = scale8(ve);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            m[e] = value8<15>(static_cast<uint32_t>(mc >> (8 * e)) & 0xFFu, ms);
-            v[e] = value8<31>(static_cast<uint32_t>(vc >> (8 * e)) & 0xFFu, vs);
+            m[e] = value8<15>(static_cast<uint32_t>(mc >> (e < 4 ? 0 : 32)), e & 3, ms);
+            v[e] = value8<31>(static_cast<uint32_t>(vc >> (e < 4 ? 0 : 32)), e & 3, vs);
         }
     }
 #pragma unroll
@@ -305,8 +322,8 @@ __global__ void __launch_bounds__(32 * AW_WARPS) k_adamw(const __grid_constant__
         const float ge = a.clipped ? __fmul_rn(g[e], s.clip) : g[e];
         m[e] = __fadd_rn(__fmul_rn(m[e], a.b1), __fmul_rn(ge, a.omb1));
         v[e] = __fadd_rn(__fmul_rn(v[e], a.b2), __fmul_rn(__fmul_rn(ge, ge), a.omb2));
-        const float d = __fadd_rn(__fmul_rn(__fsqrt_rn(v[e]), s.c2), a.eps);
-        p[e] = __fsub_rn(__fmul_rn(p[e], s.decay), __fmul_rn(__fdiv_rn(m[e], d), s.c1));
+        const float d = fmaf(sqrt_approx(v[e]), s.c2, a.eps);
+        p[e] = fmaf(-s.c1, __fmul_rn(m[e], rcp_approx(d)), __fmul_rn(p[e], s.decay));
     }
     if constexpr (sizeof(T) == 4) {
         adam_store(static_cast<float*>(t.p), i, n, vec, p);
@@ -317,36 +334,42 @@ __global__ void __launch_bounds__(32 * AW_WARPS) k_adamw(const __grid_constant__
     if constexpr (EIGHT) {
         // elements past the end are zero and lie in no code
         const uint32_t key = mix32(s.step * 0x9E3779B1u + static_cast<uint32_t>(a.place + k));
-        uint32_t rm[8], rv[8];
+        uint32_t h[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const uint32_t r = mix32(static_cast<uint32_t>(i + e) ^ key);
-            rm[e] = r & 0xFFFFu;
-            rv[e] = r >> 16;
+            h[e] = mix32(static_cast<uint32_t>(i + e) ^ key);
             if (i + e >= n) m[e] = v[e] = 0.0f;
         }
-        adam_put_codes(static_cast<unsigned char*>(t.m), i, n, vec, quantise8<15>(m, rm, t.me + block, lane));
-        adam_put_codes(static_cast<unsigned char*>(t.v), i, n, vec, quantise8<31>(v, rv, t.ve + block, lane));
+        adam_put_codes(static_cast<unsigned char*>(t.m), i, n, vec, quantise8<15>(m, h, t.me + block, lane));
+        adam_put_codes(static_cast<unsigned char*>(t.v), i, n, vec, quantise8<31>(v, h, t.ve + block, lane));
     } else {
         adam_store(static_cast<float*>(t.m), i, n, vec, m);
         adam_store(static_cast<float*>(t.v), i, n, vec, v);
     }
 }
 
-// What 8-bit codes stand for (float32 or bfloat16, which holds them exactly down to its subnormals).
+// What 8-bit codes stand for (float32 or bfloat16, which holds them exactly down to its subnormals), 16 a thread.
 template <typename T, int BIAS>
 __global__ void __launch_bounds__(256) k_values8(const unsigned char* __restrict__ code, const signed char* __restrict__ e,
                                                  int64_t n, int vec, T* __restrict__ out) {
     grid_wait();
     grid_trigger();
-    for (int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 8; i < n;
-         i += static_cast<int64_t>(gridDim.x) * 2048) {
-        const uint64_t c = adam_codes(code, i, n, vec);
-        const float s = scale8(e[i / 256]);
+    const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * 16;
+    if (i >= n) return;
+    uint32_t c[4];
+    if (vec && i + 16 <= n) {
+        *reinterpret_cast<uint4*>(c) = __ldg(reinterpret_cast<const uint4*>(code + i));
+    } else {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) *reinterpret_cast<uint64_t*>(c + 2 * q) = adam_codes(code, i + 8 * q, n, vec);
+    }
+    const float s = scale8(e[i / 256]);
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
         float f[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) f[k] = value8<BIAS>(static_cast<uint32_t>(c >> (8 * k)) & 0xFFu, s);
-        adam_store(out, i, n, vec, f);
+        for (int k = 0; k < 8; ++k) f[k] = value8<BIAS>(c[2 * q + k / 4], k & 3, s);
+        adam_store(out, i + 8 * q, n, vec, f);
     }
 }
 

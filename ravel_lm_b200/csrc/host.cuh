@@ -64,9 +64,6 @@ int device_words(DeviceWords* out);
 int encode_map_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t inner, int64_t outer,
                   int64_t pitch, int box_inner, int box_outer);
 
-// Sort keys of the event tape of streams of T events over A addresses: address << *tbits | time, in 64 bits where *key64.
-void event_keys(int64_t T, int64_t A, int* tbits, int* key64);
-
 // One timing record around the rest of the enclosing entry point (a pair of CUDA
 // events while ravel_timing_start's recording is on, nothing otherwise).
 class EntryTimer {

@@ -162,7 +162,8 @@ int ravel_state_values(const void* codes, const signed char* exponents, int64_t 
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const unsigned char* const c = static_cast<const unsigned char*>(codes);
     const int vec = on16(codes) && on16(out);
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((n + 2047) / 2048, int64_t{sm_count()} * 32)));
+    if (n > (int64_t{1} << 40)) return RAVEL_ERR_UNSUPPORTED;
+    const dim3 grid(static_cast<unsigned>((n + 4095) / 4096));
     auto go = [&](auto tv) -> int {
         using T = decltype(tv);
         if (is_signed) return launch(k_values8<T, 15>, grid, 256, 0, st, 1, c, exponents, n, vec, static_cast<T*>(out));

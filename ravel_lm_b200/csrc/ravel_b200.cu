@@ -346,12 +346,6 @@ int raise_smem(const void* kernel, size_t bytes) {
     return RAVEL_OK;
 }
 
-void event_keys(int64_t T, int64_t A, int* tbits, int* key64) {
-    const KeyLayout l = key_layout(T, A, 0);
-    *tbits = l.tbits;
-    *key64 = l.key64;
-}
-
 int device_words(DeviceWords* out) {
     static std::mutex mu;
     static std::map<int, DeviceWords> found;

@@ -40,31 +40,76 @@ int embed_tx(int64_t units) {
     return tx;
 }
 
-// Positions per range of the backward's sums: at least two waves of groups, and no range under 16 positions (a piece
+// Positions per range of the backward's sums: short enough for two waves of groups, no shorter than 16 (a piece
 // costs as much memory traffic as four 16-bit rows).
 int embed_range(int64_t N, int tx) {
-    const int64_t groups = static_cast<int64_t>(sm_count()) * 8 * (EM_THREADS / tx);
-    int64_t r = 128;
+    const int64_t groups = static_cast<int64_t>(sm_count()) * 2 * (EM_THREADS / tx);
+    int r = 64;
     while (r > 16 && N / r < groups * 2) r /= 2;
-    return static_cast<int>(r);
+    return r;
+}
+
+// ------------------------------------------------------------------ positions sorted by id
+struct IdsLayout {
+    size_t off_keys, off_other, off_count, off_live, total;
+    int passes, tiles, steps;
+};
+IdsLayout ids_layout(int64_t N, int64_t V) {
+    IdsLayout l;
+    int bits = 1;
+    while ((int64_t{1} << bits) < V) ++bits;
+    l.passes = (bits + IDS_BITS - 1) / IDS_BITS;
+    const int64_t steps = std::max<int64_t>(1, (N + IDS_STEP - 1) / IDS_STEP);
+    l.steps = static_cast<int>((steps + IDS_TILES - 1) / IDS_TILES);
+    l.tiles = static_cast<int>((steps + l.steps - 1) / l.steps);
+    l.off_keys = 0;
+    l.off_other = up256(static_cast<size_t>(N) * sizeof(uint2));
+    l.off_count = l.off_other + (l.passes > 1 ? l.off_other : 0);
+    l.off_live = l.off_count + static_cast<size_t>(IDS_TILES) * IDS_BINS * sizeof(int);
+    l.total = l.off_live + 256;
+    return l;
+}
+
+// Sorted (id, position) into the layout's keys; a: what the first pass reads.
+int sort_ids(IdsArgs a, const IdsLayout& l, char* mem, cudaStream_t st) {
+    uint2* const keys = reinterpret_cast<uint2*>(mem + l.off_keys);
+    uint2* const other = reinterpret_cast<uint2*>(mem + l.off_other);
+    int bits = 1;
+    while ((int64_t{1} << bits) < a.V) ++bits;
+    a.live = reinterpret_cast<int*>(mem + l.off_live);
+    a.count = reinterpret_cast<int*>(mem + l.off_count);
+    a.tiles = l.tiles;
+    a.steps = l.steps;
+    const dim3 grid(static_cast<unsigned>(l.tiles));
+    a.shift = 0;
+    for (int p = 0; p < l.passes; ++p) {
+        a.bits = (bits - a.shift + l.passes - p - 1) / (l.passes - p);  // even digits
+        a.out = (l.passes - 1 - p) % 2 == 0 ? keys : other;
+        if (int e = launch(p == 0 ? k_ids_count<true> : k_ids_count<false>, grid, IDS_THREADS, 0, st, 1, a)) return e;
+        if (int e = launch(p == 0 ? k_ids_place<true> : k_ids_place<false>, grid, IDS_THREADS, 0, st, 1, a)) return e;
+        a.in = a.out;
+        a.shift += a.bits;
+    }
+    return RAVEL_OK;
 }
 
 struct EmbedLayout {
-    size_t off_clean, off_present, off_part, off_tape, off_sort, total, tape_bytes, sort_bytes;
-    int64_t ranges;
+    size_t off_present, off_list, off_part, off_ids, total, zeroed;
+    int64_t K4;
+    IdsLayout ids;
 };
-// Ranges as if each row took a whole block: the most there can be.
+// With ranges of 16 positions: the most there can be.
 EmbedLayout embed_layout(int64_t N, int64_t V, int64_t K) {
     EmbedLayout l;
-    l.ranges = (N + 15) / 16;
-    l.tape_bytes = ravel_tape_bytes(1, N, 1, V + 1, 0);
-    l.sort_bytes = ravel_scratch_bytes(1, N, 1, 1, V + 1, 1, RAVEL_F32, 0);
-    l.off_clean = 0;
-    l.off_present = up256(static_cast<size_t>(N) * 4);
-    l.off_part = l.off_present + up256(static_cast<size_t>(V));
-    l.off_tape = l.off_part + up256(static_cast<size_t>(l.ranges) * 2 * static_cast<size_t>(K) * sizeof(float));
-    l.off_sort = l.off_tape + up256(l.tape_bytes);
-    l.total = l.off_sort + up256(l.sort_bytes);
+    const size_t ranges = static_cast<size_t>((N + 15) / 16);
+    l.K4 = up_to(K, 4);
+    l.ids = ids_layout(N, V);
+    l.off_present = 0;
+    l.off_list = up256(static_cast<size_t>(V));
+    l.zeroed = l.off_list + sizeof(int);
+    l.off_part = up256(l.off_list + (ranges + 1) * sizeof(int));
+    l.off_ids = l.off_part + up256(ranges * 2 * static_cast<size_t>(l.K4) * sizeof(float));
+    l.total = l.off_ids + l.ids.total;
     return l;
 }
 
@@ -357,8 +402,8 @@ int ravel_embedding_fwd(const void* ids, int ids_dtype, const void* weight, int6
     const bool vec = (K * es) % 16 == 0 && aligned16(weight) && (V == 1 || ldw * es % 16 == 0) && aligned16(y);
     const int64_t units = vec ? K * es / 16 : K;
     a.tx = embed_tx(units);
-    const int64_t blocks = (N + EM_THREADS / a.tx - 1) / (EM_THREADS / a.tx);
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(blocks, int64_t{sm_count()} * 64)));
+    const int64_t rows = static_cast<int64_t>(EM_THREADS / a.tx) * EM_ROWS;
+    const dim3 grid(static_cast<unsigned>((N + rows - 1) / rows));
     return with_float_type(dtype, [&](auto tv) -> int {
         using T = decltype(tv);
         const auto kern = vec ? k_embed<T, 16 / sizeof(T)> : k_embed<T, 1>;
@@ -387,28 +432,30 @@ int ravel_embedding_bwd(const void* ids, int ids_dtype, const void* grad_y, int6
     const EmbedLayout l = embed_layout(N, V, K);
     if (scratch == nullptr || scratch_bytes < l.total) return RAVEL_ERR_WORKSPACE;
     char* const s = static_cast<char*>(scratch);
-    EmbedArgs a;
-    std::memset(&a, 0, sizeof(a));
-    a.ids = ids; a.ids64 = ids_dtype == RAVEL_I64;
-    a.g = grad_y; a.out = grad_weight;
-    a.N = N; a.V = V; a.K = K; a.ldg = ldg; a.pad = padding_idx; a.scale = scale;
     DeviceWords words;
     if (int e = device_words(&words)) return e;
-    a.err = words.error;
-    a.clean = reinterpret_cast<int32_t*>(s + l.off_clean);
-    a.present = reinterpret_cast<unsigned char*>(s + l.off_present);
+    if (cudaMemsetAsync(s, 0, l.zeroed, st) != cudaSuccess) return RAVEL_ERR_CUDA;
+    IdsArgs q;
+    std::memset(&q, 0, sizeof(q));
+    q.ids = ids; q.ids64 = ids_dtype == RAVEL_I64;
+    q.N = N; q.V = V; q.pad = padding_idx; q.strict = 1;
+    q.err = words.error;
+    q.present = reinterpret_cast<unsigned char*>(s + l.off_present);
+    if (int e = sort_ids(q, l.ids, s + l.off_ids, st)) return e;
+    EmbedArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.g = grad_y; a.out = grad_weight;
+    a.N = N; a.V = V; a.K = K; a.ldg = ldg; a.scale = scale;
+    a.present = q.present;
+    a.keys = reinterpret_cast<const uint2*>(s + l.off_ids + l.ids.off_keys);
+    a.live = reinterpret_cast<const int*>(s + l.off_ids + l.ids.off_live);
     a.part = reinterpret_cast<float*>(s + l.off_part);
-    a.keys = s + l.off_tape;
-    event_keys(N, V + 1, &a.tbits, &a.key64);  // token above position
-    if (cudaMemsetAsync(a.present, 0, static_cast<size_t>(V), st) != cudaSuccess) return RAVEL_ERR_CUDA;
-    if (int e = launch(k_embed_ids, dim3(static_cast<unsigned>((N + 255) / 256)), 256, 0, st, 1, a)) return e;
-    if (int e = ravel_tape_build(a.clean, nullptr, RAVEL_I32, nullptr, 1, N, 1, V + 1, 0, s + l.off_tape, l.tape_bytes,
-                                 s + l.off_sort, l.sort_bytes, stream))
-        return e;
+    a.K4 = l.K4;
+    a.list = reinterpret_cast<int*>(s + l.off_list);
     const bool vec = (K * es) % 16 == 0 && aligned16(grad_y) && (N == 1 || ldg * es % 16 == 0) && aligned16(grad_weight);
     a.tx = embed_tx(vec ? K * es / 16 : K);
     a.range = embed_range(N, a.tx);
-    a.ranges = (N + a.range - 1) / a.range;
+    a.ranges = static_cast<int>((N + a.range - 1) / a.range);
     const int groups = EM_THREADS / a.tx;
     a.sum_blocks = (a.ranges + groups - 1) / groups;
     const int64_t zero_blocks = (V + EM_ZERO_ROWS - 1) / EM_ZERO_ROWS;
@@ -417,8 +464,9 @@ int ravel_embedding_bwd(const void* ids, int ids_dtype, const void* grad_y, int6
         const auto kern = vec ? k_embed_sum<T, 16 / sizeof(T)> : k_embed_sum<T, 1>;
         if (int e = launch(kern, dim3(static_cast<unsigned>(a.sum_blocks + zero_blocks)), EM_THREADS, 0, st, 1, a)) return e;
         if (a.ranges < 2) return RAVEL_OK;
-        const unsigned cols = static_cast<unsigned>(std::min<int64_t>((K + 31) / 32, 32));
-        return launch(k_embed_join<T>, dim3(static_cast<unsigned>(a.ranges - 1), cols), EM_THREADS, 0, st, 1, a);
+        const int64_t items = static_cast<int64_t>(a.ranges - 1) * ((K + EJ_COLS - 1) / EJ_COLS);
+        return launch(k_embed_join<T>, dim3(static_cast<unsigned>(std::min<int64_t>(items, int64_t{sm_count()} * 8))),
+                      32 * EJ_GROUPS, 0, st, 1, a);
     });
 }
 
