@@ -470,7 +470,7 @@ int ravel_embedding_bwd(const void* ids, int ids_dtype, const void* grad_y, int6
  * with up NULL.  work is needed during a call only.
  */
 size_t ravel_linear_ce_scratch_bytes(int64_t M, int64_t K, int64_t V);
-size_t ravel_linear_ce_work_bytes(int64_t M, int64_t K, int64_t V, int grads);
+size_t ravel_linear_ce_work_bytes(int64_t M, int64_t K, int64_t V, int grads, int dtype);
 int ravel_linear_ce_slabs(int64_t M, int64_t K, int64_t V, int64_t* sizes);
 int ravel_linear_ce_fwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* targets,
                         int target_dtype, int64_t M, int64_t K, int64_t V, int64_t ignore_index, int reduction,

@@ -150,27 +150,25 @@ __device__ __forceinline__ float value8(uint32_t c, int k, float scale) {
     return __fmul_rn(__fmul_rn(__uint_as_float(b), pow2_of(127 - BIAS)), scale);
 }
 
-// A block's exponent from its values' largest magnitude, as bits (a NaN's are above infinity's): AW_NAN for no number.
+// A block's exponent from its values' largest magnitude, as bits (a NaN's are above infinity's).  Values past
+// 1.875 2^127 have no code: AW_NAN, as for infinity.
 __device__ __forceinline__ int block_exponent(uint32_t top) {
     const uint32_t t = __reduce_max_sync(0xffffffffu, top);
-    if (t >= 0x7f800000u) return AW_NAN;
-    int e = static_cast<int>(t >> 23) - 127;
-    e = e < -126 ? -126 : e;
-    if (__uint_as_float(t) > __fmul_rn(pow2_of(e), 1.875f)) ++e;
-    return e > 127 ? 127 : e;
+    if (t > 0x7f700000u) return AW_NAN;
+    const int e = max(static_cast<int>(t >> 23) - 127, -126);
+    return __uint_as_float(t) > __fmul_rn(pow2_of(e), 1.875f) ? e + 1 : e;
 }
 
 // x rounded to a code, up or down by 16 random bits (r: those above bit 4, and 8).
 template <int BIAS>
 __device__ __forceinline__ uint32_t code8(float x, float down1, float down2, uint32_t r) {
-    const uint32_t c = (__float_as_uint(__fmul_rn(__fmul_rn(fabsf(x), down1), down2)) + r) >> 20;
-    if (BIAS == 31) return c > 255u ? 255u : c;
-    return (c > 127u ? 127u : c) | (x < 0.0f ? 0x80u : 0u);
+    const uint32_t t = __float_as_uint(__fmul_rn(__fmul_rn(x, down1), down2)) + r;  // a sign stays on top
+    return BIAS == 31 ? t >> 20 : ((t >> 20) & 0x7Fu) | ((t >> 24) & 0x80u);
 }
 
 __device__ __forceinline__ float sqrt_approx(float x) {
     float y;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 __device__ __forceinline__ float rcp_approx(float x) {
@@ -322,7 +320,8 @@ __global__ void __launch_bounds__(32 * AW_WARPS) k_adamw(const __grid_constant__
         const float ge = a.clipped ? __fmul_rn(g[e], s.clip) : g[e];
         m[e] = __fadd_rn(__fmul_rn(m[e], a.b1), __fmul_rn(ge, a.omb1));
         v[e] = __fadd_rn(__fmul_rn(v[e], a.b2), __fmul_rn(__fmul_rn(ge, ge), a.omb2));
-        const float d = fmaf(sqrt_approx(v[e]), s.c2, a.eps);
+        // subnormal v counts as the least normal number, so that eps = 0 divides by no zero but v's own
+        const float d = fmaf(sqrt_approx(v[e] == 0.0f ? 0.0f : fmaxf(v[e], 1.17549435e-38f)), s.c2, a.eps);
         p[e] = fmaf(-s.c1, __fmul_rn(m[e], rcp_approx(d)), __fmul_rn(p[e], s.decay));
     }
     if constexpr (sizeof(T) == 4) {
@@ -334,12 +333,14 @@ __global__ void __launch_bounds__(32 * AW_WARPS) k_adamw(const __grid_constant__
     if constexpr (EIGHT) {
         // elements past the end are zero and lie in no code
         const uint32_t key = mix32(s.step * 0x9E3779B1u + static_cast<uint32_t>(a.place + k));
+        if (block * 256 + 256 > n) {  // the same for the whole warp
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (i + e >= n) m[e] = v[e] = 0.0f;
+        }
         uint32_t h[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            h[e] = mix32(static_cast<uint32_t>(i + e) ^ key);
-            if (i + e >= n) m[e] = v[e] = 0.0f;
-        }
+        for (int e = 0; e < 8; ++e) h[e] = mix32((static_cast<uint32_t>(i) + e) ^ key);
         adam_put_codes(static_cast<unsigned char*>(t.m), i, n, vec, quantise8<15>(m, h, t.me + block, lane));
         adam_put_codes(static_cast<unsigned char*>(t.v), i, n, vec, quantise8<31>(v, h, t.ve + block, lane));
     } else {

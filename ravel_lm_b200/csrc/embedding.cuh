@@ -47,6 +47,10 @@ struct EmbedArgs {
     int ranges, range;         // positions per range
     int sum_blocks;
     int tx;                    // threads per group, a power of two from 32 on
+    // ADD: the sums of weighted rows are added to float32 rows
+    const float4* weight;      // [N]: each row's weight is its third component, negated
+    float* add;                // [V], rows ldo apart
+    int64_t ldo;
 };
 
 __device__ __forceinline__ int64_t embed_id(const EmbedArgs& a, int64_t i) {
@@ -107,15 +111,22 @@ __device__ __forceinline__ void embed_piece(float* p, const float (&s)[VEC]) {
     }
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool ADD>
 __device__ __forceinline__ void embed_put(const EmbedArgs& a, uint32_t id, int64_t u, const float (&s)[VEC]) {
     float f[VEC];
+    if constexpr (ADD) {
+        float* const p = a.add + id * a.ldo + u * VEC;
 #pragma unroll
-    for (int e = 0; e < VEC; ++e) f[e] = s[e] * a.scale;
-    store_pack<T, VEC>(static_cast<T*>(a.out) + id * a.K + u * VEC, from_floats<T, VEC>(f));
+        for (int e = 0; e < VEC; ++e) f[e] = p[e] + s[e];
+        embed_piece<VEC>(p, f);
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f[e] = s[e] * a.scale;
+        store_pack<T, VEC>(static_cast<T*>(a.out) + id * a.K + u * VEC, from_floats<T, VEC>(f));
+    }
 }
 
-template <typename T, int VEC>
+template <typename T, int VEC, bool ADD>
 __global__ void __launch_bounds__(EM_THREADS) k_embed_sum(const EmbedArgs a) {
     grid_wait();
     grid_trigger();
@@ -154,11 +165,13 @@ __global__ void __launch_bounds__(EM_THREADS) k_embed_sum(const EmbedArgs a) {
         for (int b = i0; b < i1; b += EM_DEPTH) {
             uint32_t id[EM_DEPTH];
             Pack<T, VEC> row[EM_DEPTH];
+            float weight[ADD ? EM_DEPTH : 1];
 #pragma unroll
             for (int k = 0; k < EM_DEPTH; ++k) {
                 if (b + k >= i1) continue;
                 const uint2 key = __ldg(keys + b + k);
                 id[k] = key.x;
+                if constexpr (ADD) weight[k] = -a.weight[key.y].z;
                 row[k] = load_pack<T, VEC>(g + static_cast<int64_t>(key.y) * a.ldg + u * VEC);
             }
 #pragma unroll
@@ -166,7 +179,7 @@ __global__ void __launch_bounds__(EM_THREADS) k_embed_sum(const EmbedArgs a) {
                 if (b + k >= i1) continue;
                 if (id[k] != cur) {  // the token ends inside the range
                     if (head) embed_piece<VEC>(part + u * VEC, s);
-                    else embed_put<T, VEC>(a, cur, u, s);
+                    else embed_put<T, VEC, ADD>(a, cur, u, s);
                     head = false;
                     cur = id[k];
 #pragma unroll
@@ -175,19 +188,19 @@ __global__ void __launch_bounds__(EM_THREADS) k_embed_sum(const EmbedArgs a) {
                 float f[VEC];
                 to_floats<T, VEC>(row[k], f);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) s[e] += f[e];
+                for (int e = 0; e < VEC; ++e) s[e] = ADD ? fmaf(weight[ADD ? k : 0], f[e], s[e]) : s[e] + f[e];
             }
         }
         // the last token: a piece where it began before the range or goes on after it
         if (head || goes) embed_piece<VEC>(part + (head ? 0 : a.K4) + u * VEC, s);
-        else embed_put<T, VEC>(a, cur, u, s);
+        else embed_put<T, VEC, ADD>(a, cur, u, s);
     }
 }
 
 // A listed range's last token: its piece there (the second slot) and the first slots of the ranges that follow, as far
 // as the token reaches, a block per EJ_COLS columns.  Groups of the block take every EJ_GROUPS-th piece, their
 // sums are added in order.
-template <typename T>
+template <typename T, bool ADD>
 __global__ void __launch_bounds__(32 * EJ_GROUPS) k_embed_join(const EmbedArgs a) {
     __shared__ float4 red[EJ_GROUPS][32];
     grid_wait();
@@ -224,11 +237,13 @@ __global__ void __launch_bounds__(32 * EJ_GROUPS) k_embed_join(const EmbedArgs a
                 const float4 w = red[k][x];
                 s.x += w.x; s.y += w.y; s.z += w.z; s.w += w.w;
             }
-            T* const o = static_cast<T*>(a.out) + v * a.K + col;
             const float f[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (col + e < a.K) o[e] = round_to<T>(f[e] * a.scale);
+            for (int e = 0; e < 4; ++e) {
+                if (col + e >= a.K) continue;
+                if constexpr (ADD) a.add[v * a.ldo + col + e] += f[e];
+                else static_cast<T*>(a.out)[v * a.K + col + e] = round_to<T>(f[e] * a.scale);
+            }
         }
         __syncthreads();
     }

@@ -7,18 +7,29 @@
 //
 // A row without a target (the ignored index) has loss 0 and gradient 0, whatever its x holds.
 //
-//   k_head_prep    targets as int32 (-1: none), and x with the rows that have none zeroed.
+//   k_head_prep    targets as int32 (-1: none), x with the rows that have none zeroed, and (fast) the targets' logits.
 //   k_head_logits  the logits' product, on the pairs and single CTAs of k_matmul.  The logits never leave the SM:
 //     HEAD_STATS   a thread owns a row of the tile and keeps the maximum and the sum of 2^((z - max) log2 e) over its
 //                  columns, the target's column apart (so that a confident row's 1 - p_t is no difference), a
 //                  part per row and half tile in memory; the target's logit is kept.
 //     HEAD_EXP     with the row's maximum and sum known: d z in 16 bits (the tensor cores' operand), for a piece
 //                  of the rows.
+//     HEAD_FAST    both in one product: E = exp(z - z_t) in 16 bits and its sums.
 //   k_head_rows    the parts of a row joined: loss, maximum, log2 of the sum, 1 - p_t.
 //   k_head_grad    d x and d W of a piece as float32 products, k divided over splits whose sums lie in slabs of their
 //                  own; d W adds up over the pieces.
 //   k_head_out     slabs added in order, scaled by the upstream gradient, rounded once.
 //   k_head_total   losses added in a fixed order, rows counted.
+//
+// A training step takes four products this way: the logits twice, d x, d W.  In bfloat16, whose range is float32's, three
+// do: with the target's own logit as the reference, E needs no maximum, and with s = sum_{v != t} E_v and f = 1 / (1 + s)
+//
+//   loss = log(1 + s),   d x = f (E W) - (1 - p_t) W_t,   d W = E^T (f x) - sum over the rows with t = v of (1 - p_t) x
+//
+// E_t left out of E; the last sums run over the positions sorted by target (embedding.cuh), in float32, so that the
+// target's term, which carries most of the gradient, is not rounded to 16 bits.  A row whose s passes 2^80 (a
+// loss above 55) or is no number flags its piece, and three launches that otherwise return at once do it by
+// HEAD_STATS and HEAD_EXP.  8192 x 1024 x 65536: 3.6 ms with four products.
 // float16: d z is kept times 2^15, so that probabilities down to 2^-29 stay normal numbers.
 // Every wait is bounded, as k_matmul's.
 #pragma once
@@ -30,19 +41,22 @@ namespace ravel {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-enum HeadMode { HEAD_STATS = 0, HEAD_EXP = 1 };
+enum HeadMode { HEAD_STATS = 0, HEAD_EXP = 1, HEAD_FAST = 2 };
+constexpr float HEAD_FAST_SUM = 1.2089258196146292e24f;  // 2^80
 
 struct HeadLogitsArgs : MmShape {
     int64_t M;                 // rows of the piece
     int V;
     const int32_t* target;     // [M], -1: none
-    float2* part;              // STATS: [2 ntiles][M]
-    float* zt;                 // STATS: [M] the target's logit
+    float2* part;              // STATS: [2 ntiles][M]; FAST: as many floats
+    float* zt;                 // [M] the target's logit, from STATS or for FAST
+    const int* only;           // null, or 0: nothing to do
+    int apart;                 // EXP: the target's term is left out
     const float4* stat;        // EXP: [M] (max, log2 sum, 1 - p_t, live)
     const float* up;           // EXP: a row's upstream gradient, or null
     const float* up_max;       //   and the largest of them
     float unit_log2;           // EXP: log2 of what d z is kept times
-    void* dz;                  // EXP: [M], rows ldz apart
+    void* dz;                  // EXP, FAST: [M], rows ldz apart
     int64_t ldz;
     unsigned int* err;
     const unsigned int* wait_limit;
@@ -54,6 +68,12 @@ struct HeadGradArgs : MmShape {
     float* out;                // [splits][M], rows ldo apart (a multiple of 4)
     int64_t ldo, slab;
     int add;                   // to what is there
+    // ROWS: out = f_m (the product) - (1 - p_t) W[target_m], the latter in the first slab
+    const float* f;            // [M]
+    const float4* stat;        // [M]
+    const int32_t* target;     // [M]
+    const void* w;             // [V, N], rows ldw apart
+    int64_t ldw;
     unsigned int* err;
     const unsigned int* wait_limit;
 };
@@ -129,6 +149,10 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
     constexpr int UNITS = BN / 64;  // 32-column units of an epilogue warp
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ unsigned char smem_raw[];
+    if (a.only != nullptr) {  // the same for every CTA
+        grid_wait();
+        if (*a.only == 0) return;
+    }
     const MmCta c = mm_begin<CG, COLS>(smem_raw, a.stages, &map_a, &map_b, a.wait_limit);
     const int tiles = a.mtiles * a.ntiles;
     const int t0 = static_cast<int>(blockIdx.x) / CG, tstep = static_cast<int>(gridDim.x) / CG;
@@ -163,6 +187,10 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
             uint32_t keep = 0u, sign = 0u;
             if (row < a.M) {
                 t = a.target[row];
+                if constexpr (MODE == HEAD_FAST) {
+                    top = a.zt[row];
+                    keep = t >= 0 ? 0xffffffffu : 0u;
+                }
                 if constexpr (MODE == HEAD_EXP) {
                     const float4 s = a.stat[row];
                     float u = 1.0f;
@@ -170,7 +198,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
                     const bool live = s.w != 0.0f && u != 0.0f;
                     top = s.x;
                     e0 = a.unit_log2 - s.y + log2f(fabsf(u));
-                    tv = -s.z * ex2(a.unit_log2) * fabsf(u);
+                    tv = a.apart ? 0.0f : -s.z * ex2(a.unit_log2) * fabsf(u);
                     keep = live ? 0xffffffffu : 0u;
                     sign = u < 0.0f ? 0x80008000u : 0u;
                 }
@@ -222,13 +250,25 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
                     for (int e = 0; e < 32; ++e) s[e & 3] += ex2(x[e]);
                     v.l += (s[0] + s[1]) + (s[2] + s[3]);
                 } else {
-                    sub_fma<32>(x, top, LOG2E, e0);
+                    if constexpr (MODE == HEAD_FAST) sub_scale<32>(x, top, LOG2E);
+                    else sub_fma<32>(x, top, LOG2E, e0);
 #pragma unroll
                     for (int e = 0; e < 32; ++e) x[e] = ex2(x[e]);
                     if (here) {
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
                             if (col + e == t) x[e] = tv;
+                    }
+                    if constexpr (MODE == HEAD_FAST) {
+                        if (col + 32 > a.V) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (col + e >= a.V) x[e] = 0.0f;
+                        }
+                        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) s[e & 3] += x[e];
+                        v.l += (s[0] + s[1]) + (s[2] + s[3]);
                     }
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
@@ -247,6 +287,9 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
             if constexpr (MODE == HEAD_STATS) {
                 if (row < a.M) a.part[static_cast<int64_t>(nt * 2 + half) * a.M + row] = make_float2(v.m, v.l);
             }
+            if constexpr (MODE == HEAD_FAST) {
+                if (row < a.M) reinterpret_cast<float*>(a.part)[static_cast<int64_t>(nt * 2 + half) * a.M + row] = v.l;
+            }
         }
     }
     mm_end<CG, COLS>(c, a.err);
@@ -254,7 +297,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
 
 // ------------------------------------------------------------------ the gradients' products
 // A: d z [rows][V] (A_MN false: d x, k over the vocabulary) or its transpose (true: d W, k over the rows); B [k][N].
-template <typename T, int CG, int BN, bool A_MN>
+template <typename T, int CG, int BN, bool A_MN, bool ROWS>
 __global__ void __launch_bounds__(MM_THREADS, 1)
     k_head_grad(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                 const __grid_constant__ HeadGradArgs a) {
@@ -292,6 +335,18 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
             const int64_t m0 = static_cast<int64_t>(mt) * (MM_BM * CG) + c.rank * MM_BM + q * 32;
             const int64_t n0 = static_cast<int64_t>(nt) * BN + half * UNITS * 32;
             float* const out = a.out + split * a.slab;
+            float f = 1.0f, hot = 0.0f;
+            const T* wt = nullptr;
+            if constexpr (ROWS) {
+                if (m0 + lane < a.M) {
+                    f = a.f[m0 + lane];
+                    const int t = a.target[m0 + lane];
+                    if (split == 0 && t >= 0) {
+                        hot = a.stat[m0 + lane].z;
+                        wt = static_cast<const T*>(a.w) + t * a.ldw;
+                    }
+                }
+            }
             const bool ok = __all_sync(0xffffffffu, mm_wait(bar_tfull + 8 * buf, (j / 2) & 1, c.limit, c.abort));
             tc_fence_after();
             if (!ok) break;
@@ -299,6 +354,16 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
 #pragma unroll 1
             for (int u = 0; u < UNITS; ++u) {
                 const int64_t col = n0 + u * 32;
+                const bool live = m0 < a.M && col < a.N;  // the same for the whole warp
+                // this lane's places in the 32 x 32 outputs, and what is there
+                float4 old[8];
+                if (a.add && live) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int64_t rw = m0 + i * 4 + (lane >> 3), cl = col + (lane & 7) * 4;
+                        if (rw < a.M && cl < a.ldo) old[i] = *reinterpret_cast<const float4*>(out + rw * a.ldo + cl);
+                    }
+                }
                 uint32_t r[32];
                 tmem_ld32(tm + u * 32, r);
                 if (u == UNITS - 1) {
@@ -306,7 +371,21 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
                     __syncwarp();
                     if (lane == 0) mbar_arrive_cluster(done_bar + 8 * buf);
                 }
-                if (m0 >= a.M || col >= a.N) continue;
+                if (!live) continue;
+                if constexpr (ROWS) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) r[e] = __float_as_uint(f * __uint_as_float(r[e]));
+                    if (wt != nullptr) {
+#pragma unroll
+                        for (int p = 0; p < 4; ++p) {
+                            float w[8];
+                            unpack8<T>(load8(wt, col + p * 8, a.N, true), w);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                r[p * 8 + e] = __float_as_uint(fmaf(-hot, w[e], __uint_as_float(r[p * 8 + e])));
+                        }
+                    }
+                }
                 // 32 rows of 128 bytes, their 16-byte pieces rotated against bank conflicts, then whole rows out
 #pragma unroll
                 for (int p = 0; p < 8; ++p)
@@ -320,8 +399,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
                         float4 v = *reinterpret_cast<const float4*>(st + rw * 128 + ((p ^ (rw & 7)) << 4));
                         float4* const o = reinterpret_cast<float4*>(out + (m0 + rw) * a.ldo + col + p * 4);
                         if (a.add) {
-                            const float4 w = *o;
-                            v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
+                            v.x += old[i].x; v.y += old[i].y; v.z += old[i].z; v.w += old[i].w;
                         }
                         *o = v;
                     }
@@ -340,9 +418,14 @@ struct HeadPrepArgs {
     int64_t M, V, ignore;
     int32_t* target;       // [M]
     const void* x;         // [M, K], rows ldx apart
-    void* clean;           // [M, K], rows ldc apart (16 bytes), or null
+    void* clean;           // [M, K], rows ldc apart (16 bytes)
     int64_t K, ldx, ldc;
     int vec;               // x has 16-byte rows
+    const void* w;         // [V, K], rows ldw apart (16 bytes)
+    int64_t ldw;
+    float* zt;             // [M] the targets' logits, or null
+    int* flags;            // one per piece, to be zeroed
+    int pieces;
     unsigned int* err;
 };
 // A warp per row.
@@ -351,6 +434,7 @@ __global__ void __launch_bounds__(256) k_head_prep(const HeadPrepArgs a) {
     grid_wait();
     grid_trigger();
     const int lane = threadIdx.x & 31;
+    for (int p = blockIdx.x * 256 + threadIdx.x; p < a.pieces; p += gridDim.x * 256) a.flags[p] = 0;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5); i < a.M;
          i += static_cast<int64_t>(gridDim.x) * 8) {
         const int64_t t = a.targets64 ? static_cast<const int64_t*>(a.targets)[i] : static_cast<const int32_t*>(a.targets)[i];
@@ -359,54 +443,120 @@ __global__ void __launch_bounds__(256) k_head_prep(const HeadPrepArgs a) {
             if (!in && t != a.ignore) atomicOr(a.err, RAVEL_DEVERR_INDEX);
             a.target[i] = live ? static_cast<int32_t>(t) : -1;
         }
-        if (a.clean == nullptr) continue;
         const T* const x = static_cast<const T*>(a.x) + i * a.ldx;
         T* const d = static_cast<T*>(a.clean) + i * a.ldc;
+        if (a.zt == nullptr || !live) {
 #pragma unroll 4
-        for (int64_t c = lane * 8; c < a.K; c += 256)
-            store8(d, c, a.K, true, live ? load8(x, c, a.K, a.vec) : make_uint4(0u, 0u, 0u, 0u));
+            for (int64_t c = lane * 8; c < a.K; c += 256)
+                store8(d, c, a.K, true, live ? load8(x, c, a.K, a.vec) : make_uint4(0u, 0u, 0u, 0u));
+            if (lane == 0 && a.zt != nullptr) a.zt[i] = 0.0f;
+            continue;
+        }
+        const T* const w = static_cast<const T*>(a.w) + t * a.ldw;
+        float z = 0.0f;
+#pragma unroll 4
+        for (int64_t c = lane * 8; c < a.K; c += 256) {
+            const uint4 xv = load8(x, c, a.K, a.vec);
+            float xf[8], wf[8];
+            unpack8<T>(xv, xf);
+            unpack8<T>(load8(w, c, a.K, true), wf);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) z = fmaf(xf[e], wf[e], z);
+            store8(d, c, a.K, true, xv);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
+        if (lane == 0) a.zt[i] = z;
     }
 }
 
 constexpr int HR_ROWS = 32, HR_GROUPS = 16;
-// loss, and stat = (max, log2 sum, 1 - p_t, live); HR_GROUPS groups of threads share a row's parts.
-__global__ void __launch_bounds__(HR_ROWS* HR_GROUPS) k_head_rows(const float2* __restrict__ part, int parts, int64_t M,
-                                                                  const int32_t* __restrict__ target,
-                                                                  const float* __restrict__ zt, float* __restrict__ losses,
-                                                                  float4* __restrict__ stat) {
+struct HeadRowsArgs {
+    const float2* part;    // [parts][M]; FAST: floats
+    int parts;
+    int64_t M;
+    const int32_t* target;
+    const float* zt;
+    float* losses;
+    float4* stat;
+    const int* only;       // null, or 0: nothing to do
+    int* bad;              // FAST: set where a row's sum is too large
+    float* f;              // the rows' factor of d x, or null; and with it
+    const void* x;         //   [M, K], rows ldc apart
+    void* scaled;          //   f x likewise
+    int64_t K, ldc;
+};
+// loss, and stat = (reference, log2 sum, 1 - p_t, live); HR_GROUPS groups of threads share a row's parts.
+template <typename T, bool FAST>
+__global__ void __launch_bounds__(HR_ROWS* HR_GROUPS) k_head_rows(const HeadRowsArgs a) {
     __shared__ MaxSum red[HR_GROUPS][HR_ROWS];
+    __shared__ float sf[HR_ROWS];
     grid_wait();
     grid_trigger();
+    if (a.only != nullptr && *a.only == 0) return;
     const int x = threadIdx.x % HR_ROWS, y = threadIdx.x / HR_ROWS;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * HR_ROWS + x;
+    const int64_t row0 = static_cast<int64_t>(blockIdx.x) * HR_ROWS, row = row0 + x;
     auto join = [](MaxSum& v, float m, float l) {
         const float t = fmaxf(v.m, m), f = finite_ref(t);
         v.l = v.l * ex2((v.m - f) * LOG2E) + l * ex2((m - f) * LOG2E);
         v.m = t;
     };
     MaxSum v = {-INFINITY, 0.0f};
-    if (row < M) {
+    if (row < a.M) {
+        if constexpr (FAST) {
+            const float* const part = reinterpret_cast<const float*>(a.part) + row;
+#pragma unroll 8
+            for (int p = y; p < a.parts; p += HR_GROUPS) v.l += part[static_cast<int64_t>(p) * a.M];
+        } else {
 #pragma unroll 4
-        for (int p = y; p < parts; p += HR_GROUPS) {
-            const float2 w = part[static_cast<int64_t>(p) * M + row];
-            join(v, w.x, w.y);
+            for (int p = y; p < a.parts; p += HR_GROUPS) {
+                const float2 w = a.part[static_cast<int64_t>(p) * a.M + row];
+                join(v, w.x, w.y);
+            }
         }
     }
     red[y][x] = v;
     __syncthreads();
-    if (y != 0 || row >= M) return;
+    if (y == 0 && row < a.M) {
+        float f = 1.0f;
 #pragma unroll
-    for (int g = 1; g < HR_GROUPS; ++g) join(v, red[g][x].m, red[g][x].l);
-    if (target[row] < 0) {
-        losses[row] = 0.0f;
-        if (stat != nullptr) stat[row] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        return;
+        for (int g = 1; g < HR_GROUPS; ++g) {
+            if constexpr (FAST) v.l += red[g][x].l;
+            else join(v, red[g][x].m, red[g][x].l);
+        }
+        if (a.target[row] < 0) {
+            a.losses[row] = 0.0f;
+            if (a.stat != nullptr) a.stat[row] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        } else if constexpr (FAST) {
+            const float l = 1.0f + v.l;
+            if (!(v.l <= HEAD_FAST_SUM)) *a.bad = 1;
+            f = 1.0f / l;
+            a.losses[row] = log1pf(v.l);
+            a.stat[row] = make_float4(a.zt[row], log2f(l), v.l * f, 1.0f);
+        } else {
+            // the others' sum and the target's term under one maximum
+            const float z = a.zt[row], m = fmaxf(v.m, z);
+            const float others = v.l * ex2((v.m - finite_ref(m)) * LOG2E), mine = ex2((z - m) * LOG2E), l = others + mine;
+            a.losses[row] = (m - z) + (mine == 1.0f ? log1pf(others) : logf(l));
+            if (a.stat != nullptr) a.stat[row] = make_float4(m, log2f(l), others / l, 1.0f);
+        }
+        if (a.f != nullptr) a.f[row] = f;
+        sf[x] = f;
     }
-    // the others' sum and the target's term under one maximum
-    const float z = zt[row], m = fmaxf(v.m, z);
-    const float others = v.l * ex2((v.m - finite_ref(m)) * LOG2E), mine = ex2((z - m) * LOG2E), l = others + mine;
-    losses[row] = (m - z) + (mine == 1.0f ? log1pf(others) : logf(l));
-    if (stat != nullptr) stat[row] = make_float4(m, log2f(l), others / l, 1.0f);
+    if (a.f == nullptr) return;
+    __syncthreads();
+    for (int r = y; r < HR_ROWS && row0 + r < a.M; r += HR_GROUPS) {
+        const T* const src = static_cast<const T*>(a.x) + (row0 + r) * a.ldc;
+        T* const dst = static_cast<T*>(a.scaled) + (row0 + r) * a.ldc;
+        const float f = sf[r];
+        for (int64_t c = x * 8; c < a.K; c += 256) {
+            float e[8];
+            unpack8<T>(load8(src, c, a.K, true), e);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) e[k] *= f;
+            store8(dst, c, a.K, true, pack8<T>(e));
+        }
+    }
 }
 
 // out = the losses' sum (MEAN: over the rows with a target), *factor = 1 or 1 / rows: one block, a fixed order.

@@ -709,7 +709,7 @@ struct CrossEntropyCall {
         losses = at::empty(rows_shape, f32);
         if (reduced) out = at::empty({}, f32);
         if (grads) make_slabs(need_x, need_w);
-        const size_t sb = ravel_linear_ce_scratch_bytes(M, K, V), wb = ravel_linear_ce_work_bytes(M, K, V, grads);
+        const size_t sb = ravel_linear_ce_scratch_bytes(M, K, V), wb = ravel_linear_ce_work_bytes(M, K, V, grads, dtype);
         scratch = bytes(sb, w.t);
         at::Tensor work = bytes(wb, w.t);
         check_status("ravel_linear_ce_fwd",
@@ -760,7 +760,7 @@ struct LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy>
             CrossEntropyCall c(Rows{saved[3], ctx->saved_data["ld"].toInt()}, M, K, V);
             c.make_slabs(need_x, need_w);
             at::Tensor scratch = saved[4];
-            const size_t wb = ravel_linear_ce_work_bytes(M, K, V, 1);
+            const size_t wb = ravel_linear_ce_work_bytes(M, K, V, 1, dtype);
             at::Tensor work = bytes(wb, up);
             check_status("ravel_linear_ce_grad",
                          ravel_linear_ce_grad(c.w.t.data_ptr(), c.w.ld, up.data_ptr<float>(), M, K, V,

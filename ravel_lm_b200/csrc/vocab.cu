@@ -113,6 +113,23 @@ EmbedLayout embed_layout(int64_t N, int64_t V, int64_t K) {
     return l;
 }
 
+// The sums over sorted positions, and their joins.
+template <typename T, bool ADD>
+int launch_sums(EmbedArgs a, bool vec, cudaStream_t st) {
+    a.tx = embed_tx(vec ? a.K * static_cast<int64_t>(sizeof(T)) / 16 : a.K);
+    a.range = embed_range(a.N, a.tx);
+    a.ranges = static_cast<int>((a.N + a.range - 1) / a.range);
+    const int groups = EM_THREADS / a.tx;
+    a.sum_blocks = (a.ranges + groups - 1) / groups;
+    const int64_t zero_blocks = ADD ? 0 : (a.V + EM_ZERO_ROWS - 1) / EM_ZERO_ROWS;
+    const auto kern = vec ? k_embed_sum<T, 16 / sizeof(T), ADD> : k_embed_sum<T, 1, ADD>;
+    if (int e = launch(kern, dim3(static_cast<unsigned>(a.sum_blocks + zero_blocks)), EM_THREADS, 0, st, 1, a)) return e;
+    if (a.ranges < 2) return RAVEL_OK;
+    const int64_t items = static_cast<int64_t>(a.ranges - 1) * ((a.K + EJ_COLS - 1) / EJ_COLS);
+    return launch(k_embed_join<T, ADD>, dim3(static_cast<unsigned>(std::min<int64_t>(items, int64_t{sm_count()} * 8))),
+                  32 * EJ_GROUPS, 0, st, 1, a);
+}
+
 int embed_check(int64_t N, int64_t V, int64_t K, int ids_dtype, int dtype) {
     if (N < 0 || V <= 0 || K < 0 || (ids_dtype != RAVEL_I32 && ids_dtype != RAVEL_I64)) return RAVEL_ERR_INVALID_ARG;
     if (dtype != RAVEL_F32 && dtype != RAVEL_BF16 && dtype != RAVEL_F16) return RAVEL_ERR_UNSUPPORTED;
@@ -128,7 +145,17 @@ struct HeadLayout {
     int64_t ldz, ldc, ldo;
     size_t off_target, off_zt, off_stat, off_up, off_clean, total;  // scratch: what the backward of single losses needs again
     size_t work, work_grads;  // the parts, and d z in their place
+    // the three-product form: d z, the parts, and
+    int pieces;
+    size_t off_part, off_flags, off_f, off_scaled, off_embed;
+    EmbedLayout embed;
 };
+
+// Three products or four, for a bfloat16 training step of a reduced loss: the sort by target, its sums and the launches
+// that wait for a flag take some 35 us, which the spared product has to pass (2 M K V at 1.4 PFLOP/s).
+bool head_fast(int64_t M, int64_t K, int64_t V, int dtype) {
+    return dtype == RAVEL_BF16 && M > 128 && static_cast<double>(M) * K * V >= 3e10;
+}
 
 // Rows of a piece: whole tiles of 256.  d W is read and written once more for every piece after the first, which at 1024
 // rows takes about as long as the piece's products.
@@ -139,8 +166,9 @@ int64_t head_piece(int64_t M, int64_t V) {
     return up_to((M + pieces - 1) / pieces, 256);
 }
 
-HeadLayout head_layout(int64_t M, int64_t K, int64_t V) {
+HeadLayout head_layout(int64_t M, int64_t K, int64_t V, bool fast) {
     HeadLayout l;
+    std::memset(&l, 0, sizeof(l));
     l.piece = head_piece(M, V);
     l.ldz = up_to(V, 8);
     l.ldc = up_to(K, 8);
@@ -148,12 +176,22 @@ HeadLayout head_layout(int64_t M, int64_t K, int64_t V) {
     l.parts = 2 * ((V + 127) / 128);
     l.off_target = 0;
     l.off_zt = up256(static_cast<size_t>(M) * 4);
-    l.off_stat = l.off_zt + up256(static_cast<size_t>(l.piece) * 4);
+    l.off_stat = l.off_zt + up256(static_cast<size_t>(M) * 4);
     l.off_up = l.off_stat + up256(static_cast<size_t>(M) * 16);
     l.off_clean = l.off_up + 256;
     l.total = l.off_clean + up256(static_cast<size_t>(M) * static_cast<size_t>(l.ldc) * 2);
     l.work = static_cast<size_t>(l.parts) * static_cast<size_t>(l.piece) * 8;
     l.work_grads = std::max(l.work, static_cast<size_t>(l.piece) * static_cast<size_t>(l.ldz) * 2);
+    l.pieces = static_cast<int>((M + l.piece - 1) / l.piece);
+    l.off_part = up256(l.work_grads);
+    l.off_flags = l.off_part + up256(l.work);
+    l.off_f = l.off_flags + up256(static_cast<size_t>(l.pieces) * 4);
+    l.off_scaled = l.off_f + up256(static_cast<size_t>(M) * 4);
+    l.off_embed = l.off_scaled + up256(static_cast<size_t>(M) * static_cast<size_t>(l.ldc) * 2);
+    if (fast) {
+        l.embed = embed_layout(M, V, K);
+        l.work_grads = l.off_embed + l.embed.total;
+    }
     return l;
 }
 
@@ -230,8 +268,9 @@ int launch_logits(const HeadOperand& X, const HeadOperand& W, int64_t K, HeadLog
 bool head_pairs(int64_t M) { return M > 128; }
 
 template <typename T, int MODE>
-int head_logits(const HeadOperand& X, const HeadOperand& W, int64_t K, const HeadLogitsArgs& a, cudaStream_t st) {
-    if (head_pairs(a.M)) return launch_logits<T, 2, 256, MODE>(X, W, K, a, st);
+int head_logits(const HeadOperand& X, const HeadOperand& W, int64_t K, bool pairs, const HeadLogitsArgs& a,
+                cudaStream_t st) {
+    if (pairs) return launch_logits<T, 2, 256, MODE>(X, W, K, a, st);
     return launch_logits<T, 1, 128, MODE>(X, W, K, a, st);
 }
 
@@ -260,9 +299,9 @@ HeadPlan plan_grad(int64_t M, int64_t N, int64_t k) {
     return best;
 }
 
-template <typename T, int CG, int BN, bool A_MN>
+template <typename T, int CG, int BN, bool A_MN, bool ROWS>
 int launch_grad(const HeadOperand& A, const HeadOperand& B, int64_t k, HeadGradArgs a, cudaStream_t st) {
-    const auto kern = k_head_grad<T, CG, BN, A_MN>;
+    const auto kern = k_head_grad<T, CG, BN, A_MN, ROWS>;
     head_shape<CG, BN, A_MN>(a, a.M, a.N, k);
     CUtensorMap ma, mb;
     if (int e = head_map<T, A_MN>(&ma, A, a.M, k, a.a_rows)) return e;
@@ -304,22 +343,54 @@ struct HeadCall {
     float *gx, *gw;    // null: not wanted
     char* scratch;
     void* work;
+    bool fast;         // three products
     HeadLayout l;
     DeviceWords words;
     cudaStream_t st;
 };
 
+// d W += the targets' terms: the rows of x times -(1 - p_t), summed by target.
+template <typename T>
+int head_targets(const HeadCall& c, const int32_t* target, const float4* stat, const char* clean, char* work) {
+    char* const e = work + c.l.off_embed;
+    const EmbedLayout& l = c.l.embed;
+    if (cudaMemsetAsync(e + l.off_list, 0, sizeof(int), c.st) != cudaSuccess) return RAVEL_ERR_CUDA;
+    IdsArgs q;
+    std::memset(&q, 0, sizeof(q));
+    q.ids = target;
+    q.N = c.M; q.V = c.V; q.pad = -1;
+    q.err = c.words.error;
+    if (int rc = sort_ids(q, l.ids, e + l.off_ids, c.st)) return rc;
+    EmbedArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.g = clean;
+    a.N = c.M; a.V = c.V; a.K = c.K; a.ldg = c.l.ldc;
+    a.keys = reinterpret_cast<const uint2*>(e + l.off_ids + l.ids.off_keys);
+    a.live = reinterpret_cast<const int*>(e + l.off_ids + l.ids.off_live);
+    a.part = reinterpret_cast<float*>(e + l.off_part);
+    a.K4 = l.K4;
+    a.list = reinterpret_cast<int*>(e + l.off_list);
+    a.weight = stat;
+    a.add = c.gw;
+    a.ldo = c.l.ldo;
+    return launch_sums<T, true>(a, c.K % 8 == 0, c.st);
+}
+
 // Statistics and losses, and the gradients' float32 sums, a piece of the rows at a time.
 template <typename T>
 int head_run(const HeadCall& c, bool stats) {
-    const bool half = std::is_same<T, __half>::value;
+    constexpr bool half = std::is_same<T, __half>::value;
     int32_t* const target = reinterpret_cast<int32_t*>(c.scratch + c.l.off_target);
     float* const zt = reinterpret_cast<float*>(c.scratch + c.l.off_zt);
     float4* const stat = reinterpret_cast<float4*>(c.scratch + c.l.off_stat);
-    float2* const part = static_cast<float2*>(c.work);
     float* const up_max = reinterpret_cast<float*>(c.scratch + c.l.off_up);
     char* const clean = c.scratch + c.l.off_clean;
-    void* const dz = c.work;  // the parts are read before it is written
+    char* const work = static_cast<char*>(c.work);
+    void* const dz = c.work;  // four products: the parts are read before it is written
+    float2* const part = reinterpret_cast<float2*>(c.fast ? work + c.l.off_part : work);
+    int* const flags = reinterpret_cast<int*>(work + c.l.off_flags);
+    float* const f = reinterpret_cast<float*>(work + c.l.off_f);
+    char* const scaled = work + c.l.off_scaled;
     const bool grads = c.gx != nullptr || c.gw != nullptr;
     const HeadOperand W{c.w, c.ldw};
     const HeadSplits sp = head_splits(c.M, c.K, c.V);
@@ -329,31 +400,49 @@ int head_run(const HeadCall& c, bool stats) {
     if (c.M == 0 && c.gw != nullptr &&
         cudaMemsetAsync(c.gw, 0, static_cast<size_t>(sp.w.splits) * c.V * c.l.ldo * sizeof(float), c.st) != cudaSuccess)
         return RAVEL_ERR_CUDA;
-    for (int64_t r0 = 0; r0 < c.M; r0 += c.l.piece) {
+    for (int64_t r0 = 0, piece = 0; r0 < c.M; r0 += c.l.piece, ++piece) {
         const int64_t rows = std::min(c.l.piece, c.M - r0);
         const HeadOperand X{clean + static_cast<size_t>(r0) * c.l.ldc * 2, c.l.ldc};
+        const HeadOperand S{scaled + static_cast<size_t>(r0) * c.l.ldc * 2, c.l.ldc};
+        const bool pairs = c.fast || head_pairs(rows);
+        const int tile = pairs ? 256 : 128;
         HeadLogitsArgs a;
         std::memset(&a, 0, sizeof(a));
         a.M = rows; a.V = static_cast<int>(c.V);
         a.target = target + r0;
-        a.err = c.words.error; a.wait_limit = c.words.wait_limit;
-        if (stats) {
-            a.part = part; a.zt = zt;
-            if (int e = head_logits<T, HEAD_STATS>(X, W, c.K, a, c.st)) return e;
-            const int tile = head_pairs(rows) ? 256 : 128;
-            const int parts = static_cast<int>((c.V + tile - 1) / tile) * 2;
-            if (int e = launch(k_head_rows, dim3(static_cast<unsigned>((rows + HR_ROWS - 1) / HR_ROWS)),
-                               HR_ROWS * HR_GROUPS, 0, c.st, 1, part, parts, rows, target + r0, zt, c.losses + r0,
-                               stat + r0))
-                return e;
-        }
-        if (!grads) continue;
+        a.part = part; a.zt = zt + r0;
         a.stat = stat + r0;
         a.up = c.up != nullptr ? c.up + r0 : nullptr;
         a.up_max = up_max;
         a.unit_log2 = half ? 15.0f : 0.0f;
+        a.apart = c.fast;
         a.dz = dz; a.ldz = c.l.ldz;
-        if (int e = head_logits<T, HEAD_EXP>(X, W, c.K, a, c.st)) return e;
+        a.err = c.words.error; a.wait_limit = c.words.wait_limit;
+        HeadRowsArgs h;
+        std::memset(&h, 0, sizeof(h));
+        h.part = part; h.parts = static_cast<int>((c.V + tile - 1) / tile) * 2;
+        h.M = rows; h.target = a.target; h.zt = a.zt;
+        h.losses = c.losses != nullptr ? c.losses + r0 : nullptr; h.stat = stat + r0;
+        if (c.fast) {
+            h.f = f + r0;
+            h.x = X.p; h.scaled = scaled + static_cast<size_t>(r0) * c.l.ldc * 2;
+            h.K = c.K; h.ldc = c.l.ldc;
+        }
+        const dim3 row_blocks(static_cast<unsigned>((rows + HR_ROWS - 1) / HR_ROWS));
+        if constexpr (!half) {
+            if (c.fast) {
+                if (int e = head_logits<T, HEAD_FAST>(X, W, c.K, true, a, c.st)) return e;
+                h.bad = flags + piece;
+                if (int e = launch(k_head_rows<T, true>, row_blocks, HR_ROWS * HR_GROUPS, 0, c.st, 1, h)) return e;
+                a.only = h.only = flags + piece;  // what follows is for a piece that needs it
+            }
+        }
+        if (stats) {
+            if (int e = head_logits<T, HEAD_STATS>(X, W, c.K, pairs, a, c.st)) return e;
+            if (int e = launch(k_head_rows<T, false>, row_blocks, HR_ROWS * HR_GROUPS, 0, c.st, 1, h)) return e;
+        }
+        if (!grads) continue;
+        if (int e = head_logits<T, HEAD_EXP>(X, W, c.K, pairs, a, c.st)) return e;
         const HeadOperand Z{dz, c.l.ldz};
         HeadGradArgs g;
         std::memset(&g, 0, sizeof(g));
@@ -362,17 +451,30 @@ int head_run(const HeadCall& c, bool stats) {
         if (c.gx != nullptr) {
             g.M = rows; g.splits = sp.x.splits;
             g.out = c.gx + r0 * c.l.ldo; g.slab = c.M * c.l.ldo; g.add = 0;
-            if (int e = sp.x.cg == 2 ? launch_grad<T, 2, 256, false>(Z, W, c.V, g, c.st)
-                                     : launch_grad<T, 1, 128, false>(Z, W, c.V, g, c.st))
-                return e;
+            g.f = f + r0; g.stat = stat + r0; g.target = a.target;
+            g.w = c.w; g.ldw = c.ldw;
+            int e = RAVEL_OK;
+            if (c.fast) {
+                if constexpr (!half)
+                    e = sp.x.cg == 2 ? launch_grad<T, 2, 256, false, true>(Z, W, c.V, g, c.st)
+                                     : launch_grad<T, 1, 128, false, true>(Z, W, c.V, g, c.st);
+            } else {
+                e = sp.x.cg == 2 ? launch_grad<T, 2, 256, false, false>(Z, W, c.V, g, c.st)
+                                 : launch_grad<T, 1, 128, false, false>(Z, W, c.V, g, c.st);
+            }
+            if (e) return e;
         }
         if (c.gw != nullptr) {
             g.M = c.V; g.splits = sp.w.splits;
             g.out = c.gw; g.slab = c.V * c.l.ldo; g.add = r0 > 0;
-            if (int e = sp.w.cg == 2 ? launch_grad<T, 2, 256, true>(Z, X, rows, g, c.st)
-                                     : launch_grad<T, 1, 128, true>(Z, X, rows, g, c.st))
+            const HeadOperand& B = c.fast ? S : X;
+            if (int e = sp.w.cg == 2 ? launch_grad<T, 2, 256, true, false>(Z, B, rows, g, c.st)
+                                     : launch_grad<T, 1, 128, true, false>(Z, B, rows, g, c.st))
                 return e;
         }
+    }
+    if constexpr (!half) {
+        if (c.fast && c.gw != nullptr) return head_targets<T>(c, target, stat, clean, work);
     }
     return RAVEL_OK;
 }
@@ -453,31 +555,20 @@ int ravel_embedding_bwd(const void* ids, int ids_dtype, const void* grad_y, int6
     a.K4 = l.K4;
     a.list = reinterpret_cast<int*>(s + l.off_list);
     const bool vec = (K * es) % 16 == 0 && aligned16(grad_y) && (N == 1 || ldg * es % 16 == 0) && aligned16(grad_weight);
-    a.tx = embed_tx(vec ? K * es / 16 : K);
-    a.range = embed_range(N, a.tx);
-    a.ranges = static_cast<int>((N + a.range - 1) / a.range);
-    const int groups = EM_THREADS / a.tx;
-    a.sum_blocks = (a.ranges + groups - 1) / groups;
-    const int64_t zero_blocks = (V + EM_ZERO_ROWS - 1) / EM_ZERO_ROWS;
     return with_float_type(dtype, [&](auto tv) -> int {
         using T = decltype(tv);
-        const auto kern = vec ? k_embed_sum<T, 16 / sizeof(T)> : k_embed_sum<T, 1>;
-        if (int e = launch(kern, dim3(static_cast<unsigned>(a.sum_blocks + zero_blocks)), EM_THREADS, 0, st, 1, a)) return e;
-        if (a.ranges < 2) return RAVEL_OK;
-        const int64_t items = static_cast<int64_t>(a.ranges - 1) * ((K + EJ_COLS - 1) / EJ_COLS);
-        return launch(k_embed_join<T>, dim3(static_cast<unsigned>(std::min<int64_t>(items, int64_t{sm_count()} * 8))),
-                      32 * EJ_GROUPS, 0, st, 1, a);
+        return launch_sums<T, false>(a, vec, st);
     });
 }
 
 size_t ravel_linear_ce_scratch_bytes(int64_t M, int64_t K, int64_t V) {
     if (head_check(M, K, V, RAVEL_I64, RAVEL_BF16) != RAVEL_OK) return 0;
-    return head_layout(M, K, V).total;
+    return head_layout(M, K, V, false).total;
 }
 
-size_t ravel_linear_ce_work_bytes(int64_t M, int64_t K, int64_t V, int grads) {
-    if (head_check(M, K, V, RAVEL_I64, RAVEL_BF16) != RAVEL_OK) return 0;
-    const HeadLayout l = head_layout(M, K, V);
+size_t ravel_linear_ce_work_bytes(int64_t M, int64_t K, int64_t V, int grads, int dtype) {
+    if (head_check(M, K, V, RAVEL_I64, dtype) != RAVEL_OK) return 0;
+    const HeadLayout l = head_layout(M, K, V, head_fast(M, K, V, dtype));
     return grads ? l.work_grads : l.work;
 }
 
@@ -504,7 +595,8 @@ int ravel_linear_ce_fwd(const void* x, int64_t ldx, const void* weight, int64_t 
         !aligned16(weight) || ldw % 8 != 0 || !aligned16(slabs_x) || !aligned16(slabs_w))
         return RAVEL_ERR_INVALID_ARG;
     HeadCall c;
-    c.l = head_layout(M, K, V);
+    c.fast = grads && head_fast(M, K, V, dtype);
+    c.l = head_layout(M, K, V, c.fast);
     if (scratch == nullptr || scratch_bytes < c.l.total || work == nullptr ||
         work_bytes < (grads ? c.l.work_grads : c.l.work) || !aligned16(scratch) || !aligned16(work))
         return RAVEL_ERR_WORKSPACE;
@@ -526,6 +618,12 @@ int ravel_linear_ce_fwd(const void* x, int64_t ldx, const void* weight, int64_t 
             p.x = x; p.clean = c.scratch + c.l.off_clean;
             p.K = K; p.ldx = ldx; p.ldc = c.l.ldc;
             p.vec = aligned16(x) && (M == 1 || ldx % 8 == 0);
+            p.w = weight; p.ldw = ldw;
+            if (c.fast) {
+                p.zt = reinterpret_cast<float*>(c.scratch + c.l.off_zt);
+                p.flags = reinterpret_cast<int*>(static_cast<char*>(work) + c.l.off_flags);
+                p.pieces = c.l.pieces;
+            }
             p.err = c.words.error;
             const dim3 grid(static_cast<unsigned>(std::min<int64_t>((M + 7) / 8, int64_t{sm_count()} * 32)));
             if (int e = launch(k_head_prep<T>, grid, 256, 0, c.st, 1, p)) return e;
@@ -546,7 +644,8 @@ int ravel_linear_ce_grad(const void* weight, int64_t ldw, const float* up, int64
         (M > 0 && up == nullptr) || !aligned16(slabs_x) || !aligned16(slabs_w))
         return RAVEL_ERR_INVALID_ARG;
     HeadCall c;
-    c.l = head_layout(M, K, V);
+    c.fast = false;
+    c.l = head_layout(M, K, V, false);
     if (scratch == nullptr || scratch_bytes < c.l.total || work == nullptr || work_bytes < c.l.work_grads ||
         !aligned16(scratch) || !aligned16(work))
         return RAVEL_ERR_WORKSPACE;
