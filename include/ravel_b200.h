@@ -465,7 +465,7 @@ int ravel_embedding_bwd(const void* ids, int ids_dtype, const void* grad_y, int6
  * sizes[1] slabs of V rows, rows sizes[2] floats apart (ravel_linear_ce_slabs);
  * factor (one float) goes with them.  ravel_linear_ce_bwd adds the slabs up, scales
  * them by *up (device) and rounds: grad_x [M, K], grad_w [V, K], contiguous.
- * Single rows' losses (RAVEL_REDUCE_NONE) get their gradients from
+ * Single rows' losses (RAVEL_REDUCE_NONE, keep set in the forward) get their gradients from
  * ravel_linear_ce_grad, given the forward's scratch and up [M]; then ravel_linear_ce_bwd
  * with up NULL.  work is needed during a call only.
  */
@@ -473,7 +473,7 @@ size_t ravel_linear_ce_scratch_bytes(int64_t M, int64_t K, int64_t V);
 size_t ravel_linear_ce_work_bytes(int64_t M, int64_t K, int64_t V, int grads, int dtype);
 int ravel_linear_ce_slabs(int64_t M, int64_t K, int64_t V, int64_t* sizes);
 int ravel_linear_ce_fwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* targets,
-                        int target_dtype, int64_t M, int64_t K, int64_t V, int64_t ignore_index, int reduction,
+                        int target_dtype, int64_t M, int64_t K, int64_t V, int64_t ignore_index, int reduction, int keep,
                         float* losses, float* out, float* factor, float* slabs_x, float* slabs_w, int dtype,
                         void* scratch, size_t scratch_bytes, void* work, size_t work_bytes, void* stream);
 int ravel_linear_ce_grad(const void* weight, int64_t ldw, const float* up, int64_t M, int64_t K, int64_t V, float* factor,
@@ -514,15 +514,16 @@ int ravel_grad_norm(const ravel_adamw_tensor* tensors, int64_t count, int dtype,
 /*
  * One AdamW step (decoupled weight decay; the reference's optimizer is FlatAdamW,
  * ravel_lm/runtime.py:44): *step (device) counts up by one, then for every element in float32
- *   g' = g min(1, max_norm / (*norm + 1e-6))   (norm, from ravel_grad_norm, NULL: g)
+ *   g' = g min(1, max_norm / (norm + 1e-6))    (max_norm 0: g)
  *   m = beta1 m + (1 - beta1) g',  v = beta2 v + (1 - beta2) g'^2
  *   p = p (1 - lr wd) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
- * lr_device (one float32 on the device) is taken in place of lr where given.
+ * norm: *norm where given (ravel_grad_norm's, over this list and others), else over
+ * this list.  lr_device (one float32 on the device) is taken in place of lr where given.
  * norm_out (NULL: not wanted) receives the norm in float32.  8-bit states are
  * rounded stochastically by a hash of the step, the tensor's place in the list and
  * the element: the same call gives the same bits.  No tensor may appear twice.
  */
-size_t ravel_adamw_scratch_bytes(void);
+size_t ravel_adamw_scratch_bytes(const ravel_adamw_tensor* tensors, int64_t count, double max_norm);
 int ravel_adamw(const ravel_adamw_tensor* tensors, int64_t count, int dtype, int state_bits, int64_t* step, double lr,
                 const float* lr_device, double beta1, double beta2, double eps, double weight_decay, double max_norm,
                 const double* norm, float* norm_out, void* scratch, size_t scratch_bytes, void* stream);

@@ -105,14 +105,14 @@ SIGNATURES = {
     "ravel_linear_ce_scratch_bytes": (_c_sz, [_c_i64] * 3),
     "ravel_linear_ce_work_bytes": (_c_sz, [_c_i64] * 3 + [_c_int, _c_int]),
     "ravel_linear_ce_slabs": (_c_int, [_c_i64] * 3 + [ctypes.POINTER(_c_i64)]),
-    "ravel_linear_ce_fwd": (_c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_int] + [_c_i64] * 4 + [_c_int] + [_c_vp] * 5 +
+    "ravel_linear_ce_fwd": (_c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_int] + [_c_i64] * 4 + [_c_int, _c_int] + [_c_vp] * 5 +
                             [_c_int, _c_vp, _c_sz, _c_vp, _c_sz, _c_vp]),
     "ravel_linear_ce_grad": (_c_int, [_c_vp, _c_i64, _c_vp] + [_c_i64] * 3 + [_c_vp] * 3 +
                              [_c_int, _c_vp, _c_sz, _c_vp, _c_sz, _c_vp]),
     "ravel_linear_ce_bwd": (_c_int, [_c_vp] * 4 + [_c_i64] * 3 + [_c_vp, _c_vp, _c_int, _c_vp]),
     "ravel_grad_norm_scratch_bytes": (_c_sz, [ctypes.POINTER(AdamTensor), _c_i64]),
     "ravel_grad_norm": (_c_int, [ctypes.POINTER(AdamTensor), _c_i64, _c_int, _c_vp, _c_vp, _c_sz, _c_vp]),
-    "ravel_adamw_scratch_bytes": (_c_sz, []),
+    "ravel_adamw_scratch_bytes": (_c_sz, [ctypes.POINTER(AdamTensor), _c_i64, ctypes.c_double]),
     "ravel_adamw": (_c_int, [ctypes.POINTER(AdamTensor), _c_i64, _c_int, _c_int, _c_vp, ctypes.c_double, _c_vp] +
                     [ctypes.c_double] * 5 + [_c_vp, _c_vp, _c_vp, _c_sz, _c_vp]),
     "ravel_state_values": (_c_int, [_c_vp, _c_vp, _c_i64, _c_int, _c_vp, _c_int, _c_vp]),

@@ -9,8 +9,8 @@
 // the reciprocal are the hardware's approximations (2^-22 of a step that is a small part of p).
 //
 //   k_grad_norm      sums of squares in float64, a part per block (any float32 gradient's square is finite there, and the
-//                    sum is the same to float32 whatever its order).
-//   k_adamw_scalars  the next step number and what every element needs of it and of the norm; the step lives on the
+//                    sum is the same to float32 whatever its order); k_norm_total adds the parts for callers of the norm.
+//   k_adamw_scalars  the norm, the next step number and what every element needs of them; the step lives on the
 //                    device, so that a captured step counts on when it is replayed.
 //   k_adamw          a warp per block of 256 elements of a tensor.
 //
@@ -233,44 +233,52 @@ __global__ void __launch_bounds__(32 * AW_WARPS) k_grad_norm(const __grid_consta
     }
 }
 
-// norm = sqrt(sum of the parts), in float64 and float32.
-__global__ void __launch_bounds__(1024) k_norm_total(const double* __restrict__ part, int parts, double* norm) {
+// The norm from its parts, by a block of 1024; thread 0 has it.
+__device__ __forceinline__ double norm_of(const double* part, int parts) {
     __shared__ double red[32];
-    grid_wait();
-    grid_trigger();
     double s = 0.0;
+#pragma unroll 4
     for (int i = threadIdx.x; i < parts; i += 1024) s += part[i];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0)
         for (int w = 1; w < 32; ++w) s += red[w];
-        *norm = sqrt(s);
-    }
+    return sqrt(s);
+}
+__global__ void __launch_bounds__(1024) k_norm_total(const double* __restrict__ part, int parts, double* norm) {
+    grid_wait();
+    grid_trigger();
+    const double n = norm_of(part, parts);
+    if (threadIdx.x == 0) *norm = n;
 }
 
 struct AdamStep {
     int64_t* step;
     const float* lr_dev;  // the learning rate on the device, or null
-    double lr, b1, b2, wd, max_norm;
-    const double* norm;   // null: no clipping
+    double lr, b1, b2, wd, max_norm;  // max_norm 0: no clipping
+    const double* norm;   // the norm, or null: from its parts
+    const double* part;
+    int parts;
     float* norm32;        // the norm in float32, or null
     AdamScalars* s;
 };
-__global__ void k_adamw_scalars(const AdamStep a) {
+__global__ void __launch_bounds__(1024) k_adamw_scalars(const AdamStep a) {
     grid_wait();
     grid_trigger();
+    double norm = 0.0;
+    if (a.max_norm > 0.0) norm = a.norm != nullptr ? *a.norm : norm_of(a.part, a.parts);
     if (threadIdx.x != 0) return;
     const int64_t t = *a.step + 1;
     *a.step = t;
     const double lr = a.lr_dev != nullptr ? static_cast<double>(*a.lr_dev) : a.lr, n = static_cast<double>(t);
     AdamScalars s;
     s.clip = 1.0f;
-    if (a.norm != nullptr) {
-        const double c = a.max_norm / (*a.norm + 1e-6);
+    if (a.max_norm > 0.0) {
+        const double c = a.max_norm / (norm + 1e-6);
         s.clip = c >= 1.0 ? 1.0f : static_cast<float>(c);  // a NaN stays one
-        if (a.norm32 != nullptr) *a.norm32 = static_cast<float>(*a.norm);
+        if (a.norm32 != nullptr) *a.norm32 = static_cast<float>(norm);
     }
     s.decay = static_cast<float>(1.0 - lr * a.wd);
     s.c1 = static_cast<float>(lr / (1.0 - pow(a.b1, n)));

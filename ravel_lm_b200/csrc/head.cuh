@@ -9,9 +9,9 @@
 //
 //   k_head_prep    targets as int32 (-1: none), x with the rows that have none zeroed, and (fast) the targets' logits.
 //   k_head_logits  the logits' product, on the pairs and single CTAs of k_matmul.  The logits never leave the SM:
-//     HEAD_STATS   a thread owns a row of the tile and keeps the maximum and the sum of 2^((z - max) log2 e) over its
-//                  columns, the target's column apart (so that a confident row's 1 - p_t is no difference), a
-//                  part per row and half tile in memory; the target's logit is kept.
+//     HEAD_STATS   a thread owns a row of the tile and keeps the maximum and the sum of exp(z - max) over its
+//                  columns, the target's column apart (so that a confident row's 1 - p_t is no difference), a few
+//                  parts per row and tile in memory; the target's logit is kept.
 //     HEAD_EXP     with the row's maximum and sum known: d z in 16 bits (the tensor cores' operand), for a piece
 //                  of the rows.
 //     HEAD_FAST    both in one product: E = exp(z - z_t) in 16 bits and its sums.
@@ -44,15 +44,34 @@ constexpr float LOG2E = 1.4426950408889634f;
 enum HeadMode { HEAD_STATS = 0, HEAD_EXP = 1, HEAD_FAST = 2 };
 constexpr float HEAD_FAST_SUM = 1.2089258196146292e24f;  // 2^80
 
+// The rows' targets: as k_head_prep leaves them (int32, -1: none), or as the caller gave them, where x needs no copy.
+struct HeadTargets {
+    const void* p;
+    int kind;                  // 0: prepared; 1, 2: int32, int64 as given
+    int V;
+    int64_t ignore;
+    __device__ __forceinline__ int at(int64_t row) const {
+        if (kind == 0) return static_cast<const int32_t*>(p)[row];
+        const int64_t t = kind == 2 ? static_cast<const int64_t*>(p)[row] : static_cast<const int32_t*>(p)[row];
+        return t >= 0 && t < V && t != ignore ? static_cast<int>(t) : -1;
+    }
+    // a target outside the vocabulary that is not the ignored index
+    __device__ __forceinline__ bool bad(int64_t row) const {
+        if (kind == 0) return false;
+        const int64_t t = kind == 2 ? static_cast<const int64_t*>(p)[row] : static_cast<const int32_t*>(p)[row];
+        return (t < 0 || t >= V) && t != ignore;
+    }
+};
+
 struct HeadLogitsArgs : MmShape {
     int64_t M;                 // rows of the piece
     int V;
-    const int32_t* target;     // [M], -1: none
-    float2* part;              // STATS: [2 ntiles][M]; FAST: as many floats
+    HeadTargets target;        // [M]
+    float2* part;              // STATS: [head_parts ntiles][M]; FAST: as many floats
     float* zt;                 // [M] the target's logit, from STATS or for FAST
     const int* only;           // null, or 0: nothing to do
     int apart;                 // EXP: the target's term is left out
-    const float4* stat;        // EXP: [M] (max, log2 sum, 1 - p_t, live)
+    const float4* stat;        // EXP: [M] (reference in base 2, log2 sum, 1 - p_t, live)
     const float* up;           // EXP: a row's upstream gradient, or null
     const float* up_max;       //   and the largest of them
     float unit_log2;           // EXP: log2 of what d z is kept times
@@ -86,7 +105,7 @@ struct MmCta {
     int warp, lane;
 };
 // Barriers, tensor memory and (pairs) the other CTA; returns with the previous kernel's writes visible.
-template <int CG, uint32_t COLS>
+template <int CG, uint32_t COLS, int EPI>
 __device__ __forceinline__ MmCta mm_begin(unsigned char* smem_raw, int stages, const CUtensorMap* map_a,
                                           const CUtensorMap* map_b, const unsigned int* wait_limit) {
     MmCta c;
@@ -107,7 +126,7 @@ __device__ __forceinline__ MmCta mm_begin(unsigned char* smem_raw, int stages, c
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(bar_tfull + 8 * b, 1);
-            mbar_init(bar_tempty + 8 * b, CG * MM_EPI_WARPS);
+            mbar_init(bar_tempty + 8 * b, CG * EPI);
         }
         *c.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -141,19 +160,31 @@ __device__ __forceinline__ void mm_end(const MmCta& c, unsigned int* err) {
 
 // ------------------------------------------------------------------ the logits
 // T: element type.  CG, BN as k_matmul's: CTAs per product and a tile's columns.
+//
+// The epilogue's exponentials (one an element) take 1.1 us of the special-function units for a CTA's 128 x 256, its other
+// instructions less: with 8 warps, two a scheduler, each waited for its own chain of tensor-memory load, exponentials,
+// sum and store, 5 to 6.6 us a tile, more than the tile's products at k = 1024 (4.5).  16 warps take it: warp w the rows
+// 32 (w % 4) .. and every fourth 32-column unit.  Exponents are one fused multiply-add, z log2 e - c; c is
+// rounded once a row and is itself the reference that is kept.
+constexpr int HEAD_EPI_WARPS = 16;
+constexpr int HEAD_THREADS = 128 + 32 * HEAD_EPI_WARPS;
+constexpr uint32_t HEAD_EPI_BYTES = 2048;  // per epilogue warp: 32 rows x 32 columns
+static_assert(HEAD_EPI_WARPS * HEAD_EPI_BYTES <= MM_EPI_WARPS * MM_EPI_BYTES, "staging");
+__host__ __device__ constexpr int head_parts(int bn) { return bn >= 128 ? 4 : bn / 32; }  // of a row and tile
+
 template <typename T, int CG, int BN, int MODE>
-__global__ void __launch_bounds__(MM_THREADS, 1)
+__global__ void __launch_bounds__(HEAD_THREADS, 1)
     k_head_logits(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                   const __grid_constant__ HeadLogitsArgs a) {
     constexpr uint32_t COLS = 2 * BN;
-    constexpr int UNITS = BN / 64;  // 32-column units of an epilogue warp
+    constexpr int PARTS = head_parts(BN);
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     extern __shared__ unsigned char smem_raw[];
     if (a.only != nullptr) {  // the same for every CTA
         grid_wait();
         if (*a.only == 0) return;
     }
-    const MmCta c = mm_begin<CG, COLS>(smem_raw, a.stages, &map_a, &map_b, a.wait_limit);
+    const MmCta c = mm_begin<CG, COLS, HEAD_EPI_WARPS>(smem_raw, a.stages, &map_a, &map_b, a.wait_limit);
     const int tiles = a.mtiles * a.ntiles;
     const int t0 = static_cast<int>(blockIdx.x) / CG, tstep = static_cast<int>(gridDim.x) / CG;
     const auto unit = [&](int j, int& mt, int& nt, int& c0, int& c1) {
@@ -169,89 +200,80 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
     } else if (c.warp == 1 && (CG == 1 || c.rank == 0) && elect_one()) {
         mm_issue<CG, BN, false, false, 2, BF16>(a, c.base, c.sbar, c.tmem, c.limit, c.abort, unit);
     } else if (c.warp >= 4) {
-        const int q = c.warp & 3, half = (c.warp - 4) >> 2, lane = c.lane;
-        unsigned char* const st = c.gen + MM_RING + (c.warp - 4) * MM_EPI_BYTES;
+        const int q = c.warp & 3, h = (c.warp - 4) >> 2, lane = c.lane;
+        unsigned char* const st = c.gen + MM_RING + (c.warp - 4) * HEAD_EPI_BYTES;
         const uint32_t bar_tfull = c.sbar + 16 * MM_MAX_STAGES, bar_tempty = bar_tfull + 16;
         const uint32_t done_bar = map_to_rank(bar_tempty, 0u);
         int mt, nt, k0, k1;
         for (uint32_t j = 0; unit(static_cast<int>(j), mt, nt, k0, k1); ++j) {
             const uint32_t buf = j % 2;
             const int64_t m0 = static_cast<int64_t>(mt) * (MM_BM * CG) + c.rank * MM_BM + q * 32, row = m0 + lane;
-            const int n0 = nt * BN + half * UNITS * 32;
-            const bool rows = m0 < a.M;  // the same for the whole warp
+            const bool rows = m0 < a.M && h < PARTS;  // the same for the whole warp
             int t = -1;
-            MaxSum v = {-INFINITY, 0.0f};
-            float zt = 0.0f;
-            // EXP: d z = +- 2^((z - max) log2 e + e0), the target's column, and which bits of a packed pair live
-            float top = 0.0f, e0 = 0.0f, tv = 0.0f;
+            MaxSum v = {-INFINITY, 0.0f};  // in base 2: the reference c, the sum of 2^(z log2 e - c)
+            // EXP, FAST: E = 2^(z log2 e - ref), the target's column; EXP: and which bits of a packed pair live
+            float ref = INFINITY, tv = 0.0f;
             uint32_t keep = 0u, sign = 0u;
             if (row < a.M) {
-                t = a.target[row];
+                t = a.target.at(row);
                 if constexpr (MODE == HEAD_FAST) {
-                    top = a.zt[row];
-                    keep = t >= 0 ? 0xffffffffu : 0u;
+                    if (t >= 0) ref = a.zt[row] * LOG2E;
                 }
                 if constexpr (MODE == HEAD_EXP) {
                     const float4 s = a.stat[row];
                     float u = 1.0f;
                     if (a.up != nullptr) u = a.up[row] / *a.up_max;
-                    const bool live = s.w != 0.0f && u != 0.0f;
-                    top = s.x;
-                    e0 = a.unit_log2 - s.y + log2f(fabsf(u));
+                    ref = s.x - (a.unit_log2 - s.y + log2f(fabsf(u)));
                     tv = a.apart ? 0.0f : -s.z * ex2(a.unit_log2) * fabsf(u);
-                    keep = live ? 0xffffffffu : 0u;
+                    keep = s.w != 0.0f && u != 0.0f ? 0xffffffffu : 0u;
                     sign = u < 0.0f ? 0x80008000u : 0u;
                 }
             }
             const bool ok = __all_sync(0xffffffffu, mm_wait(bar_tfull + 8 * buf, (j / 2) & 1, c.limit, c.abort));
             tc_fence_after();
             if (!ok) break;
-            const uint32_t tm = c.tmem + buf * BN + (static_cast<uint32_t>(q * 32) << 16) + half * UNITS * 32;
+            const uint32_t tm = c.tmem + buf * BN + (static_cast<uint32_t>(q * 32) << 16);
 #pragma unroll 1
-            for (int u = 0; u < UNITS; ++u) {
-                const int col = n0 + u * 32;
+            for (int u = h; u < BN / 32; u += 4) {
+                const int col = nt * BN + u * 32;
+                if (!rows || col >= a.V) continue;
                 uint32_t r[32];
                 tmem_ld32(tm + u * 32, r);
-                if (u == UNITS - 1) {  // this warp has read its part of the accumulator
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(done_bar + 8 * buf);
-                }
-                if (!rows || col >= a.V) continue;
                 float x[32];
 #pragma unroll
                 for (int e = 0; e < 32; ++e) x[e] = __uint_as_float(r[e]);
-                const bool here = __any_sync(0xffffffffu, t >= col && t < col + 32);
+                const bool here = __any_sync(0xffffffffu, static_cast<unsigned>(t - col) < 32u);
+                const bool tail = col + 32 > a.V;
                 if constexpr (MODE == HEAD_STATS) {
                     if (here) {
+                        float zt = 0.0f;
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
                             if (col + e == t) {
                                 zt = x[e];
                                 x[e] = -INFINITY;
                             }
+                        if (static_cast<unsigned>(t - col) < 32u) a.zt[row] = zt;
                     }
-                    if (col + 32 > a.V) {
+                    if (tail) {
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
                             if (col + e >= a.V) x[e] = -INFINITY;
                     }
-                    if (here && t >= col && t < col + 32) a.zt[row] = zt;
-                    float m = -INFINITY;
+                    float m = x[0];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) m = fmaxf(m, x[e]);
+                    for (int e = 1; e < 32; ++e) m = fmaxf(m, x[e]);
+                    m *= LOG2E;
                     if (m > v.m) {
-                        v.l *= ex2((v.m - m) * LOG2E);
+                        v.l *= ex2(v.m - m);
                         v.m = m;
                     }
-                    sub_scale<32>(x, finite_ref(v.m), LOG2E);
-                    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    scale_sub<32>(x, LOG2E, finite_ref(v.m));
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) s[e & 3] += ex2(x[e]);
-                    v.l += (s[0] + s[1]) + (s[2] + s[3]);
+                    for (int e = 0; e < 32; ++e) x[e] = ex2(x[e]);
+                    v.l += sum_of<32>(x);
                 } else {
-                    if constexpr (MODE == HEAD_FAST) sub_scale<32>(x, top, LOG2E);
-                    else sub_fma<32>(x, top, LOG2E, e0);
+                    scale_sub<32>(x, LOG2E, ref);
 #pragma unroll
                     for (int e = 0; e < 32; ++e) x[e] = ex2(x[e]);
                     if (here) {
@@ -260,23 +282,22 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
                             if (col + e == t) x[e] = tv;
                     }
                     if constexpr (MODE == HEAD_FAST) {
-                        if (col + 32 > a.V) {
+                        if (tail) {
 #pragma unroll
                             for (int e = 0; e < 32; ++e)
                                 if (col + e >= a.V) x[e] = 0.0f;
                         }
-                        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) s[e & 3] += x[e];
-                        v.l += (s[0] + s[1]) + (s[2] + s[3]);
+                        v.l += sum_of<32>(x);
                     }
 #pragma unroll
                     for (int p = 0; p < 4; ++p) {
                         uint4 w;
                         uint32_t* const wp = reinterpret_cast<uint32_t*>(&w);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            wp[e] = (pack2<T>(x[p * 8 + 2 * e], x[p * 8 + 2 * e + 1]) ^ sign) & keep;
+                        for (int e = 0; e < 4; ++e) {
+                            wp[e] = pack2<T>(x[p * 8 + 2 * e], x[p * 8 + 2 * e + 1]);
+                            if constexpr (MODE == HEAD_EXP) wp[e] = (wp[e] ^ sign) & keep;
+                        }
                         *reinterpret_cast<uint4*>(st + epi_piece(lane, p)) = w;
                     }
                     __syncwarp();
@@ -284,11 +305,14 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
                     __syncwarp();
                 }
             }
-            if constexpr (MODE == HEAD_STATS) {
-                if (row < a.M) a.part[static_cast<int64_t>(nt * 2 + half) * a.M + row] = make_float2(v.m, v.l);
-            }
-            if constexpr (MODE == HEAD_FAST) {
-                if (row < a.M) reinterpret_cast<float*>(a.part)[static_cast<int64_t>(nt * 2 + half) * a.M + row] = v.l;
+            // this warp has read its part of the accumulator
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(done_bar + 8 * buf);
+            if (MODE != HEAD_EXP && row < a.M && h < PARTS) {
+                const int64_t at = static_cast<int64_t>(nt * PARTS + h) * a.M + row;
+                if constexpr (MODE == HEAD_STATS) a.part[at] = make_float2(v.m, v.l);
+                else reinterpret_cast<float*>(a.part)[at] = v.l;
             }
         }
     }
@@ -306,7 +330,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1)
     constexpr bool BF16 = std::is_same<T, __nv_bfloat16>::value;
     static_assert(BN / CG % 64 == 0, "MN-major tiles come in blocks of 64");
     extern __shared__ unsigned char smem_raw[];
-    const MmCta c = mm_begin<CG, COLS>(smem_raw, a.stages, &map_a, &map_b, a.wait_limit);
+    const MmCta c = mm_begin<CG, COLS, MM_EPI_WARPS>(smem_raw, a.stages, &map_a, &map_b, a.wait_limit);
     const int units = a.mtiles * a.ntiles * a.splits;
     const int t0 = static_cast<int>(blockIdx.x) / CG, tstep = static_cast<int>(gridDim.x) / CG;
     int split = 0;
@@ -470,15 +494,16 @@ __global__ void __launch_bounds__(256) k_head_prep(const HeadPrepArgs a) {
     }
 }
 
-constexpr int HR_ROWS = 32, HR_GROUPS = 16;
+constexpr int HR_THREADS = 512;
 struct HeadRowsArgs {
     const float2* part;    // [parts][M]; FAST: floats
     int parts;
     int64_t M;
-    const int32_t* target;
+    HeadTargets target;
     const float* zt;
     float* losses;
     float4* stat;
+    unsigned int* err;
     const int* only;       // null, or 0: nothing to do
     int* bad;              // FAST: set where a row's sum is too large
     float* f;              // the rows' factor of d x, or null; and with it
@@ -486,9 +511,12 @@ struct HeadRowsArgs {
     void* scaled;          //   f x likewise
     int64_t K, ldc;
 };
-// loss, and stat = (reference, log2 sum, 1 - p_t, live); HR_GROUPS groups of threads share a row's parts.
-template <typename T, bool FAST>
-__global__ void __launch_bounds__(HR_ROWS* HR_GROUPS) k_head_rows(const HeadRowsArgs a) {
+// loss, and stat = (reference in base 2, log2 sum, 1 - p_t, live).  HR_ROWS rows a block, whose other threads share a
+// row's parts: 32 rows, so that 128 bytes of a part are read together, or 8 where there are few (24 rows of 1000
+// parts: 9.7 us with 32).
+template <typename T, bool FAST, int HR_ROWS>
+__global__ void __launch_bounds__(HR_THREADS) k_head_rows(const HeadRowsArgs a) {
+    constexpr int HR_GROUPS = HR_THREADS / HR_ROWS;
     __shared__ MaxSum red[HR_GROUPS][HR_ROWS];
     __shared__ float sf[HR_ROWS];
     grid_wait();
@@ -498,10 +526,10 @@ __global__ void __launch_bounds__(HR_ROWS* HR_GROUPS) k_head_rows(const HeadRows
     const int64_t row0 = static_cast<int64_t>(blockIdx.x) * HR_ROWS, row = row0 + x;
     auto join = [](MaxSum& v, float m, float l) {
         const float t = fmaxf(v.m, m), f = finite_ref(t);
-        v.l = v.l * ex2((v.m - f) * LOG2E) + l * ex2((m - f) * LOG2E);
+        v.l = v.l * ex2(v.m - f) + l * ex2(m - f);
         v.m = t;
     };
-    MaxSum v = {-INFINITY, 0.0f};
+    MaxSum v = {-INFINITY, 0.0f};  // base 2
     if (row < a.M) {
         if constexpr (FAST) {
             const float* const part = reinterpret_cast<const float*>(a.part) + row;
@@ -519,25 +547,27 @@ __global__ void __launch_bounds__(HR_ROWS* HR_GROUPS) k_head_rows(const HeadRows
     __syncthreads();
     if (y == 0 && row < a.M) {
         float f = 1.0f;
-#pragma unroll
+#pragma unroll 16
         for (int g = 1; g < HR_GROUPS; ++g) {
             if constexpr (FAST) v.l += red[g][x].l;
             else join(v, red[g][x].m, red[g][x].l);
         }
-        if (a.target[row] < 0) {
+        if (a.target.bad(row)) atomicOr(a.err, RAVEL_DEVERR_INDEX);
+        if (a.target.at(row) < 0) {
             a.losses[row] = 0.0f;
             if (a.stat != nullptr) a.stat[row] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         } else if constexpr (FAST) {
-            const float l = 1.0f + v.l;
+            // the reference was z_t log2 e rounded: E = d exp(z - z_t)
+            const float z = a.zt[row], d = ex2(fmaf(z, LOG2E, -(z * LOG2E))), s = v.l / d, l = 1.0f + s;
             if (!(v.l <= HEAD_FAST_SUM)) *a.bad = 1;
-            f = 1.0f / l;
-            a.losses[row] = log1pf(v.l);
-            a.stat[row] = make_float4(a.zt[row], log2f(l), v.l * f, 1.0f);
+            f = 1.0f / (l * d);
+            a.losses[row] = log1pf(s);
+            a.stat[row] = make_float4(z * LOG2E, log2f(l), s / l, 1.0f);
         } else {
             // the others' sum and the target's term under one maximum
-            const float z = a.zt[row], m = fmaxf(v.m, z);
-            const float others = v.l * ex2((v.m - finite_ref(m)) * LOG2E), mine = ex2((z - m) * LOG2E), l = others + mine;
-            a.losses[row] = (m - z) + (mine == 1.0f ? log1pf(others) : logf(l));
+            const float z = a.zt[row], m = fmaxf(v.m, z * LOG2E), d = fmaf(z, LOG2E, -m);  // d <= 0, but for a rounding
+            const float others = v.l * ex2(v.m - finite_ref(m)), mine = ex2(d), l = others + mine;
+            a.losses[row] = d >= 0.0f ? log1pf(others / mine) : logf(l) - d * 0.6931471805599453f;
             if (a.stat != nullptr) a.stat[row] = make_float4(m, log2f(l), others / l, 1.0f);
         }
         if (a.f != nullptr) a.f[row] = f;
@@ -545,11 +575,12 @@ __global__ void __launch_bounds__(HR_ROWS* HR_GROUPS) k_head_rows(const HeadRows
     }
     if (a.f == nullptr) return;
     __syncthreads();
-    for (int r = y; r < HR_ROWS && row0 + r < a.M; r += HR_GROUPS) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int r = warp; r < HR_ROWS && row0 + r < a.M; r += HR_THREADS / 32) {
         const T* const src = static_cast<const T*>(a.x) + (row0 + r) * a.ldc;
         T* const dst = static_cast<T*>(a.scaled) + (row0 + r) * a.ldc;
         const float f = sf[r];
-        for (int64_t c = x * 8; c < a.K; c += 256) {
+        for (int64_t c = lane * 8; c < a.K; c += 256) {
             float e[8];
             unpack8<T>(load8(src, c, a.K, true), e);
 #pragma unroll
@@ -561,8 +592,7 @@ __global__ void __launch_bounds__(HR_ROWS* HR_GROUPS) k_head_rows(const HeadRows
 
 // out = the losses' sum (MEAN: over the rows with a target), *factor = 1 or 1 / rows: one block, a fixed order.
 template <bool MEAN>
-__global__ void __launch_bounds__(1024) k_head_total(const float* __restrict__ losses, const int32_t* __restrict__ target,
-                                                     int64_t M, float* __restrict__ out, float* __restrict__ factor) {
+__global__ void __launch_bounds__(1024) k_head_total(const float* __restrict__ losses, const HeadTargets target, int64_t M, float* __restrict__ out, float* __restrict__ factor) {
     __shared__ float rs[32];
     __shared__ int rn[32];
     grid_wait();
@@ -572,7 +602,7 @@ __global__ void __launch_bounds__(1024) k_head_total(const float* __restrict__ l
 #pragma unroll 4
     for (int64_t i = threadIdx.x; i < M; i += 1024) {
         s += losses[i];
-        if (MEAN) n += target[i] >= 0;
+        if (MEAN) n += target.at(i) >= 0;
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -611,32 +641,62 @@ __global__ void __launch_bounds__(1024) k_head_up_max(const float* __restrict__ 
     *up_max = m > 0.0f ? m : 1.0f;
 }
 
-// out[r][c] = (sum of the slabs) up factor unit, rows of N; a thread per 4 columns.
+// Two outputs in one launch (d x, then d W from block `first` on).
+struct HeadOut {
+    const float* slabs;    // [splits] slabs of M rows, ldo apart
+    int64_t slab, ldo, M;
+    int splits;
+    int vec;               // 8-byte stores
+    void* out;             // [M, N]
+};
+struct HeadOutArgs {
+    HeadOut o[2];
+    int first;
+    int64_t N;
+    const float* up;       // null: 1
+    const float* factor;
+    float unit;
+};
+constexpr int HO_DEPTH = 4;  // 4-column groups of a thread, their loads in flight together
+// out[r][c] = (sum of the slabs) up factor unit.
 template <typename T>
-__global__ void __launch_bounds__(256) k_head_out(const float* __restrict__ slabs, int splits, int64_t slab, int64_t ldo,
-                                                  int64_t M, int64_t N, int vec, const float* __restrict__ up,
-                                                  const float* __restrict__ factor, float unit, T* __restrict__ out) {
+__global__ void __launch_bounds__(256) k_head_out(const HeadOutArgs a) {
     grid_wait();
     grid_trigger();
-    const float f = (up != nullptr ? *up : 1.0f) * *factor * unit;
-    const int64_t per = (N + 3) / 4, total = M * per;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total;
-         i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t r = i / per, c = (i - r * per) * 4;
-        const float* p = slabs + r * ldo + c;
-        float4 v = __ldcs(reinterpret_cast<const float4*>(p));
-        for (int s = 1; s < splits; ++s) {
-            const float4 w = __ldcs(reinterpret_cast<const float4*>(p + s * slab));
-            v.x += w.x; v.y += w.y; v.z += w.z; v.w += w.w;
-        }
-        T* const o = out + r * N + c;
-        if (vec) {
-            *reinterpret_cast<uint2*>(o) = make_uint2(pack2<T>(v.x * f, v.y * f), pack2<T>(v.z * f, v.w * f));
-        } else {
-            const float e[4] = {v.x, v.y, v.z, v.w};
+    const bool second = static_cast<int>(blockIdx.x) >= a.first;
+    const HeadOut& o = a.o[second];
+    const float f = (a.up != nullptr ? *a.up : 1.0f) * *a.factor * a.unit;
+    const int64_t per = (a.N + 3) / 4, total = o.M * per;
+    const int64_t i0 = static_cast<int64_t>(static_cast<int>(blockIdx.x) - (second ? a.first : 0)) * (256 * HO_DEPTH) + threadIdx.x;
+    float4 v[HO_DEPTH];
+    int64_t r[HO_DEPTH], c[HO_DEPTH];
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (c + k < N) o[k] = round_to<T>(e[k] * f);
+    for (int k = 0; k < HO_DEPTH; ++k) {
+        const int64_t i = i0 + k * 256;
+        if (i >= total) continue;
+        r[k] = i / per;
+        c[k] = (i - r[k] * per) * 4;
+        v[k] = __ldcs(reinterpret_cast<const float4*>(o.slabs + r[k] * o.ldo + c[k]));
+    }
+    for (int s = 1; s < o.splits; ++s) {
+#pragma unroll
+        for (int k = 0; k < HO_DEPTH; ++k) {
+            if (i0 + k * 256 >= total) continue;
+            const float4 w = __ldcs(reinterpret_cast<const float4*>(o.slabs + s * o.slab + r[k] * o.ldo + c[k]));
+            v[k].x += w.x; v[k].y += w.y; v[k].z += w.z; v[k].w += w.w;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < HO_DEPTH; ++k) {
+        if (i0 + k * 256 >= total) continue;
+        T* const p = static_cast<T*>(o.out) + r[k] * a.N + c[k];
+        if (o.vec) {
+            *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(v[k].x * f, v[k].y * f), pack2<T>(v[k].z * f, v[k].w * f));
+        } else {
+            const float e[4] = {v[k].x, v[k].y, v[k].z, v[k].w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (c[k] + q < a.N) p[q] = round_to<T>(e[q] * f);
         }
     }
 }

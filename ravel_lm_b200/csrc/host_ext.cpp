@@ -247,14 +247,15 @@ Rows rows_of(const at::Tensor& x) {
     return {t, m > 1 ? t.stride(0) : up8(n)};
 }
 
-// The same for an operand that TMA reads: 16-byte aligned rows, copied to such a pitch when
-// the tensor has none.
-Rows tma_rows(const at::Tensor& x) {
+// The same for an operand that TMA reads: 16-byte aligned rows, copied to such a pitch (of a multiple of
+// `multiple` elements) when the tensor has none.
+Rows tma_rows(const at::Tensor& x, int64_t multiple = 8) {
     Rows r = rows_of(x);
     const int64_t m = r.t.size(0), n = r.t.size(1);
     if (m == 0 || n == 0) return r;
     if (r.ld % 8 == 0 && reinterpret_cast<uintptr_t>(r.t.data_ptr()) % 16 == 0) return r;
-    Rows p{at::empty({m, up8(n)}, r.t.options()), up8(n)};
+    const int64_t pitch = (n + multiple - 1) / multiple * multiple;
+    Rows p{at::empty({m, pitch}, r.t.options()), pitch};
     check_status("ravel_pad_rows", ravel_pad_rows(r.t.data_ptr(), r.ld, m, n, p.t.data_ptr(), p.ld,
                                                   payload_code(r.t.scalar_type()), stream_of(r.t)));
     return p;
@@ -681,44 +682,58 @@ at::Tensor token_embedding(const at::Tensor& ids, const at::Tensor& weight, doub
     return embedding_forward(idc, rows_of(weight), scale);
 }
 
-// The tensors of a cross entropy call, its forward, and the gradients' float32 sums.
+// A cross entropy call's forward, and the gradients' float32 sums: slabs of d x, slabs of d W and their factor in one
+// allocation.
 struct CrossEntropyCall {
     Rows w;
     int64_t M, K, V;
     int dtype;
-    at::Tensor losses, out, factor, scratch, slabs_x, slabs_w;
+    at::Tensor out, scratch, sums;
+    int64_t nx = 0;  // floats of d x's slabs
+    float *slabs_x = nullptr, *slabs_w = nullptr, *factor = nullptr;
 
     // w: rows that TMA can read, of K elements and perhaps padding
     CrossEntropyCall(const Rows& w_, int64_t M_, int64_t K_, int64_t V_)
         : w(w_), M(M_), K(K_), V(V_), dtype(payload_code(w_.t.scalar_type())) {}
 
-    void make_slabs(bool need_x, bool need_w) {
+    void make_sums(bool need_x, bool need_w) {
         int64_t sizes[3];
         check_status("ravel_linear_ce_slabs", ravel_linear_ce_slabs(M, K, V, sizes));
-        const auto f32 = w.t.options().dtype(at::kFloat);
-        if (need_x) slabs_x = at::empty({sizes[0], M, sizes[2]}, f32);
-        if (need_w) slabs_w = at::empty({sizes[1], V, sizes[2]}, f32);
-        factor = at::empty({}, f32);
+        const int64_t n = need_x ? sizes[0] * M * sizes[2] : 0, nw = need_w ? sizes[1] * V * sizes[2] : 0;
+        hold(at::empty({n + nw + 1}, w.t.options().dtype(at::kFloat)), n);
     }
-    float* slab(at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+    void hold(const at::Tensor& t, int64_t n) {  // rows of whole 4 floats: every slab is 16-byte aligned
+        sums = t;
+        nx = n;
+        const int64_t all = sums.numel() - 1;
+        float* const p = sums.data_ptr<float>();
+        slabs_x = nx > 0 ? p : nullptr;
+        slabs_w = all > nx ? p + nx : nullptr;
+        factor = p + all;
+    }
 
+    // keep: what the backward of single rows' losses needs stays in scratch
     at::Tensor forward(const Rows& x, const at::Tensor& targets, int64_t ignore, int reduction, bool need_x, bool need_w,
-                       at::IntArrayRef rows_shape) {
+                       bool keep, at::IntArrayRef rows_shape) {
         const auto f32 = w.t.options().dtype(at::kFloat);
         const bool reduced = reduction != RAVEL_REDUCE_NONE, grads = reduced && (need_x || need_w);
-        losses = at::empty(rows_shape, f32);
-        if (reduced) out = at::empty({}, f32);
-        if (grads) make_slabs(need_x, need_w);
-        const size_t sb = ravel_linear_ce_scratch_bytes(M, K, V), wb = ravel_linear_ce_work_bytes(M, K, V, grads, dtype);
-        scratch = bytes(sb, w.t);
-        at::Tensor work = bytes(wb, w.t);
+        out = reduced ? at::empty({}, f32) : at::empty(rows_shape, f32);
+        if (grads) make_sums(need_x, need_w);
+        const size_t sb = ravel_linear_ce_scratch_bytes(M, K, V);
+        const size_t wb = ravel_linear_ce_work_bytes(M, K, V, grads, dtype);
+        // a reduced loss needs nothing of it later: losses, scratch and work in one
+        const size_t lb = reduced ? (static_cast<size_t>(M) * 4 + 255) / 256 * 256 : 0;
+        at::Tensor work = bytes(lb + (keep ? 0 : sb) + wb, w.t);
+        char* const p = static_cast<char*>(work.data_ptr());
+        if (keep) scratch = bytes(sb, w.t);
         check_status("ravel_linear_ce_fwd",
                      ravel_linear_ce_fwd(x.t.data_ptr(), x.ld, w.t.data_ptr(), w.ld, targets.data_ptr(),
-                                         index_code(targets, "targets"), M, K, V, ignore, reduction,
-                                         losses.data_ptr<float>(), reduced ? out.data_ptr<float>() : nullptr,
-                                         grads ? factor.data_ptr<float>() : nullptr, slab(slabs_x), slab(slabs_w), dtype,
-                                         scratch.data_ptr(), sb, work.data_ptr(), wb, stream_of(w.t)));
-        return reduced ? out : losses;
+                                         index_code(targets, "targets"), M, K, V, ignore, reduction, keep,
+                                         reduced ? reinterpret_cast<float*>(p) : out.data_ptr<float>(),
+                                         reduced ? out.data_ptr<float>() : nullptr, factor, slabs_x, slabs_w, dtype,
+                                         keep ? scratch.data_ptr() : p + lb, sb, p + lb + (keep ? 0 : sb), wb,
+                                         stream_of(w.t)));
+        return out;
     }
 };
 
@@ -727,12 +742,12 @@ struct LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy>
                               const at::Tensor& targets, int64_t ignore, int64_t reduction) {
         // A reduced loss's gradients are made here, a piece of the rows at a time, while their logits exist, up to a
         // factor that the backward applies: float32 sums, so that nothing depends on the size of the upstream gradient.
-        CrossEntropyCall c(tma_rows(weight), leading(x), weight.size(1), weight.size(0));
-        at::Tensor loss = c.forward(rows_of(x), targets, ignore, static_cast<int>(reduction), x.requires_grad(),
-                                    weight.requires_grad(), targets.sizes());
+        CrossEntropyCall c(tma_rows(weight, 64), leading(x), weight.size(1), weight.size(0));
         const bool reduced = reduction != RAVEL_REDUCE_NONE;
-        ctx->save_for_backward({c.slabs_x, c.slabs_w, c.factor, reduced ? at::Tensor() : c.w.t,
-                                reduced ? at::Tensor() : c.scratch});
+        at::Tensor loss = c.forward(rows_of(x), targets, ignore, static_cast<int>(reduction), x.requires_grad(),
+                                    weight.requires_grad(), !reduced, targets.sizes());
+        ctx->save_for_backward({c.sums, reduced ? at::Tensor() : c.w.t, c.scratch});
+        ctx->saved_data["nx"] = c.nx;
         ctx->saved_data["ld"] = c.w.ld;
         ctx->saved_data["M"] = c.M;
         ctx->saved_data["K"] = c.K;
@@ -753,31 +768,26 @@ struct LinearCrossEntropy : public torch::autograd::Function<LinearCrossEntropy>
         const c10::cuda::CUDAGuard guard(up.device());
         const int64_t M = ctx->saved_data["M"].toInt(), K = ctx->saved_data["K"].toInt(), V = ctx->saved_data["V"].toInt();
         const int dtype = static_cast<int>(ctx->saved_data["dtype"].toInt());
-        at::Tensor slabs_x = saved[0], slabs_w = saved[1], factor = saved[2];
         void* const st = stream_of(up);
-        const bool reduced = factor.defined();
-        if (!reduced) {
-            CrossEntropyCall c(Rows{saved[3], ctx->saved_data["ld"].toInt()}, M, K, V);
-            c.make_slabs(need_x, need_w);
-            at::Tensor scratch = saved[4];
+        const bool reduced = saved[0].defined();
+        CrossEntropyCall c(Rows{reduced ? saved[0] : saved[1], ctx->saved_data["ld"].toInt()}, M, K, V);
+        if (reduced) {  // which sums there are was settled by the forward
+            c.hold(saved[0], ctx->saved_data["nx"].toInt());
+        } else {
+            c.make_sums(need_x, need_w);
+            at::Tensor scratch = saved[2];
             const size_t wb = ravel_linear_ce_work_bytes(M, K, V, 1, dtype);
             at::Tensor work = bytes(wb, up);
             check_status("ravel_linear_ce_grad",
                          ravel_linear_ce_grad(c.w.t.data_ptr(), c.w.ld, up.data_ptr<float>(), M, K, V,
-                                              c.factor.data_ptr<float>(), c.slab(c.slabs_x), c.slab(c.slabs_w), dtype,
-                                              scratch.data_ptr(), static_cast<size_t>(scratch.numel()), work.data_ptr(),
-                                              wb, st));
-            slabs_x = c.slabs_x;
-            slabs_w = c.slabs_w;
-            factor = c.factor;
+                                              c.factor, c.slabs_x, c.slabs_w, dtype, scratch.data_ptr(),
+                                              static_cast<size_t>(scratch.numel()), work.data_ptr(), wb, st));
         }
         const auto like = up.options().dtype(dtype == RAVEL_F16 ? at::kHalf : at::kBFloat16);
         if (need_x) out[0] = at::empty(ctx->saved_data["x_shape"].toIntVector(), like);
         if (need_w) out[1] = at::empty({V, K}, like);
         check_status("ravel_linear_ce_bwd",
-                     ravel_linear_ce_bwd(need_x ? slabs_x.data_ptr<float>() : nullptr,
-                                         need_w ? slabs_w.data_ptr<float>() : nullptr,
-                                         reduced ? up.data_ptr<float>() : nullptr, factor.data_ptr<float>(), M, K, V,
+                     ravel_linear_ce_bwd(c.slabs_x, c.slabs_w, reduced ? up.data_ptr<float>() : nullptr, c.factor, M, K, V,
                                          need_x ? out[0].data_ptr() : nullptr, need_w ? out[1].data_ptr() : nullptr,
                                          dtype, st));
         return out;
@@ -802,8 +812,8 @@ at::Tensor linear_cross_entropy(const at::Tensor& x, const at::Tensor& weight, c
     const at::Tensor tc = targets.contiguous();
     if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad()))
         return LinearCrossEntropy::apply(x, weight, tc, ignore, reduction);
-    CrossEntropyCall c(tma_rows(weight), leading(x), weight.size(1), weight.size(0));
-    return c.forward(rows_of(x), tc, ignore, static_cast<int>(reduction), false, false, tc.sizes());
+    CrossEntropyCall c(tma_rows(weight, 64), leading(x), weight.size(1), weight.size(0));
+    return c.forward(rows_of(x), tc, ignore, static_cast<int>(reduction), false, false, false, tc.sizes());
 }
 
 // ------------------------------------------------------------------ the optimizer step
@@ -815,15 +825,6 @@ void written(const at::Tensor& t) {  // autograd counts writes in place
 }
 
 std::string at_place(const char* what, size_t i) { return std::string(what) + "[" + std::to_string(i) + "]"; }
-
-// A list's 2-norm (float64, 0-dim) of tensors of one dtype, as the library takes them.
-void list_norm(const std::vector<ravel_adamw_tensor>& list, const at::Tensor& like, double* norm) {
-    const size_t sb = ravel_grad_norm_scratch_bytes(list.data(), static_cast<int64_t>(list.size()));
-    at::Tensor scratch = bytes(sb, like);
-    check_status("ravel_grad_norm",
-                 ravel_grad_norm(list.data(), static_cast<int64_t>(list.size()), payload_code(like.scalar_type()), norm,
-                                 scratch.data_ptr(), sb, stream_of(like)));
-}
 
 at::Tensor global_norm(const TensorList& tensors) {
     if (tensors.empty()) throw py::value_error("global_norm expects at least one tensor");
@@ -847,7 +848,12 @@ at::Tensor global_norm(const TensorList& tensors) {
             if (first == nullptr) first = &t;
             list.push_back({nullptr, held.back().data_ptr(), nullptr, nullptr, nullptr, nullptr, nullptr, t.numel()});
         }
-        list_norm(list, *first, norms.data_ptr<double>() + k);
+        const int64_t count = static_cast<int64_t>(list.size());
+        const size_t sb = ravel_grad_norm_scratch_bytes(list.data(), count);
+        at::Tensor scratch = bytes(sb, *first);
+        check_status("ravel_grad_norm",
+                     ravel_grad_norm(list.data(), count, payload_code(types[k]), norms.data_ptr<double>() + k,
+                                     scratch.data_ptr(), sb, stream_of(*first)));
     }
     return types.size() == 1 ? norms[0] : at::norm(norms);
 }
@@ -935,24 +941,14 @@ OptTensor adamw_step(const TensorList& params, const TensorList& grads, const Te
                    eight ? static_cast<signed char*>((*avg_exps)[i].data_ptr()) : nullptr,
                    eight ? static_cast<signed char*>((*sq_exps)[i].data_ptr()) : nullptr, params[i].numel()};
     }
-    at::Tensor own_norm, norm32;
-    const double* norm_ptr = nullptr;
-    if (max_norm) {
-        if (norm) {
-            norm_ptr = norm->data_ptr<double>();
-        } else {
-            own_norm = at::empty({}, first.options().dtype(at::kDouble).requires_grad(false));
-            list_norm(list, first, own_norm.data_ptr<double>());
-            norm_ptr = own_norm.data_ptr<double>();
-        }
-        norm32 = at::empty({}, first.options().dtype(at::kFloat));
-    }
-    const size_t sb = ravel_adamw_scratch_bytes();
+    at::Tensor norm32;
+    if (max_norm) norm32 = at::empty({}, at::TensorOptions().device(first.device()).dtype(at::kFloat));
+    const size_t sb = ravel_adamw_scratch_bytes(list.data(), static_cast<int64_t>(n), max_norm.value_or(0.0));
     at::Tensor scratch = bytes(sb, first);
     check_status("ravel_adamw",
                  ravel_adamw(list.data(), static_cast<int64_t>(n), payload_code(dt), eight ? 8 : 32,
                              step.data_ptr<int64_t>(), lr, lr_tensor ? lr_tensor->data_ptr<float>() : nullptr, beta1,
-                             beta2, eps, weight_decay, max_norm.value_or(0.0), norm_ptr,
+                             beta2, eps, weight_decay, max_norm.value_or(0.0), norm ? norm->data_ptr<double>() : nullptr,
                              max_norm ? norm32.data_ptr<float>() : nullptr, scratch.data_ptr(), sb, stream_of(first)));
     written(step);
     for (size_t i = 0; i < n; ++i) {

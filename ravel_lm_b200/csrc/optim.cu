@@ -71,6 +71,28 @@ int check_list(const ravel_adamw_tensor* tensors, int64_t count) {
     return RAVEL_OK;
 }
 
+constexpr size_t kScalarBytes = 64;
+static_assert(sizeof(AdamScalars) <= kScalarBytes, "scratch");
+
+size_t norm_bytes(const ravel_adamw_tensor* tensors, int64_t count) {
+    return static_cast<size_t>(std::max<int64_t>(1, launch_bound(tensors, count))) * AW_NORM_BLOCKS * sizeof(double);
+}
+
+// The parts of the list's norm.
+int norm_parts(const ravel_adamw_tensor* tensors, int64_t count, int dtype, double* part, int* parts, cudaStream_t st) {
+    return with_param_type(dtype, [&](auto tv) -> int {
+        using T = decltype(tv);
+        return launches(tensors, count, [&](auto& a, int chunks) -> int {
+            constexpr int CAP = sizeof(a.t) / sizeof(a.t[0]);
+            if (chunks == 0) return RAVEL_OK;
+            a.part = part + *parts;
+            const int blocks = std::min(chunks, AW_NORM_BLOCKS);
+            *parts += blocks;
+            return launch(k_grad_norm<T, CAP>, dim3(static_cast<unsigned>(blocks)), 32 * AW_WARPS, 0, st, 1, a);
+        });
+    });
+}
+
 }  // namespace
 }  // namespace ravel
 
@@ -80,7 +102,7 @@ extern "C" {
 
 size_t ravel_grad_norm_scratch_bytes(const ravel_adamw_tensor* tensors, int64_t count) {
     if (check_list(tensors, count) != RAVEL_OK) return 0;
-    return static_cast<size_t>(std::max<int64_t>(1, launch_bound(tensors, count))) * AW_NORM_BLOCKS * sizeof(double);
+    return norm_bytes(tensors, count);
 }
 
 int ravel_grad_norm(const ravel_adamw_tensor* tensors, int64_t count, int dtype, double* norm, void* scratch,
@@ -89,26 +111,18 @@ int ravel_grad_norm(const ravel_adamw_tensor* tensors, int64_t count, int dtype,
     if (int e = check_list(tensors, count)) return e;
     if (dtype != RAVEL_F32 && dtype != RAVEL_BF16 && dtype != RAVEL_F16) return RAVEL_ERR_UNSUPPORTED;
     if (norm == nullptr) return RAVEL_ERR_INVALID_ARG;
-    if (scratch == nullptr || scratch_bytes < ravel_grad_norm_scratch_bytes(tensors, count)) return RAVEL_ERR_WORKSPACE;
+    if (scratch == nullptr || scratch_bytes < norm_bytes(tensors, count)) return RAVEL_ERR_WORKSPACE;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     double* const part = static_cast<double*>(scratch);
     int parts = 0;
-    const int rc = with_param_type(dtype, [&](auto tv) -> int {
-        using T = decltype(tv);
-        return launches(tensors, count, [&](auto& a, int chunks) -> int {
-            constexpr int CAP = sizeof(a.t) / sizeof(a.t[0]);
-            if (chunks == 0) return RAVEL_OK;
-            a.part = part + parts;
-            const int blocks = std::min(chunks, AW_NORM_BLOCKS);
-            parts += blocks;
-            return launch(k_grad_norm<T, CAP>, dim3(static_cast<unsigned>(blocks)), 32 * AW_WARPS, 0, st, 1, a);
-        });
-    });
-    if (rc != RAVEL_OK) return rc;
+    if (int e = norm_parts(tensors, count, dtype, part, &parts, st)) return e;
     return launch(k_norm_total, dim3(1), 1024, 0, st, 1, part, parts, norm);
 }
 
-size_t ravel_adamw_scratch_bytes(void) { return sizeof(AdamScalars); }
+size_t ravel_adamw_scratch_bytes(const ravel_adamw_tensor* tensors, int64_t count, double max_norm) {
+    if (check_list(tensors, count) != RAVEL_OK) return 0;
+    return kScalarBytes + (max_norm > 0.0 ? norm_bytes(tensors, count) : 0);
+}
 
 int ravel_adamw(const ravel_adamw_tensor* tensors, int64_t count, int dtype, int state_bits, int64_t* step, double lr,
                 const float* lr_device, double beta1, double beta2, double eps, double weight_decay, double max_norm,
@@ -118,7 +132,7 @@ int ravel_adamw(const ravel_adamw_tensor* tensors, int64_t count, int dtype, int
     if (dtype != RAVEL_F32 && dtype != RAVEL_BF16 && dtype != RAVEL_F16) return RAVEL_ERR_UNSUPPORTED;
     if (state_bits != 8 && state_bits != 32) return RAVEL_ERR_UNSUPPORTED;
     if (step == nullptr || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0) ||
-        (norm != nullptr && !(max_norm > 0.0)))
+        !(max_norm >= 0.0) || (norm != nullptr && max_norm == 0.0))
         return RAVEL_ERR_INVALID_ARG;
     for (int64_t i = 0; i < count; ++i) {
         const ravel_adamw_tensor& t = tensors[i];
@@ -128,11 +142,18 @@ int ravel_adamw(const ravel_adamw_tensor* tensors, int64_t count, int dtype, int
             (state_bits == 8 && (t.exp_avg_exponents == nullptr || t.exp_avg_sq_exponents == nullptr)))
             return RAVEL_ERR_INVALID_ARG;
     }
-    if (scratch == nullptr || scratch_bytes < sizeof(AdamScalars)) return RAVEL_ERR_WORKSPACE;
+    const bool own_norm = max_norm > 0.0 && norm == nullptr;
+    if (scratch == nullptr || scratch_bytes < kScalarBytes + (own_norm ? norm_bytes(tensors, count) : 0))
+        return RAVEL_ERR_WORKSPACE;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     AdamScalars* const s = static_cast<AdamScalars*>(scratch);
-    const AdamStep as = {step, lr_device, lr, beta1, beta2, weight_decay, max_norm, norm, norm_out, s};
-    if (int e = launch(k_adamw_scalars, dim3(1), 32, 0, st, 1, as)) return e;
+    double* const part = reinterpret_cast<double*>(static_cast<char*>(scratch) + kScalarBytes);
+    int parts = 0;
+    if (own_norm) {
+        if (int e = norm_parts(tensors, count, dtype, part, &parts, st)) return e;
+    }
+    const AdamStep as = {step, lr_device, lr, beta1, beta2, weight_decay, max_norm, norm, part, parts, norm_out, s};
+    if (int e = launch(k_adamw_scalars, dim3(1), own_norm ? 1024 : 32, 0, st, 1, as)) return e;
     return with_param_type(dtype, [&](auto tv) -> int {
         using T = decltype(tv);
         return launches(tensors, count, [&](auto& a, int chunks) -> int {
@@ -144,7 +165,7 @@ int ravel_adamw(const ravel_adamw_tensor* tensors, int64_t count, int dtype, int
             a.b2 = static_cast<float>(beta2);
             a.omb2 = static_cast<float>(1.0 - beta2);
             a.eps = static_cast<float>(eps);
-            a.clipped = norm != nullptr;
+            a.clipped = max_norm > 0.0;
             const dim3 grid(static_cast<unsigned>(chunks));
             if (state_bits == 8) return launch(k_adamw<T, true, CAP>, grid, 32 * AW_WARPS, 0, st, 1, a);
             return launch(k_adamw<T, false, CAP>, grid, 32 * AW_WARPS, 0, st, 1, a);

@@ -26,19 +26,35 @@ __device__ __forceinline__ void sub_scale(float (&x)[E], float m, float c) {
             : "l"(m2), "l"(c2));
 }
 
-// x[i] = (x[i] - m) c + d.
+// x[i] = x[i] c - d.
 template <int E>
-__device__ __forceinline__ void sub_fma(float (&x)[E], float m, float c, float d) {
-    uint64_t m2, c2, d2;
-    asm("mov.b64 %0, {%1, %1};" : "=l"(m2) : "f"(-m));
+__device__ __forceinline__ void scale_sub(float (&x)[E], float c, float d) {
+    uint64_t c2, d2;
     asm("mov.b64 %0, {%1, %1};" : "=l"(c2) : "f"(c));
-    asm("mov.b64 %0, {%1, %1};" : "=l"(d2) : "f"(d));
+    asm("mov.b64 %0, {%1, %1};" : "=l"(d2) : "f"(-d));
 #pragma unroll
     for (int e = 0; e < E; e += 2)
-        asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%0, %1};\n\tadd.rn.f32x2 t, t, %2;\n\tfma.rn.f32x2 t, t, %3, %4;\n\t"
-            "mov.b64 {%0, %1}, t;\n\t}"
+        asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%0, %1};\n\tfma.rn.f32x2 t, t, %2, %3;\n\tmov.b64 {%0, %1}, t;\n\t}"
             : "+f"(x[e]), "+f"(x[e + 1])
-            : "l"(m2), "l"(c2), "l"(d2));
+            : "l"(c2), "l"(d2));
+}
+
+// The sum of x, in four chains.
+template <int E>
+__device__ __forceinline__ float sum_of(const float (&x)[E]) {
+    static_assert(E % 4 == 0 && E >= 8, "two pairs at a time");
+    uint64_t a, b;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "f"(x[0]), "f"(x[1]));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "f"(x[2]), "f"(x[3]));
+#pragma unroll
+    for (int e = 4; e < E; e += 4) {
+        asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tadd.rn.f32x2 %0, %0, t;\n\t}" : "+l"(a) : "f"(x[e]), "f"(x[e + 1]));
+        asm("{\n\t.reg .b64 t;\n\tmov.b64 t, {%1, %2};\n\tadd.rn.f32x2 %0, %0, t;\n\t}" : "+l"(b) : "f"(x[e + 2]), "f"(x[e + 3]));
+    }
+    float a0, a1, b0, b1;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(a));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(b0), "=f"(b1) : "l"(b));
+    return (a0 + a1) + (b0 + b1);
 }
 
 // Running (maximum, sum of 2^((x - maximum) c)); an empty one is (-inf, 0).

@@ -160,7 +160,7 @@ bool head_fast(int64_t M, int64_t K, int64_t V, int dtype) {
 // Rows of a piece: whole tiles of 256.  d W is read and written once more for every piece after the first, which at 1024
 // rows takes about as long as the piece's products.
 int64_t head_piece(int64_t M, int64_t V) {
-    const int64_t most = std::max<int64_t>(1024, static_cast<int64_t>(kHeadPieceBytes / 2) / up_to(V, 8) / 256 * 256);
+    const int64_t most = std::max<int64_t>(1024, static_cast<int64_t>(kHeadPieceBytes / 2) / up_to(V, 64) / 256 * 256);
     if (M <= most) return std::max<int64_t>(M, 1);
     const int64_t pieces = (M + most - 1) / most;
     return up_to((M + pieces - 1) / pieces, 256);
@@ -170,10 +170,11 @@ HeadLayout head_layout(int64_t M, int64_t K, int64_t V, bool fast) {
     HeadLayout l;
     std::memset(&l, 0, sizeof(l));
     l.piece = head_piece(M, V);
-    l.ldz = up_to(V, 8);
-    l.ldc = up_to(K, 8);
+    // whole 128-byte lines: a TMA row that straddles two reads both (1021 x 515 -> 32003: d x 45 us, XX with)
+    l.ldz = up_to(V, 64);
+    l.ldc = up_to(K, 64);
     l.ldo = up_to(K, 4);
-    l.parts = 2 * ((V + 127) / 128);
+    l.parts = head_parts(32) * ((V + 31) / 32);  // as many as the narrowest tiles make
     l.off_target = 0;
     l.off_zt = up256(static_cast<size_t>(M) * 4);
     l.off_stat = l.off_zt + up256(static_cast<size_t>(M) * 4);
@@ -196,7 +197,7 @@ HeadLayout head_layout(int64_t M, int64_t K, int64_t V, bool fast) {
 }
 
 // Clusters of two product CTAs that fit the device at once (queried once per kernel and device).
-int resident_pairs(const void* kernel) {
+int resident_pairs(const void* kernel, int threads) {
     static std::mutex mu;
     static std::map<std::pair<const void*, int>, int> known;
     int dev = 0;
@@ -211,7 +212,7 @@ int resident_pairs(const void* kernel) {
     at.val.clusterDim.x = 2;
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.gridDim = dim3(static_cast<unsigned>(sm_count() / 2 * 2));
-    cfg.blockDim = dim3(MM_THREADS);
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
     cfg.dynamicSmemBytes = MM_SMEM;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
@@ -260,8 +261,8 @@ int launch_logits(const HeadOperand& X, const HeadOperand& W, int64_t K, HeadLog
     if (int e = head_map<T, false>(&mb, W, a.V, K, BN / CG)) return e;
     if (int e = set_smem(kern, MM_SMEM)) return e;
     const int64_t tiles = static_cast<int64_t>(a.mtiles) * a.ntiles;
-    const int64_t fit = CG == 2 ? resident_pairs(reinterpret_cast<const void*>(kern)) : sm_count();
-    return launch(kern, dim3(static_cast<unsigned>(std::min(tiles, fit) * CG)), MM_THREADS, MM_SMEM, st, CG, ma, mb, a);
+    const int64_t fit = CG == 2 ? resident_pairs(reinterpret_cast<const void*>(kern), HEAD_THREADS) : sm_count();
+    return launch(kern, dim3(static_cast<unsigned>(std::min(tiles, fit) * CG)), HEAD_THREADS, MM_SMEM, st, CG, ma, mb, a);
 }
 
 // Pairs where two row tiles exist, single CTAs for fewer rows.
@@ -275,25 +276,29 @@ int head_logits(const HeadOperand& X, const HeadOperand& W, int64_t K, bool pair
 }
 
 struct HeadPlan {
-    int cg, splits;
+    int cg, bn, splits;
 };
-// A gradient's launch shape and the CTAs (or pairs) that share its k, by an estimate in microseconds: waves of units, each
-// the larger of its chunks and its epilogue, and the slabs' traffic.
+// A gradient's launch shape and the CTAs (or pairs) that share its k, by an estimate in microseconds: the launch, waves of
+// units, each the larger of its chunks (as measured with every SM busy) and its epilogue, and the slabs' traffic.
+// Measured, us (rows x k; outputs; shape): d x 4096 x 16384, 1024: pairs 256 96, pairs 128 113, single 128 122;
+// d W 16384 x 4096, 512: pairs 256 in two parts 55, in one 82, pairs 128 62; d x 24 x 32000, 2048: single 128
+// in eight parts 21, pairs 256 30.
 HeadPlan plan_grad(int64_t M, int64_t N, int64_t k) {
     const double sms = sm_count(), kc = static_cast<double>((k + MM_BK - 1) / MM_BK);
     struct Kind {
         int cg, bn;
-        double chunk, epilogue;
+        double fixed, chunk, epilogue;
     };
-    const Kind kinds[] = {{2, 256, 0.280, 3.0}, {1, 128, 0.160, 1.6}};
-    HeadPlan best = {1, 1};
+    const Kind kinds[] = {{2, 256, 5.5, 0.34, 3.0}, {2, 128, 4.4, 0.21, 1.6}, {1, 128, 4.2, 0.25, 1.6},
+                          {1, 64, 3.4, 0.20, 1.0}};
+    HeadPlan best = {1, 128, 1};
     double cost = 1e30;
     for (const Kind& q : kinds) {
         const double tiles = std::ceil(M / (128.0 * q.cg)) * std::ceil(static_cast<double>(N) / q.bn);
-        for (int s = 1; s <= 32 && kc >= 4 * s; s *= 2) {
+        for (int s = 1; s <= 32 && kc >= 4 * s; ++s) {
             const double waves = std::ceil(tiles * s / std::floor(sms / q.cg));
-            const double us = waves * std::max(std::ceil(kc / s) * q.chunk, q.epilogue) + (s - 1) * (M * N) * 8.0 / 5e6;
-            if (us < cost) cost = us, best = {q.cg, s};
+            const double us = q.fixed + waves * std::max(std::ceil(kc / s) * q.chunk, q.epilogue) + (s - 1) * (M * N) * 8.0 / 5e6;
+            if (us < cost) cost = us, best = {q.cg, q.bn, s};
         }
     }
     return best;
@@ -308,8 +313,17 @@ int launch_grad(const HeadOperand& A, const HeadOperand& B, int64_t k, HeadGradA
     if (int e = head_map<T, true>(&mb, B, a.N, k, 0)) return e;
     if (int e = set_smem(kern, MM_SMEM)) return e;
     const int64_t units = static_cast<int64_t>(a.mtiles) * a.ntiles * a.splits;
-    const int64_t fit = CG == 2 ? resident_pairs(reinterpret_cast<const void*>(kern)) : sm_count();
+    const int64_t fit = CG == 2 ? resident_pairs(reinterpret_cast<const void*>(kern), MM_THREADS) : sm_count();
     return launch(kern, dim3(static_cast<unsigned>(std::min(units, fit) * CG)), MM_THREADS, MM_SMEM, st, CG, ma, mb, a);
+}
+
+template <typename T, bool A_MN, bool ROWS>
+int head_grad(const HeadPlan& p, const HeadOperand& A, const HeadOperand& B, int64_t k, HeadGradArgs a, cudaStream_t st) {
+    a.splits = p.splits;
+    if (p.cg == 2 && p.bn == 256) return launch_grad<T, 2, 256, A_MN, ROWS>(A, B, k, a, st);
+    if (p.cg == 2) return launch_grad<T, 2, 128, A_MN, ROWS>(A, B, k, a, st);
+    if (p.bn == 128) return launch_grad<T, 1, 128, A_MN, ROWS>(A, B, k, a, st);
+    return launch_grad<T, 1, 64, A_MN, ROWS>(A, B, k, a, st);
 }
 
 // The split counts of a whole call: of its full pieces for d W and of the first piece for d x.
@@ -336,8 +350,10 @@ int head_check(int64_t M, int64_t K, int64_t V, int t_dtype, int dtype) {
 }
 
 struct HeadCall {
-    const void *x, *w;
-    int64_t ldx, ldw, M, K, V;
+    const void* w;
+    int64_t ldw, M, K, V;
+    HeadTargets target;
+    HeadOperand x;     // rows that TMA can read, those without a target zero where gradients are wanted
     float* losses;     // null: the statistics are there (the gradient of given upstream values)
     const float* up;   // [M] or null
     float *gx, *gw;    // null: not wanted
@@ -348,6 +364,13 @@ struct HeadCall {
     DeviceWords words;
     cudaStream_t st;
 };
+
+template <typename T, bool FAST>
+int head_rows(const HeadRowsArgs& h, cudaStream_t st) {
+    if (h.M < 16 * static_cast<int64_t>(sm_count()))
+        return launch(k_head_rows<T, FAST, 8>, dim3(static_cast<unsigned>((h.M + 7) / 8)), HR_THREADS, 0, st, 1, h);
+    return launch(k_head_rows<T, FAST, 32>, dim3(static_cast<unsigned>((h.M + 31) / 32)), HR_THREADS, 0, st, 1, h);
+}
 
 // d W += the targets' terms: the rows of x times -(1 - p_t), summed by target.
 template <typename T>
@@ -380,11 +403,10 @@ int head_targets(const HeadCall& c, const int32_t* target, const float4* stat, c
 template <typename T>
 int head_run(const HeadCall& c, bool stats) {
     constexpr bool half = std::is_same<T, __half>::value;
-    int32_t* const target = reinterpret_cast<int32_t*>(c.scratch + c.l.off_target);
+    const int32_t* const target = static_cast<const int32_t*>(c.target.p);  // with gradients: prepared
     float* const zt = reinterpret_cast<float*>(c.scratch + c.l.off_zt);
     float4* const stat = reinterpret_cast<float4*>(c.scratch + c.l.off_stat);
     float* const up_max = reinterpret_cast<float*>(c.scratch + c.l.off_up);
-    char* const clean = c.scratch + c.l.off_clean;
     char* const work = static_cast<char*>(c.work);
     void* const dz = c.work;  // four products: the parts are read before it is written
     float2* const part = reinterpret_cast<float2*>(c.fast ? work + c.l.off_part : work);
@@ -402,14 +424,15 @@ int head_run(const HeadCall& c, bool stats) {
         return RAVEL_ERR_CUDA;
     for (int64_t r0 = 0, piece = 0; r0 < c.M; r0 += c.l.piece, ++piece) {
         const int64_t rows = std::min(c.l.piece, c.M - r0);
-        const HeadOperand X{clean + static_cast<size_t>(r0) * c.l.ldc * 2, c.l.ldc};
+        const HeadOperand X{static_cast<const char*>(c.x.p) + static_cast<size_t>(r0) * c.x.ld * 2, c.x.ld};
         const HeadOperand S{scaled + static_cast<size_t>(r0) * c.l.ldc * 2, c.l.ldc};
         const bool pairs = c.fast || head_pairs(rows);
         const int tile = pairs ? 256 : 128;
         HeadLogitsArgs a;
         std::memset(&a, 0, sizeof(a));
         a.M = rows; a.V = static_cast<int>(c.V);
-        a.target = target + r0;
+        a.target = c.target;
+        a.target.p = static_cast<const char*>(c.target.p) + static_cast<size_t>(r0) * (c.target.kind == 2 ? 8 : 4);
         a.part = part; a.zt = zt + r0;
         a.stat = stat + r0;
         a.up = c.up != nullptr ? c.up + r0 : nullptr;
@@ -420,26 +443,26 @@ int head_run(const HeadCall& c, bool stats) {
         a.err = c.words.error; a.wait_limit = c.words.wait_limit;
         HeadRowsArgs h;
         std::memset(&h, 0, sizeof(h));
-        h.part = part; h.parts = static_cast<int>((c.V + tile - 1) / tile) * 2;
+        h.part = part; h.parts = static_cast<int>((c.V + tile - 1) / tile) * head_parts(tile);
         h.M = rows; h.target = a.target; h.zt = a.zt;
         h.losses = c.losses != nullptr ? c.losses + r0 : nullptr; h.stat = stat + r0;
+        h.err = c.words.error;
         if (c.fast) {
             h.f = f + r0;
             h.x = X.p; h.scaled = scaled + static_cast<size_t>(r0) * c.l.ldc * 2;
             h.K = c.K; h.ldc = c.l.ldc;
         }
-        const dim3 row_blocks(static_cast<unsigned>((rows + HR_ROWS - 1) / HR_ROWS));
         if constexpr (!half) {
             if (c.fast) {
                 if (int e = head_logits<T, HEAD_FAST>(X, W, c.K, true, a, c.st)) return e;
                 h.bad = flags + piece;
-                if (int e = launch(k_head_rows<T, true>, row_blocks, HR_ROWS * HR_GROUPS, 0, c.st, 1, h)) return e;
+                if (int e = head_rows<T, true>(h, c.st)) return e;
                 a.only = h.only = flags + piece;  // what follows is for a piece that needs it
             }
         }
         if (stats) {
             if (int e = head_logits<T, HEAD_STATS>(X, W, c.K, pairs, a, c.st)) return e;
-            if (int e = launch(k_head_rows<T, false>, row_blocks, HR_ROWS * HR_GROUPS, 0, c.st, 1, h)) return e;
+            if (int e = head_rows<T, false>(h, c.st)) return e;
         }
         if (!grads) continue;
         if (int e = head_logits<T, HEAD_EXP>(X, W, c.K, pairs, a, c.st)) return e;
@@ -449,32 +472,27 @@ int head_run(const HeadCall& c, bool stats) {
         g.N = c.K; g.ldo = c.l.ldo;
         g.err = c.words.error; g.wait_limit = c.words.wait_limit;
         if (c.gx != nullptr) {
-            g.M = rows; g.splits = sp.x.splits;
+            g.M = rows;
             g.out = c.gx + r0 * c.l.ldo; g.slab = c.M * c.l.ldo; g.add = 0;
-            g.f = f + r0; g.stat = stat + r0; g.target = a.target;
+            g.f = f + r0; g.stat = stat + r0; g.target = target + r0;
             g.w = c.w; g.ldw = c.ldw;
             int e = RAVEL_OK;
             if (c.fast) {
-                if constexpr (!half)
-                    e = sp.x.cg == 2 ? launch_grad<T, 2, 256, false, true>(Z, W, c.V, g, c.st)
-                                     : launch_grad<T, 1, 128, false, true>(Z, W, c.V, g, c.st);
+                if constexpr (!half) e = head_grad<T, false, true>(sp.x, Z, W, c.V, g, c.st);
             } else {
-                e = sp.x.cg == 2 ? launch_grad<T, 2, 256, false, false>(Z, W, c.V, g, c.st)
-                                 : launch_grad<T, 1, 128, false, false>(Z, W, c.V, g, c.st);
+                e = head_grad<T, false, false>(sp.x, Z, W, c.V, g, c.st);
             }
             if (e) return e;
         }
         if (c.gw != nullptr) {
-            g.M = c.V; g.splits = sp.w.splits;
+            g.M = c.V;
             g.out = c.gw; g.slab = c.V * c.l.ldo; g.add = r0 > 0;
             const HeadOperand& B = c.fast ? S : X;
-            if (int e = sp.w.cg == 2 ? launch_grad<T, 2, 256, true, false>(Z, B, rows, g, c.st)
-                                     : launch_grad<T, 1, 128, true, false>(Z, B, rows, g, c.st))
-                return e;
+            if (int e = head_grad<T, true, false>(sp.w, Z, B, rows, g, c.st)) return e;
         }
     }
     if constexpr (!half) {
-        if (c.fast && c.gw != nullptr) return head_targets<T>(c, target, stat, clean, work);
+        if (c.fast && c.gw != nullptr) return head_targets<T>(c, target, stat, static_cast<const char*>(c.x.p), work);
     }
     return RAVEL_OK;
 }
@@ -583,7 +601,7 @@ int ravel_linear_ce_slabs(int64_t M, int64_t K, int64_t V, int64_t* sizes) {
 }
 
 int ravel_linear_ce_fwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* targets,
-                        int target_dtype, int64_t M, int64_t K, int64_t V, int64_t ignore_index, int reduction,
+                        int target_dtype, int64_t M, int64_t K, int64_t V, int64_t ignore_index, int reduction, int keep,
                         float* losses, float* out, float* factor, float* slabs_x, float* slabs_w, int dtype,
                         void* scratch, size_t scratch_bytes, void* work, size_t work_bytes, void* stream) {
     RAVEL_TIMED("ravel_linear_ce_fwd", stream);
@@ -601,20 +619,25 @@ int ravel_linear_ce_fwd(const void* x, int64_t ldx, const void* weight, int64_t 
         work_bytes < (grads ? c.l.work_grads : c.l.work) || !aligned16(scratch) || !aligned16(work))
         return RAVEL_ERR_WORKSPACE;
     if (int e = device_words(&c.words)) return e;
-    c.x = x; c.w = weight; c.ldx = ldx; c.ldw = ldw;
+    c.w = weight; c.ldw = ldw;
     c.M = M; c.K = K; c.V = V;
     c.losses = losses; c.up = nullptr; c.gx = slabs_x; c.gw = slabs_w;
     c.scratch = static_cast<char*>(scratch);
     c.work = work;
     c.st = static_cast<cudaStream_t>(stream);
-    int32_t* const target = reinterpret_cast<int32_t*>(c.scratch + c.l.off_target);
+    // x and the targets as they are, where only losses are wanted (a row without a target then has any logits) and TMA can
+    // read x; else prepared
+    c.target = {targets, target_dtype == RAVEL_I64 ? 2 : 1, static_cast<int>(V), ignore_index};
+    c.x = {x, M > 1 ? ldx : up_to(K, 8)};
+    const bool prepare = grads || keep || !aligned16(x) || c.x.ld % 8 != 0;
     return with_half_type(dtype, [&](auto tv) -> int {
         using T = decltype(tv);
-        if (M > 0) {
+        if (M > 0 && prepare) {
             HeadPrepArgs p;
             std::memset(&p, 0, sizeof(p));
             p.targets = targets; p.targets64 = target_dtype == RAVEL_I64;
-            p.M = M; p.V = V; p.ignore = ignore_index; p.target = target;
+            p.M = M; p.V = V; p.ignore = ignore_index;
+            p.target = reinterpret_cast<int32_t*>(c.scratch + c.l.off_target);
             p.x = x; p.clean = c.scratch + c.l.off_clean;
             p.K = K; p.ldx = ldx; p.ldc = c.l.ldc;
             p.vec = aligned16(x) && (M == 1 || ldx % 8 == 0);
@@ -627,11 +650,14 @@ int ravel_linear_ce_fwd(const void* x, int64_t ldx, const void* weight, int64_t 
             p.err = c.words.error;
             const dim3 grid(static_cast<unsigned>(std::min<int64_t>((M + 7) / 8, int64_t{sm_count()} * 32)));
             if (int e = launch(k_head_prep<T>, grid, 256, 0, c.st, 1, p)) return e;
+            c.target.p = p.target;
+            c.target.kind = 0;
+            c.x = {p.clean, p.ldc};
         }
         if (int e = head_run<T>(c, true)) return e;
         if (reduction == RAVEL_REDUCE_NONE) return RAVEL_OK;
         return launch(reduction == RAVEL_REDUCE_MEAN ? k_head_total<true> : k_head_total<false>, dim3(1), 1024, 0, c.st, 1,
-                      losses, target, M, out, factor);
+                      losses, c.target, M, out, factor);
     });
 }
 
@@ -650,12 +676,14 @@ int ravel_linear_ce_grad(const void* weight, int64_t ldw, const float* up, int64
         !aligned16(scratch) || !aligned16(work))
         return RAVEL_ERR_WORKSPACE;
     if (int e = device_words(&c.words)) return e;
-    c.x = nullptr; c.w = weight; c.ldx = 0; c.ldw = ldw;
+    c.w = weight; c.ldw = ldw;
     c.M = M; c.K = K; c.V = V;
     c.losses = nullptr; c.up = up; c.gx = slabs_x; c.gw = slabs_w;
     c.scratch = static_cast<char*>(scratch);
     c.work = work;
     c.st = static_cast<cudaStream_t>(stream);
+    c.target = {c.scratch + c.l.off_target, 0, static_cast<int>(V), 0};
+    c.x = {c.scratch + c.l.off_clean, c.l.ldc};
     const int rc = with_half_type(dtype, [&](auto tv) -> int { return head_run<decltype(tv)>(c, false); });
     if (rc != RAVEL_OK) return rc;
     return cudaMemcpyAsync(factor, c.scratch + c.l.off_up, sizeof(float), cudaMemcpyDeviceToDevice, c.st) == cudaSuccess
@@ -674,17 +702,22 @@ int ravel_linear_ce_bwd(const float* slabs_x, const float* slabs_w, const float*
     const int64_t ldo = up_to(K, 4);
     return with_half_type(dtype, [&](auto tv) -> int {
         using T = decltype(tv);
-        const float unit = std::is_same<T, __half>::value ? 1.0f / 32768.0f : 1.0f;
-        auto out = [&](const float* slabs, int splits, int64_t rows, void* g) -> int {
-            if (g == nullptr || rows == 0) return RAVEL_OK;
-            const int64_t units = rows * ((K + 3) / 4);
-            const dim3 grid(static_cast<unsigned>(std::min<int64_t>((units + 255) / 256, int64_t{sm_count()} * 32)));
-            const int vec = K % 4 == 0 && reinterpret_cast<uintptr_t>(g) % 8 == 0;
-            return launch(k_head_out<T>, grid, 256, 0, st, 1, slabs, splits, rows * ldo, ldo, rows, K, vec, up, factor, unit,
-                          static_cast<T*>(g));
+        HeadOutArgs a;
+        std::memset(&a, 0, sizeof(a));
+        a.N = K; a.up = up; a.factor = factor;
+        a.unit = std::is_same<T, __half>::value ? 1.0f / 32768.0f : 1.0f;
+        int64_t blocks[2] = {0, 0};
+        auto fill = [&](int k, const float* slabs, int splits, int64_t rows, void* g) {
+            if (g == nullptr || rows == 0) return;
+            a.o[k] = {slabs, rows * ldo, ldo, rows, splits, K % 4 == 0 && reinterpret_cast<uintptr_t>(g) % 8 == 0, g};
+            blocks[k] = (rows * ((K + 3) / 4) + 256 * HO_DEPTH - 1) / (256 * HO_DEPTH);
         };
-        if (int e = out(slabs_x, s.x.splits, M, grad_x)) return e;
-        return out(slabs_w, s.w.splits, V, grad_w);
+        fill(0, slabs_x, s.x.splits, M, grad_x);
+        fill(1, slabs_w, s.w.splits, V, grad_w);
+        if (blocks[0] + blocks[1] == 0) return RAVEL_OK;
+        if (blocks[0] + blocks[1] > 2147483647LL) return RAVEL_ERR_UNSUPPORTED;
+        a.first = static_cast<int>(blocks[0]);
+        return launch(k_head_out<T>, dim3(static_cast<unsigned>(blocks[0] + blocks[1])), 256, 0, st, 1, a);
     });
 }
 
