@@ -1,19 +1,22 @@
-"""A RAVEL language model trained on a teacher's top logits, and decoded token by token.
+"""A RAVEL language model trained on a teacher's top logits or on the next tokens, and decoded token by token.
 
-Every dense piece around the event memory runs on this package's kernels:
+Every piece around the event memory runs on this package's kernels:
 
+    token_embedding
     layer_norm -> fused_linear (packed input projection, bias)
                -> memory_lookups (literal addresses of the token ids, latest value)
                -> fused_linear (read-out, residual)
     layer_norm -> fused_linear (feed-forward, SiLU) -> fused_linear (residual)
     layer_norm -> fused_linear (the tied head) -> distill_topk_loss
+               or linear_cross_entropy (the tied head and the loss of the next tokens)
+    AdamW (float32 masters; float32 or 8-bit states)
 
 in bfloat16.  The teacher is a fixed random bigram table whose k largest logits per
 position are known, as they would be from a stored corpus.  Decoding runs the same
 weights one token at a time: ``RavelLayerCache.step`` in place of the lookups, and the
 projections' form for few rows.
 
-    python examples/distill_student.py [--steps 200]
+    python examples/distill_student.py [--steps 200] [--labels] [--state-bits 8]
 """
 from __future__ import annotations
 
@@ -31,6 +34,8 @@ from ravel_lm_b200 import RavelLayerCache, literal_addresses_from_tokens, memory
 from ravel_lm_b200.dense import fused_linear  # noqa: E402
 from ravel_lm_b200.distill import distill_topk_loss  # noqa: E402
 from ravel_lm_b200.glue import layer_norm  # noqa: E402
+from ravel_lm_b200.optim import AdamW  # noqa: E402
+from ravel_lm_b200.vocab import linear_cross_entropy, token_embedding  # noqa: E402
 
 Tensor = torch.Tensor
 
@@ -85,11 +90,18 @@ class Student(torch.nn.Module):
     def head(self, x: Tensor) -> Tensor:
         return fused_linear(layer_norm(x, self.nw, self.nb), self.embed)
 
-    def forward(self, tokens: Tensor) -> Tensor:
-        x = torch.nn.functional.embedding(tokens, self.embed)
+    def body(self, tokens: Tensor) -> Tensor:
+        x = token_embedding(tokens, self.embed)
         for block in self.blocks:
             x = block(x, tokens)
-        return self.head(x)
+        return x
+
+    def forward(self, tokens: Tensor) -> Tensor:
+        return self.head(self.body(tokens))
+
+    def loss(self, tokens: Tensor, targets: Tensor) -> Tensor:
+        """Mean cross entropy of the next tokens (-100: none); the logits are never kept."""
+        return linear_cross_entropy(layer_norm(self.body(tokens), self.nw, self.nb), self.embed, targets)
 
     def caches(self, streams: int) -> list[RavelLayerCache]:
         return [RavelLayerCache.empty(streams, self.heads, self.space, b.payload, device=self.embed.device,
@@ -101,7 +113,7 @@ class Student(torch.nn.Module):
         hash it and the two before it); the caches hold the tokens before it."""
         addresses = literal_addresses_from_tokens(history, address_space=self.space, n_heads=self.heads,
                                                   bos_token_id=0)[:, -1]
-        x = torch.nn.functional.embedding(history[:, -1], self.embed)
+        x = token_embedding(history[:, -1], self.embed)
         for block, cache in zip(self.blocks, caches):
             x = block.step(x, addresses, cache)
         return self.head(x)
@@ -115,18 +127,32 @@ def teacher(vocab: int, k: int, seed: int = 0, device: str = "cuda") -> tuple[Te
     return ids, logits.bfloat16()
 
 
+def next_tokens(ids: Tensor, logits: Tensor, batch: int, length: int, generator: torch.Generator) -> Tensor:
+    """[batch, length + 1] tokens drawn from the teacher, each after the one before it."""
+    out = [torch.randint(1, ids.shape[0], (batch,), generator=generator, device=ids.device)]
+    for _ in range(length):
+        p = torch.softmax(logits[out[-1]].float(), 1)
+        out.append(ids[out[-1]].gather(1, torch.multinomial(p, 1, generator=generator))[:, 0])
+    return torch.stack(out, 1)
+
+
 def train(steps: int = 200, batch: int = 16, length: int = 256, k: int = 16, lr: float = 2e-3, seed: int = 0,
-          report: bool = False) -> tuple[Student, list[float]]:
+          report: bool = False, labels: bool = False, state_bits: int = 32) -> tuple[Student, list[float]]:
+    """On the teacher's top logits, or (``labels``) on the next tokens of sequences drawn from it."""
     torch.manual_seed(seed)
     student = Student().cuda()
     vocab = student.embed.shape[0]
     ids, logits = teacher(vocab, k, seed)
-    opt = torch.optim.AdamW(student.parameters(), lr=lr, weight_decay=0.0)
+    opt = AdamW(student.parameters(), lr=lr, weight_decay=0.0, state_bits=state_bits, max_norm=1.0)
     g = torch.Generator(device="cuda").manual_seed(seed + 1)
     losses = []
     for i in range(steps):
-        tokens = torch.randint(1, vocab, (batch, length), generator=g, device="cuda")
-        loss = distill_topk_loss(student(tokens), ids[tokens], logits[tokens], temperature=2.0)
+        if labels:
+            text = next_tokens(ids, logits, batch, length, g)
+            loss = student.loss(text[:, :-1], text[:, 1:])
+        else:
+            tokens = torch.randint(1, vocab, (batch, length), generator=g, device="cuda")
+            loss = distill_topk_loss(student(tokens), ids[tokens], logits[tokens], temperature=2.0)
         opt.zero_grad(set_to_none=True)
         loss.backward()
         opt.step()
@@ -139,8 +165,10 @@ def train(steps: int = 200, batch: int = 16, length: int = 256, k: int = 16, lr:
 def main() -> None:
     ap = argparse.ArgumentParser(description=__doc__.split("\n\n")[0])
     ap.add_argument("--steps", type=int, default=200)
+    ap.add_argument("--labels", action="store_true", help="train on the next tokens")
+    ap.add_argument("--state-bits", type=int, default=32, choices=(8, 32))
     a = ap.parse_args()
-    student, losses = train(a.steps, report=True)
+    student, losses = train(a.steps, report=True, labels=a.labels, state_bits=a.state_bits)
     print(f"loss {losses[0]:.4f} -> {losses[-1]:.4f}")
     tokens = torch.randint(1, student.embed.shape[0], (4, 16), device="cuda")
     caches = student.caches(4)

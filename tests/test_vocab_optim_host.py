@@ -1,0 +1,189 @@
+"""CPU-only checks of the vocabulary operators' and the optimizer step's boundary: C-ABI refusals before any launch,
+workspace sizes, and the Python functions' refusals (no CPU path)."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+INVALID, WORKSPACE, UNSUPPORTED = 1, 2, 4
+P = 4096  # a pointer that is never followed (16-byte aligned)
+
+
+@pytest.fixture(scope="module")
+def lib():
+    import ravel_lm_b200._lib as L
+    return L.load()
+
+
+def test_embedding_refuses_on_the_host(lib):
+    def fwd(ids=P, it=1, w=P, ldw=8, N=4, V=9, K=8, y=P, dt=0):
+        return lib.ravel_embedding_fwd(ids, it, w, ldw, N, V, K, 1.0, y, dt, None)
+    assert fwd(N=-1) == INVALID and fwd(V=0) == INVALID and fwd(it=7) == INVALID
+    assert fwd(dt=3) == UNSUPPORTED and fwd(N=(1 << 30) + 1) == UNSUPPORTED
+    assert fwd(ids=None) == INVALID and fwd(w=None) == INVALID and fwd(y=None) == INVALID and fwd(ldw=7) == INVALID
+    assert fwd(N=0, ids=None, y=None) == 0 and fwd(K=0) == 0
+
+    def bwd(g=P, ldg=8, N=4, V=9, K=8, dw=P, dt=0, scratch=P, sb=None):
+        sb = lib.ravel_embedding_scratch_bytes(N, V, K) if sb is None else sb
+        return lib.ravel_embedding_bwd(P, 1, g, ldg, N, V, K, 1.0, -1, dw, dt, scratch, sb, None)
+    assert bwd(dw=None) == INVALID and bwd(g=None) == INVALID and bwd(ldg=7) == INVALID
+    assert bwd(scratch=None) == WORKSPACE and bwd(sb=100) == WORKSPACE
+    assert lib.ravel_embedding_scratch_bytes(-1, 9, 8) == 0
+    assert lib.ravel_embedding_scratch_bytes(1 << 20, 1 << 17, 1024) > (1 << 17) + 16 * (1 << 20)
+
+
+def test_cross_entropy_refuses_on_the_host(lib):
+    def fwd(x=P, ldx=64, w=P, ldw=64, t=P, tt=1, M=8, K=64, V=100, red=2, losses=P, out=P, factor=P, sx=P, sw=P, dt=1,
+            scratch=P, sb=1 << 40, work=P, wb=1 << 40):
+        return lib.ravel_linear_ce_fwd(x, ldx, w, ldw, t, tt, M, K, V, -100, red, 0, losses, out, factor, sx, sw, dt,
+                                       scratch, sb, work, wb, None)
+    assert fwd(M=-1) == INVALID and fwd(K=0) == INVALID and fwd(V=0) == INVALID and fwd(tt=5) == INVALID
+    assert fwd(dt=0) == UNSUPPORTED and fwd(V=1 << 30) == UNSUPPORTED
+    assert fwd(x=None) == INVALID and fwd(w=None) == INVALID and fwd(t=None) == INVALID and fwd(losses=None) == INVALID
+    assert fwd(ldx=63) == INVALID and fwd(ldw=63) == INVALID and fwd(ldw=68) == INVALID and fwd(w=P + 2) == INVALID
+    assert fwd(red=3) == INVALID and fwd(out=None) == INVALID and fwd(factor=None) == INVALID
+    assert fwd(red=0) == INVALID                     # single losses have no gradient for an upstream gradient of 1
+    assert fwd(sw=P + 4) == INVALID
+    assert fwd(scratch=None) == WORKSPACE and fwd(sb=64) == WORKSPACE and fwd(wb=64) == WORKSPACE
+    sizes = (ctypes.c_int64 * 3)()
+    assert lib.ravel_linear_ce_slabs(8, 64, 100, sizes) == 0 and sizes[0] >= 1 and sizes[1] >= 1 and sizes[2] == 64
+    assert lib.ravel_linear_ce_slabs(8, 65, 100, sizes) == 0 and sizes[2] == 68
+    assert lib.ravel_linear_ce_slabs(8, 0, 100, sizes) == INVALID
+    # never the logits of every row: at most 512 MB of them, or of 1024 rows
+    for M, V in ((1 << 20, 50000), (1 << 17, 1 << 18)):
+        per_row = 2 * V + 4 * (V // 32 + 1) * 2
+        assert lib.ravel_linear_ce_work_bytes(M, 64, V, 1, 2) <= max((512 << 20), 1024 * per_row) * 1.2
+    assert lib.ravel_linear_ce_scratch_bytes(8, 0, 100) == 0
+
+    def grad(w=P, ldw=64, up=P, M=8, K=64, V=100, factor=P, sx=P, sw=P, dt=1, scratch=P, sb=1 << 40, work=P, wb=1 << 40):
+        return lib.ravel_linear_ce_grad(w, ldw, up, M, K, V, factor, sx, sw, dt, scratch, sb, work, wb, None)
+    assert grad(up=None) == INVALID and grad(factor=None) == INVALID and grad(w=None) == INVALID
+    assert grad(wb=10) == WORKSPACE and grad(dt=3) == UNSUPPORTED
+
+    def bwd(sx=P, sw=P, up=P, factor=P, gx=P, gw=P, dt=1):
+        return lib.ravel_linear_ce_bwd(sx, sw, up, factor, 8, 64, 100, gx, gw, dt, None)
+    assert bwd(sx=None) == INVALID and bwd(sw=None) == INVALID and bwd(factor=None) == INVALID
+    assert bwd(sx=None, sw=None, gx=None, gw=None) == 0
+
+
+def test_adamw_refuses_on_the_host(lib):
+    import ravel_lm_b200._lib as L
+
+    def tensors(**k):
+        t = dict(param=P, grad=P, master=None, exp_avg=P, exp_avg_sq=P, exp_avg_exponents=None, exp_avg_sq_exponents=None,
+                 n=5)
+        t.update(k)
+        return (L.AdamTensor * 1)(L.AdamTensor(**t))
+
+    def go(t=None, count=1, dt=0, bits=32, st=P, lr=1e-3, b1=0.9, b2=0.99, eps=1e-8, mx=0.0, norm=None, scratch=P, sb=1 << 30):
+        return lib.ravel_adamw(t or tensors(), count, dt, bits, st, lr, None, b1, b2, eps, 0.0, mx, norm, None, scratch, sb,
+                               None)
+    assert go(count=-1) == INVALID and go(dt=3) == UNSUPPORTED and go(bits=16) == UNSUPPORTED
+    assert go(st=None) == INVALID and go(b1=1.0) == INVALID and go(b2=-0.1) == INVALID and go(eps=-1.0) == INVALID
+    assert go(mx=-1.0) == INVALID and go(norm=P) == INVALID
+    assert go(tensors(n=-1)) == INVALID and go(tensors(grad=None)) == INVALID and go(tensors(param=None)) == INVALID
+    assert go(tensors(exp_avg=None)) == INVALID
+    assert go(dt=1) == INVALID                                     # a 16-bit parameter without a master
+    assert go(bits=8) == INVALID                                   # 8-bit states without exponents
+    assert go(scratch=None) == WORKSPACE and go(sb=8) == WORKSPACE and go(mx=1.0, sb=64) == WORKSPACE
+    t = tensors()
+    assert lib.ravel_grad_norm(t, 1, 0, None, P, 1 << 30, None) == INVALID
+    assert lib.ravel_grad_norm(t, 1, 0, P, P, 8, None) == WORKSPACE
+    assert lib.ravel_adamw_scratch_bytes(t, 1, 1.0) >= 64 + lib.ravel_grad_norm_scratch_bytes(t, 1)
+    assert lib.ravel_state_values(P, P, -1, 1, P, 0, None) == INVALID
+    assert lib.ravel_state_values(P, P, 4, 1, P, 2, None) == UNSUPPORTED
+    assert lib.ravel_state_values(None, None, 0, 1, None, 0, None) == 0
+
+
+def test_vocab_functions_refuse():
+    from ravel_lm_b200.vocab import linear_cross_entropy, token_embedding
+    ids, w = torch.zeros(3, dtype=torch.long), torch.zeros(5, 8)
+    with pytest.raises(ValueError, match=r"weight \[V, K\]"):
+        token_embedding(ids, w[0])
+    with pytest.raises(ValueError, match=r"weight \[V, K\]"):
+        token_embedding(ids, w[:0])
+    with pytest.raises(TypeError, match="int32 or int64"):
+        token_embedding(ids.float(), w)
+    with pytest.raises(TypeError, match="float32, bfloat16 or float16"):
+        token_embedding(ids, w.double())
+    with pytest.raises(ValueError, match="padding_idx"):
+        token_embedding(ids, w, padding_idx=5)
+    with pytest.raises(ValueError, match="finite"):
+        token_embedding(ids, w, scale=float("inf"))
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        token_embedding(ids, w)
+    x, h = torch.zeros(3, 8).bfloat16(), w.bfloat16()
+    with pytest.raises(ValueError, match="reduction must be"):
+        linear_cross_entropy(x, h, ids, reduction="max")
+    with pytest.raises(ValueError, match=r"x \[..., K\]"):
+        linear_cross_entropy(x, h[:, :4], ids)
+    with pytest.raises(ValueError, match="leading dimensions"):
+        linear_cross_entropy(x, h, ids[:2])
+    with pytest.raises(TypeError, match="bfloat16 or float16"):
+        linear_cross_entropy(x.float(), w, ids)
+    with pytest.raises(TypeError, match="one dtype"):
+        linear_cross_entropy(x, h.half(), ids)
+    with pytest.raises(TypeError, match="int32 or int64"):
+        linear_cross_entropy(x, h, ids.bool())
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        linear_cross_entropy(x, h, ids)
+
+
+def test_optimizer_functions_refuse():
+    from ravel_lm_b200.optim import AdamW, adamw_step, global_norm, state_values
+    p, g, m, v = ([torch.zeros(300)] for _ in range(4))
+    step = torch.zeros(1, dtype=torch.long)
+
+    def go(p=p, g=g, m=m, v=v, step=step, **k):
+        return adamw_step(p, g, m, v, step, **{"lr": 1e-3, **k})
+    with pytest.raises(ValueError, match="at least one"):
+        go([], [], [], [])
+    with pytest.raises(ValueError, match="one length"):
+        go(g=g * 2)
+    with pytest.raises(ValueError, match="masters"):
+        go(masters=p)
+    with pytest.raises(ValueError, match="masters"):
+        go([p[0].half()], [g[0].half()])
+    with pytest.raises(ValueError, match="come together"):
+        go(exp_avg_exponents=m)
+    with pytest.raises(ValueError, match="wrong number"):
+        go(m=[torch.zeros(299)])
+    with pytest.raises(TypeError, match=r"exp_avgs\[0\] must be Byte"):
+        e = [torch.zeros(2, dtype=torch.int8)]
+        go(exp_avg_exponents=e, exp_avg_sq_exponents=e)
+    with pytest.raises(ValueError, match="contiguous"):
+        go([torch.zeros(20, 15).t()], [torch.zeros(15, 20)], [torch.zeros(15, 20)], [torch.zeros(15, 20)])
+    with pytest.raises(ValueError, match="parameter's shape"):
+        go(g=[torch.zeros(3, 100)])
+    with pytest.raises(TypeError, match="parameter's dtype"):
+        go(g=[g[0].half()])
+    with pytest.raises(TypeError, match="one int64"):
+        go(step=step.int())
+    with pytest.raises(TypeError, match="float32"):
+        go(lr=torch.zeros(1, dtype=torch.float64))
+    with pytest.raises(ValueError, match="betas"):
+        go(betas=(1.0, 0.9))
+    with pytest.raises(ValueError, match="negative"):
+        go(lr=-1.0)
+    with pytest.raises(ValueError, match="max_norm"):
+        go(max_norm=0.0)
+    with pytest.raises(ValueError, match="with max_norm only"):
+        go(norm=torch.zeros((), dtype=torch.float64))
+    with pytest.raises(ValueError, match="twice"):
+        go(p * 2, g * 2, m * 2, v * 2)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        go()
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        global_norm(g)
+    with pytest.raises(ValueError, match="at least one"):
+        global_norm([])
+    with pytest.raises(TypeError, match="float32 or bfloat16"):
+        state_values(torch.zeros(4, dtype=torch.uint8), torch.zeros(1, dtype=torch.int8), signed=True, dtype=torch.float16)
+    with pytest.raises(ValueError, match="one exponent per block"):
+        state_values(torch.zeros(4, dtype=torch.uint8), torch.zeros(2, dtype=torch.int8), signed=True)
+    for k in (dict(lr=-1.0), dict(eps=-1.0), dict(weight_decay=-1.0), dict(betas=(0.9, 1.0)), dict(state_bits=16),
+              dict(max_norm=-1.0)):
+        with pytest.raises(ValueError):
+            AdamW([torch.nn.Parameter(torch.zeros(3))], **k)
