@@ -100,7 +100,7 @@ __device__ __forceinline__ void adam_store(T* p, int64_t i, int64_t n, bool vec,
     constexpr int E = 16 / sizeof(T);
     if (vec && i + 8 <= n) {
 #pragma unroll
-        for (int q = 0; q < 8 / E; ++q) store_pack<T, E>(p + i + q * E, from_floats<T, E>(f + q * E));
+        for (int q = 0; q < 8 / E; ++q) store_pack_stream<T, E>(p + i + q * E, from_floats<T, E>(f + q * E));
         return;
     }
 #pragma unroll
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(1024) k_adamw_scalars(const AdamStep a) {
 
 // ------------------------------------------------------------------ the step
 template <typename T, bool EIGHT, int CAP>
-__global__ void __launch_bounds__(32 * AW_WARPS) k_adamw(const __grid_constant__ AdamArgs<CAP> a) {
+__global__ void __launch_bounds__(32 * AW_WARPS, 4) k_adamw(const __grid_constant__ AdamArgs<CAP> a) {
     grid_wait();
     grid_trigger();
     const int lane = threadIdx.x & 31;

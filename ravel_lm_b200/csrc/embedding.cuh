@@ -8,8 +8,9 @@
 //   k_embed          rows gathered and scaled.
 //   k_embed_sum      backward, over the sorted positions (idsort.cuh): a group of threads per range of them; a token
 //                    whose rows lie in one range is finished there, the pieces of the others are kept in float32 and
-//                    their first ranges listed.  The last blocks write the zeros of tokens that do not occur.
-//   k_embed_join     the pieces of a listed token, added in their order.
+//                    their first ranges listed.
+//   k_embed_join     the pieces of a listed token, added in their order; the last blocks, under those chains of loads, write
+//                    the zeros of tokens that do not occur.
 // Sums are float32 in a fixed order without atomics: the same inputs give the same bits.
 // Bound by HBM: N rows read and N (forward) or V (backward) rows written.
 #pragma once
@@ -23,8 +24,9 @@ namespace ravel {
 
 constexpr int EM_THREADS = 256;
 constexpr int EM_ROWS = 4;         // rows in flight per group, forward
-constexpr int EM_DEPTH = 8;        // and backward
-constexpr int EM_ZERO_ROWS = 64;   // vocabulary rows a zeroing block looks through
+constexpr int EM_RING = 12;        // and on their way to a thread, backward
+constexpr size_t EM_SMEM = EM_RING * EM_THREADS * 16, EM_SMEM_ADD = EM_SMEM + EM_RING * EM_THREADS * 4;
+constexpr int EM_ZERO_ROWS = 64;   // vocabulary rows a block looks through for absent ones
 constexpr int EJ_COLS = 128;       // columns of a joining block: 32 threads of 4
 constexpr int EJ_GROUPS = 8;       // groups that share a long token's pieces
 
@@ -45,7 +47,7 @@ struct EmbedArgs {
     int64_t K4;
     int* list;                 // [0]: how many; then the ranges in which a token begins that goes on
     int ranges, range;         // positions per range
-    int sum_blocks;
+    int join_blocks;           // of k_embed_join; the others write zeros
     int tx;                    // threads per group, a power of two from 32 on
     // ADD: the sums of weighted rows are added to float32 rows
     const float4* weight;      // [N]: each row's weight is its third component, negated
@@ -126,25 +128,67 @@ __device__ __forceinline__ void embed_put(const EmbedArgs& a, uint32_t id, int64
     }
 }
 
+// A range's rows as they pass a thread: its 16 bytes of each come by cp.async, EM_RING rows ahead, into a ring that
+// only this thread reads (no barrier).  With eight rows in registers instead two blocks fit an SM and a pass over
+// 131072 x 1024 took 94 us whatever the range, 62 being its bytes.
+template <typename T, int VEC, bool ADD>
+struct EmbedRows {
+    static constexpr bool RING = VEC * sizeof(T) == 16;
+    const EmbedArgs& a;
+    unsigned char* ring;
+    float* weights;
+    const uint2* key;  // of the range's first row
+    const T* g;        // the thread's column of row 0
+    int n;
+    uint32_t next;     // the position of the next row to be fetched
+
+    __device__ __forceinline__ EmbedRows(const EmbedArgs& a_, unsigned char* smem, const uint2* key_, const T* g_, int n_)
+        : a(a_), ring(smem + threadIdx.x * 16),
+          weights(reinterpret_cast<float*>(smem + EM_RING * EM_THREADS * 16) + threadIdx.x), key(key_), g(g_), n(n_) {
+        if constexpr (RING) {
+            next = __ldg(&key[0].y);
+#pragma unroll 4
+            for (int k = 0; k < EM_RING; ++k) fetch(k);
+        }
+    }
+    __device__ __forceinline__ void fetch(int k) {
+        if (k < n) {
+            const int slot = k % EM_RING;
+            const uint32_t pos = next;
+            if (k + 1 < n) next = __ldg(&key[k + 1].y);
+            cp_async16_zfill(static_cast<uint32_t>(__cvta_generic_to_shared(ring + slot * (EM_THREADS * 16))),
+                             g + static_cast<int64_t>(pos) * a.ldg, true);
+            if constexpr (ADD)
+                cp_async4(static_cast<uint32_t>(__cvta_generic_to_shared(weights + slot * EM_THREADS)), &a.weight[pos].z);
+        }
+        cp_async_commit();
+    }
+    // row k (in order) added to s
+    __device__ __forceinline__ void add(int k, float (&s)[VEC]) {
+        float f[VEC], w = 0.0f;
+        if constexpr (RING) {
+            cp_async_wait<EM_RING - 1>();
+            const int slot = k % EM_RING;
+            to_floats<T, VEC>(*reinterpret_cast<const Pack<T, VEC>*>(ring + slot * (EM_THREADS * 16)), f);
+            if constexpr (ADD) w = weights[slot * EM_THREADS];
+        } else {
+            const uint32_t pos = __ldg(&key[k].y);
+            to_floats<T, VEC>(load_pack<T, VEC>(g + static_cast<int64_t>(pos) * a.ldg), f);
+            if constexpr (ADD) w = a.weight[pos].z;
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) s[e] = ADD ? fmaf(-w, f[e], s[e]) : s[e] + f[e];
+        if constexpr (RING) fetch(k + EM_RING);
+    }
+};
+
 template <typename T, int VEC, bool ADD>
 __global__ void __launch_bounds__(EM_THREADS) k_embed_sum(const EmbedArgs a) {
+    extern __shared__ __align__(16) unsigned char em_smem[];
     grid_wait();
     grid_trigger();
     const int64_t units = a.K / VEC;
     const int tx = threadIdx.x & (a.tx - 1), ty = threadIdx.x / a.tx, groups = EM_THREADS / a.tx;
-    if (static_cast<int>(blockIdx.x) >= a.sum_blocks) {
-        // zeros of the tokens that do not occur, a group per vocabulary row
-        const int64_t v0 = static_cast<int64_t>(static_cast<int>(blockIdx.x) - a.sum_blocks) * EM_ZERO_ROWS;
-        float z[VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) z[e] = 0.0f;
-        const Pack<T, VEC> zero = from_floats<T, VEC>(z);
-        for (int64_t v = v0 + ty; v < v0 + EM_ZERO_ROWS && v < a.V; v += groups) {
-            if (a.present[v]) continue;
-            for (int64_t u = tx; u < units; u += a.tx) store_pack<T, VEC>(static_cast<T*>(a.out) + v * a.K + u * VEC, zero);
-        }
-        return;
-    }
     const int r = static_cast<int>(blockIdx.x) * groups + ty, n = *a.live;
     const int i0 = r * a.range, i1 = min(i0 + a.range, n);
     if (r >= a.ranges || i0 >= n) return;
@@ -154,7 +198,6 @@ __global__ void __launch_bounds__(EM_THREADS) k_embed_sum(const EmbedArgs a) {
     const bool goes = i1 < n && keys[i1].x == last;        // the last one goes on
     const bool one = first == last;                        // the range has one token only
     if (tx == 0 && goes && !(one && began)) a.list[1 + atomicAdd(a.list, 1)] = r;  // any order: the joins are apart
-    const T* const g = static_cast<const T*>(a.g);
     float* const part = a.part + static_cast<int64_t>(r) * 2 * a.K4;
     for (int64_t u = tx; u < units; u += a.tx) {
         float s[VEC];
@@ -162,34 +205,21 @@ __global__ void __launch_bounds__(EM_THREADS) k_embed_sum(const EmbedArgs a) {
         for (int e = 0; e < VEC; ++e) s[e] = 0.0f;
         uint32_t cur = first;
         bool head = began;  // the running sum belongs to a token that began before this range
-        for (int b = i0; b < i1; b += EM_DEPTH) {
-            uint32_t id[EM_DEPTH];
-            Pack<T, VEC> row[EM_DEPTH];
-            float weight[ADD ? EM_DEPTH : 1];
+        EmbedRows<T, VEC, ADD> rows(a, em_smem, keys + i0, static_cast<const T*>(a.g) + u * VEC, i1 - i0);
+        uint32_t id = first;
+#pragma unroll EmbedRows<T, VEC, ADD>::RING ? 4 : 8
+        for (int k = 0; k < i1 - i0; ++k) {
+            const uint32_t now = id;
+            if (k + 1 < i1 - i0) id = __ldg(&keys[i0 + k + 1].x);
+            if (now != cur) {  // the token ends inside the range
+                if (head) embed_piece<VEC>(part + u * VEC, s);
+                else embed_put<T, VEC, ADD>(a, cur, u, s);
+                head = false;
+                cur = now;
 #pragma unroll
-            for (int k = 0; k < EM_DEPTH; ++k) {
-                if (b + k >= i1) continue;
-                const uint2 key = __ldg(keys + b + k);
-                id[k] = key.x;
-                if constexpr (ADD) weight[k] = -a.weight[key.y].z;
-                row[k] = load_pack<T, VEC>(g + static_cast<int64_t>(key.y) * a.ldg + u * VEC);
+                for (int e = 0; e < VEC; ++e) s[e] = 0.0f;
             }
-#pragma unroll
-            for (int k = 0; k < EM_DEPTH; ++k) {
-                if (b + k >= i1) continue;
-                if (id[k] != cur) {  // the token ends inside the range
-                    if (head) embed_piece<VEC>(part + u * VEC, s);
-                    else embed_put<T, VEC, ADD>(a, cur, u, s);
-                    head = false;
-                    cur = id[k];
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) s[e] = 0.0f;
-                }
-                float f[VEC];
-                to_floats<T, VEC>(row[k], f);
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) s[e] = ADD ? fmaf(weight[ADD ? k : 0], f[e], s[e]) : s[e] + f[e];
-            }
+            rows.add(k, s);
         }
         // the last token: a piece where it began before the range or goes on after it
         if (head || goes) embed_piece<VEC>(part + (head ? 0 : a.K4) + u * VEC, s);
@@ -197,55 +227,108 @@ __global__ void __launch_bounds__(EM_THREADS) k_embed_sum(const EmbedArgs a) {
     }
 }
 
+// Zeros of the tokens that do not occur, a warp per vocabulary row, EM_ZERO_ROWS rows a block.
+template <typename T>
+__device__ __forceinline__ void embed_zeros(const EmbedArgs& a, int block) {
+    const int lane = threadIdx.x & 31;
+    constexpr int E = 16 / sizeof(T);
+    const int64_t v0 = static_cast<int64_t>(block) * EM_ZERO_ROWS;
+    for (int64_t v = v0 + (threadIdx.x >> 5); v < v0 + EM_ZERO_ROWS && v < a.V; v += 32 * EJ_GROUPS / 32) {
+        if (a.present[v]) continue;
+        T* const o = static_cast<T*>(a.out) + v * a.K;
+        const int64_t head = min(a.K, static_cast<int64_t>((16 - (reinterpret_cast<uintptr_t>(o) & 15)) & 15) / sizeof(T));
+        const int64_t vecs = (a.K - head) / E;
+        for (int64_t u = lane; u < head; u += 32) o[u] = round_to<T>(0.0f);
+        for (int64_t u = lane; u < vecs; u += 32) __stcs(reinterpret_cast<uint4*>(o + head) + u, make_uint4(0u, 0u, 0u, 0u));
+        for (int64_t u = head + vecs * E + lane; u < a.K; u += 32) o[u] = round_to<T>(0.0f);
+    }
+}
+
+// The sum of a listed token's columns col .. col + 3 into the output.
+template <typename T, bool ADD>
+__device__ __forceinline__ void embed_finish(const EmbedArgs& a, uint32_t v, int64_t col, const float4& s) {
+    const float f[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (col + e >= a.K) continue;
+        if constexpr (ADD) a.add[v * a.ldo + col + e] += f[e];
+        else static_cast<T*>(a.out)[v * a.K + col + e] = round_to<T>(f[e] * a.scale);
+    }
+}
+__device__ __forceinline__ void add4(float4& s, const float4& w) {
+    s.x += w.x; s.y += w.y; s.z += w.z; s.w += w.w;
+}
+
 // A listed range's last token: its piece there (the second slot) and the first slots of the ranges that follow, as far
-// as the token reaches, a block per EJ_COLS columns.  Groups of the block take every EJ_GROUPS-th piece, their
-// sums are added in order.
+// as the token reaches, added in order, EJ_COLS columns at a time.  A warp does an item (a token's columns) of up to
+// 32 following pieces, a lane 4 columns; a block together the few items with more: its warps take every
+// EJ_GROUPS-th piece.  Most tokens have two or three pieces, and a block each left seven warps idle (131072 x 1024: 26 us).
 template <typename T, bool ADD>
 __global__ void __launch_bounds__(32 * EJ_GROUPS) k_embed_join(const EmbedArgs a) {
     __shared__ float4 red[EJ_GROUPS][32];
     grid_wait();
     grid_trigger();
+    if constexpr (!ADD) {
+        if (static_cast<int>(blockIdx.x) >= a.join_blocks) return embed_zeros<T>(a, blockIdx.x - a.join_blocks);
+    }
+    const int step = a.join_blocks;
     const int slabs = static_cast<int>((a.K + EJ_COLS - 1) / EJ_COLS), items = a.list[0] * slabs, n = *a.live;
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
-    for (int item = blockIdx.x; item < items; item += gridDim.x) {
-        const int r = a.list[1 + item / slabs];
-        const int64_t col = static_cast<int64_t>(item % slabs) * EJ_COLS + x * 4;
-        const int i1 = (r + 1) * a.range;
+    const int64_t part_ld = 2 * a.K4;
+    auto first_of = [&](int item) { return (a.list[1 + item / slabs] + 1) * static_cast<int64_t>(a.range); };
+    // the range `k` after the listed one starts with the token
+    auto reaches = [&](int64_t i1, uint32_t v, int k) {
+        const int64_t i = i1 + static_cast<int64_t>(k) * a.range;
+        return i < n && a.keys[i].x == v;
+    };
+    for (int item = blockIdx.x * EJ_GROUPS + y; item < items; item += step * EJ_GROUPS) {
+        const int64_t i1 = first_of(item), col = static_cast<int64_t>(item % slabs) * EJ_COLS + x * 4;
         const uint32_t v = a.keys[i1].x;
-        int pieces = 0;  // of the following ranges: those that start with the token
-        for (bool more = true; more; ) {
-            const int64_t i = static_cast<int64_t>(i1) + static_cast<int64_t>(pieces + x) * a.range;
-            const unsigned no = __ballot_sync(0xffffffffu, !(i < n && a.keys[i].x == v));
-            pieces += no ? __ffs(no) - 1 : 32;
-            more = no == 0u;
-        }
-        float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (col < a.K4) {
-            const float* const p = a.part + static_cast<int64_t>(r) * 2 * a.K4 + col;
-            if (y == 0) s = *reinterpret_cast<const float4*>(p + a.K4);
+        const unsigned no = __ballot_sync(0xffffffffu, !reaches(i1, v, x));
+        if (no == 0u && reaches(i1, v, 32)) continue;  // the same for the whole warp
+        const int pieces = no ? __ffs(no) - 1 : 32;
+        if (col >= a.K4) continue;
+        const float* const p = a.part + (i1 / a.range - 1) * part_ld + col;
+        float4 s = *reinterpret_cast<const float4*>(p + a.K4);
 #pragma unroll 4
-            for (int k = y; k < pieces; k += EJ_GROUPS) {
-                const float4 w = *reinterpret_cast<const float4*>(p + static_cast<int64_t>(k + 1) * 2 * a.K4);
-                s.x += w.x; s.y += w.y; s.z += w.z; s.w += w.w;
-            }
+        for (int k = 1; k <= pieces; ++k) add4(s, *reinterpret_cast<const float4*>(p + k * part_ld));
+        embed_finish<T, ADD>(a, v, col, s);
+    }
+    for (int item0 = blockIdx.x; item0 < items; item0 += step * 32) {
+        // a lane looks at one of this block's next 32 items
+        const int mine = item0 + x * step;
+        bool longer = false;
+        if (mine < items) {
+            const int64_t i1 = first_of(mine);
+            longer = reaches(i1, a.keys[i1].x, 32);
         }
-        red[y][x] = s;
-        __syncthreads();
-        if (y == 0) {
-#pragma unroll
-            for (int k = 1; k < EJ_GROUPS; ++k) {
-                const float4 w = red[k][x];
-                s.x += w.x; s.y += w.y; s.z += w.z; s.w += w.w;
+        unsigned todo = __ballot_sync(0xffffffffu, longer);  // the same in every warp
+        for (; todo != 0u; todo &= todo - 1u) {
+            const int item = item0 + (__ffs(todo) - 1) * step;
+            const int64_t i1 = first_of(item), col = static_cast<int64_t>(item % slabs) * EJ_COLS + x * 4;
+            const uint32_t v = a.keys[i1].x;
+            int pieces = 32;
+            for (bool more = true; more;) {
+                const unsigned no = __ballot_sync(0xffffffffu, !reaches(i1, v, pieces + x));
+                pieces += no ? __ffs(no) - 1 : 32;
+                more = no == 0u;
             }
-            const float f[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (col + e >= a.K) continue;
-                if constexpr (ADD) a.add[v * a.ldo + col + e] += f[e];
-                else static_cast<T*>(a.out)[v * a.K + col + e] = round_to<T>(f[e] * a.scale);
+            float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (col < a.K4) {
+                const float* const p = a.part + (i1 / a.range - 1) * part_ld + col;
+                if (y == 0) s = *reinterpret_cast<const float4*>(p + a.K4);
+#pragma unroll 8
+                for (int k = y + 1; k <= pieces; k += EJ_GROUPS) add4(s, *reinterpret_cast<const float4*>(p + k * part_ld));
             }
+            red[y][x] = s;
+            __syncthreads();
+            if (y == 0 && col < a.K4) {
+#pragma unroll
+                for (int k = 1; k < EJ_GROUPS; ++k) add4(s, red[k][x]);
+                embed_finish<T, ADD>(a, v, col, s);
+            }
+            __syncthreads();
         }
-        __syncthreads();
     }
 }
 

@@ -40,12 +40,13 @@ int embed_tx(int64_t units) {
     return tx;
 }
 
-// Positions per range of the backward's sums: short enough for two waves of groups, no shorter than 16 (a piece
-// costs as much memory traffic as four 16-bit rows).
+// Positions per range of the backward's sums: short enough that every SM has two blocks, no shorter than 16 (a piece
+// costs as much memory traffic as four 16-bit rows).  131072 x 1024 in ranges of 32 / 64 / 128 / 256: sums 64 / 66 / 68 /
+// 82 us, joins (with the zeros) 40 / 28 / 22 / 19.
 int embed_range(int64_t N, int tx) {
     const int64_t groups = static_cast<int64_t>(sm_count()) * 2 * (EM_THREADS / tx);
-    int r = 64;
-    while (r > 16 && N / r < groups * 2) r /= 2;
+    int r = 128;
+    while (r > 16 && N / r < groups) r /= 2;
     return r;
 }
 
@@ -94,7 +95,7 @@ int sort_ids(IdsArgs a, const IdsLayout& l, char* mem, cudaStream_t st) {
 }
 
 struct EmbedLayout {
-    size_t off_present, off_list, off_part, off_ids, total, zeroed;
+    size_t off_present, off_list, off_part, off_ids, total;
     int64_t K4;
     IdsLayout ids;
 };
@@ -106,7 +107,6 @@ EmbedLayout embed_layout(int64_t N, int64_t V, int64_t K) {
     l.ids = ids_layout(N, V);
     l.off_present = 0;
     l.off_list = up256(static_cast<size_t>(V));
-    l.zeroed = l.off_list + sizeof(int);
     l.off_part = up256(l.off_list + (ranges + 1) * sizeof(int));
     l.off_ids = l.off_part + up256(ranges * 2 * static_cast<size_t>(l.K4) * sizeof(float));
     l.total = l.off_ids + l.ids.total;
@@ -120,14 +120,16 @@ int launch_sums(EmbedArgs a, bool vec, cudaStream_t st) {
     a.range = embed_range(a.N, a.tx);
     a.ranges = static_cast<int>((a.N + a.range - 1) / a.range);
     const int groups = EM_THREADS / a.tx;
-    a.sum_blocks = (a.ranges + groups - 1) / groups;
-    const int64_t zero_blocks = ADD ? 0 : (a.V + EM_ZERO_ROWS - 1) / EM_ZERO_ROWS;
     const auto kern = vec ? k_embed_sum<T, 16 / sizeof(T), ADD> : k_embed_sum<T, 1, ADD>;
-    if (int e = launch(kern, dim3(static_cast<unsigned>(a.sum_blocks + zero_blocks)), EM_THREADS, 0, st, 1, a)) return e;
-    if (a.ranges < 2) return RAVEL_OK;
+    const size_t smem = vec ? (ADD ? EM_SMEM_ADD : EM_SMEM) : 0;
+    if (int e = set_smem(kern, smem)) return e;
+    if (int e = launch(kern, dim3(static_cast<unsigned>((a.ranges + groups - 1) / groups)), EM_THREADS, smem, st, 1, a))
+        return e;
     const int64_t items = static_cast<int64_t>(a.ranges - 1) * ((a.K + EJ_COLS - 1) / EJ_COLS);
-    return launch(k_embed_join<T, ADD>, dim3(static_cast<unsigned>(std::min<int64_t>(items, int64_t{sm_count()} * 8))),
-                  32 * EJ_GROUPS, 0, st, 1, a);
+    a.join_blocks = static_cast<int>(std::min<int64_t>((items + EJ_GROUPS - 1) / EJ_GROUPS, int64_t{sm_count()} * 8));
+    const int64_t zero_blocks = ADD ? 0 : (a.V + EM_ZERO_ROWS - 1) / EM_ZERO_ROWS;
+    if (a.join_blocks + zero_blocks == 0) return RAVEL_OK;
+    return launch(k_embed_join<T, ADD>, dim3(static_cast<unsigned>(a.join_blocks + zero_blocks)), 32 * EJ_GROUPS, 0, st, 1, a);
 }
 
 int embed_check(int64_t N, int64_t V, int64_t K, int ids_dtype, int dtype) {
@@ -377,11 +379,11 @@ template <typename T>
 int head_targets(const HeadCall& c, const int32_t* target, const float4* stat, const char* clean, char* work) {
     char* const e = work + c.l.off_embed;
     const EmbedLayout& l = c.l.embed;
-    if (cudaMemsetAsync(e + l.off_list, 0, sizeof(int), c.st) != cudaSuccess) return RAVEL_ERR_CUDA;
     IdsArgs q;
     std::memset(&q, 0, sizeof(q));
     q.ids = target;
     q.N = c.M; q.V = c.V; q.pad = -1;
+    q.zero = reinterpret_cast<int*>(e + l.off_list);
     q.err = c.words.error;
     if (int rc = sort_ids(q, l.ids, e + l.off_ids, c.st)) return rc;
     EmbedArgs a;
@@ -554,13 +556,13 @@ int ravel_embedding_bwd(const void* ids, int ids_dtype, const void* grad_y, int6
     char* const s = static_cast<char*>(scratch);
     DeviceWords words;
     if (int e = device_words(&words)) return e;
-    if (cudaMemsetAsync(s, 0, l.zeroed, st) != cudaSuccess) return RAVEL_ERR_CUDA;
     IdsArgs q;
     std::memset(&q, 0, sizeof(q));
     q.ids = ids; q.ids64 = ids_dtype == RAVEL_I64;
     q.N = N; q.V = V; q.pad = padding_idx; q.strict = 1;
     q.err = words.error;
     q.present = reinterpret_cast<unsigned char*>(s + l.off_present);
+    q.zero = reinterpret_cast<int*>(s + l.off_list);
     if (int e = sort_ids(q, l.ids, s + l.off_ids, st)) return e;
     EmbedArgs a;
     std::memset(&a, 0, sizeof(a));
