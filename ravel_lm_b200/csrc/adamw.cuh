@@ -4,9 +4,8 @@
 //   m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2
 //   p = p (1 - lr wd) - lr / (1 - b1^t)  m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
-// in float32 (p: the float32 master of a 16-bit parameter, which gets its rounding in the same pass).  The states'
-// operations are rounded one by one, so that a state does not depend on what a compiler contracts; the root and
-// the reciprocal are the hardware's approximations (2^-22 of a step that is a small part of p).
+// in float32 (p: the float32 master of a 16-bit parameter, which gets its rounding in the same pass), two elements an
+// instruction; the root and the reciprocal are the hardware's approximations (2^-22 of a step that is a small part of p).
 //
 //   k_grad_norm      sums of squares in float64, a part per block (any float32 gradient's square is finite there, and the
 //                    sum is the same to float32 whatever its order); k_norm_total adds the parts for callers of the norm.
@@ -137,33 +136,57 @@ constexpr int AW_NAN = -128;  // the exponent of a block that stands for NaN
 __device__ __forceinline__ float pow2_of(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 __device__ __forceinline__ float scale8(int e) { return e == AW_NAN ? __int_as_float(0x7fc00000) : pow2_of(e); }
 
-// The value of byte k of c (its block's scale: scale8 of the exponent).
-template <int BIAS>
-__device__ __forceinline__ float value8(uint32_t c, int k, float scale) {
-    uint32_t b;
-    if constexpr (BIAS == 15) {
-        const uint32_t t = c << (24 - 8 * k);  // the byte on top: its sign is float32's
-        b = ((t >> 4) & 0x07f00000u) | (t & 0x80000000u);
-    } else {
-        b = (k < 3 ? c << (k < 3 ? 20 - 8 * k : 0) : c >> 4) & 0x0ff00000u;
-    }
-    return __fmul_rn(__fmul_rn(__uint_as_float(b), pow2_of(127 - BIAS)), scale);
+// Two floats an instruction (each rounded as by itself).
+__device__ __forceinline__ uint64_t two(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void split(uint64_t v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
 }
 
-// A block's exponent from its values' largest magnitude, as bits (a NaN's are above infinity's).  Values past
+// Byte k of c as float32 bits: its value times 2^(BIAS - 127).  Shifts to the left are products, on the pipe that is idle.
+template <int BIAS>
+__device__ __forceinline__ float bits8(uint32_t c, int k) {
+    const uint32_t u = k < 3 ? c * (1u << (k < 3 ? 20 - 8 * k : 0)) : c >> 4;  // the byte at bits 27 .. 20
+    if constexpr (BIAS == 31) return __uint_as_float(u & 0x0ff00000u);
+    const uint32_t t = k < 3 ? u * 16u : c;  // and on top, for its sign
+    return __uint_as_float((u & 0x07f00000u) | (t & 0x80000000u));
+}
+// The values of 8 codes (their block's scale: scale8 of the exponent).
+template <int BIAS>
+__device__ __forceinline__ void values8(uint32_t lo, uint32_t hi, float scale, float (&f)[8]) {
+    const uint64_t up = two(pow2_of(127 - BIAS), pow2_of(127 - BIAS)), s = two(scale, scale);
+#pragma unroll
+    for (int k = 0; k < 8; k += 2) {
+        const uint32_t c = k < 4 ? lo : hi;
+        split(mul2(mul2(two(bits8<BIAS>(c, k & 3), bits8<BIAS>(c, (k & 3) + 1)), up), s), f[k], f[k + 1]);
+    }
+}
+
+// A block's exponent from its values' largest magnitude; odd: some value is no finite number.  Values past
 // 1.875 2^127 have no code: AW_NAN, as for infinity.
-__device__ __forceinline__ int block_exponent(uint32_t top) {
-    const uint32_t t = __reduce_max_sync(0xffffffffu, top);
+__device__ __forceinline__ int block_exponent(float top, bool odd) {
+    const uint32_t t = __reduce_max_sync(0xffffffffu, odd ? 0x7fffffffu : __float_as_uint(top));  // they order as their bits
     if (t > 0x7f700000u) return AW_NAN;
     const int e = max(static_cast<int>(t >> 23) - 127, -126);
     return __uint_as_float(t) > __fmul_rn(pow2_of(e), 1.875f) ? e + 1 : e;
-}
-
-// x rounded to a code, up or down by 16 random bits (r: those above bit 4, and 8).
-template <int BIAS>
-__device__ __forceinline__ uint32_t code8(float x, float down1, float down2, uint32_t r) {
-    const uint32_t t = __float_as_uint(__fmul_rn(__fmul_rn(x, down1), down2)) + r;  // a sign stays on top
-    return BIAS == 31 ? t >> 20 : ((t >> 20) & 0x7Fu) | ((t >> 24) & 0x80u);
 }
 
 __device__ __forceinline__ float sqrt_approx(float x) {
@@ -184,25 +207,40 @@ __device__ __forceinline__ uint32_t mix32(uint32_t i) {
     return i ^ (i >> 16);
 }
 
-// 8 values of a lane as codes, their block's exponent into *e; the random bits are h's low or high halves.
+// 8 values of a lane as codes, their block's exponent into *e.  Each is rounded up or down by 16 random bits, h's low
+// or high half, and half of one more, added below the code's last place.  The integer and logic pipe, half as fast as the
+// multiply-add pipe, bounds the 8-bit step: the value's bits go up by 4 (the code becomes the top byte) and meet the random
+// ones in one integer multiply-add, one byte permutation lays out the latter, and sums of x * 0 find what is not finite.
 template <int BIAS>
 __device__ __forceinline__ uint64_t quantise8(const float (&x)[8], const uint32_t (&h)[8], signed char* e, int lane) {
-    uint32_t top = 0u;
+    float top = 0.0f;
+    uint64_t odd = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(x[k]) & 0x7fffffffu);
-    const int b = block_exponent(top);
+    for (int k = 0; k < 8; k += 2) {
+        top = fmaxf(top, fmaxf(fabsf(x[k]), fabsf(x[k + 1])));
+        odd = fma2(two(x[k], x[k + 1]), 0, odd);
+    }
+    float odd0, odd1;
+    split(odd, odd0, odd1);
+    const int b = block_exponent(top, !(odd0 + odd1 == 0.0f));
     if (lane == 0) *e = static_cast<signed char>(b);
     if (b == AW_NAN) return 0;
     const int s = BIAS - 127 - b, s1 = s >> 1;  // -239 <= s <= 30, in two steps
-    const float d1 = pow2_of(s1), d2 = pow2_of(s - s1);
-    uint32_t c[8];
+    const uint64_t d1 = two(pow2_of(s1), pow2_of(s1)), d2 = two(pow2_of(s - s1), pow2_of(s - s1));
+    uint32_t c[8];  // the code in the top byte
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const uint32_t r = BIAS == 15 ? (h[k] & 0xFFFFu) * 16u + 8u : ((h[k] >> 12) & 0xFFFF0u) + 8u;
-        c[k] = code8<BIAS>(x[k], d1, d2, r);
+    for (int k = 0; k < 8; k += 2) {
+        float y[2];
+        split(mul2(mul2(two(x[k], x[k + 1]), d1), d2), y[0], y[1]);
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            const uint32_t r = __byte_perm(h[k + q], 0x80u, BIAS == 15 ? 0x5104 : 0x5324);
+            const uint32_t t = __float_as_uint(y[q]) * 16u + r;
+            c[k + q] = BIAS == 31 ? t : (t & 0x7fffffffu) | (__float_as_uint(y[q]) & 0x80000000u);
+        }
     }
-    const uint32_t lo = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
-    const uint32_t hi = __byte_perm(__byte_perm(c[4], c[5], 0x0040), __byte_perm(c[6], c[7], 0x0040), 0x5410);
+    const uint32_t lo = __byte_perm(__byte_perm(c[0], c[1], 0x0073), __byte_perm(c[2], c[3], 0x0073), 0x5410);
+    const uint32_t hi = __byte_perm(__byte_perm(c[4], c[5], 0x0073), __byte_perm(c[6], c[7], 0x0073), 0x5410);
     return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
@@ -288,72 +326,95 @@ __global__ void __launch_bounds__(1024) k_adamw_scalars(const AdamStep a) {
 }
 
 // ------------------------------------------------------------------ the step
+// The step of 8 elements, in pairs.  A subnormal v counts as the least normal number where eps = 0, so that nothing but a
+// zero v divides by zero.
+template <int CAP>
+__device__ __forceinline__ void adam_update(const AdamArgs<CAP>& a, const AdamScalars& s, const float (&g)[8], float (&m)[8],
+                                            float (&v)[8], float (&p)[8]) {
+    const uint64_t clip = two(s.clip, s.clip), decay = two(s.decay, s.decay), c1 = two(-s.c1, -s.c1), c2 = two(s.c2, s.c2);
+    const uint64_t b1 = two(a.b1, a.b1), omb1 = two(a.omb1, a.omb1), b2 = two(a.b2, a.b2), omb2 = two(a.omb2, a.omb2);
+    const uint64_t eps = two(a.eps, a.eps);
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        uint64_t g2 = two(g[e], g[e + 1]);
+        if (a.clipped) g2 = mul2(g2, clip);
+        split(fma2(g2, omb1, mul2(two(m[e], m[e + 1]), b1)), m[e], m[e + 1]);
+        split(fma2(mul2(g2, g2), omb2, mul2(two(v[e], v[e + 1]), b2)), v[e], v[e + 1]);
+        float r[2], d[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+            r[q] = sqrt_approx(a.eps != 0.0f || v[e + q] == 0.0f ? v[e + q] : fmaxf(v[e + q], 1.17549435e-38f));
+        split(fma2(two(r[0], r[1]), c2, eps), d[0], d[1]);
+        const uint64_t q2 = mul2(two(m[e], m[e + 1]), two(rcp_approx(d[0]), rcp_approx(d[1])));
+        split(fma2(c1, q2, mul2(two(p[e], p[e + 1]), decay)), p[e], p[e + 1]);
+    }
+}
+
+// Where a warp's block of 256 elements lies.
+struct AdamPlace {
+    int k;          // the tensor
+    int64_t block;  // of it
+    int64_t i, n;   // the lane's first element; the tensor's
+    bool live, whole;  // the block exists; the lane's 8 elements do, on 16 bytes
+    template <int CAP>
+    __device__ __forceinline__ AdamPlace(const AdamArgs<CAP>& a, int chunk) {
+        live = chunk < a.first[a.count];
+        k = live ? adam_tensor(a, chunk) : 0;
+        n = a.t[k].n;
+        block = static_cast<int64_t>(chunk - a.first[k]) * AW_WARPS + (threadIdx.x >> 5);
+        i = block * 256 + (threadIdx.x & 31) * 8;
+        live = live && block * 256 < n;
+        whole = live && a.vec[k] && i + 8 <= n;
+    }
+};
+
 template <typename T, bool EIGHT, int CAP>
 __global__ void __launch_bounds__(32 * AW_WARPS, 4) k_adamw(const __grid_constant__ AdamArgs<CAP> a) {
     grid_wait();
     grid_trigger();
-    const int lane = threadIdx.x & 31;
-    const int k = adam_tensor(a, blockIdx.x);
-    const AdamTensor& t = a.t[k];
-    const int64_t block = static_cast<int64_t>(static_cast<int>(blockIdx.x) - a.first[k]) * AW_WARPS + (threadIdx.x >> 5);
-    const int64_t i = block * 256 + lane * 8, n = t.n;
-    if (block * 256 >= n) return;
-    const bool vec = a.vec[k];
+    const AdamPlace at(a, blockIdx.x);
+    if (!at.live) return;
+    const int64_t i = at.i, n = at.n;
+    const AdamTensor& t = a.t[at.k];
+    float* const master = sizeof(T) == 4 ? static_cast<float*>(t.p) : t.master;
     float g[8], m[8], v[8], p[8];
-    adam_load(static_cast<const T*>(t.g), i, n, vec, g);
+    adam_load(static_cast<const T*>(t.g), i, n, at.whole, g);
     uint64_t mc = 0, vc = 0;
     int me = 0, ve = 0;
     if constexpr (EIGHT) {
-        mc = adam_codes(static_cast<const unsigned char*>(t.m), i, n, vec);
-        vc = adam_codes(static_cast<const unsigned char*>(t.v), i, n, vec);
-        me = t.me[block];
-        ve = t.ve[block];
+        mc = adam_codes(static_cast<const unsigned char*>(t.m), i, n, at.whole);
+        vc = adam_codes(static_cast<const unsigned char*>(t.v), i, n, at.whole);
+        me = t.me[at.block];
+        ve = t.ve[at.block];
     } else {
-        adam_load(static_cast<const float*>(t.m), i, n, vec, m);
-        adam_load(static_cast<const float*>(t.v), i, n, vec, v);
+        adam_load(static_cast<const float*>(t.m), i, n, at.whole, m);
+        adam_load(static_cast<const float*>(t.v), i, n, at.whole, v);
     }
-    if constexpr (sizeof(T) == 4) adam_load(static_cast<const float*>(t.p), i, n, vec, p);
-    else adam_load(static_cast<const float*>(t.master), i, n, vec, p);
+    adam_load(master, i, n, at.whole, p);
     const AdamScalars s = *a.s;
     if constexpr (EIGHT) {
-        const float ms = scale8(me), vs = scale8(ve);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            m[e] = value8<15>(static_cast<uint32_t>(mc >> (e < 4 ? 0 : 32)), e & 3, ms);
-            v[e] = value8<31>(static_cast<uint32_t>(vc >> (e < 4 ? 0 : 32)), e & 3, vs);
-        }
+        values8<15>(static_cast<uint32_t>(mc), static_cast<uint32_t>(mc >> 32), scale8(me), m);
+        values8<31>(static_cast<uint32_t>(vc), static_cast<uint32_t>(vc >> 32), scale8(ve), v);
     }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const float ge = a.clipped ? __fmul_rn(g[e], s.clip) : g[e];
-        m[e] = __fadd_rn(__fmul_rn(m[e], a.b1), __fmul_rn(ge, a.omb1));
-        v[e] = __fadd_rn(__fmul_rn(v[e], a.b2), __fmul_rn(__fmul_rn(ge, ge), a.omb2));
-        // subnormal v counts as the least normal number, so that eps = 0 divides by no zero but v's own
-        const float d = fmaf(sqrt_approx(v[e] == 0.0f ? 0.0f : fmaxf(v[e], 1.17549435e-38f)), s.c2, a.eps);
-        p[e] = fmaf(-s.c1, __fmul_rn(m[e], rcp_approx(d)), __fmul_rn(p[e], s.decay));
-    }
-    if constexpr (sizeof(T) == 4) {
-        adam_store(static_cast<float*>(t.p), i, n, vec, p);
-    } else {
-        adam_store(static_cast<float*>(t.master), i, n, vec, p);
-        adam_store(static_cast<T*>(t.p), i, n, vec, p);
-    }
+    adam_update(a, s, g, m, v, p);
+    adam_store(master, i, n, at.whole, p);
+    if constexpr (sizeof(T) != 4) adam_store(static_cast<T*>(t.p), i, n, at.whole, p);
     if constexpr (EIGHT) {
-        // elements past the end are zero and lie in no code
-        const uint32_t key = mix32(s.step * 0x9E3779B1u + static_cast<uint32_t>(a.place + k));
-        if (block * 256 + 256 > n) {  // the same for the whole warp
+        const int lane = threadIdx.x & 31;
+        if (at.block * 256 + 256 > n) {  // elements past the end are zero and lie in no code; the same for the whole warp
 #pragma unroll
             for (int e = 0; e < 8; ++e)
                 if (i + e >= n) m[e] = v[e] = 0.0f;
         }
+        const uint32_t key = mix32(s.step * 0x9E3779B1u + static_cast<uint32_t>(a.place + at.k));
         uint32_t h[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) h[e] = mix32((static_cast<uint32_t>(i) + e) ^ key);
-        adam_put_codes(static_cast<unsigned char*>(t.m), i, n, vec, quantise8<15>(m, h, t.me + block, lane));
-        adam_put_codes(static_cast<unsigned char*>(t.v), i, n, vec, quantise8<31>(v, h, t.ve + block, lane));
+        adam_put_codes(static_cast<unsigned char*>(t.m), i, n, at.whole, quantise8<15>(m, h, t.me + at.block, lane));
+        adam_put_codes(static_cast<unsigned char*>(t.v), i, n, at.whole, quantise8<31>(v, h, t.ve + at.block, lane));
     } else {
-        adam_store(static_cast<float*>(t.m), i, n, vec, m);
-        adam_store(static_cast<float*>(t.v), i, n, vec, v);
+        adam_store(static_cast<float*>(t.m), i, n, at.whole, m);
+        adam_store(static_cast<float*>(t.v), i, n, at.whole, v);
     }
 }
 
@@ -376,8 +437,7 @@ __global__ void __launch_bounds__(256) k_values8(const unsigned char* __restrict
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
         float f[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) f[k] = value8<BIAS>(c[2 * q + k / 4], k & 3, s);
+        values8<BIAS>(c[2 * q], c[2 * q + 1], s, f);
         adam_store(out, i + 8 * q, n, vec, f);
     }
 }
