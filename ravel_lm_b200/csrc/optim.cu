@@ -184,7 +184,7 @@ int ravel_state_values(const void* codes, const signed char* exponents, int64_t 
     const unsigned char* const c = static_cast<const unsigned char*>(codes);
     const int vec = on16(codes) && on16(out);
     if (n > (int64_t{1} << 40)) return RAVEL_ERR_UNSUPPORTED;
-    const dim3 grid(static_cast<unsigned>((n + 4095) / 4096));
+    const dim3 grid(static_cast<unsigned>((n + 2048 * VA_DEPTH - 1) / (2048 * VA_DEPTH)));
     auto go = [&](auto tv) -> int {
         using T = decltype(tv);
         if (is_signed) return launch(k_values8<T, 15>, grid, 256, 0, st, 1, c, exponents, n, vec, static_cast<T*>(out));
