@@ -111,7 +111,7 @@ int ravel_grad_norm(const ravel_adamw_tensor* tensors, int64_t count, int dtype,
     if (int e = check_list(tensors, count)) return e;
     if (dtype != RAVEL_F32 && dtype != RAVEL_BF16 && dtype != RAVEL_F16) return RAVEL_ERR_UNSUPPORTED;
     if (norm == nullptr) return RAVEL_ERR_INVALID_ARG;
-    if (scratch == nullptr || scratch_bytes < norm_bytes(tensors, count)) return RAVEL_ERR_WORKSPACE;
+    if (scratch == nullptr || scratch_bytes < norm_bytes(tensors, count) || !on16(scratch)) return RAVEL_ERR_WORKSPACE;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     double* const part = static_cast<double*>(scratch);
     int parts = 0;
@@ -143,7 +143,8 @@ int ravel_adamw(const ravel_adamw_tensor* tensors, int64_t count, int dtype, int
             return RAVEL_ERR_INVALID_ARG;
     }
     const bool own_norm = max_norm > 0.0 && norm == nullptr;
-    if (scratch == nullptr || scratch_bytes < kScalarBytes + (own_norm ? norm_bytes(tensors, count) : 0))
+    if (scratch == nullptr || !on16(scratch) ||
+        scratch_bytes < kScalarBytes + (own_norm ? norm_bytes(tensors, count) : 0))
         return RAVEL_ERR_WORKSPACE;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     AdamScalars* const s = static_cast<AdamScalars*>(scratch);

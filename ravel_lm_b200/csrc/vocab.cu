@@ -84,7 +84,7 @@ int sort_ids(IdsArgs a, const IdsLayout& l, char* mem, cudaStream_t st) {
     const dim3 grid(static_cast<unsigned>(l.tiles));
     a.shift = 0;
     for (int p = 0; p < l.passes; ++p) {
-        a.bits = (bits - a.shift + l.passes - p - 1) / (l.passes - p);  // even digits
+        a.bits = (bits - a.shift + l.passes - p - 1) / (l.passes - p);  // digits of a size, at least a bit each
         a.out = (l.passes - 1 - p) % 2 == 0 ? keys : other;
         if (int e = launch(p == 0 ? k_ids_count<true> : k_ids_count<false>, grid, IDS_THREADS, 0, st, 1, a)) return e;
         if (int e = launch(p == 0 ? k_ids_place<true> : k_ids_place<false>, grid, IDS_THREADS, 0, st, 1, a)) return e;
@@ -99,10 +99,11 @@ struct EmbedLayout {
     int64_t K4;
     IdsLayout ids;
 };
-// With ranges of 16 positions: the most there can be.
+// With the shortest ranges that a width or an alignment can lead to.
 EmbedLayout embed_layout(int64_t N, int64_t V, int64_t K) {
     EmbedLayout l;
-    const size_t ranges = static_cast<size_t>((N + 15) / 16);
+    const int64_t shortest = embed_range(N, 32);
+    const size_t ranges = static_cast<size_t>((N + shortest - 1) / shortest);
     l.K4 = up_to(K, 4);
     l.ids = ids_layout(N, V);
     l.off_present = 0;
@@ -552,7 +553,7 @@ int ravel_embedding_bwd(const void* ids, int ids_dtype, const void* grad_y, int6
         return cudaMemsetAsync(grad_weight, 0, static_cast<size_t>(V) * K * es, st) == cudaSuccess ? RAVEL_OK
                                                                                                      : RAVEL_ERR_CUDA;
     const EmbedLayout l = embed_layout(N, V, K);
-    if (scratch == nullptr || scratch_bytes < l.total) return RAVEL_ERR_WORKSPACE;
+    if (scratch == nullptr || scratch_bytes < l.total || !aligned16(scratch)) return RAVEL_ERR_WORKSPACE;
     char* const s = static_cast<char*>(scratch);
     DeviceWords words;
     if (int e = device_words(&words)) return e;

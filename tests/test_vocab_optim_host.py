@@ -29,9 +29,11 @@ def test_embedding_refuses_on_the_host(lib):
         sb = lib.ravel_embedding_scratch_bytes(N, V, K) if sb is None else sb
         return lib.ravel_embedding_bwd(P, 1, g, ldg, N, V, K, 1.0, -1, dw, dt, scratch, sb, None)
     assert bwd(dw=None) == INVALID and bwd(g=None) == INVALID and bwd(ldg=7) == INVALID
-    assert bwd(scratch=None) == WORKSPACE and bwd(sb=100) == WORKSPACE
+    assert bwd(scratch=None) == WORKSPACE and bwd(sb=100) == WORKSPACE and bwd(scratch=P + 8) == WORKSPACE
     assert lib.ravel_embedding_scratch_bytes(-1, 9, 8) == 0
     assert lib.ravel_embedding_scratch_bytes(1 << 20, 1 << 17, 1024) > (1 << 17) + 16 * (1 << 20)
+    # the pieces of sums are a part of the gradients read, not more
+    assert lib.ravel_embedding_scratch_bytes(1 << 20, 1 << 17, 1024) < (1 << 20) * 1024 * 2 // 8
 
 
 def test_cross_entropy_refuses_on_the_host(lib):
@@ -88,6 +90,7 @@ def test_adamw_refuses_on_the_host(lib):
     assert go(dt=1) == INVALID                                     # a 16-bit parameter without a master
     assert go(bits=8) == INVALID                                   # 8-bit states without exponents
     assert go(scratch=None) == WORKSPACE and go(sb=8) == WORKSPACE and go(mx=1.0, sb=64) == WORKSPACE
+    assert go(scratch=P + 4) == WORKSPACE
     t = tensors()
     assert lib.ravel_grad_norm(t, 1, 0, None, P, 1 << 30, None) == INVALID
     assert lib.ravel_grad_norm(t, 1, 0, P, P, 8, None) == WORKSPACE
