@@ -173,7 +173,8 @@ HeadLayout head_layout(int64_t M, int64_t K, int64_t V, bool fast) {
     HeadLayout l;
     std::memset(&l, 0, sizeof(l));
     l.piece = head_piece(M, V);
-    // whole 128-byte lines: a TMA row that straddles two reads both (1021 x 515 -> 32003: d x 45 us, XX with)
+    // whole 128-byte lines: a TMA row that straddles two reads both (1021 x 515 -> 32003 float16, rows of 16 and of 128
+    // bytes: d x 45 / 38 us, d W 62 / 44)
     l.ldz = up_to(V, 64);
     l.ldc = up_to(K, 64);
     l.ldo = up_to(K, 4);

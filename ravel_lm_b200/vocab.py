@@ -1,10 +1,9 @@
 """The vocabulary's two ends: token embedding, and cross entropy over the vocabulary without its logits.
 
 ``token_embedding`` looks rows up and scales them; its
-gradient adds the rows of every token in the order of its positions: the ids are sorted
-with their positions (the event memory's sort), sums run over sorted ranges in
-float32 without atomics, and tokens that do not occur get their zeros in the same
-pass.  The same inputs give the same bits.
+gradient adds the rows of every token in the order of its positions: positions are sorted
+by id (a radix sort), sums run over sorted ranges in float32 without atomics, and tokens
+that do not occur get their zeros in the same pass.  The same inputs give the same bits.
 
 ``linear_cross_entropy`` is the head and the loss of ``RavelLM.forward`` (``ravel_lm/model.py:506``) in one:
 
@@ -12,13 +11,14 @@ pass.  The same inputs give the same bits.
 
 The [rows, V] logits are never kept: a tensor-core kernel reduces each tile of them to
 a maximum and a sum per row where they are made.  A training step makes the gradients of
-a reduced loss in its forward, piece of rows by piece of rows: the logits' product again, this
-time as ``softmax - onehot`` in 16 bits (at most 512 MB or 1024 rows of them), and the two
-products of it, in float32.  These float32 gradients are held until the graph goes; the
+a reduced loss in its forward, piece of rows by piece of rows: ``softmax - onehot`` in
+16 bits (at most 512 MB or 1024 rows of it) from the logits' product done again -- large
+bfloat16 steps get it from the first, as exp(z - z_target) and a factor per row -- and
+its two products, in float32.  These float32 gradients are held until the graph goes; the
 backward scales them by the upstream gradient and rounds them once, so that it may be run again,
 and a float16 loss scale loses nothing.  Single rows' losses (``reduction="none"``) get their
 gradients in the backward, where the rows' upstream gradients are known.
-Probabilities enter the gradients' products rounded to 16 bits.
+Probabilities enter the gradients' products rounded to 16 bits; everything else is float32.
 
 There is no CPU path, no float32 form of the cross entropy (parameters kept in float32, as under
 autocast, are cast by the caller), no second derivative and no forward-mode one.
