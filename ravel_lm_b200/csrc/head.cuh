@@ -668,6 +668,7 @@ __global__ void __launch_bounds__(256) k_head_out(const HeadOutArgs a) {
     const HeadOut& o = a.o[second];
     const float f = (a.up != nullptr ? *a.up : 1.0f) * *a.factor * a.unit;
     const int64_t per = (a.N + 3) / 4, total = o.M * per;
+    const bool flat = o.ldo == a.N;
     const int64_t i0 = static_cast<int64_t>(static_cast<int>(blockIdx.x) - (second ? a.first : 0)) * (256 * HO_DEPTH) + threadIdx.x;
     float4 v[HO_DEPTH];
     int64_t r[HO_DEPTH], c[HO_DEPTH];
@@ -675,8 +676,12 @@ __global__ void __launch_bounds__(256) k_head_out(const HeadOutArgs a) {
     for (int k = 0; k < HO_DEPTH; ++k) {
         const int64_t i = i0 + k * 256;
         if (i >= total) continue;
-        r[k] = i / per;
-        c[k] = (i - r[k] * per) * 4;
+        r[k] = 0;  // rows without padding are one array
+        c[k] = i * 4;
+        if (!flat) {
+            r[k] = i / per;
+            c[k] = (i - r[k] * per) * 4;
+        }
         v[k] = __ldcs(reinterpret_cast<const float4*>(o.slabs + r[k] * o.ldo + c[k]));
     }
     for (int s = 1; s < o.splits; ++s) {

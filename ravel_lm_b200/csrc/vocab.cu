@@ -155,7 +155,9 @@ struct HeadLayout {
 };
 
 // Three products or four, for a bfloat16 training step of a reduced loss: the sort by target, its sums and the launches
-// that wait for a flag take some 35 us, which the spared product has to pass (2 M K V at 1.4 PFLOP/s).
+// that wait for a flag take some 35 us, which the spared product has to pass (2 M K V at 1.4 PFLOP/s).  Measured, us
+// with three / four (replayed graphs): 2048 x 1024 x 8192 148 / 129, 4096 x 256 x 16384 178 / 162, 4096 x 512 x 16384
+// (3.4e10) 227 / 234, 8192 x 256 x 32768 479 / 578, 8192 x 1024 x 32768 1325 / 1818.
 bool head_fast(int64_t M, int64_t K, int64_t V, int dtype) {
     return dtype == RAVEL_BF16 && M > 128 && static_cast<double>(M) * K * V >= 3e10;
 }
@@ -269,7 +271,8 @@ int launch_logits(const HeadOperand& X, const HeadOperand& W, int64_t K, HeadLog
     return launch(kern, dim3(static_cast<unsigned>(std::min(tiles, fit) * CG)), HEAD_THREADS, MM_SMEM, st, CG, ma, mb, a);
 }
 
-// Pairs where two row tiles exist, single CTAs for fewer rows.
+// Pairs where two row tiles exist, single CTAs for fewer rows.  Losses alone, us with pairs / single CTAs: 129 x 1024 x
+// 32000 43 / 48, 512 x 2048 x 8192 35 / 37, 1024 x 256 x 4096 21 / 21, 256 x 256 x 1024 19 / 17.
 bool head_pairs(int64_t M) { return M > 128; }
 
 template <typename T, int MODE>
@@ -369,9 +372,11 @@ struct HeadCall {
     cudaStream_t st;
 };
 
+// Rows a block, by the whole call's time (losses alone, V 32000), us with 8 / 32: 128 rows 25 / 37, 1024 43 / 49, 4096
+// 105 / 111, 8192 170 / 140.
 template <typename T, bool FAST>
 int head_rows(const HeadRowsArgs& h, cudaStream_t st) {
-    if (h.M < 16 * static_cast<int64_t>(sm_count()))
+    if (h.M < 32 * static_cast<int64_t>(sm_count()))
         return launch(k_head_rows<T, FAST, 8>, dim3(static_cast<unsigned>((h.M + 7) / 8)), HR_THREADS, 0, st, 1, h);
     return launch(k_head_rows<T, FAST, 32>, dim3(static_cast<unsigned>((h.M + 31) / 32)), HR_THREADS, 0, st, 1, h);
 }
