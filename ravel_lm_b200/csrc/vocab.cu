@@ -180,7 +180,8 @@ HeadLayout head_layout(int64_t M, int64_t K, int64_t V, bool fast) {
     l.ldz = up_to(V, 64);
     l.ldc = up_to(K, 64);
     l.ldo = up_to(K, 4);
-    l.parts = head_parts(32) * ((V + 31) / 32);  // as many as the narrowest tiles make
+    // as many as either launch shape makes: every part of a tile is written, those behind the vocabulary too
+    l.parts = std::max<int64_t>(head_parts(128) * ((V + 127) / 128), head_parts(256) * ((V + 255) / 256));
     l.off_target = 0;
     l.off_zt = up256(static_cast<size_t>(M) * 4);
     l.off_stat = l.off_zt + up256(static_cast<size_t>(M) * 4);

@@ -58,6 +58,13 @@ def test_cross_entropy_refuses_on_the_host(lib):
         per_row = 2 * V + 4 * (V // 32 + 1) * 2
         assert lib.ravel_linear_ce_work_bytes(M, 64, V, 1, 2) <= max((512 << 20), 1024 * per_row) * 1.2
     assert lib.ravel_linear_ce_scratch_bytes(8, 0, 100) == 0
+    # a tile of 128 or 256 columns writes four parts (a maximum and a sum) a row, whatever the vocabulary leaves of it
+    for M in (1, 100, 128, 129, 5000):
+        for V in (1, 6, 96, 97, 128, 129, 224, 256, 257, 300, 32003):
+            parts = 4 * -(-V // 128) if M <= 128 else 4 * -(-V // 256)
+            for dt in (1, 2):
+                assert lib.ravel_linear_ce_work_bytes(M, 64, V, 0, dt) >= parts * M * 8, (M, V)
+                assert lib.ravel_linear_ce_work_bytes(M, 64, V, 1, dt) >= max(parts * M * 8, M * V * 2), (M, V)
 
     def grad(w=P, ldw=64, up=P, M=8, K=64, V=100, factor=P, sx=P, sw=P, dt=1, scratch=P, sb=1 << 40, work=P, wb=1 << 40):
         return lib.ravel_linear_ce_grad(w, ldw, up, M, K, V, factor, sx, sw, dt, scratch, sb, work, wb, None)
