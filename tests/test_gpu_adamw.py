@@ -289,6 +289,41 @@ def test_captured_steps_count_on(bits):
         assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_offsets_past_32_bits(bits):
+    n, k = (1 << 31) + 1000, 5000
+    big = Case([k], torch.bfloat16, bits, seed=12)
+    small = Case([k], torch.bfloat16, bits, seed=12)
+    tail = (n - k) // 256 * 256  # a block's start, so that the small case has the same blocks
+    cut = n - tail
+
+    def grow(t, dt):
+        out = torch.zeros(n, dtype=dt, device="cuda")
+        out[tail:] = torch.nn.functional.pad(t, (0, cut - k)) if cut > k else t[:cut]
+        return out
+    for c in (big.p, big.g, big.masters, big.m, big.v):
+        c[0] = grow(c[0], c[0].dtype)
+    for c in (small.p, small.g, small.masters, small.m, small.v):
+        c[0] = torch.nn.functional.pad(c[0], (0, cut - k))
+    if bits == 8:
+        for name in ("me", "ve"):
+            e = torch.full(((n + 255) // 256,), -126, dtype=torch.int8, device="cuda")
+            se = torch.full(((cut + 255) // 256,), -126, dtype=torch.int8, device="cuda")
+            se[:(k + 255) // 256] = getattr(small, name)[0]
+            e[tail // 256:] = se
+            setattr(big, name, [e])
+            setattr(small, name, [se.clone()])
+    big.run(max_norm=0.5)
+    small.run(max_norm=0.5)
+    assert torch.equal(big.masters[0][tail:], small.masters[0]) and torch.equal(big.p[0][tail:], small.p[0])
+    assert not big.masters[0][:1 << 20].any() and not big.m[0][tail - (1 << 20):tail].any()
+    if bits == 32:
+        assert torch.equal(big.m[0][tail:], small.m[0]) and torch.equal(big.v[0][tail:], small.v[0])
+    else:  # other random bits: the codes around the same values
+        m, v = values(big.m[0][tail:], big.me[0][tail // 256:], True), values(small.m[0], small.me[0], True)
+        assert bool(((m - v).abs() <= around(torch.maximum(m.abs(), v.abs()), small.me[0], True, cut)).all())
+
+
 def test_another_stream_and_gradients_laid_out_otherwise():
     a, b = Case([64 * 48], torch.float32, 32, seed=11), Case([64 * 48], torch.float32, 32, seed=11)
     st = torch.cuda.Stream()

@@ -366,6 +366,26 @@ def test_offsets_past_32_bits():
         within(dw[v], want, 2.0 ** -7 * top + 2.0 ** -8 * want.abs() + 1e-30, f"d weight[{v}]")
 
 
+def test_rows_past_32_bits():
+    M, K, V = 70000, 32768, 6
+    g = torch.Generator(device="cuda").manual_seed(17)
+    x = torch.zeros(M, K, dtype=torch.bfloat16, device="cuda")
+    x[-200:] = torch.randn(200, K, generator=g, device="cuda").bfloat16()
+    w = (torch.randn(V, K, generator=g, device="cuda") * K ** -0.5).bfloat16()
+    t = torch.randint(0, V, (M,), generator=g, device="cuda")
+    x.requires_grad_(True)
+    loss = ce(x, w, t, reduction="none")
+    want, d, dl, _ = reference(x[-200:], w, t[-200:])
+    within(loss[-200:].detach(), want, dl + 4 * E * want.abs(), "losses")
+    assert torch.allclose(loss[:1000].detach(), torch.full((1000,), math.log(V), device="cuda"))
+    up = torch.zeros(M, device="cuda")
+    up[-200:] = 1.0
+    dx, = torch.autograd.grad(loss, x, up)
+    wx = d @ w.double()
+    within(dx[-200:], wx, (d.abs() * (2.0 ** -7 + 2 * dl[:, None])) @ w.double().abs() + 2.0 ** -8 * wx.abs() + 1e-30, "d x")
+    assert not dx[:1000].any() and not dx[-1000:-200].any()
+
+
 def test_non_finite_inputs_show():
     x, w, t = make(20, 16, 40, torch.bfloat16, seed=14, ignored=False)
     x[3, 2] = float("nan")

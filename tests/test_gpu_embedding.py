@@ -195,6 +195,22 @@ def test_offsets_past_32_bits():
     assert not d[1:V - 3].any() and not d[V - 2].any()
 
 
+def test_outputs_past_32_bits():
+    N, V, K = 70000, 3, 32768
+    g = torch.Generator(device="cuda").manual_seed(8)
+    w = torch.randn(V, K, generator=g, device="cuda").bfloat16().requires_grad_(True)
+    ids = torch.randint(0, 2, (N,), generator=g, device="cuda")
+    ids[-2:] = 2
+    y = embed(ids, w)
+    for i in (0, 65535, 65536, N - 1):
+        assert torch.equal(y[i], w[ids[i]])
+    gy = torch.zeros(N, K, dtype=torch.bfloat16, device="cuda")
+    gy[-3:] = torch.randn(3, K, generator=g, device="cuda").bfloat16()
+    d, = torch.autograd.grad(y, w, gy)
+    assert torch.equal(d[2], (gy[-2].float() + gy[-1].float()).bfloat16())
+    assert torch.equal(d[ids[-3]], gy[-3]) and not d[1 - ids[-3]].any()
+
+
 def test_second_derivatives_and_tangents_are_refused():
     ids, w, gy = make(5, 9, 8, torch.float32, seed=9)
     w.requires_grad_(True)
