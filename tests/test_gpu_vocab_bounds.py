@@ -1,0 +1,143 @@
+"""The vocabulary operators and the optimizer step write nothing outside the buffers they are given: each output and
+workspace lies at its exact size between guard bytes, which have to be as they were."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+GUARD = 8192
+MARK = 0xA5
+
+
+@pytest.fixture(scope="module")
+def lib():
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    import ravel_lm_b200._lib as L
+    yield L.load()
+    torch.cuda.synchronize()
+    assert L.device_error(torch.cuda.current_stream().cuda_stream) == 0
+
+
+class Guarded:
+    def __init__(self):
+        self.all = []
+
+    def __call__(self, nbytes, fill=MARK):
+        t = torch.full((nbytes + 2 * GUARD,), MARK, dtype=torch.uint8, device="cuda")
+        if fill != MARK:
+            t[GUARD:GUARD + nbytes] = fill
+        self.all.append((t, nbytes))
+        return t.data_ptr() + GUARD
+
+    def tensor(self, src):
+        """A copy of ``src`` between guards: its pointer, and the tensor."""
+        n = src.numel() * src.element_size()
+        p = self(n)
+        v = self.all[-1][0][GUARD:GUARD + n].view(src.dtype).view(src.shape)
+        v.copy_(src)
+        return p, v
+
+    def check(self, what):
+        torch.cuda.synchronize()
+        for i, (t, n) in enumerate(self.all):
+            assert bool((t[:GUARD] == MARK).all()) and bool((t[GUARD + n:] == MARK).all()), (what, i)
+
+
+@pytest.mark.parametrize("dt,code", [(torch.float32, 0), (torch.bfloat16, 1), (torch.float16, 2)])
+def test_embedding(lib, dt, code):
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    es = torch.tensor([], dtype=dt).element_size()
+    for N, V, K in ((1, 1, 1), (7, 3, 5), (100, 17, 8), (129, 1025, 33), (1025, 40, 24), (3000, 70000, 12), (5000, 9, 260)):
+        for bad in (False, True):
+            g = Guarded()
+            ids = torch.randint(0, V, (N,), generator=gen, device="cuda")
+            pi, _ = g.tensor(ids)
+            pw, _ = g.tensor(torch.randn(V, K, generator=gen, device="cuda").to(dt))
+            pg, _ = g.tensor(torch.randn(N, K, generator=gen, device="cuda").to(dt))
+            y, dw = g(N * K * es), g(V * K * es)
+            sb = lib.ravel_embedding_scratch_bytes(N, V, K)
+            scratch = g(sb, 0xFF if bad else 0)  # whatever a workspace held before
+            assert lib.ravel_embedding_fwd(pi, 1, pw, K, N, V, K, 1.0, y, code, None) == 0
+            assert lib.ravel_embedding_bwd(pi, 1, pg, K, N, V, K, 1.0, -1, dw, code, scratch, sb, None) == 0
+            g.check((N, V, K))
+
+
+CE_SIZES = [(1, 8, 1), (3, 16, 6), (100, 24, 96), (128, 40, 300), (129, 8, 129), (257, 33, 97), (1000, 72, 224), (40, 264, 1000),
+            (300, 8, 20000), (2000, 16, 33)]
+
+
+@pytest.mark.parametrize("code", [1, 2])
+@pytest.mark.parametrize("M,K,V", CE_SIZES + [(1500, 1000, 24003)])
+def test_cross_entropy(lib, code, M, K, V):
+    dt = torch.bfloat16 if code == 1 else torch.float16
+    gen = torch.Generator(device="cuda").manual_seed(M + V)
+    ld = (K + 7) // 8 * 8
+    for reduction, grads in ((2, True), (2, False), (0, True)):
+        g = Guarded()
+        px, _ = g.tensor(torch.randn(M, K, generator=gen, device="cuda").to(dt))
+        pw, _ = g.tensor((torch.randn(V, ld, generator=gen, device="cuda") * K ** -0.5).to(dt))
+        t = torch.randint(0, V, (M,), generator=gen, device="cuda")
+        t[::5] = -100
+        pt, _ = g.tensor(t)
+        sizes = (ctypes.c_int64 * 3)()
+        assert lib.ravel_linear_ce_slabs(M, K, V, sizes) == 0
+        losses, out, factor = g(4 * M), g(4), g(4)
+        sx = g(sizes[0] * M * sizes[2] * 4) if grads else None
+        sw = g(sizes[1] * V * sizes[2] * 4) if grads else None
+        sb = lib.ravel_linear_ce_scratch_bytes(M, K, V)
+        wb = lib.ravel_linear_ce_work_bytes(M, K, V, int(grads and reduction == 2), code)
+        scratch, work = g(sb, 0xFF), g(wb, 0xFF)
+        first = (sx, sw) if reduction == 2 else (None, None)
+        assert lib.ravel_linear_ce_fwd(px, K, pw, ld, pt, 1, M, K, V, -100, reduction, int(reduction == 0), losses,
+                                       out if reduction else None, factor if grads else None, *first, code, scratch, sb,
+                                       work, wb, None) == 0
+        g.check(("fwd", reduction, grads))
+        if not grads:
+            continue
+        up = None
+        if reduction == 0:
+            pu, _ = g.tensor(torch.randn(M, generator=gen, device="cuda"))
+            wb2 = lib.ravel_linear_ce_work_bytes(M, K, V, 1, code)
+            work2 = g(wb2, 0xFF)
+            assert lib.ravel_linear_ce_grad(pw, ld, pu, M, K, V, factor, sx, sw, code, scratch, sb, work2, wb2, None) == 0
+            g.check("grad")
+        else:
+            up, _ = g.tensor(torch.ones(1, device="cuda"))
+        dx, dw = g(M * K * 2), g(V * K * 2)
+        assert lib.ravel_linear_ce_bwd(sx, sw, up, factor, M, K, V, dx, dw, code, None) == 0
+        g.check("bwd")
+        n = M * K * 2
+        got = next(b[GUARD:GUARD + n] for b, m in g.all if b.data_ptr() + GUARD == dx).view(dt)
+        assert bool(torch.isfinite(got).all())  # no leftovers of a workspace
+
+
+@pytest.mark.parametrize("code,dt", [(0, torch.float32), (1, torch.bfloat16)])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw(lib, code, dt, bits):
+    import ravel_lm_b200._lib as L
+    for sizes in ([1], [255, 257], [2048, 7, 4097], [33] * 60):
+        for off in (0, 1):
+            g = Guarded()
+            arr = (L.AdamTensor * len(sizes))()
+            for a, n in zip(arr, sizes):
+                def buf(kind, count=n, fill=0):
+                    es = torch.tensor([], dtype=kind).element_size()
+                    return g(count * es, fill) if not off else g.tensor(torch.zeros(count + 1, dtype=kind))[0] + es
+                a.param, a.grad = buf(dt), buf(dt)
+                a.master = buf(torch.float32) if code else None
+                state = torch.float32 if bits == 32 else torch.uint8
+                a.exp_avg, a.exp_avg_sq = buf(state), buf(state)
+                if bits == 8:
+                    a.exp_avg_exponents, a.exp_avg_sq_exponents = g((n + 255) // 256, 0), g((n + 255) // 256, 0)
+                a.n = n
+            step, norm = g(8, 0), g(4, 0)
+            sb = lib.ravel_adamw_scratch_bytes(arr, len(sizes), 1.0)
+            scratch = g(sb, 0xFF)
+            for _ in range(2):
+                assert lib.ravel_adamw(arr, len(sizes), code, bits, step, 1e-3, None, 0.9, 0.99, 1e-8, 0.0, 1.0, None, norm,
+                                       scratch, sb, None) == 0
+            g.check((sizes, off))
