@@ -447,7 +447,7 @@ int ravel_embedding_fwd(const void* ids, int ids_dtype, const void* weight, int6
  * Its gradient: grad_weight[v] = scale sum over the i with ids[i] = v of grad_y[i], all V rows
  * written (contiguous); none from rows whose id is padding_idx or outside [0, V).
  * Sums in float32 in a fixed order of the sorted positions, without atomics.
- * scratch: 16-byte aligned, as the scratch and work of the entry points below.
+ * scratch: 16-byte aligned, as the scratch and work of the entry points below; a few ids need none (0 bytes).
  */
 size_t ravel_embedding_scratch_bytes(int64_t N, int64_t V, int64_t K);
 int ravel_embedding_bwd(const void* ids, int ids_dtype, const void* grad_y, int64_t ldg, int64_t N, int64_t V, int64_t K,

@@ -11,6 +11,7 @@
 //                    their first ranges listed.
 //   k_embed_join     the pieces of a listed token, added in their order; the last blocks, under those chains of loads, write
 //                    the zeros of tokens that do not occur.
+//   k_embed_few      up to 512 ids: the whole gradient in one launch, without a sort.
 // Sums are float32 in a fixed order without atomics: the same inputs give the same bits.
 // Bound by HBM: N rows read and N (forward) or V (backward) rows written.
 #pragma once
@@ -328,6 +329,141 @@ __global__ void __launch_bounds__(32 * EJ_GROUPS) k_embed_join(const EmbedArgs a
                 embed_finish<T, ADD>(a, v, col, s);
             }
             __syncthreads();
+        }
+    }
+}
+
+// ------------------------------------------------------------------ few ids
+constexpr int ES_IDS = 512;      // at most
+constexpr int ES_ROWS = 2048;    // vocabulary rows of a block at most
+constexpr int ES_EACH = 2;       // ids a thread looks at together
+constexpr int ES_DEPTH = 8;      // rows in flight
+
+// The whole gradient in one launch, without a sort: a block per slice of the vocabulary reads every id and lists, in order,
+// the positions of those in its slice; it then writes the slice's rows: zeros, or the sums over the list's entries of a
+// token, a group of threads per token -- or, where tokens have many entries, all groups together, each a part of the
+// list, their sums added in order.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(EM_THREADS) k_embed_few(const EmbedArgs a, int slice, int64_t pad) {
+    __shared__ uint32_t list[ES_IDS];            // row of the slice << 16 | position
+    __shared__ unsigned int present[ES_ROWS / 32];
+    __shared__ int wsum[EM_THREADS / 32];
+    __shared__ float red[EM_THREADS * VEC];
+    grid_wait();
+    grid_trigger();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t v0 = static_cast<int64_t>(blockIdx.x) * slice, v1 = min(v0 + slice, a.V);
+    const int rows = static_cast<int>(v1 - v0);
+    for (int w = threadIdx.x; w < ES_ROWS / 32; w += EM_THREADS) present[w] = 0u;
+    __syncthreads();
+    int n = 0;
+    for (int64_t i0 = 0; i0 < a.N; i0 += EM_THREADS * ES_EACH) {
+        int64_t id[ES_EACH];
+        const int64_t i = i0 + threadIdx.x * ES_EACH;
+#pragma unroll
+        for (int e = 0; e < ES_EACH; ++e) id[e] = i + e < a.N ? embed_id(a, i + e) : v0 - 1;
+        int mine = 0;
+#pragma unroll
+        for (int e = 0; e < ES_EACH; ++e) {
+            if (blockIdx.x == 0 && i + e < a.N && (id[e] < 0 || id[e] >= a.V)) atomicOr(a.err, RAVEL_DEVERR_INDEX);
+            if (id[e] == pad || id[e] < v0 || id[e] >= v1) id[e] = -1;
+            mine += id[e] >= 0;
+        }
+        int incl = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += v;
+        }
+        if (lane == 31) wsum[warp] = incl;
+        __syncthreads();
+        int at = n + incl - mine;
+        for (int w = 0; w < EM_THREADS / 32; ++w) {
+            if (w < warp) at += wsum[w];
+            n += wsum[w];
+        }
+#pragma unroll
+        for (int e = 0; e < ES_EACH; ++e)
+            if (id[e] >= 0) {
+                const uint32_t r = static_cast<uint32_t>(id[e] - v0);
+                list[at++] = r << 16 | static_cast<uint32_t>(i + e);
+                atomicOr(&present[r / 32], 1u << (r % 32));
+            }
+        __syncthreads();
+    }
+    // zeros, a warp per row
+    constexpr int E = 16 / sizeof(T);
+    for (int r = warp; r < rows; r += EM_THREADS / 32) {
+        if (present[r / 32] >> (r % 32) & 1u) continue;
+        T* const o = static_cast<T*>(a.out) + (v0 + r) * a.K;
+        if constexpr (VEC == E) {
+            for (int64_t u = lane; u < a.K / E; u += 32) __stcs(reinterpret_cast<uint4*>(o) + u, make_uint4(0u, 0u, 0u, 0u));
+        } else {
+            for (int64_t c = lane; c < a.K; c += 32) o[c] = round_to<T>(0.0f);
+        }
+    }
+    int tokens = 0;
+    for (int w = 0; w < (rows + 31) / 32; ++w) tokens += __popc(present[w]);
+    const int64_t units = a.K / VEC;
+    const int tx = threadIdx.x & (a.tx - 1), ty = threadIdx.x / a.tx, groups = EM_THREADS / a.tx;
+    const bool together = n > 8 * tokens && groups > 1;  // the same for the block
+    const T* const g = static_cast<const T*>(a.g);
+    // s += the rows of the entries l0 .. l1 of token r, in their order
+    auto sum = [&](uint32_t r, int l0, int l1, int64_t u, float (&s)[VEC]) {
+        for (int l = l0; l < l1; l += 32) {
+            const uint32_t entry = l + lane < l1 ? list[l + lane] : 0xffffffffu;
+            unsigned todo = __ballot_sync(0xffffffffu, entry >> 16 == r && l + lane < l1);
+            while (todo != 0u) {
+                Pack<T, VEC> row[ES_DEPTH];
+                unsigned had = 0u;
+#pragma unroll
+                for (int k = 0; k < ES_DEPTH; ++k) {
+                    const int from = todo != 0u ? __ffs(todo) - 1 : 0;
+                    const uint32_t pos = __shfl_sync(0xffffffffu, entry, from) & 0xffffu;
+                    if (todo != 0u) {
+                        had |= 1u << k;
+                        if (u < units) row[k] = load_pack<T, VEC>(g + static_cast<int64_t>(pos) * a.ldg + u * VEC);
+                    }
+                    todo &= todo - 1u;
+                }
+#pragma unroll
+                for (int k = 0; k < ES_DEPTH; ++k)
+                    if ((had >> k & 1u) && u < units) {
+                        float f[VEC];
+                        to_floats<T, VEC>(row[k], f);
+#pragma unroll
+                        for (int e = 0; e < VEC; ++e) s[e] += f[e];
+                    }
+            }
+        }
+    };
+    int ordinal = 0;
+    for (int w = 0; w < (rows + 31) / 32; ++w) {
+        for (unsigned bits = present[w]; bits != 0u; bits &= bits - 1u, ++ordinal) {
+            const uint32_t r = static_cast<uint32_t>(w * 32 + __ffs(bits) - 1);
+            if (!together && ordinal % groups != ty) continue;
+            const int l0 = together ? static_cast<int>(static_cast<int64_t>(n) * ty / groups) : 0;
+            const int l1 = together ? static_cast<int>(static_cast<int64_t>(n) * (ty + 1) / groups) : n;
+            for (int64_t u0 = 0; u0 < units; u0 += a.tx) {
+                const int64_t u = u0 + tx;
+                float s[VEC];
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) s[e] = 0.0f;
+                sum(r, l0, l1, u, s);
+                if (together) {
+                    float* const mine = red + threadIdx.x * VEC;
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) mine[e] = s[e];
+                    __syncthreads();
+                    if (ty == 0) {
+                        for (int q = 1; q < groups; ++q)
+#pragma unroll
+                            for (int e = 0; e < VEC; ++e) s[e] += red[(q * a.tx + tx) * VEC + e];
+                    }
+                    __syncthreads();
+                }
+                if ((ty == 0 || !together) && u < units) embed_put<T, VEC, false>(a, static_cast<uint32_t>(v0 + r), u, s);
+            }
         }
     }
 }

@@ -648,12 +648,14 @@ struct TokenEmbedding : public torch::autograd::Function<TokenEmbedding> {
         const Rows gy = rows_of(grads[0]);
         at::Tensor dw = at::empty({V, K}, gy.t.options());
         const size_t sb = ravel_embedding_scratch_bytes(N, V, K);
-        at::Tensor scratch = bytes(sb, gy.t);
+        at::Tensor scratch;
+        if (sb > 0) scratch = bytes(sb, gy.t);
         check_status("ravel_embedding_bwd",
                      ravel_embedding_bwd(ids.data_ptr(), index_code(ids, "ids"), gy.t.data_ptr(), gy.ld, N, V, K,
                                          static_cast<float>(ctx->saved_data["scale"].toDouble()),
                                          ctx->saved_data["padding"].toInt(), dw.data_ptr(),
-                                         payload_code(dw.scalar_type()), scratch.data_ptr(), sb, stream_of(gy.t)));
+                                         payload_code(dw.scalar_type()), sb > 0 ? scratch.data_ptr() : nullptr, sb,
+                                         stream_of(gy.t)));
         out[1] = dw;
         return out;
     }

@@ -114,6 +114,15 @@ EmbedLayout embed_layout(int64_t N, int64_t V, int64_t K) {
     return l;
 }
 
+// Vocabulary rows of a block of the one-launch gradient, or 0 where the ids are sorted.  Lookup and gradient, us in one
+// launch / sorted, replayed from a graph (and eager): 24 x 2048 of 65536 tokens 50 / 58 (55 / 73), 512 x 512 of 8192
+// 14 / 21 (51 / 65; all of them one token, which one block then sums, 23 / 21), 1024 x 1024 of 65536 33 / 42 (58 / 70; one
+// token 79 / 38), 2048 x 512 of 1000 22 / 20 (55 / 61; one token 70 / 19), 8192 x 256 of 1024 50 / 25.
+int embed_slice(int64_t N, int64_t V) {
+    const int64_t slice = (V + sm_count() * 4 - 1) / (sm_count() * 4);
+    return N <= ES_IDS && slice <= ES_ROWS ? static_cast<int>(slice) : 0;
+}
+
 // The sums over sorted positions, and their joins.
 template <typename T, bool ADD>
 int launch_sums(EmbedArgs a, bool vec, cudaStream_t st) {
@@ -543,7 +552,7 @@ int ravel_embedding_fwd(const void* ids, int ids_dtype, const void* weight, int6
 
 size_t ravel_embedding_scratch_bytes(int64_t N, int64_t V, int64_t K) {
     if (N < 0 || V <= 0 || K < 0 || N > kMaxRows || V >= kMaxRows || K > kMaxRows) return 0;
-    return embed_layout(N, V, K).total;
+    return embed_slice(N, V) > 0 ? 0 : embed_layout(N, V, K).total;
 }
 
 int ravel_embedding_bwd(const void* ids, int ids_dtype, const void* grad_y, int64_t ldg, int64_t N, int64_t V, int64_t K,
@@ -559,11 +568,28 @@ int ravel_embedding_bwd(const void* ids, int ids_dtype, const void* grad_y, int6
     if (N == 0)
         return cudaMemsetAsync(grad_weight, 0, static_cast<size_t>(V) * K * es, st) == cudaSuccess ? RAVEL_OK
                                                                                                      : RAVEL_ERR_CUDA;
+    const int slice = embed_slice(N, V);
     const EmbedLayout l = embed_layout(N, V, K);
-    if (scratch == nullptr || scratch_bytes < l.total || !aligned16(scratch)) return RAVEL_ERR_WORKSPACE;
-    char* const s = static_cast<char*>(scratch);
+    if (slice == 0 && (scratch == nullptr || scratch_bytes < l.total || !aligned16(scratch))) return RAVEL_ERR_WORKSPACE;
     DeviceWords words;
     if (int e = device_words(&words)) return e;
+    const bool vec = (K * es) % 16 == 0 && aligned16(grad_y) && (N == 1 || ldg * es % 16 == 0) && aligned16(grad_weight);
+    if (slice > 0) {
+        EmbedArgs a;
+        std::memset(&a, 0, sizeof(a));
+        a.ids = ids; a.ids64 = ids_dtype == RAVEL_I64;
+        a.g = grad_y; a.out = grad_weight;
+        a.N = N; a.V = V; a.K = K; a.ldg = ldg; a.scale = scale;
+        a.err = words.error;
+        a.tx = embed_tx(vec ? K * es / 16 : K);
+        return with_float_type(dtype, [&](auto tv) -> int {
+            using T = decltype(tv);
+            const auto kern = vec ? k_embed_few<T, 16 / sizeof(T)> : k_embed_few<T, 1>;
+            return launch(kern, dim3(static_cast<unsigned>((V + slice - 1) / slice)), EM_THREADS, 0, st, 1, a, slice,
+                          padding_idx);
+        });
+    }
+    char* const s = static_cast<char*>(scratch);
     IdsArgs q;
     std::memset(&q, 0, sizeof(q));
     q.ids = ids; q.ids64 = ids_dtype == RAVEL_I64;
@@ -582,7 +608,6 @@ int ravel_embedding_bwd(const void* ids, int ids_dtype, const void* grad_y, int6
     a.part = reinterpret_cast<float*>(s + l.off_part);
     a.K4 = l.K4;
     a.list = reinterpret_cast<int*>(s + l.off_list);
-    const bool vec = (K * es) % 16 == 0 && aligned16(grad_y) && (N == 1 || ldg * es % 16 == 0) && aligned16(grad_weight);
     return with_float_type(dtype, [&](auto tv) -> int {
         using T = decltype(tv);
         return launch_sums<T, false>(a, vec, st);

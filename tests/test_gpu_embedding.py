@@ -70,11 +70,11 @@ def make(N, V, K, dt, seed, zipf=False):
     return ids, w, torch.randn(N, K, generator=g, device="cuda").to(dt)
 
 
-# one of everything; ranges of the sums that end inside, at and behind tokens; odd widths; several digits of ids
-# (2^9 and 2^18 are the borders of one and two passes); several steps a tile (past 262144 ids)
+# one of everything; up to 512 ids in one launch, then ranges of sums that end inside, at and behind tokens; odd widths;
+# several digits of ids (2^10 and 2^20 are the borders of one and two passes); several steps a tile (past 131072 ids)
 SHAPES = [(1, 1, 1), (1, 7, 8), (2, 2, 3), (15, 1, 4), (16, 3, 5), (17, 300, 64), (64, 512, 33), (65, 513, 40),
-          (1000, 5, 256), (2048, 1000, 100), (2049, 1025, 1), (4097, 32003, 24), (9000, 40, 520), (300, 262145, 8),
-          (300001, 700, 4), (20000, 65536, 16)]
+          (512, 1025, 40), (513, 1024, 8), (1000, 5, 256), (2048, 1000, 100), (2049, 1025, 1), (4097, 32003, 24),
+          (9000, 40, 520), (300, 262145, 8), (300, 1300000, 4), (2000, 1050000, 4), (300001, 700, 4), (20000, 65536, 16)]
 
 
 @pytest.mark.parametrize("dt", DTYPES)
@@ -84,7 +84,7 @@ def test_sizes(dt, N, V, K):
 
 
 @pytest.mark.parametrize("dt", DTYPES)
-@pytest.mark.parametrize("N,V,K", [(5000, 50, 128), (40000, 1000, 96), (70000, 30000, 33)])
+@pytest.mark.parametrize("N,V,K", [(512, 3, 520), (500, 40, 17), (5000, 50, 128), (40000, 1000, 96), (70000, 30000, 33)])
 def test_frequent_tokens(dt, N, V, K):
     check(*make(N, V, K, dt, seed=7, zipf=True), scale=-3.0)
     ids, w, gy = make(N, V, K, dt, seed=8)
@@ -117,8 +117,9 @@ def test_leading_dimensions_strides_and_alignment(ids_dtype):
     assert torch.equal(d, check_n[:, None].expand(90, 72))
 
 
-def test_padding_id_and_no_ids():
-    ids, w, gy = make(3000, 60, 40, torch.float32, seed=2)
+@pytest.mark.parametrize("N", [400, 3000])  # in one launch, and sorted
+def test_padding_id_and_no_ids(N):
+    ids, w, gy = make(N, 60, 40, torch.float32, seed=2)
     _, d = check(ids, w, gy, pad=11)
     assert not d[11].any() and d[12].any()
     _, d2 = check(ids, w, gy, pad=11 - 60)
@@ -134,12 +135,13 @@ def test_padding_id_and_no_ids():
     y = embed(none, leaf)
     assert y.shape == (0, 40) and not torch.autograd.grad(y.sum(), leaf)[0].any()
     empty = torch.zeros(60, 0, device="cuda", requires_grad=True)
-    assert embed(ids, empty).shape == (3000, 0)
+    assert embed(ids, empty).shape == (N, 0)
 
 
-def test_ids_outside_the_vocabulary_are_reported_and_not_used():
+@pytest.mark.parametrize("N", [500, 1500])
+def test_ids_outside_the_vocabulary_are_reported_and_not_used(N):
     import ravel_lm_b200._lib as L
-    ids, w, gy = make(500, 60, 40, torch.bfloat16, seed=3)
+    ids, w, gy = make(N, 60, 40, torch.bfloat16, seed=3)
     ids[3], ids[77], ids[400] = 60, -1, 1 << 40
     ok = (ids >= 0) & (ids < 60)
     leaf = w.clone().requires_grad_(True)
@@ -155,8 +157,9 @@ def test_ids_outside_the_vocabulary_are_reported_and_not_used():
     assert L.device_error(st) == 0
 
 
-def test_the_same_bits_every_time_on_any_stream_and_replayed():
-    ids, w, gy = make(30000, 2000, 64, torch.float32, seed=4, zipf=True)
+@pytest.mark.parametrize("N", [512, 30000])
+def test_the_same_bits_every_time_on_any_stream_and_replayed(N):
+    ids, w, gy = make(N, 2000, 64, torch.float32, seed=4, zipf=True)
     y, d = check(ids, w, gy)
     leaf = w.clone().requires_grad_(True)
     st = torch.cuda.Stream()
@@ -170,7 +173,7 @@ def test_the_same_bits_every_time_on_any_stream_and_replayed():
     with torch.cuda.graph(graph):
         y3 = embed(ids, leaf, scale=2.0)
         d3, = torch.autograd.grad(y3, leaf, gy)
-    ids2, _, gy2 = make(30000, 2000, 64, torch.float32, seed=5)
+    ids2, _, gy2 = make(N, 2000, 64, torch.float32, seed=5)
     ids.copy_(ids2)
     gy.copy_(gy2)
     for _ in range(2):

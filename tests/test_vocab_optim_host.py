@@ -25,12 +25,15 @@ def test_embedding_refuses_on_the_host(lib):
     assert fwd(ids=None) == INVALID and fwd(w=None) == INVALID and fwd(y=None) == INVALID and fwd(ldw=7) == INVALID
     assert fwd(N=0, ids=None, y=None) == 0 and fwd(K=0) == 0
 
-    def bwd(g=P, ldg=8, N=4, V=9, K=8, dw=P, dt=0, scratch=P, sb=None):
+    def bwd(g=P, ldg=8, N=10000, V=9, K=8, dw=P, dt=0, scratch=P, sb=None):
         sb = lib.ravel_embedding_scratch_bytes(N, V, K) if sb is None else sb
         return lib.ravel_embedding_bwd(P, 1, g, ldg, N, V, K, 1.0, -1, dw, dt, scratch, sb, None)
     assert bwd(dw=None) == INVALID and bwd(g=None) == INVALID and bwd(ldg=7) == INVALID
     assert bwd(scratch=None) == WORKSPACE and bwd(sb=100) == WORKSPACE and bwd(scratch=P + 8) == WORKSPACE
     assert lib.ravel_embedding_scratch_bytes(-1, 9, 8) == 0
+    # a few ids take one launch without scratch, unless the vocabulary has too many rows for its blocks
+    assert lib.ravel_embedding_scratch_bytes(512, 65536, 8) == 0 and lib.ravel_embedding_scratch_bytes(513, 65536, 8) > 0
+    assert lib.ravel_embedding_scratch_bytes(512, 1 << 24, 8) > 0
     assert lib.ravel_embedding_scratch_bytes(1 << 20, 1 << 17, 1024) > (1 << 17) + 16 * (1 << 20)
     # the pieces of sums are a part of the gradients read, not more
     assert lib.ravel_embedding_scratch_bytes(1 << 20, 1 << 17, 1024) < (1 << 20) * 1024 * 2 // 8
