@@ -647,7 +647,7 @@ struct HeadOut {
     const float* slabs;    // [splits] slabs of M rows, ldo apart
     int64_t slab, ldo, M;
     int splits;
-    int vec;               // 8-byte stores
+    int vec;               // 8-byte stores: the output starts on 8 bytes, N is a multiple of 4
     void* out;             // [M, N]
 };
 struct HeadOutArgs {
@@ -668,7 +668,7 @@ __global__ void __launch_bounds__(256) k_head_out(const HeadOutArgs a) {
     const HeadOut& o = a.o[second];
     const float f = (a.up != nullptr ? *a.up : 1.0f) * *a.factor * a.unit;
     const int64_t per = (a.N + 3) / 4, total = o.M * per;
-    const bool flat = o.ldo == a.N;
+    const bool flat = o.vec && o.ldo == a.N;  // without `vec` elements are bounded by their row
     const int64_t i0 = static_cast<int64_t>(static_cast<int>(blockIdx.x) - (second ? a.first : 0)) * (256 * HO_DEPTH) + threadIdx.x;
     float4 v[HO_DEPTH];
     int64_t r[HO_DEPTH], c[HO_DEPTH];

@@ -141,3 +141,46 @@ def test_adamw(lib, code, dt, bits):
                 assert lib.ravel_adamw(arr, len(sizes), code, bits, step, 1e-3, None, 0.9, 0.99, 1e-8, 0.0, 1.0, None, norm,
                                        scratch, sb, None) == 0
             g.check((sizes, off))
+
+
+def ce_slabs(lib, g, M, K, V, dt, code, seed):
+    """A mean loss's gradient sums by ``ravel_linear_ce_fwd``: slabs of d x and of d W, an upstream gradient of 1, the factor."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    px, _ = g.tensor(torch.randn(M, K, generator=gen, device="cuda").to(dt))
+    ld = (K + 7) // 8 * 8
+    pw, _ = g.tensor((torch.randn(V, ld, generator=gen, device="cuda") * K ** -0.5).to(dt))
+    pt, _ = g.tensor(torch.randint(0, V, (M,), generator=gen, device="cuda"))
+    up, _ = g.tensor(torch.ones(1, device="cuda"))
+    sizes = (ctypes.c_int64 * 3)()
+    assert lib.ravel_linear_ce_slabs(M, K, V, sizes) == 0
+    sx, sw = g(sizes[0] * M * sizes[2] * 4), g(sizes[1] * V * sizes[2] * 4)
+    losses, out, factor = g(4 * M), g(4), g(4)
+    sb, wb = lib.ravel_linear_ce_scratch_bytes(M, K, V), lib.ravel_linear_ce_work_bytes(M, K, V, 1, code)
+    assert lib.ravel_linear_ce_fwd(px, K, pw, ld, pt, 1, M, K, V, -100, 2, 0, losses, out, factor, sx, sw, code, g(sb), sb,
+                                   g(wb), wb, None) == 0
+    return sx, sw, up, factor
+
+
+@pytest.mark.parametrize("code", [1, 2])
+@pytest.mark.parametrize("M,K,V", [(8, 64, 40), (3, 4, 2), (300, 72, 500), (7, 65, 30), (5, 66, 9)])
+def test_cross_entropy_gradients_at_any_address(lib, code, M, K, V):
+    """Gradients inside a flat buffer: off 16 and off 8 bytes, either or both, they are the aligned ones."""
+    dt = torch.bfloat16 if code == 1 else torch.float16
+    g = Guarded()
+    sx, sw, up, factor = ce_slabs(lib, g, M, K, V, dt, code, seed=M)
+
+    def run(off_x, off_w):
+        got = []
+        ptrs = []
+        for n, off in ((M * K, off_x), (V * K, off_w)):
+            ptrs.append(g(2 * (n + off)) + 2 * off)
+            got.append(g.all[-1][0])
+        assert lib.ravel_linear_ce_bwd(sx, sw, up, factor, M, K, V, *ptrs, code, None) == 0
+        g.check((off_x, off_w))
+        for t, off in zip(got, (off_x, off_w)):
+            assert bool((t[:GUARD + 2 * off] == MARK).all())  # nothing before it either
+        return [t[GUARD + 2 * off:-GUARD].view(torch.int16).clone() for t, off in zip(got, (off_x, off_w))]
+    want = run(0, 0)
+    for off_x, off_w in ((1, 0), (0, 1), (1, 1), (2, 3), (4, 8)):
+        got = run(off_x, off_w)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), (off_x, off_w)
