@@ -435,7 +435,7 @@ int head_run(const HeadCall& c, bool stats) {
     const bool grads = c.gx != nullptr || c.gw != nullptr;
     const HeadOperand W{c.w, c.ldw};
     const HeadSplits sp = head_splits(c.M, c.K, c.V);
-    if (grads && c.up != nullptr) {
+    if (!stats) {  // single losses' gradients: the factor of the sums, without rows too (then 1)
         if (int e = launch(k_head_up_max, dim3(1), 1024, 0, c.st, 1, c.up, target, c.M, up_max)) return e;
     }
     if (c.M == 0 && c.gw != nullptr &&

@@ -403,3 +403,15 @@ def test_second_derivatives_and_tangents_are_refused():
         dual = fwad.make_dual(x.detach(), torch.ones_like(x))
         with pytest.raises(RuntimeError, match="forward-mode"):
             ce(dual, w, t)
+
+
+def test_gradients_of_single_losses_without_rows():
+    w = torch.randn(50, 16, device="cuda").bfloat16().requires_grad_(True)
+    x = torch.zeros(0, 16, device="cuda").bfloat16().requires_grad_(True)
+    t = torch.zeros(0, dtype=torch.int64, device="cuda")
+    for _ in range(3):
+        dirt = torch.full((1 << 20,), float("nan"), device="cuda")  # what the allocator hands out next
+        del dirt
+        loss = ce(x, w, t, reduction="none")
+        dx, dw = torch.autograd.grad(loss, [x, w], torch.zeros(0, device="cuda"))
+        assert dx.shape == (0, 16) and dw.shape == (50, 16) and not dw.any()

@@ -184,3 +184,24 @@ def test_cross_entropy_gradients_at_any_address(lib, code, M, K, V):
     for off_x, off_w in ((1, 0), (0, 1), (1, 1), (2, 3), (4, 8)):
         got = run(off_x, off_w)
         assert all(torch.equal(a, b) for a, b in zip(got, want)), (off_x, off_w)
+
+
+@pytest.mark.parametrize("code", [1, 2])
+def test_single_losses_of_no_rows_have_a_gradient_of_zero(lib, code):
+    """Whatever stood in the workspaces: there is no row, and no upstream gradient."""
+    K, V = 16, 50
+    g = Guarded()
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    pw, _ = g.tensor(torch.randn(V, K, generator=gen, device="cuda").to(torch.bfloat16 if code == 1 else torch.float16))
+    sizes = (ctypes.c_int64 * 3)()
+    assert lib.ravel_linear_ce_slabs(0, K, V, sizes) == 0
+    sw = g(sizes[1] * V * sizes[2] * 4, 0xFF)
+    sb, wb = lib.ravel_linear_ce_scratch_bytes(0, K, V), lib.ravel_linear_ce_work_bytes(0, K, V, 1, code)
+    scratch, work, factor, dw = g(sb, 0xFF), g(wb, 0xFF), g(4, 0xFF), g(V * K * 2, 0xFF)
+    assert lib.ravel_linear_ce_fwd(None, K, pw, K, None, 1, 0, K, V, -100, 0, 1, None, None, None, None, None, code, scratch,
+                                   sb, work, wb, None) == 0
+    assert lib.ravel_linear_ce_grad(pw, K, None, 0, K, V, factor, None, sw, code, scratch, sb, work, wb, None) == 0
+    assert lib.ravel_linear_ce_bwd(None, sw, None, factor, 0, K, V, None, dw, code, None) == 0
+    g.check("no rows")
+    got = next(b[GUARD:GUARD + V * K * 2] for b, _ in g.all if b.data_ptr() + GUARD == dw)
+    assert not got.any()
