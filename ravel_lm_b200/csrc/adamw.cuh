@@ -66,7 +66,8 @@ struct AdamArgs {
     int place;           // tensors of the list before this launch's
     const AdamScalars* s;
     double* part;        // norm: this launch's parts
-    float b1, omb1, b2, omb2, eps;
+    float b1, omb1, b2, omb2;
+    float eps;           // 0 or a normal number
     int clipped;
 };
 
@@ -189,9 +190,9 @@ __device__ __forceinline__ int block_exponent(float top, bool odd) {
     return __uint_as_float(t) > __fmul_rn(pow2_of(e), 1.875f) ? e + 1 : e;
 }
 
-__device__ __forceinline__ float sqrt_approx(float x) {
+__device__ __forceinline__ float sqrt_approx(float x) {  // of subnormal numbers too
     float y;
-    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 __device__ __forceinline__ float rcp_approx(float x) {
@@ -326,8 +327,8 @@ __global__ void __launch_bounds__(1024) k_adamw_scalars(const AdamStep a) {
 }
 
 // ------------------------------------------------------------------ the step
-// The step of 8 elements, in pairs.  A subnormal v counts as the least normal number where eps = 0, so that nothing but a
-// zero v divides by zero.
+// The step of 8 elements, in pairs.  A subnormal v has its root (at least 3.7e-23), and the caller gives no subnormal eps,
+// so that the reciprocal, which would take a subnormal divisor for 0, never meets one: only v = 0 with eps = 0 divides by 0.
 template <int CAP>
 __device__ __forceinline__ void adam_update(const AdamArgs<CAP>& a, const AdamScalars& s, const float (&g)[8], float (&m)[8],
                                             float (&v)[8], float (&p)[8]) {
@@ -340,11 +341,8 @@ __device__ __forceinline__ void adam_update(const AdamArgs<CAP>& a, const AdamSc
         if (a.clipped) g2 = mul2(g2, clip);
         split(fma2(g2, omb1, mul2(two(m[e], m[e + 1]), b1)), m[e], m[e + 1]);
         split(fma2(mul2(g2, g2), omb2, mul2(two(v[e], v[e + 1]), b2)), v[e], v[e + 1]);
-        float r[2], d[2];
-#pragma unroll
-        for (int q = 0; q < 2; ++q)
-            r[q] = sqrt_approx(a.eps != 0.0f || v[e + q] == 0.0f ? v[e + q] : fmaxf(v[e + q], 1.17549435e-38f));
-        split(fma2(two(r[0], r[1]), c2, eps), d[0], d[1]);
+        float d[2];
+        split(fma2(two(sqrt_approx(v[e]), sqrt_approx(v[e + 1])), c2, eps), d[0], d[1]);
         const uint64_t q2 = mul2(two(m[e], m[e + 1]), two(rcp_approx(d[0]), rcp_approx(d[1])));
         split(fma2(c1, q2, mul2(two(p[e], p[e + 1]), decay)), p[e], p[e + 1]);
     }

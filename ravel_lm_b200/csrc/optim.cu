@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <limits>
 
 #include "adamw.cuh"
 
@@ -165,7 +166,8 @@ int ravel_adamw(const ravel_adamw_tensor* tensors, int64_t count, int dtype, int
             a.omb1 = static_cast<float>(1.0 - beta1);
             a.b2 = static_cast<float>(beta2);
             a.omb2 = static_cast<float>(1.0 - beta2);
-            a.eps = static_cast<float>(eps);
+            // a positive eps below float32's normal numbers is the least of them: roots of v are 0 or far above it
+            a.eps = eps > 0.0 ? std::max(static_cast<float>(eps), std::numeric_limits<float>::min()) : 0.0f;
             a.clipped = max_norm > 0.0;
             const dim3 grid(static_cast<unsigned>(chunks));
             if (state_bits == 8) return launch(k_adamw<T, true, CAP>, grid, 32 * AW_WARPS, 0, st, 1, a);

@@ -441,3 +441,49 @@ def test_optimizer_closure_no_gradients_and_capture():
     torch.cuda.synchronize()
     for p, q in zip(m.parameters(), twin[0].parameters()):
         assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("eps", [1e-20, 1e-40, 1e-50, 0.0])
+def test_gradients_whose_squares_are_subnormal(bits, eps):
+    """A first step from states of zero moves by lr g / (|g| + eps), whatever the size of g and eps; no gradient, no step.
+
+    v = (1 - b2) g^2 lies on the grid of subnormal numbers, off by at most 2^-149 (g^2 and the sum, half of a
+    smallest number each): at most 0.4% of v for |g| >= 2e-20, and half of it in the root; lr g / |g| has the usual rest.
+    """
+    n = 3000
+    gen = torch.Generator(device="cuda").manual_seed(20)
+    size = torch.exp(torch.empty(n, device="cuda").uniform_(math.log(2e-20), math.log(1e-17), generator=gen))
+    g = size * torch.where(torch.rand(n, generator=gen, device="cuda") < 0.5, -1.0, 1.0)
+    if eps > 0.0:
+        g[::7] = 0.0
+    p = torch.zeros(n, device="cuda")
+    blocks = (n + 255) // 256
+    m, v = (torch.zeros(n, dtype=torch.float32 if bits == 32 else torch.uint8, device="cuda") for _ in range(2))
+    ex = {}
+    if bits == 8:
+        ex = {k: [torch.full((blocks,), -126, dtype=torch.int8, device="cuda")]
+              for k in ("exp_avg_exponents", "exp_avg_sq_exponents")}
+    t = torch.zeros(1, dtype=torch.int64, device="cuda")
+    hyper = dict(lr=1e-2, betas=(0.9, 0.999), eps=eps, weight_decay=0.0)
+    step([p], [g], [m], [v], t, **ex, **hyper)
+    gd = g.double()
+    want = torch.where(gd == 0, 0.0, -1e-2 * gd / (gd.abs() + eps))
+    tol = want.abs() * (2.0 ** -149 / (1e-3 * gd * gd).clamp_min(1e-300) + 2.0 ** -20)
+    tol[gd == 0] = 0.0
+    assert bool(((p.double() - want).abs() <= tol).all()), float((p.double() - want).abs().max())
+    for _ in range(3):
+        step([p], [g], [m], [v], t, **ex, **hyper)
+    assert not p[g == 0].any() and bool(torch.isfinite(p).all())
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-8])
+def test_a_second_moment_of_nan_shows(eps):
+    c = Case([600], torch.float32, 32, seed=21)
+    c.v[0][300] = float("nan")
+    c.run(eps=eps)
+    assert torch.isnan(c.p[0]).nonzero().flatten().tolist() == [300]
+    e = Case([600], torch.float32, 8, seed=21)
+    e.ve[0][1] = -128  # a block that stands for NaN
+    e.run(eps=eps)
+    assert torch.isnan(e.p[0]).nonzero().flatten().tolist() == list(range(256, 512))
