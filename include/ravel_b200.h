@@ -506,6 +506,14 @@ typedef struct {
     int64_t n;
 } ravel_adamw_tensor;
 
+/*
+ * With state_bits 8, or'ed: a positive exp_avg_sq has code 1 at least, so that code 0 is exactly 0.  Without it values
+ * below 2^-33 of the block's largest are mostly rounded to 0, and where exp_avg is not, whose smallest step is 2^-17 of
+ * its block's largest, the next step divides by little more than eps: hundreds of lr in blocks whose gradients differ by
+ * factors past 1e4.
+ */
+#define RAVEL_STATE_POSITIVE 0x100
+
 /* *norm (float64, device) = the 2-norm over every tensor's gradient; param and
  * states are not read.  Deterministic: a part per block, added in order. */
 size_t ravel_grad_norm_scratch_bytes(const ravel_adamw_tensor* tensors, int64_t count);

@@ -29,6 +29,7 @@ RAVEL_TAPE_WRITE_MASK = 2
 RAVEL_NOALLOC_SCRATCH_BYTES = 32 << 20
 RAVEL_DEVERR_SPIN = 1
 RAVEL_DEVERR_INDEX = 2
+RAVEL_STATE_POSITIVE = 0x100
 
 _c_i64 = ctypes.c_int64
 _c_int = ctypes.c_int

@@ -20,7 +20,10 @@
 // them; m is kept as sign, 4 bits of exponent and 3 of mantissa below that, v (never negative, its range the
 // square) as 5 and 3.  A power of two leaves the grid where it was when a block's largest value moves, and rounding
 // is stochastic: v moves by a thousandth of itself a step, a hundredth of a grid step, which rounding to nearest
-// would drop for ever.  The random bits are a hash of (step, tensor, element): the same call gives the same
+// would drop for ever.  With RAVEL_STATE_POSITIVE a positive v has code 1 at least, 2^-33 2^e, and code 0 is exactly 0:
+// where elements of very different gradients share a block, a small one's m may round up to 2^-17 of the
+// block's largest, and over a v rounded to 0 that is a step of m / eps (gradients about 1, 1e-5 times
+// that in half of each block, 300 steps: up to 1400 lr; so, 1.8 lr).  The random bits are a hash of (step, tensor, element): the same call gives the same
 // bits.  A block that meets a NaN or an infinity is marked (exponent -128) and stands for NaN from then on.
 //
 // Bound by HBM.
@@ -69,6 +72,7 @@ struct AdamArgs {
     float b1, omb1, b2, omb2;
     float eps;           // 0 or a normal number
     int clipped;
+    uint32_t least;      // quantise8's, of v
 };
 
 // The tensor of a chunk.
@@ -212,8 +216,10 @@ __device__ __forceinline__ uint32_t mix32(uint32_t i) {
 // or high half, and half of one more, added below the code's last place.  The integer and logic pipe, half as fast as the
 // multiply-add pipe, bounds the 8-bit step: the value's bits go up by 4 (the code becomes the top byte) and meet the random
 // ones in one integer multiply-add, one byte permutation lays out the latter, and sums of x * 0 find what is not finite.
+// BIAS 31: a positive value's bits are at least `least` (0, or 2^24: code 1).
 template <int BIAS>
-__device__ __forceinline__ uint64_t quantise8(const float (&x)[8], const uint32_t (&h)[8], signed char* e, int lane) {
+__device__ __forceinline__ uint64_t quantise8(const float (&x)[8], const uint32_t (&h)[8], uint32_t least, signed char* e,
+                                              int lane) {
     float top = 0.0f;
     uint64_t odd = 0;
 #pragma unroll
@@ -237,7 +243,8 @@ __device__ __forceinline__ uint64_t quantise8(const float (&x)[8], const uint32_
         for (int q = 0; q < 2; ++q) {
             const uint32_t r = __byte_perm(h[k + q], 0x80u, BIAS == 15 ? 0x5104 : 0x5324);
             const uint32_t t = __float_as_uint(y[q]) * 16u + r;
-            c[k + q] = BIAS == 31 ? t : (t & 0x7fffffffu) | (__float_as_uint(y[q]) & 0x80000000u);
+            if constexpr (BIAS == 31) c[k + q] = x[k + q] != 0.0f ? max(t, least) : t;
+            else c[k + q] = (t & 0x7fffffffu) | (__float_as_uint(y[q]) & 0x80000000u);
         }
     }
     const uint32_t lo = __byte_perm(__byte_perm(c[0], c[1], 0x0073), __byte_perm(c[2], c[3], 0x0073), 0x5410);
@@ -410,8 +417,8 @@ __global__ void __launch_bounds__(32 * AW_WARPS, EIGHT ? 5 : 4) k_adamw(const __
         uint32_t h[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) h[e] = mix32((static_cast<uint32_t>(i) + e) ^ key);
-        adam_put_codes(static_cast<unsigned char*>(t.m), i, n, at.whole, quantise8<15>(m, h, t.me + at.block, lane));
-        adam_put_codes(static_cast<unsigned char*>(t.v), i, n, at.whole, quantise8<31>(v, h, t.ve + at.block, lane));
+        adam_put_codes(static_cast<unsigned char*>(t.m), i, n, at.whole, quantise8<15>(m, h, 0u, t.me + at.block, lane));
+        adam_put_codes(static_cast<unsigned char*>(t.v), i, n, at.whole, quantise8<31>(v, h, a.least, t.ve + at.block, lane));
     } else {
         adam_store(static_cast<float*>(t.m), i, n, at.whole, m);
         adam_store(static_cast<float*>(t.v), i, n, at.whole, v);

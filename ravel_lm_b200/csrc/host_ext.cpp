@@ -863,7 +863,8 @@ at::Tensor global_norm(const TensorList& tensors) {
 OptTensor adamw_step(const TensorList& params, const TensorList& grads, const TensorList& avgs, const TensorList& sqs,
                      const at::Tensor& step, const OptTensorList& masters, const OptTensorList& avg_exps,
                      const OptTensorList& sq_exps, double lr, const OptTensor& lr_tensor, double beta1, double beta2,
-                     double eps, double weight_decay, std::optional<double> max_norm, const OptTensor& norm) {
+                     double eps, double weight_decay, std::optional<double> max_norm, const OptTensor& norm,
+                     bool positive) {
     const size_t n = params.size();
     if (n == 0) throw py::value_error("adamw_step expects at least one tensor");
     if (grads.size() != n || avgs.size() != n || sqs.size() != n || (masters && masters->size() != n) ||
@@ -877,6 +878,7 @@ OptTensor adamw_step(const TensorList& params, const TensorList& grads, const Te
         throw py::value_error("lr, eps and weight_decay must not be negative");
     if (max_norm && !(*max_norm > 0.0)) throw py::value_error("max_norm must be positive");
     if (norm && !max_norm) throw py::value_error("norm is used with max_norm only");
+    if (positive && !avg_exps) throw py::value_error("positive_exp_avg_sq is for 8-bit states only");
     const at::Tensor& first = params[0];
     const auto dt = first.scalar_type();
     const bool eight = avg_exps.has_value(), half = dt != at::kFloat;
@@ -948,7 +950,8 @@ OptTensor adamw_step(const TensorList& params, const TensorList& grads, const Te
     const size_t sb = ravel_adamw_scratch_bytes(list.data(), static_cast<int64_t>(n), max_norm.value_or(0.0));
     at::Tensor scratch = bytes(sb, first);
     check_status("ravel_adamw",
-                 ravel_adamw(list.data(), static_cast<int64_t>(n), payload_code(dt), eight ? 8 : 32,
+                 ravel_adamw(list.data(), static_cast<int64_t>(n), payload_code(dt),
+                             eight ? (positive ? 8 | RAVEL_STATE_POSITIVE : 8) : 32,
                              step.data_ptr<int64_t>(), lr, lr_tensor ? lr_tensor->data_ptr<float>() : nullptr, beta1,
                              beta2, eps, weight_decay, max_norm.value_or(0.0), norm ? norm->data_ptr<double>() : nullptr,
                              max_norm ? norm32.data_ptr<float>() : nullptr, scratch.data_ptr(), sb, stream_of(first)));

@@ -131,6 +131,8 @@ int ravel_adamw(const ravel_adamw_tensor* tensors, int64_t count, int dtype, int
     RAVEL_TIMED("ravel_adamw", stream);
     if (int e = check_list(tensors, count)) return e;
     if (dtype != RAVEL_F32 && dtype != RAVEL_BF16 && dtype != RAVEL_F16) return RAVEL_ERR_UNSUPPORTED;
+    const bool positive = state_bits == (8 | RAVEL_STATE_POSITIVE);
+    if (positive) state_bits = 8;
     if (state_bits != 8 && state_bits != 32) return RAVEL_ERR_UNSUPPORTED;
     if (step == nullptr || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) || !(eps >= 0.0) ||
         !(max_norm >= 0.0) || (norm != nullptr && max_norm == 0.0))
@@ -169,6 +171,7 @@ int ravel_adamw(const ravel_adamw_tensor* tensors, int64_t count, int dtype, int
             // a positive eps below float32's normal numbers is the least of them: roots of v are 0 or far above it
             a.eps = eps > 0.0 ? std::max(static_cast<float>(eps), std::numeric_limits<float>::min()) : 0.0f;
             a.clipped = max_norm > 0.0;
+            a.least = positive ? 1u << 24 : 0u;
             const dim3 grid(static_cast<unsigned>(chunks));
             if (state_bits == 8) return launch(k_adamw<T, true, CAP>, grid, 32 * AW_WARPS, 0, st, 1, a);
             return launch(k_adamw<T, false, CAP>, grid, 32 * AW_WARPS, 0, st, 1, a);

@@ -11,7 +11,8 @@ clipping by the global norm (``runtime.py:9``).  Per element, in float32:
 A 16-bit parameter is the rounding of a float32 master that takes the steps.  8-bit
 states share a power of two per block of 256 elements, sign + 4 + 3 bits for m and 5 + 3
 for v, and are rounded stochastically (the random bits are a hash of step, tensor and
-element: a run repeats bit for bit).  A block that meets a NaN or an infinity stands for
+element: a run repeats bit for bit).  ``AdamW`` keeps every positive v positive, so that
+a block may hold elements of very different gradients.  A block that meets a NaN or an infinity stands for
 NaN as a whole from then on.
 
 The step count lives on the device and the learning rate may too, so that a step
@@ -40,7 +41,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
                betas: tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
                masters: Optional[Sequence[Tensor]] = None, exp_avg_exponents: Optional[Sequence[Tensor]] = None,
                exp_avg_sq_exponents: Optional[Sequence[Tensor]] = None, max_norm: Optional[float] = None,
-               norm: Optional[Tensor] = None) -> Optional[Tensor]:
+               norm: Optional[Tensor] = None, positive_exp_avg_sq: bool = False) -> Optional[Tensor]:
     """One AdamW step in place on every tensor of the lists; all of one dtype, contiguous, on one device, none twice.
 
     Args:
@@ -52,6 +53,9 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
         lr:          a number, or one float32 on the device.
         max_norm:    gradients are scaled down to this norm over all of them, or by ``norm``
                      (``global_norm``'s) where other tensors share in it.
+        positive_exp_avg_sq: 8-bit states: a positive second moment has code 1 at least (``AdamW``'s way).  Without it
+                     one below 2^-33 of its block's largest may be rounded to 0 while the first
+                     moment is not: in blocks whose gradients differ by factors past 1e4 steps of hundreds of lr.
     Returns:
         the norm (float32, 0-dim) with ``max_norm``, else None.
     """
@@ -60,7 +64,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     lists = [None if v is None else list(v) for v in (masters, exp_avg_exponents, exp_avg_sq_exponents)]
     return _lib.host().adamw_step(list(params), list(grads), list(exp_avgs), list(exp_avg_sqs), step, *lists,
                                   0.0 if on_device else float(lr), lr if on_device else None, float(b1), float(b2),
-                                  float(eps), float(weight_decay), max_norm, norm)
+                                  float(eps), float(weight_decay), max_norm, norm, bool(positive_exp_avg_sq))
 
 
 def state_values(codes: Tensor, exponents: Tensor, *, signed: bool, dtype: torch.dtype = torch.float32) -> Tensor:
@@ -163,7 +167,8 @@ class AdamW(torch.optim.Optimizer):
                 adamw_step(ps, [p.grad for p in ps], each("exp_avg"), each("exp_avg_sq"), sts[0]["step"],
                            lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
                            masters=each("master"), exp_avg_exponents=each("exp_avg_exponents"),
-                           exp_avg_sq_exponents=each("exp_avg_sq_exponents"), max_norm=self.max_norm, norm=norm)
+                           exp_avg_sq_exponents=each("exp_avg_sq_exponents"), max_norm=self.max_norm, norm=norm,
+                           positive_exp_avg_sq=self.state_bits == 8)
         return loss
 
     def load_state_dict(self, state_dict: dict) -> None:

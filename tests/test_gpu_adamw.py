@@ -487,3 +487,52 @@ def test_a_second_moment_of_nan_shows(eps):
     e.ve[0][1] = -128  # a block that stands for NaN
     e.run(eps=eps)
     assert torch.isnan(e.p[0]).nonzero().flatten().tolist() == list(range(256, 512))
+
+
+@pytest.mark.parametrize("r", [1e-5, 1e-6])
+def test_blocks_with_a_wide_range_take_steps_of_lr(r):
+    """Half of each block has gradients r times the other half's.  A small element's second moment must not be rounded to 0
+    while its first moment is not, which would divide the one by eps.
+
+    With b1 = 0.9, b2 = 0.999 Cauchy's inequality gives |m| <= 7.3 sqrt(v) in exact arithmetic, a block's largest values
+    among them.  m's smallest step is 2^-17 2^e <= 2^-17 1.07 max |m|, v's smallest value 2^-33 2^e >= 2^-33 max v / 1.875,
+    so that one step of m over the root of v's smallest value is at most 7.3 * 1.07 * 1.37 / sqrt(2) = 7.6; with the value
+    that was rounded (7.3) and the new gradient's part (0.1 / sqrt(0.001) = 3.2) no step passes 18.1 lr, or 20.4 with the
+    values' own roundings of 1/8 (bias correction: sqrt(1 - b2^t) / (1 - b1^t) <= 1).
+    """
+    from ravel_lm_b200.optim import AdamW, state_values
+    n = 64 * 256
+    gen = torch.Generator(device="cuda").manual_seed(22)
+    small = torch.arange(n, device="cuda") % 256 >= 128
+    p = torch.nn.Parameter(torch.zeros(n, device="cuda"))
+    opt = AdamW([p], lr=1.0, betas=(0.9, 0.999), weight_decay=0.0, state_bits=8)
+    worst = torch.zeros((), device="cuda")
+    for _ in range(100):
+        p.grad = torch.randn(n, generator=gen, device="cuda") * torch.where(small, r, 1.0)
+        p.data.zero_()
+        opt.step()
+        worst = torch.maximum(worst, p.detach().abs().max())
+    assert float(worst) <= 20.4
+    st = opt.state[p]
+    assert bool((st["exp_avg_sq"] > 0).all())
+    assert bool((state_values(st["exp_avg_sq"], st["exp_avg_sq_exponents"], signed=False) > 0).all())
+
+
+@pytest.mark.parametrize("n,off", [(1000, 0), (1000, 1), (4096, 0)])
+def test_positive_second_moments(n, off):
+    """Exactly 0 keeps code 0, a positive value has code 1 at least; all else is as without the option."""
+    def go(**k):
+        c = Case([n], torch.float32, 8, seed=23, offset=off)
+        c.g[0].zero_()
+        c.g[0][::3] = 1e-2
+        c.g[0][1::3] = 1e-11
+        c.m[0].zero_(), c.v[0].zero_()
+        c.run(**k)
+        return c
+    a, b = go(), go(positive_exp_avg_sq=True)
+    none = torch.arange(n, device="cuda") % 3 == 2
+    assert not b.v[0][none].any() and bool((b.v[0][~none] > 0).all()) and not a.v[0][1::3].any()
+    assert torch.equal(b.v[0], torch.where(none, a.v[0], a.v[0].clamp_min(1))) and torch.equal(a.ve[0], b.ve[0])
+    assert torch.equal(a.m[0], b.m[0]) and torch.equal(a.me[0], b.me[0]) and torch.equal(a.p[0], b.p[0])
+    with pytest.raises(ValueError, match="8-bit states only"):
+        Case([n], torch.float32, 32).run(positive_exp_avg_sq=True)

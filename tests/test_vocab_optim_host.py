@@ -200,3 +200,17 @@ def test_optimizer_functions_refuse():
               dict(max_norm=-1.0)):
         with pytest.raises(ValueError):
             AdamW([torch.nn.Parameter(torch.zeros(3))], **k)
+
+
+def test_the_option_for_positive_second_moments(lib):
+    import ravel_lm_b200._lib as L
+    t = (L.AdamTensor * 1)(L.AdamTensor(param=P, grad=P, exp_avg=P, exp_avg_sq=P, n=5))
+
+    def go(bits):
+        return lib.ravel_adamw(t, 1, 0, bits, P, 1e-3, None, 0.9, 0.99, 1e-8, 0.0, 0.0, None, None, P, 1 << 30, None)
+    assert go(8 | L.RAVEL_STATE_POSITIVE) == INVALID == go(8)  # 8-bit states: exponents are missing
+    assert go(32 | L.RAVEL_STATE_POSITIVE) == UNSUPPORTED and go(16 | L.RAVEL_STATE_POSITIVE) == UNSUPPORTED
+    from ravel_lm_b200.optim import adamw_step
+    z = [torch.zeros(3)]
+    with pytest.raises(ValueError, match="8-bit states only"):
+        adamw_step(z, z, z, z, torch.zeros(1, dtype=torch.long), lr=1e-3, positive_exp_avg_sq=True)
