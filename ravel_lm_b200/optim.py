@@ -84,6 +84,7 @@ class AdamW(torch.optim.Optimizer):
 
     A parameter counts the steps in which it had a gradient.  Masters are made from 16-bit parameters at their
     first step: parameters overwritten later need ``reset_masters()``.  ``lr`` may be a float32 CUDA tensor.
+    A step may be captured in a CUDA graph after an eager one with gradients for the same parameters.
     """
 
     def __init__(self, params, lr: Union[float, Tensor] = 1e-3, betas: tuple[float, float] = (0.9, 0.999),
@@ -125,7 +126,8 @@ class AdamW(torch.optim.Optimizer):
 
     def _buckets(self, group: dict) -> list[list[Tensor]]:
         """The group's parameters with gradients, by the step tensor they share: those of one dtype and device that have
-        counted the same steps.  Where one of them has no gradient now, the others go on with a copy."""
+        counted the same steps.  Where one of them has no gradient now, the others go on with a copy.  Neither new
+        states nor copies are made inside a capture: every replay would make them again."""
         idle = {id(self.state[p]["step"]) for p in group["params"] if p.grad is None and self.state.get(p)}
         fresh: dict = {}
         moved: dict = {}
@@ -134,6 +136,10 @@ class AdamW(torch.optim.Optimizer):
             if p.grad is None:
                 continue
             st = self.state.get(p)
+            if (not st or id(st["step"]) in idle) and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: take a step with gradients for the same parameters before a capture; a "
+                                   + ("new state" if not st else "step count copied for some of them")
+                                   + " would start again in every replay")
             if not st:
                 kind = (p.dtype, p.device)
                 if kind not in fresh:
@@ -153,22 +159,22 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        buckets = [(group, ps) for group in self.param_groups for ps in self._buckets(group)]
         norm = None
         if self.max_norm is not None:
             grads = [p.grad for g in self.param_groups for p in g["params"] if p.grad is not None]
             norm = global_norm(grads) if grads else None
             self.grad_norm = norm
-        for group in self.param_groups:
-            for ps in self._buckets(group):
-                sts = [self.state[p] for p in ps]
+        for group, ps in buckets:
+            sts = [self.state[p] for p in ps]
 
-                def each(name):
-                    return [st[name] for st in sts] if name in sts[0] else None
-                adamw_step(ps, [p.grad for p in ps], each("exp_avg"), each("exp_avg_sq"), sts[0]["step"],
-                           lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
-                           masters=each("master"), exp_avg_exponents=each("exp_avg_exponents"),
-                           exp_avg_sq_exponents=each("exp_avg_sq_exponents"), max_norm=self.max_norm, norm=norm,
-                           positive_exp_avg_sq=self.state_bits == 8)
+            def each(name):
+                return [st[name] for st in sts] if name in sts[0] else None
+            adamw_step(ps, [p.grad for p in ps], each("exp_avg"), each("exp_avg_sq"), sts[0]["step"],
+                       lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
+                       masters=each("master"), exp_avg_exponents=each("exp_avg_exponents"),
+                       exp_avg_sq_exponents=each("exp_avg_sq_exponents"), max_norm=self.max_norm, norm=norm,
+                       positive_exp_avg_sq=self.state_bits == 8)
         return loss
 
     def load_state_dict(self, state_dict: dict) -> None:

@@ -536,3 +536,40 @@ def test_positive_second_moments(n, off):
     assert torch.equal(a.m[0], b.m[0]) and torch.equal(a.me[0], b.me[0]) and torch.equal(a.p[0], b.p[0])
     with pytest.raises(ValueError, match="8-bit states only"):
         Case([n], torch.float32, 32).run(positive_exp_avg_sq=True)
+
+
+def test_a_capture_refuses_what_a_replay_would_repeat():
+    """States made, or a step count copied, inside a capture would start again in every replay."""
+    from ravel_lm_b200.optim import AdamW
+    m = model(4)
+    o = AdamW(m.parameters(), lr=1e-2, max_norm=1.0)
+    grads(m, 0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="before a capture"):
+        with torch.cuda.graph(graph):
+            o.step()
+    assert not any(o.state.values())
+    o.step()
+    gone = m[2].bias.grad
+    m[2].bias.grad = None  # has counted a step, and has no gradient now
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="before a capture"):
+        with torch.cuda.graph(graph):
+            o.step()
+    o.step()  # as the message says
+    twin = copy.deepcopy((m, o))
+    for p, q in zip(m.parameters(), twin[0].parameters()):
+        q.grad = None if p.grad is None else p.grad.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o.step()
+    for _ in range(3):
+        graph.replay()
+        twin[1].step()
+    torch.cuda.synchronize()
+    assert gone is not None and [int(o.state[p]["step"]) for p in m.parameters()] == [5, 5, 5, 1]
+    for p, q in zip(m.parameters(), twin[0].parameters()):
+        assert torch.equal(p, q)

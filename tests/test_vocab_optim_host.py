@@ -214,3 +214,34 @@ def test_the_option_for_positive_second_moments(lib):
     z = [torch.zeros(3)]
     with pytest.raises(ValueError, match="8-bit states only"):
         adamw_step(z, z, z, z, torch.zeros(1, dtype=torch.long), lr=1e-3, positive_exp_avg_sq=True)
+
+
+def _stepped(bits):
+    """An optimizer of two CPU parameters with states as after a step (no kernel runs here)."""
+    from ravel_lm_b200.optim import AdamW
+    ps = [torch.nn.Parameter(torch.full((300,), float(i))) for i in range(2)]
+    o = AdamW(ps, lr=1e-2, state_bits=bits)
+    step = torch.ones(1, dtype=torch.int64)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+        o.state[p] = o._new_state(p, step)
+    return ps, o
+
+
+def test_a_capture_makes_no_states_and_copies_no_count(monkeypatch):
+    ps, o = _stepped(32)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    group = o.param_groups[0]
+    assert o._buckets(group) == [ps]  # every state is there
+    step = o.state[ps[1]]["step"]
+    ps[0].grad = None
+    with pytest.raises(RuntimeError, match="before a capture"):
+        o._buckets(group)
+    assert o.state[ps[1]]["step"] is step
+    ps[0].grad = torch.ones(300)
+    del o.state[ps[0]]
+    with pytest.raises(RuntimeError, match="before a capture"):
+        o._buckets(group)
+    assert ps[0] not in o.state
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    assert o._buckets(group) == [[ps[0]], [ps[1]]]
