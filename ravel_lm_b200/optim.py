@@ -117,6 +117,13 @@ class AdamW(torch.optim.Optimizer):
             st["master"] = p.detach().float()
         return st
 
+    def _state_names(self, p: Tensor) -> set[str]:
+        """The names of ``_new_state(p, step)``."""
+        names = {"step", "exp_avg", "exp_avg_sq"}
+        if self.state_bits == 8:
+            names |= {"exp_avg_exponents", "exp_avg_sq_exponents"}
+        return names if p.dtype == torch.float32 else names | {"master"}
+
     @torch.no_grad()
     def reset_masters(self) -> None:
         """Take the float32 masters from the parameters as they are now."""
@@ -178,17 +185,24 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict: dict) -> None:
-        """As ``torch.optim.Optimizer``'s, with the states in their own types (not cast to their parameters')."""
-        super().load_state_dict(state_dict)
+        """As ``torch.optim.Optimizer``'s, with the states in their own types (not cast to their parameters').  States of
+        another ``state_bits`` or another optimizer are refused before anything is loaded."""
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
-        shared: dict = {}
         owned = [(p, k) for k, g in enumerate(self.param_groups) for p in g["params"]]
+        for i, (p, _) in zip(ids, owned):
+            src = state_dict["state"].get(i)
+            if not src:
+                continue
+            if "exp_avg" in src and (src["exp_avg"].dtype == torch.uint8) != (self.state_bits == 8):
+                raise ValueError(f"the loaded states do not have state_bits={self.state_bits}")
+            if set(src) != self._state_names(p) or getattr(src["step"], "dtype", None) != torch.int64:
+                raise ValueError(f"the loaded states are not this optimizer's for a parameter of {p.dtype}")
+        super().load_state_dict(state_dict)
+        shared: dict = {}
         for i, (p, g) in zip(ids, owned):
             src = state_dict["state"].get(i)
             if not src:
                 continue
-            if (src["exp_avg"].dtype == torch.uint8) != (self.state_bits == 8):
-                raise ValueError(f"the loaded states do not have state_bits={self.state_bits}")
             st = {k: v.detach().to(p.device, copy=True) for k, v in src.items()}
             st["step"] = shared.setdefault((g, p.dtype, p.device, int(st["step"])), st["step"])
             self.state[p] = st

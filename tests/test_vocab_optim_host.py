@@ -245,3 +245,40 @@ def test_a_capture_makes_no_states_and_copies_no_count(monkeypatch):
     assert ps[0] not in o.state
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     assert o._buckets(group) == [[ps[0]], [ps[1]]]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_refused_state_dict_changes_nothing(bits):
+    _, src = _stepped(40 - bits)
+    src.param_groups[0]["lr"] = 0.5
+    ps, o = _stepped(bits)
+    kept = {p: dict(o.state[p]) for p in ps}
+    with pytest.raises(ValueError, match="state_bits"):
+        o.load_state_dict(src.state_dict())
+    assert o.param_groups[0]["lr"] == 1e-2 and all(a is b for a, b in zip(o.param_groups[0]["params"], ps))
+    assert set(o.state) == set(ps)
+    for p in ps:
+        assert o.state[p].keys() == kept[p].keys() and all(o.state[p][k] is v for k, v in kept[p].items())
+
+
+def test_states_of_another_optimizer_or_dtype_are_refused():
+    ps, o = _stepped(32)
+    for p in ps:
+        assert set(o.state[p]) == o._state_names(p)
+    other = torch.optim.AdamW([torch.nn.Parameter(torch.zeros(300)) for _ in range(2)], lr=0.5)
+    for p in other.param_groups[0]["params"]:
+        p.grad = torch.ones_like(p)
+    other.step()
+    with pytest.raises(ValueError, match="not this optimizer's"):
+        o.load_state_dict(other.state_dict())
+    from ravel_lm_b200.optim import AdamW
+    half = AdamW([torch.nn.Parameter(torch.zeros(300).bfloat16()) for _ in range(2)], lr=1e-2)
+    p = half.param_groups[0]["params"][0]
+    assert set(half._new_state(p, torch.ones(1, dtype=torch.int64))) == half._state_names(p)
+    with pytest.raises(ValueError, match="parameter of torch.bfloat16"):  # there is no master
+        half.load_state_dict(o.state_dict())
+    assert o.param_groups[0]["lr"] == 1e-2 and not half.state
+    fresh = AdamW([torch.nn.Parameter(torch.zeros(300)) for _ in range(2)], lr=0.1)
+    fresh.load_state_dict(o.state_dict())
+    a, b = (fresh.state[q] for q in fresh.param_groups[0]["params"])
+    assert a["step"] is b["step"] and int(a["step"]) == 1 and fresh.param_groups[0]["lr"] == 1e-2
