@@ -195,7 +195,8 @@ class AdamW(torch.optim.Optimizer):
                 continue
             if "exp_avg" in src and (src["exp_avg"].dtype == torch.uint8) != (self.state_bits == 8):
                 raise ValueError(f"the loaded states do not have state_bits={self.state_bits}")
-            if set(src) != self._state_names(p) or getattr(src["step"], "dtype", None) != torch.int64:
+            if (not self._state_names(p) <= set(src) or ("master" in src) != (p.dtype != torch.float32)
+                    or getattr(src["step"], "dtype", None) != torch.int64):
                 raise ValueError(f"the loaded states are not this optimizer's for a parameter of {p.dtype}")
         super().load_state_dict(state_dict)
         shared: dict = {}

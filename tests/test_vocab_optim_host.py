@@ -282,3 +282,11 @@ def test_states_of_another_optimizer_or_dtype_are_refused():
     fresh.load_state_dict(o.state_dict())
     a, b = (fresh.state[q] for q in fresh.param_groups[0]["params"])
     assert a["step"] is b["step"] and int(a["step"]) == 1 and fresh.param_groups[0]["lr"] == 1e-2
+
+
+def test_a_users_own_entries_in_the_states_are_loaded():
+    ps, o = _stepped(32)
+    o.state[ps[0]]["mine"] = torch.ones(2)
+    d = o.state_dict()
+    o.load_state_dict(d)
+    assert torch.equal(o.state[ps[0]]["mine"], torch.ones(2)) and "mine" not in o.state[ps[1]]
