@@ -415,3 +415,43 @@ def test_gradients_of_single_losses_without_rows():
         loss = ce(x, w, t, reduction="none")
         dx, dw = torch.autograd.grad(loss, [x, w], torch.zeros(0, device="cuda"))
         assert dx.shape == (0, 16) and dw.shape == (50, 16) and not dw.any()
+
+
+@pytest.mark.parametrize("dt,reduction,M,K,V", [
+    (torch.bfloat16, "sum", 200, 256, 900), (torch.float16, "sum", 200, 256, 900), (torch.bfloat16, "none", 100, 256, 900),
+    (torch.bfloat16, "sum", 1400, 512, 48000)])  # the last: the three-product form
+def test_gradients_of_confident_rows_are_as_exact_as_others(dt, reduction, M, K, V):
+    """Targets with 1 - p_t of 1e-4 to 1e-7, every row of its own token: relative to |d z|, of which the target's part
+    is 1 - p_t, so that a difference 1 - p_t taken in float32 (off by 2^-24 of 1) would show.
+
+    A logit's error moves 1 - p_t by p_t dl and hence by dl of itself (d log(1 - p_t) / d z_t = -p_t), another
+    column's probability likewise: 2 dl of |d z| holds both, and no term of p_t is added.
+    """
+    u = torch.finfo(dt).eps / 2
+    x, w, _ = make(M, K, V, dt, seed=18, scale=0.5, ignored=False)
+    t = torch.arange(M, device="cuda") * (V // M) + 1
+    # z_t = |x|^2 c, about log V + 9 to log V + 16; the other rows' logits with W_t are about N(0, c^2 K), small against it
+    c = torch.linspace(math.log(V) + 9, math.log(V) + 16, M, device="cuda") / K
+    w[t] = (x.float() * c[:, None]).to(dt)
+    want, d, dl, _ = reference(x, w, t)
+    rest = -torch.expm1(-want)  # 1 - p_t
+    assert float(rest.max()) < 3e-3 and float(rest.median()) < 1e-5 and float(rest.min()) < 1e-6
+    # from the other columns' probabilities, as a float64 difference at 1 - p_t = 1e-7 has 1e-9 of itself
+    d.scatter_(1, t[:, None], 0.0)
+    d.scatter_(1, t[:, None], -d.sum(1, keepdim=True))
+    xl, wl = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    got = torch.autograd.grad(ce(xl, wl, t, reduction=reduction), [xl, wl],
+                              torch.ones(M, device="cuda") if reduction == "none" else None)
+    xa, wa = x.double(), w.double()
+    rel = 2 * u + 2 * dl[:, None]
+    low = 2.0 ** -40 if dt == torch.float16 else 0.0
+    want_x, want_w = d @ wa, d.T @ xa
+    tx = (d.abs() * (rel + (V / 8 + 16) * 2.0 ** -23)) @ wa.abs() + low * wa.abs().sum(0) + (u + 4 * E) * want_x.abs()
+    tw = (d.abs() * (rel + (M / 8 + 16) * 2.0 ** -23)).T @ xa.abs() + low * xa.abs().sum(0) + (u + 4 * E) * want_w.abs()
+    within(got[0], want_x, tx + TINY[dt], "d x")
+    within(got[1], want_w, tw + TINY[dt], "d weight")
+    # and the bounds tell: gradients without the target's term lie beyond them in most elements
+    without = d.clone()
+    without.scatter_(1, t[:, None], 0.0)
+    assert float(((without @ wa - want_x).abs() > tx + TINY[dt]).double().mean()) > 0.5
+    assert float(((without.T @ xa - want_w).abs() > tw + TINY[dt])[t].double().mean()) > 0.5
