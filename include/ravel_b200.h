@@ -473,6 +473,9 @@ int ravel_embedding_bwd(const void* ids, int ids_dtype, const void* grad_y, int6
 size_t ravel_linear_ce_scratch_bytes(int64_t M, int64_t K, int64_t V);
 size_t ravel_linear_ce_work_bytes(int64_t M, int64_t K, int64_t V, int grads, int dtype);
 int ravel_linear_ce_slabs(int64_t M, int64_t K, int64_t V, int64_t* sizes);
+/* The launch shapes of the gradients' products on the current device (M > 0): for d x plan[0] CTAs per product (1, or 2: a
+ * pair), plan[1] columns of a tile, plan[2] CTAs that divide k; plan[3] to plan[5] for d W. */
+int ravel_linear_ce_plan(int64_t M, int64_t K, int64_t V, int* plan);
 int ravel_linear_ce_fwd(const void* x, int64_t ldx, const void* weight, int64_t ldw, const void* targets,
                         int target_dtype, int64_t M, int64_t K, int64_t V, int64_t ignore_index, int reduction, int keep,
                         float* losses, float* out, float* factor, float* slabs_x, float* slabs_w, int dtype,

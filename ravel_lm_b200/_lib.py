@@ -106,6 +106,7 @@ SIGNATURES = {
     "ravel_linear_ce_scratch_bytes": (_c_sz, [_c_i64] * 3),
     "ravel_linear_ce_work_bytes": (_c_sz, [_c_i64] * 3 + [_c_int, _c_int]),
     "ravel_linear_ce_slabs": (_c_int, [_c_i64] * 3 + [ctypes.POINTER(_c_i64)]),
+    "ravel_linear_ce_plan": (_c_int, [_c_i64] * 3 + [ctypes.POINTER(_c_int)]),
     "ravel_linear_ce_fwd": (_c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_int] + [_c_i64] * 4 + [_c_int, _c_int] + [_c_vp] * 5 +
                             [_c_int, _c_vp, _c_sz, _c_vp, _c_sz, _c_vp]),
     "ravel_linear_ce_grad": (_c_int, [_c_vp, _c_i64, _c_vp] + [_c_i64] * 3 + [_c_vp] * 3 +

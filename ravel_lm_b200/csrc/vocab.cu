@@ -300,8 +300,10 @@ struct HeadPlan {
 // Measured, us (rows x k; outputs; shape): d x 4096 x 16384, 1024: pairs 256 96, pairs 128 113, single 128 122;
 // d W 16384 x 4096, 512: pairs 256 in two parts 55, in one 82, pairs 128 62; d x 24 x 32000, 2048: single 128
 // in eight parts 21, pairs 256 30.
-HeadPlan plan_grad(int64_t M, int64_t N, int64_t k) {
+// least: the k of the call's shortest piece, of which every part needs a few chunks too.
+HeadPlan plan_grad(int64_t M, int64_t N, int64_t k, int64_t least) {
     const double sms = sm_count(), kc = static_cast<double>((k + MM_BK - 1) / MM_BK);
+    const int64_t least_kc = (least + MM_BK - 1) / MM_BK;
     struct Kind {
         int cg, bn;
         double fixed, chunk, epilogue;
@@ -312,7 +314,7 @@ HeadPlan plan_grad(int64_t M, int64_t N, int64_t k) {
     double cost = 1e30;
     for (const Kind& q : kinds) {
         const double tiles = std::ceil(M / (128.0 * q.cg)) * std::ceil(static_cast<double>(N) / q.bn);
-        for (int s = 1; s <= 32 && kc >= 4 * s; ++s) {
+        for (int s = 1; s <= 32 && (s == 1 || least_kc >= 4 * s); ++s) {
             const double waves = std::ceil(tiles * s / std::floor(sms / q.cg));
             const double us = q.fixed + waves * std::max(std::ceil(kc / s) * q.chunk, q.epilogue) + (s - 1) * (M * N) * 8.0 / 5e6;
             if (us < cost) cost = us, best = {q.cg, q.bn, s};
@@ -343,16 +345,14 @@ int head_grad(const HeadPlan& p, const HeadOperand& A, const HeadOperand& B, int
     return launch_grad<T, 1, 64, A_MN, ROWS>(A, B, k, a, st);
 }
 
-// The split counts of a whole call: of its full pieces for d W and of the first piece for d x.
+// The launch shapes and split counts of a whole call, by its full pieces; slabs are the same for every piece.
 struct HeadSplits {
     HeadPlan x, w;
 };
 HeadSplits head_splits(int64_t M, int64_t K, int64_t V) {
     const int64_t piece = head_piece(M, V);
-    // the last piece may have fewer rows: its k must still hold every split
-    const int64_t last = M - (std::max<int64_t>(M, 1) - 1) / piece * piece;
-    HeadSplits s = {plan_grad(piece, K, V), plan_grad(V, K, std::max<int64_t>(1, std::min(piece, last)))};
-    return s;
+    const int64_t last = M - (std::max<int64_t>(M, 1) - 1) / piece * piece;  // the last piece may have one row only
+    return {plan_grad(piece, K, V, V), plan_grad(V, K, piece, std::max<int64_t>(1, std::min(piece, last)))};
 }
 
 int head_check(int64_t M, int64_t K, int64_t V, int t_dtype, int dtype) {
@@ -632,6 +632,15 @@ int ravel_linear_ce_slabs(int64_t M, int64_t K, int64_t V, int64_t* sizes) {
     sizes[0] = s.x.splits;
     sizes[1] = s.w.splits;
     sizes[2] = up_to(K, 4);
+    return RAVEL_OK;
+}
+
+int ravel_linear_ce_plan(int64_t M, int64_t K, int64_t V, int* plan) {
+    if (plan == nullptr || M <= 0) return RAVEL_ERR_INVALID_ARG;
+    if (int e = head_check(M, K, V, RAVEL_I64, RAVEL_BF16)) return e;
+    const HeadSplits s = head_splits(M, K, V);
+    plan[0] = s.x.cg, plan[1] = s.x.bn, plan[2] = s.x.splits;
+    plan[3] = s.w.cg, plan[4] = s.w.bn, plan[5] = s.w.splits;
     return RAVEL_OK;
 }
 

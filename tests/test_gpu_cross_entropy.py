@@ -455,3 +455,9 @@ def test_gradients_of_confident_rows_are_as_exact_as_others(dt, reduction, M, K,
     without.scatter_(1, t[:, None], 0.0)
     assert float(((without @ wa - want_x).abs() > tx + TINY[dt]).double().mean()) > 0.5
     assert float(((without.T @ xa - want_w).abs() > tw + TINY[dt])[t].double().mean()) > 0.5
+
+
+@pytest.mark.parametrize("dt,K", [(torch.float16, 16), (torch.bfloat16, 16), (torch.bfloat16, 40)])
+def test_a_last_piece_of_one_row(dt, K):
+    """1024 rows a piece, four and a row; the last case takes three products."""
+    check(*make(4097, K, 210000, dt, seed=19))

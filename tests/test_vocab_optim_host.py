@@ -290,3 +290,24 @@ def test_a_users_own_entries_in_the_states_are_loaded():
     d = o.state_dict()
     o.load_state_dict(d)
     assert torch.equal(o.state[ps[0]]["mine"], torch.ones(2)) and "mine" not in o.state[ps[1]]
+
+
+def test_a_short_last_piece_does_not_choose_the_launch_shape(lib):
+    """Rows go in pieces; d weight's shape is the full pieces', and only its parts have to fit the last one's rows."""
+    def plan(M, K, V):
+        p = (ctypes.c_int * 6)()
+        assert lib.ravel_linear_ce_plan(M, K, V, p) == 0
+        sizes = (ctypes.c_int64 * 3)()
+        assert lib.ravel_linear_ce_slabs(M, K, V, sizes) == 0 and [p[2], p[5]] == list(sizes[:2])
+        return list(p)
+    for M, K, V in ((16384, 512, 131072), (16384, 1024, 131072), (4096, 64, 262144), (4096, 2048, 262144)):
+        even = plan(M, K, V)
+        for rest in (1, 100, 193):
+            assert plan(M + rest, K, V)[:5] == even[:5], (M, K, V, rest)
+        assert plan(M + 1, K, V)[5] == 1  # one row: a single part
+    for M in (1, 24, 128, 192):  # few rows: tiles by the estimate, in one part (a part has 4 chunks of 64 at least)
+        for K, V in ((2048, 32000), (64, 300)):
+            assert plan(M, K, V)[5] == 1
+    p = (ctypes.c_int * 6)()
+    assert lib.ravel_linear_ce_plan(0, 8, 8, p) == INVALID and lib.ravel_linear_ce_plan(8, 8, 8, None) == INVALID
+    assert lib.ravel_linear_ce_plan(8, 0, 8, p) == INVALID
