@@ -464,7 +464,7 @@ int ravel_embedding_bwd(const void* ids, int ids_dtype, const void* grad_y, int6
  * A training step gives slabs_x and slabs_w (either may be NULL): float32
  * sums of the gradients for an upstream gradient of 1, sizes[0] slabs of M rows and
  * sizes[1] slabs of V rows, rows sizes[2] floats apart (ravel_linear_ce_slabs);
- * factor (one float) goes with them.  ravel_linear_ce_bwd adds the slabs up, scales
+ * factor (one float) goes with them; slabs start on 16 bytes.  ravel_linear_ce_bwd adds the slabs up, scales
  * them by *up (device) and rounds: grad_x [M, K], grad_w [V, K], contiguous.
  * Single rows' losses (RAVEL_REDUCE_NONE, keep set in the forward) get their gradients from
  * ravel_linear_ce_grad, given the forward's scratch and up [M]; then ravel_linear_ce_bwd

@@ -739,7 +739,8 @@ int ravel_linear_ce_bwd(const float* slabs_x, const float* slabs_w, const float*
                         int64_t K, int64_t V, void* grad_x, void* grad_w, int dtype, void* stream) {
     RAVEL_TIMED("ravel_linear_ce_bwd", stream);
     if (int e = head_check(M, K, V, RAVEL_I64, dtype)) return e;
-    if (factor == nullptr || (grad_x != nullptr && M > 0 && slabs_x == nullptr) || (grad_w != nullptr && slabs_w == nullptr))
+    if (factor == nullptr || (grad_x != nullptr && M > 0 && slabs_x == nullptr) || (grad_w != nullptr && slabs_w == nullptr) ||
+        !aligned16(slabs_x) || !aligned16(slabs_w))
         return RAVEL_ERR_INVALID_ARG;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const HeadSplits s = head_splits(M, K, V);

@@ -311,3 +311,10 @@ def test_a_short_last_piece_does_not_choose_the_launch_shape(lib):
     p = (ctypes.c_int * 6)()
     assert lib.ravel_linear_ce_plan(0, 8, 8, p) == INVALID and lib.ravel_linear_ce_plan(8, 8, 8, None) == INVALID
     assert lib.ravel_linear_ce_plan(8, 0, 8, p) == INVALID
+
+
+def test_unaligned_gradient_sums_are_refused(lib):
+    """The outputs' kernel reads slabs 16 bytes at a time."""
+    def bwd(sx=P, sw=P):
+        return lib.ravel_linear_ce_bwd(sx, sw, P, P, 8, 64, 100, P, P, 1, None)
+    assert bwd(sx=P + 4) == INVALID and bwd(sw=P + 8) == INVALID
