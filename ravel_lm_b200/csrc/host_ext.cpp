@@ -667,7 +667,7 @@ at::Tensor token_embedding(const at::Tensor& ids, const at::Tensor& weight, doub
         throw py::value_error("token_embedding expects a weight [V, K] with V >= 1");
     index_code(ids, "ids");
     float_code(weight, "token_embedding");
-    if (!std::isfinite(scale)) throw py::value_error("scale must be finite");
+    if (!std::isfinite(static_cast<float>(scale))) throw py::value_error("scale must be finite (in float32)");
     const int64_t V = weight.size(0);
     int64_t padding = -1;
     if (padding_idx) {

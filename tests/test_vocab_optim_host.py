@@ -318,3 +318,11 @@ def test_unaligned_gradient_sums_are_refused(lib):
     def bwd(sx=P, sw=P):
         return lib.ravel_linear_ce_bwd(sx, sw, P, P, 8, 64, 100, P, P, 1, None)
     assert bwd(sx=P + 4) == INVALID and bwd(sw=P + 8) == INVALID
+
+
+def test_a_scale_past_float32_is_refused():
+    from ravel_lm_b200.vocab import token_embedding
+    ids, w = torch.zeros(3, dtype=torch.long), torch.zeros(5, 8)
+    for scale in (1e39, -1e300):
+        with pytest.raises(ValueError, match="finite"):  # it would be an infinity to the kernel
+            token_embedding(ids, w, scale=scale)
