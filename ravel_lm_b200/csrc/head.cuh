@@ -623,7 +623,8 @@ __global__ void __launch_bounds__(1024) k_head_total(const float* __restrict__ l
     if (factor != nullptr) *factor = 1.0f / rows;
 }
 
-// *up_max = the largest |up| of a row with a target (1 where that is 0): one block.
+// *up_max = the largest finite |up| of a row with a target (1 where that is 0): one block.  Rows are kept relative to it, so
+// that one infinity among them would leave no other.
 __global__ void __launch_bounds__(1024) k_head_up_max(const float* __restrict__ up, const int32_t* __restrict__ target,
                                                       int64_t M, float* __restrict__ up_max) {
     __shared__ float red[32];
@@ -632,7 +633,7 @@ __global__ void __launch_bounds__(1024) k_head_up_max(const float* __restrict__ 
     float m = 0.0f;
 #pragma unroll 4
     for (int64_t i = threadIdx.x; i < M; i += 1024)
-        if (target[i] >= 0) m = fmaxf(m, fabsf(up[i]));
+        if (target[i] >= 0 && fabsf(up[i]) < INFINITY) m = fmaxf(m, fabsf(up[i]));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;

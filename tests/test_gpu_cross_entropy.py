@@ -461,3 +461,18 @@ def test_gradients_of_confident_rows_are_as_exact_as_others(dt, reduction, M, K,
 def test_a_last_piece_of_one_row(dt, K):
     """1024 rows a piece, four and a row; the last case takes three products."""
     check(*make(4097, K, 210000, dt, seed=19))
+
+
+@pytest.mark.parametrize("dt", DTYPES)
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_a_row_whose_upstream_gradient_is_no_number_leaves_the_others(dt, bad):
+    x, w, t = make(200, 64, 300, dt, seed=24, ignored=False)
+    x.requires_grad_(True)
+    loss = ce(x, w, t, reduction="none")
+    up = torch.linspace(-1.0, 2.0, 200, device="cuda")
+    up[3] = 0.0
+    want, = torch.autograd.grad(loss, x, up, retain_graph=True)
+    up[3] = bad
+    got, = torch.autograd.grad(loss, x, up)
+    rest = torch.arange(200, device="cuda") != 3
+    assert torch.equal(got[rest], want[rest]) and torch.isfinite(want).all() and not torch.isfinite(got[3]).any()
