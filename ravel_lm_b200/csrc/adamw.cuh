@@ -373,10 +373,11 @@ struct AdamPlace {
     }
 };
 
-// 8-bit states: bound by issue slots and the latency of their chains, some 70 instructions an element; five blocks an SM
-// (48 registers) beat four and six (118 M bfloat16 parameters with their values read back: 508 us, 550, 514).
+// 8-bit states: bound by issue slots and the latency of their chains, some 70 instructions an element; six blocks an SM
+// (40 registers) beat five and four (118 M bfloat16 parameters with their values read back: 492 us, 509, 526; 24 M float16,
+// clipped: 119, 124, 128).
 template <typename T, bool EIGHT, int CAP>
-__global__ void __launch_bounds__(32 * AW_WARPS, EIGHT ? 5 : 4) k_adamw(const __grid_constant__ AdamArgs<CAP> a) {
+__global__ void __launch_bounds__(32 * AW_WARPS, EIGHT ? 6 : 4) k_adamw(const __grid_constant__ AdamArgs<CAP> a) {
     grid_wait();
     grid_trigger();
     const AdamPlace at(a, blockIdx.x);
