@@ -529,6 +529,7 @@ int ravel_grad_norm(const ravel_adamw_tensor* tensors, int64_t count, int dtype,
  *   g' = g min(1, max_norm / (norm + 1e-6))    (max_norm 0: g)
  *   m = beta1 m + (1 - beta1) g',  v = beta2 v + (1 - beta2) g'^2
  *   p = p (1 - lr wd) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * A positive eps below 2^-126 counts as 2^-126.
  * norm: *norm where given (ravel_grad_norm's, over this list and others), else over
  * this list.  lr_device (one float32 on the device) is taken in place of lr where given.
  * norm_out (NULL: not wanted) receives the norm in float32.  8-bit states are

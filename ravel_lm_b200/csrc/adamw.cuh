@@ -4,8 +4,8 @@
 //   m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2
 //   p = p (1 - lr wd) - lr / (1 - b1^t)  m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
-// in float32 (p: the float32 master of a 16-bit parameter, which gets its rounding in the same pass), two elements an
-// instruction; the root and the reciprocal are the hardware's approximations (2^-22 of a step that is a small part of p).
+// in float32 (p: the float32 master of a 16-bit parameter, which gets its rounding in the same pass; an eps below
+// float32's least normal number counts as that), two elements an instruction; the root and the reciprocal are the hardware's approximations (2^-22 of a step that is a small part of p).
 //
 //   k_grad_norm      sums of squares in float64, a part per block (any float32 gradient's square is finite there, and the
 //                    sum is the same to float32 whatever its order); k_norm_total adds the parts for callers of the norm.
@@ -205,7 +205,8 @@ __device__ __forceinline__ float rcp_approx(float x) {
     return y;
 }
 
-// Well-mixed bits of 32: two multiplications between shifted exclusive ors.
+// Well-mixed bits of 32: two multiplications between shifted exclusive ors, with the shifts and multipliers of
+// C. Wellons, "Prospecting for Hash Functions" (2018).
 __device__ __forceinline__ uint32_t mix32(uint32_t i) {
     i = (i ^ (i >> 16)) * 0x7FEB352Du;
     i = (i ^ (i >> 15)) * 0x846CA68Bu;
@@ -373,7 +374,7 @@ struct AdamPlace {
     }
 };
 
-// 8-bit states: bound by issue slots and the latency of their chains, some 70 instructions an element; six blocks an SM
+// 8-bit states: bound by issue slots and the latency of their chains, some 80 instructions an element; six blocks an SM
 // (40 registers) beat five and four (118 M bfloat16 parameters with their values read back: 492 us, 509, 526; 24 M float16,
 // clipped: 119, 124, 128).
 template <typename T, bool EIGHT, int CAP>

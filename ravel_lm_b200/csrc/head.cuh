@@ -13,7 +13,8 @@
 //                  columns, the target's column apart (so that a confident row's 1 - p_t is no difference), a few
 //                  parts per row and tile in memory; the target's logit is kept.
 //     HEAD_EXP     with the row's maximum and sum known: d z in 16 bits (the tensor cores' operand), for a piece
-//                  of the rows.
+//                  of the rows.  The target's term is among them: -1 is exact, u (p_t - 1) with upstream gradients
+//                  per row is one rounding more (errors of d x and d W 1.35 times an output's rounding alone).
 //     HEAD_FAST    both in one product: E = exp(z - z_t) in 16 bits and its sums.
 //   k_head_rows    the parts of a row joined: loss, maximum, log2 of the sum, 1 - p_t.
 //   k_head_grad    d x and d W of a piece as float32 products, k divided over splits whose sums lie in slabs of their
@@ -26,7 +27,7 @@
 //
 //   loss = log(1 + s),   d x = f (E W) - (1 - p_t) W_t,   d W = E^T (f x) - sum over the rows with t = v of (1 - p_t) x
 //
-// E_t left out of E; the last sums run over the positions sorted by target (embedding.cuh), in float32, so that the
+// E_t left out of E, and f x rounded to bfloat16 for d W's product as E is; the last sums run over the positions sorted by target (embedding.cuh), in float32, so that the
 // target's term, which carries most of the gradient, is not rounded to 16 bits.  A row whose s passes 2^80 (a
 // loss above 55) or is no number flags its piece, and three launches that otherwise return at once do it by
 // HEAD_STATS and HEAD_EXP.  8192 x 1024 x 65536: 2.9 ms, 3.6 with four products (power-capped: the products run at

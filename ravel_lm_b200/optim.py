@@ -8,12 +8,12 @@ clipping by the global norm (``runtime.py:9``).  Per element, in float32:
     m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2
     p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 
-A 16-bit parameter is the rounding of a float32 master that takes the steps.  8-bit
-states share a power of two per block of 256 elements, sign + 4 + 3 bits for m and 5 + 3
-for v, and are rounded stochastically (the random bits are a hash of step, tensor and
-element: a run repeats bit for bit).  ``AdamW`` keeps every positive v positive, so that
-a block may hold elements of very different gradients.  A block that meets a NaN or an infinity stands for
-NaN as a whole from then on.
+(a positive eps below 2^-126 counts as 2^-126).  A 16-bit parameter is the rounding of a
+float32 master that takes the steps.  8-bit states share a power of two per block of 256
+elements, sign + 4 + 3 bits for m and 5 + 3 for v, and are rounded stochastically (the
+random bits are a hash of step, tensor and element: a run repeats bit for bit).  ``AdamW``
+keeps every positive v positive, so that a block may hold elements of very different
+gradients.  A block that meets a NaN or an infinity stands for NaN as a whole from then on.
 
 The step count lives on the device and the learning rate may too, so that a step
 captured in a CUDA graph counts on in every replay.

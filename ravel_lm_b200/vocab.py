@@ -14,11 +14,15 @@ a maximum and a sum per row where they are made.  A training step makes the grad
 a reduced loss in its forward, piece of rows by piece of rows: ``softmax - onehot`` in
 16 bits (at most 512 MB or 1024 rows of it) from the logits' product done again -- large
 bfloat16 steps get it from the first, as exp(z - z_target) and a factor per row -- and
-its two products, in float32.  These float32 gradients are held until the graph goes; the
-backward scales them by the upstream gradient and rounds them once, so that it may be run again,
+its two products, in float32.  These float32 gradients (several slabs of one, where its product has few tiles) are held
+until the graph goes; the backward scales them by the upstream gradient and rounds them once, so that it may be run again,
 and a float16 loss scale loses nothing.  Single rows' losses (``reduction="none"``) get their
 gradients in the backward, where the rows' upstream gradients are known.
-Probabilities enter the gradients' products rounded to 16 bits; everything else is float32.
+Sums are float32.  What enters the gradients' products is rounded to 16 bits: the operands of either product, with
+``reduction="none"`` the upstream gradient times ``softmax - onehot`` as a whole, in the three-product form (large
+bfloat16 steps) exp(z - z_target) and, for the weight's gradient, x times the row's factor; the target's
+own term, which carries most of a gradient, stays in float32 there.  In float16 what lies below 2^-40 of the
+largest upstream gradient is dropped.
 
 There is no CPU path, no float32 form of the cross entropy (parameters kept in float32, as under
 autocast, are cast by the caller), no second derivative and no forward-mode one.
