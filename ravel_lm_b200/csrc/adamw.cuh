@@ -5,7 +5,8 @@
 //   p = p (1 - lr wd) - lr / (1 - b1^t)  m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // in float32 (p: the float32 master of a 16-bit parameter, which gets its rounding in the same pass; an eps below
-// float32's least normal number counts as that), two elements an instruction; the root and the reciprocal are the hardware's approximations (2^-22 of a step that is a small part of p).
+// float32's least normal number counts as that), two elements an instruction; the root and the reciprocal are the
+// hardware's approximations (2^-22 of a step that is a small part of p).
 //
 //   k_grad_norm      sums of squares in float64, a part per block (any float32 gradient's square is finite there, and the
 //                    sum is the same to float32 whatever its order); k_norm_total adds the parts for callers of the norm.
@@ -23,8 +24,8 @@
 // would drop for ever.  With RAVEL_STATE_POSITIVE a positive v has code 1 at least, 2^-33 2^e, and code 0 is exactly 0:
 // where elements of very different gradients share a block, a small one's m may round up to 2^-17 of the
 // block's largest, and over a v rounded to 0 that is a step of m / eps (gradients about 1, 1e-5 times
-// that in half of each block, 300 steps: up to 1400 lr; so, 1.8 lr).  The random bits are a hash of (step, tensor, element): the same call gives the same
-// bits.  A block that meets a NaN or an infinity is marked (exponent -128) and stands for NaN from then on.
+// that in half of each block, 300 steps: up to 1400 lr; so, 1.8 lr).  The random bits are a hash of (step, tensor, element):
+// the same call gives the same bits.  A block that meets a NaN or an infinity is marked (exponent -128) and stands for NaN from then on.
 //
 // Bound by HBM.
 #pragma once

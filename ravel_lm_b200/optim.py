@@ -143,7 +143,7 @@ class AdamW(torch.optim.Optimizer):
             if p.grad is None:
                 continue
             st = self.state.get(p)
-            if (not st or id(st["step"]) in idle) and torch.cuda.is_current_stream_capturing():
+            if (not st or id(st["step"]) in idle) and torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("AdamW: take a step with gradients for the same parameters before a capture; a "
                                    + ("new state" if not st else "step count copied for some of them")
                                    + " would start again in every replay")

@@ -230,6 +230,7 @@ def _stepped(bits):
 
 def test_a_capture_makes_no_states_and_copies_no_count(monkeypatch):
     ps, o = _stepped(32)
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
     group = o.param_groups[0]
     assert o._buckets(group) == [ps]  # every state is there
@@ -326,3 +327,12 @@ def test_a_scale_past_float32_is_refused():
     for scale in (1e39, -1e300):
         with pytest.raises(ValueError, match="finite"):  # it would be an infinity to the kernel
             token_embedding(ids, w, scale=scale)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_the_optimizer_refuses_cpu_parameters_without_a_gpu_too(bits):
+    from ravel_lm_b200.optim import AdamW
+    p = torch.nn.Parameter(torch.zeros(3))
+    p.grad = torch.ones(3)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        AdamW([p], state_bits=bits).step()
